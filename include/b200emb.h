@@ -364,6 +364,129 @@ int b200emb_op_add_ln(const void* x, const void* y, const float* gamma, const fl
 int b200emb_op_pool(const void* x, const int32_t* d_cu_seqlens, int32_t n_seqs, int32_t hidden, int32_t pooling,
                     int32_t normalize, void* out, int64_t out_row_stride, int32_t out_bf16, void* stream);
 
+/* ---- the attention block of models with relative positions ---------------------
+ * Rotary positions, a paged key / value cache, and attention whose scores are capped, biased by distance or
+ * masked. Device pointers on the current device, bf16 storage, fp32 (angles: fp64) arithmetic; asynchronous on
+ * `stream`, no allocation, capturable into a CUDA graph. cu_seqlens and kv_lens are read on the DEVICE only, so a
+ * captured graph follows their values; nothing in them can move an access out of its buffer: sequences are
+ * cut to [0, n_tokens), a page index outside [0, n_pages) reads as zeros and is never written. Rows from
+ * cu_seqlens[n_seqs] on are left as they were. Empty sequences are allowed. n_tokens == 0 or n_seqs == 0: nothing
+ * is done. None has a counterpart function in the reference: its models reach such attention through
+ * third-party torch code behind sentence_transformer.py:124. */
+
+/* b200emb_rope_desc.layout */
+#define B200EMB_ROPE_HALF 0        /* element i of the rotated part pairs with i + rot_dim / 2 */
+#define B200EMB_ROPE_INTERLEAVED 1 /* element 2i pairs with 2i + 1 */
+/* b200emb_rope_desc.scaling: angle per position of pair i, w_i = theta^(-2i / rot_dim) unscaled */
+#define B200EMB_ROPE_SCALE_NONE 0
+#define B200EMB_ROPE_SCALE_LINEAR 1 /* w_i / factor */
+#define B200EMB_ROPE_SCALE_NTK 2    /* theta replaced by theta * factor^(rot_dim / (rot_dim - 2)); rot_dim > 2 */
+/* With t_i = original_max_pos * w_i / 2 pi (rotations over the trained length): w_i kept where t_i >= high, w_i / factor
+ * where t_i <= low, in between w_i (k + (1 - k) / factor) with k = (t_i - low) / (high - low). 0 <= low < high. */
+#define B200EMB_ROPE_SCALE_BANDS 3
+/* YaRN: with d(n) = rot_dim ln(original_max_pos / (2 pi n)) / (2 ln theta), a = max(0, floor(d(low))),
+ * b = min(rot_dim - 1, ceil(d(high))) and k = clamp((i - a) / max(b - a, 0.001), 0, 1): w_i (1 - k) + w_i / factor * k. Here
+ * low is the FAST edge (usually 32 rotations) and high the SLOW one (usually 1): 0 < high <= low; theta != 1. */
+#define B200EMB_ROPE_SCALE_YARN 4
+
+typedef struct b200emb_rope_desc {
+  int32_t rot_dim;          /* the first rot_dim elements of every head are rotated, the rest passes through; even, 2 .. 256 */
+  int32_t layout;
+  int32_t scaling;
+  int32_t original_max_pos; /* BANDS and YARN: trained length, > 0 */
+  float theta;              /* > 0 */
+  float factor;             /* every scaling but NONE: > 0 */
+  float low, high;          /* BANDS and YARN, see above */
+  float magnitude;          /* cos and sin are multiplied by it; 0 = 1, with YARN 0.1 ln(max(factor, 1)) + 1 */
+  int32_t inverse;          /* 1: rotate by the negative angle (the transpose: the gradient, or positions taken back) */
+  int32_t reserved[6];      /* zero */
+} b200emb_rope_desc;
+
+/* out[t, h, :] = rotation of x[t, h, :] by the position of token t, for the first n_heads heads of every row
+ * (x row stride x_row_stride, out row stride out_row_stride elements; out == x rotates in place, other overlaps are not
+ * allowed). Position: positions[t] when given (then cu_seqlens and pos_start are not read), else
+ * pos_start[s] (0 when null) + t - cu_seqlens[s] for token t of sequence s. With `positions` every row below n_tokens is
+ * rotated and n_seqs is ignored. Angles are formed and reduced in fp64, so far positions lose nothing.
+ * head_dim >= rot_dim; rows of any alignment (16-byte aligned rows are fastest). */
+int b200emb_op_rope(const void* x, int64_t x_row_stride, void* out, int64_t out_row_stride, const int32_t* positions,
+                    const int32_t* d_cu_seqlens, const int32_t* d_pos_start, int32_t n_seqs, int32_t n_tokens,
+                    int32_t n_heads, int32_t head_dim, const b200emb_rope_desc* rope, void* stream);
+
+/* A paged key / value cache: element (page p, token o, head h, j) of k and of v lies at
+ * p * page_stride + o * token_stride + h * head_stride + j (elements), so pages may hold tokens of all heads
+ * ([page_size, n_kv_heads, head_dim]) or heads of all tokens ([n_kv_heads, page_size, head_dim]). Key j of sequence s is in
+ * page page_table[s * table_stride + j / page_size] at j % page_size; table entries past the sequence's last page are
+ * not used. Several sequences may share pages that they only read. */
+typedef struct b200emb_kv_cache {
+  void* k;
+  void* v;                   /* device, bf16 */
+  const int32_t* page_table; /* device [n_seqs, table_stride] */
+  int32_t n_pages, page_size, n_kv_heads, head_dim;
+  int32_t table_stride;      /* pages of the longest sequence, at least */
+  int32_t reserved;          /* zero */
+  int64_t page_stride, token_stride, head_stride;
+} b200emb_kv_cache;
+
+/* Writes the keys and values of the new tokens into the cache and, with `rope`, rotates queries and keys on the way.
+ * qkv is the packed buffer of b200emb_op_attention with row stride qkv_row_stride. kv_lens[s] counts the keys of
+ * sequence s INCLUDING its new tokens: token t of sequence s gets position kv_lens[s] - (new tokens of s) + t - cu_seqlens[s].
+ * q_out [n_tokens, n_heads * head_dim] (row stride q_out_row_stride) receives the queries (copied when rope is null);
+ * q_out null: they are not touched. Tokens at a negative position, past the page table or on a page outside [0, n_pages)
+ * are not stored. A slot written by two tokens holds one of the two. */
+int b200emb_op_kv_append(const void* qkv, int64_t qkv_row_stride, const int32_t* d_cu_seqlens, const int32_t* d_kv_lens,
+                         int32_t n_seqs, int32_t n_tokens, int32_t n_heads, const b200emb_rope_desc* rope, void* q_out,
+                         int64_t q_out_row_stride, const b200emb_kv_cache* cache, void* stream);
+
+/* What the attention below does to its scores. Query i and key j are positions within the sequence; h is the query head.
+ *   s = scale * q_i . k_j;  cap > 0: s = cap * tanh(s / cap);  slopes: s -= slopes[h] * |i - j|;
+ *   bias: s += bias[h * (2 R + 1) + clamp(j - i, -R, R) + R], R = bias_radius
+ * Key j is visible to query i when (j <= i + window_right and j >= i - window_left) or j < prefix_lens[s], and with
+ * doc_ids only when doc_ids of both tokens are equal and not negative. A row that sees no key (or only -inf) is zero.
+ * Masked scores are selected away, so keys may hold anything there; a VALUE that is not finite reaches every row of its own
+ * sequence whose tiles cover it (0 * inf), never another sequence, and slots past the sequence's end never count. */
+typedef struct b200emb_attn_opts {
+  float scale;              /* 0 = 1 / sqrt(head_dim) */
+  float cap;                /* 0 = none */
+  int32_t causal;           /* 1 = window_right 0 (window_right must then be <= 0) */
+  int32_t window_left;      /* < 0 = unlimited */
+  int32_t window_right;     /* < 0 = unlimited */
+  int32_t bias_radius;      /* 0 .. 1023 */
+  const float* slopes;      /* device [n_heads] or null */
+  const float* bias;        /* device [n_heads, 2 * bias_radius + 1] or null; not together with slopes */
+  const int32_t* prefix_lens; /* device [n_seqs] or null */
+  const int32_t* doc_ids;   /* device [n_tokens] or null; packed attention only */
+  int32_t reserved[4];      /* zero */
+} b200emb_attn_opts;
+
+/* Bytes of device workspace (256-byte aligned) the two attention calls below need for these sizes; enough for every smaller
+ * n_seqs and n_tokens too. The contents need no initialisation. Two calls that may run at the same time need two workspaces.
+ * Negative status for sizes the calls refuse. */
+int64_t b200emb_attention_workspace_bytes(int32_t n_seqs, int32_t n_tokens, int32_t n_heads, int32_t n_kv_heads,
+                                          int32_t head_dim);
+
+/* Waits for the stream and reports whether a bounded device-side wait of the last attention call on this workspace gave up
+ * (B200EMB_ERR_DEVICE_WAIT; its output is then not valid). The calls themselves do not wait and so cannot report it. */
+int b200emb_op_workspace_status(const void* workspace, void* stream);
+
+/* Packed variable-length attention: q [n_tokens, n_heads * head_dim], k and v [n_tokens, n_kv_heads * head_dim], out
+ * [n_tokens, n_heads * head_dim], each with its own row stride (elements, a multiple of 8) and 16-byte aligned, so the packed qkv
+ * buffer serves with three pointers. n_heads a multiple of n_kv_heads and at most 128 times it; head_dim a multiple of 8, 8 .. 128.
+ * opts null: plain bidirectional attention. Query i of a sequence is at position i. */
+int b200emb_op_attention_scored(const void* q, int64_t q_row_stride, const void* k, int64_t k_row_stride, const void* v,
+                                int64_t v_row_stride, void* out, int64_t out_row_stride, const int32_t* d_cu_seqlens,
+                                int32_t n_seqs, int32_t n_tokens, int32_t n_heads, int32_t n_kv_heads, int32_t head_dim,
+                                const b200emb_attn_opts* opts, void* workspace, int64_t workspace_bytes, void* stream);
+
+/* Attention of new tokens (a chunk of any length, or one) over the paged cache, which already holds their own keys
+ * (b200emb_op_kv_append). The new tokens of sequence s are rows cu_seqlens[s] .. cu_seqlens[s + 1] - 1 of q and out and take the last
+ * positions below kv_lens[s]. kv_lens is cut to table_stride * page_size. page_size a multiple of 8; the three cache
+ * strides multiples of 8, k and v 16-byte aligned. opts null: causal. Few rows over long caches are split over the keys
+ * and joined in a fixed order: results depend on the batch's lengths and the device alone. */
+int b200emb_op_attention_paged(const void* q, int64_t q_row_stride, void* out, int64_t out_row_stride,
+                               const int32_t* d_cu_seqlens, const int32_t* d_kv_lens, int32_t n_seqs, int32_t n_tokens,
+                               int32_t n_heads, const b200emb_kv_cache* cache, const b200emb_attn_opts* opts, void* workspace,
+                               int64_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

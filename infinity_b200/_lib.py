@@ -23,6 +23,8 @@ EMB_NUMPY = {"float32": "float32", "int8": "int8", "uint8": "uint8", "binary": "
 HEAD = {"none": 0, "classifier": 1}
 WFMT = {"bf16": 0, "mxfp8": 1, "nvfp4": 2}
 EPI = {"bias": 0, "gelu": 1, "tanh": 2, "swiglu": 3}
+ROPE_LAYOUT = {"half": 0, "interleaved": 1}
+ROPE_SCALING = {"none": 0, "linear": 1, "ntk": 2, "bands": 3, "yarn": 4}
 
 
 class ModelDesc(C.Structure):
@@ -43,6 +45,30 @@ class Timing(C.Structure):
         ("d2h_ms", C.c_float), ("total_ms", C.c_float), ("launches", C.c_int32),
         ("kclass_ms", C.c_float * N_KCLASS), ("kclass_launches", C.c_int32 * N_KCLASS),
         ("gemm_flops", C.c_double),
+    ]
+
+
+class RopeDesc(C.Structure):
+    _fields_ = [
+        ("rot_dim", C.c_int32), ("layout", C.c_int32), ("scaling", C.c_int32), ("original_max_pos", C.c_int32),
+        ("theta", C.c_float), ("factor", C.c_float), ("low", C.c_float), ("high", C.c_float), ("magnitude", C.c_float),
+        ("inverse", C.c_int32), ("reserved", C.c_int32 * 6),
+    ]
+
+
+class KvCache(C.Structure):
+    _fields_ = [
+        ("k", C.c_void_p), ("v", C.c_void_p), ("page_table", C.c_void_p), ("n_pages", C.c_int32),
+        ("page_size", C.c_int32), ("n_kv_heads", C.c_int32), ("head_dim", C.c_int32), ("table_stride", C.c_int32),
+        ("reserved", C.c_int32), ("page_stride", C.c_int64), ("token_stride", C.c_int64), ("head_stride", C.c_int64),
+    ]
+
+
+class AttnOpts(C.Structure):
+    _fields_ = [
+        ("scale", C.c_float), ("cap", C.c_float), ("causal", C.c_int32), ("window_left", C.c_int32),
+        ("window_right", C.c_int32), ("bias_radius", C.c_int32), ("slopes", C.c_void_p), ("bias", C.c_void_p),
+        ("prefix_lens", C.c_void_p), ("doc_ids", C.c_void_p), ("reserved", C.c_int32 * 4),
     ]
 
 
@@ -82,6 +108,14 @@ SIGNATURES = {
     "b200emb_op_pool": (C.c_int, [_P, _P, C.c_int32, C.c_int32, C.c_int32, C.c_int32, _P, C.c_int64, C.c_int32, _P]),
     "b200emb_forward_quantized": (C.c_int, [_P, _P, _P, _P, C.c_int32, C.c_int32, C.c_int32, _P, _P, C.c_int64, C.POINTER(Timing)]),
     "b200emb_op_quantize_embeddings": (C.c_int, [_P, C.c_int32, C.c_int32, C.c_int64, C.c_int32, _P, _P, C.c_int64, _P]),
+    "b200emb_op_rope": (C.c_int, [_P, C.c_int64, _P, C.c_int64, _P, _P, _P, C.c_int32, C.c_int32, C.c_int32, C.c_int32, _P, _P]),
+    "b200emb_op_kv_append": (C.c_int, [_P, C.c_int64, _P, _P, C.c_int32, C.c_int32, C.c_int32, _P, _P, C.c_int64, _P, _P]),
+    "b200emb_attention_workspace_bytes": (C.c_int64, [C.c_int32, C.c_int32, C.c_int32, C.c_int32, C.c_int32]),
+    "b200emb_op_workspace_status": (C.c_int, [_P, _P]),
+    "b200emb_op_attention_scored": (C.c_int, [_P, C.c_int64, _P, C.c_int64, _P, C.c_int64, _P, C.c_int64, _P, C.c_int32, C.c_int32,
+                                              C.c_int32, C.c_int32, C.c_int32, _P, _P, C.c_int64, _P]),
+    "b200emb_op_attention_paged": (C.c_int, [_P, C.c_int64, _P, C.c_int64, _P, _P, C.c_int32, C.c_int32, C.c_int32, _P, _P, _P,
+                                             C.c_int64, _P]),
 }
 
 _lib = None

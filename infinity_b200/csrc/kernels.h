@@ -190,4 +190,8 @@ int launch_small_proj(const void* x, const void* W, const float* bias, int n_row
 // softmax over each row's n_labels logits (logistic function when n_labels == 1), in place
 int launch_label_scores(float* logits, int n_rows, int n_labels, int64_t row_stride, cudaStream_t stream);
 
+// ---- paged cache (rope.cu) ----
+// Status of a cache descriptor; `who` names the entry point in the message.
+int check_kv_cache(const b200emb_kv_cache* c, const char* who);
+
 }  // namespace b2
