@@ -1,20 +1,56 @@
-// Attention with modified scores over a packed batch, and the same over a paged key / value cache.
+// Attention with modified scores over a packed batch, and the same over a paged key / value cache, on the 5th-generation
+// tensor cores.
 //
-// One warp per (query token, head): the lanes share the head dimension, the keys are walked once with a running
-// maximum and sum (m, l, o) <- (m', l e^(m - m') + e^(s - m'), o e^(m - m') + e^(s - m') v).
+// Rows. The G query heads that share a key head are packed into one 128-row tile: row r of a tile is token r / G, head
+// r % G, so a single new token of a grouped model fills G rows of one tile instead of one row of G tiles, and its keys are read
+// once. An item is a query tile of one key head with the key tiles (128 keys) its masks can reach: at most two runs of
+// tiles, the prefix and the window (a document mask cuts both to the tiles whose documents meet the query tile's).
+//
+// Split. A planning kernel (one block) lists the items and cuts the row of all (item, key tile) steps into equal parts, one
+// per stream of the grid, wherever the cuts fall: few rows over long caches and many short sequences are balanced by the same
+// rule. An item that a cut divides leaves partial results (fp32 numerators, maximum, denominator) in the workspace; the
+// stream that finishes last joins them in the order of the parts, so the result depends on the lengths and not on timing.
+//
+// A CTA (one per SM) runs two streams, A and B, each with its own 128-row tile, softmax warpgroup and tensor-memory
+// accumulators, so that one stream's exponentials run under the other's matrix products. With long queries the two streams take
+// neighbouring tiles of the same item row and share every key and value tile ("pair"); otherwise each walks its own part.
+// Per step of a stream:
+//   S = Q K^T     tcgen05.mma 128 x N x 16 (N = valid keys rounded up to 16), fp32 in tensor memory
+//   softmax       128 threads, one row each: the whole score row is read into registers, modified and masked there, and reduced to
+//                 its maximum; the reference of the exponentials moves only when the maximum passes it by 2^8
+//                 (probabilities then stay below 2^8, sums far inside fp32), which is when O is rescaled
+//   O += P V      P rounded to bf16 (the tensor core's operand type; half a step of 2^-8 per probability) in tensor memory, V as an MN-major
+//                 shared-memory operand
+// Warps: 0-3 softmax A, 4-7 softmax B, 8 loads Q and K, 9 loads V, 10 issues the matrix instructions, 11 idle (it completes the
+// warpgroup whose registers go to the softmax warps).
+#include <cuda.h>
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
+#include <float.h>
 #include <limits.h>
 #include <math.h>
 #include <stdint.h>
 
 #include "kernels.h"
+// waits here are short and on the chain softmax -> MMA -> softmax: plain polling, as in attention_tc2.cu
+#define B2_MBAR_SUSPEND_NS 0
+#include "ptx.cuh"
 
 namespace b2 {
 
 static constexpr int AS_MAX_RADIUS = 1023;
 static constexpr int AS_MAX_GROUP = 128;
 static constexpr int64_t AS_ALIGN = 256;
+static constexpr int AS_MAX_CTAS = 160;
+static constexpr int AS_MAX_SLOTS = 2 * AS_MAX_CTAS;
+static constexpr int AS_THREADS = 384;
+static constexpr int AS_PLAN_THREADS = 1024;
+static constexpr int AS_KV = 128;                  // keys of a step
+static constexpr int AS_BLOCK = 128 * 64 * 2;      // 128 rows x 64 columns, 128-byte swizzle
+static constexpr int AS_PACKED_BOX = 32;           // rows of one copy of a packed key tile: short sequences copy few rows
+static constexpr int AS_TABLE = 2048;              // floats of a stream's staged bias tables
+static constexpr float AS_LOG2E = 1.4426950408889634f;
+static constexpr float AS_LAZY = 8.f;              // the softmax reference moves when the maximum passes it by 2^AS_LAZY
 
 struct AttnMod {
   float scale, cap;
@@ -25,103 +61,948 @@ struct AttnMod {
   const int32_t* docs;
 };
 
-struct AttnIo {
-  const __nv_bfloat16* q;
-  const __nv_bfloat16* k;
-  const __nv_bfloat16* v;
+// One query tile (PAIR: two neighbouring ones) of one sequence; the same for every key head.
+struct __align__(16) AttnEntry {
+  int32_t seq, tok0, n_tok, pos0;     // first row of q and out, tokens, position of the first
+  int32_t kv_len, kv_row0, prefix, n; // keys; packed: first row of k and v; visible prefix; key tiles visited
+  int32_t a0, n0, a1, pad;            // visited tiles: a0 .. a0 + n0 - 1, then a1 ..
+  int64_t before;                     // tiles of the entries in front (per key head)
+  int64_t pad2;
+};
+static_assert(sizeof(AttnEntry) == 64, "entry layout");
+
+struct AttnSlot {  // where a stream starts, and its steps
+  int32_t e, h, k, count;
+};
+
+struct AttnPlan {  // views into the workspace
+  int32_t* status;
+  int64_t* bound;        // [slots + 1] first step of each slot
+  AttnSlot* slot;        // [slots]
+  int32_t* counter;      // [2 * slots] finished parts of the item that starts in a slot (PAIR: per stream)
+  int32_t* seq_first;    // [n_seqs + 1] first entry of a sequence
+  int2* doc_range;       // [n_tokens / 128 + n_seqs + 1] smallest and largest document of a key tile
+  AttnEntry* entry;
+  float2* part_ml;       // [2 * slots * streams][rows] maximum (log2 units) and denominator
+  float* part_o;         // [...][rows][Dp]
+  int32_t max_entries, rows;
+};
+
+struct AttnJob {
   __nv_bfloat16* out;
-  int64_t q_stride, k_stride, v_stride, out_stride;
+  int64_t out_stride;
   const int32_t* cu;
   const int32_t* kv_lens;
   const int32_t* page_table;
-  int64_t page_stride, token_stride, head_stride;
-  int n_seqs, n_tokens, n_heads, n_kv_heads, head_dim;
-  int n_pages, page_size, table_stride;
+  int n_seqs, n_tokens, n_heads, n_kv_heads, head_dim, group, tile_tokens;
+  int n_pages, page_size, table_stride, box_rows, head_first;
 };
 
-__device__ __forceinline__ void load4(const __nv_bfloat16* p, float (&x)[4]) {
-  const uint2 u = *reinterpret_cast<const uint2*>(p);
-  const float2 a = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&u.x));
-  const float2 b = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&u.y));
-  x[0] = a.x;
-  x[1] = a.y;
-  x[2] = b.x;
-  x[3] = b.y;
+__device__ __forceinline__ float as_ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ float as_rcp(float x) {
+  float y;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ float as_max3(float a, float b, float c) {
+  float d;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
+// 32-bit mask of the x lowest bits, x clamped to 0 .. 32
+__device__ __forceinline__ uint32_t as_below(int x) {
+  uint32_t m;
+  asm("bmsk.clamp.b32 %0, 0, %1;" : "=r"(m) : "r"(max(x, 0)));
+  return m;
 }
 
-template <bool PAGED>
-__global__ void __launch_bounds__(256) attn_rows_kernel(const AttnIo io, const AttnMod mod, int* __restrict__ status) {
-  if (blockIdx.x == 0 && threadIdx.x == 0) *status = 0;
-  const int64_t row = static_cast<int64_t>(blockIdx.x) * 8 + (threadIdx.x >> 5);
-  const int lane = threadIdx.x & 31;
-  if (row >= static_cast<int64_t>(io.n_tokens) * io.n_heads) return;
-  const int t = static_cast<int>(row / io.n_heads), h = static_cast<int>(row % io.n_heads);
-  const int hk = h / (io.n_heads / io.n_kv_heads);
-  int lo = 0, hi = io.n_seqs;
-  while (hi - lo > 1) {
-    const int mid = (lo + hi) >> 1;
-    if (io.cu[mid] <= t) lo = mid;
-    else hi = mid;
+// ---- planning -------------------------------------------------------------------------
+
+// Tokens of sequence s, cut to the buffer.
+__device__ __forceinline__ int2 as_rows_of(const AttnJob& j, int s) {
+  const int first = min(max(j.cu[s], 0), j.n_tokens);
+  return make_int2(first, min(max(j.cu[s + 1], first), j.n_tokens));
+}
+
+// Exclusive sum over the block of v, plus *carry, which then grows by the block's total.
+__device__ int64_t as_block_sum(int64_t v, int64_t* carry, int64_t* scratch) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  int64_t x = v;
+#pragma unroll
+  for (int d = 1; d < 32; d <<= 1) {
+    const int64_t y = __shfl_up_sync(0xffffffffu, x, d);
+    if (lane >= d) x += y;
   }
-  const int first = max(io.cu[lo], 0), end = min(io.cu[lo + 1], io.n_tokens);
-  if (t < first || t >= end) return;
-  int kv_len = end - first;
-  if (PAGED) kv_len = min(max(io.kv_lens[lo], 0), io.table_stride * io.page_size);
-  const int pos = kv_len - (end - first) + (t - first);
-  const int prefix = mod.prefix != nullptr ? mod.prefix[lo] : 0;
-  const int doc = mod.docs != nullptr ? mod.docs[t] : 0;
-  const bool on = lane * 4 < io.head_dim;
-  float q[4] = {}, o[4] = {}, k[4] = {}, v[4] = {};
-  if (on) load4(io.q + t * io.q_stride + static_cast<int64_t>(h) * io.head_dim + lane * 4, q);
-  float m = -INFINITY, l = 0.f;
-  for (int j = 0; j < kv_len; ++j) {
-    const int d = j - pos;
-    bool seen = (d <= mod.right && d >= -mod.left) || j < prefix;
-    if (mod.docs != nullptr) seen = seen && doc >= 0 && mod.docs[first + j] == doc;
-    if (!seen) continue;
-    const __nv_bfloat16* kp = nullptr;
-    const __nv_bfloat16* vp = nullptr;
-    if (PAGED) {
-      const int page = io.page_table[static_cast<int64_t>(lo) * io.table_stride + j / io.page_size];
-      if (page >= 0 && page < io.n_pages) {
-        const int64_t at = page * io.page_stride + (j % io.page_size) * io.token_stride + hk * io.head_stride;
-        kp = io.k + at;
-        vp = io.v + at;
+  if (lane == 31) scratch[warp] = x;
+  __syncthreads();
+  if (warp == 0) {
+    int64_t w = scratch[lane];
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+      const int64_t y = __shfl_up_sync(0xffffffffu, w, d);
+      if (lane >= d) w += y;
+    }
+    scratch[lane] = w;
+  }
+  __syncthreads();
+  const int64_t base = *carry + (warp ? scratch[warp - 1] : 0);
+  const int64_t total = scratch[31];
+  __syncthreads();
+  if (threadIdx.x == 0) *carry += total;
+  __syncthreads();
+  return base + x - v;
+}
+
+// First key tile record of sequence s: (first token / 128) + s never runs into the next sequence's.
+__device__ __forceinline__ int as_doc_base(int first, int s) { return first / AS_KV + s; }
+
+__global__ void __launch_bounds__(AS_PLAN_THREADS, 1)
+attn_plan_kernel(const AttnJob j, const AttnMod mod, const AttnPlan p, int tokens_per_entry, int max_slots) {
+  __shared__ int64_t scratch[32];
+  __shared__ int64_t carry;
+  pdl_launch_dependents();
+  pdl_wait();
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  if (tid == 0) {
+    *p.status = 0;
+    carry = 0;
+  }
+  for (int i = tid; i < 2 * max_slots; i += AS_PLAN_THREADS) p.counter[i] = 0;
+  for (int i = tid; i < max_slots; i += AS_PLAN_THREADS) p.slot[i] = AttnSlot{0, 0, 0, 0};
+  __syncthreads();
+  // entries of each sequence
+  for (int base = 0; base < j.n_seqs; base += AS_PLAN_THREADS) {
+    const int s = base + tid;
+    int count = 0;
+    if (s < j.n_seqs) {
+      const int2 r = as_rows_of(j, s);
+      count = (r.y - r.x + tokens_per_entry - 1) / tokens_per_entry;
+    }
+    const int64_t at = as_block_sum(count, &carry, scratch);
+    if (s < j.n_seqs) p.seq_first[s] = static_cast<int>(min(at, static_cast<int64_t>(p.max_entries)));
+  }
+  const int n_entries = static_cast<int>(min(carry, static_cast<int64_t>(p.max_entries)));
+  if (tid == 0) p.seq_first[j.n_seqs] = n_entries;
+  __syncthreads();
+  if (mod.docs != nullptr) {
+    // documents of every 128-token tile (tokens of no document left out)
+    const int records = j.n_tokens / AS_KV + j.n_seqs;
+    for (int i = warp; i < records; i += AS_PLAN_THREADS / 32) {
+      int lo = 0, hi = j.n_seqs;
+      while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        if (as_doc_base(as_rows_of(j, mid).x, mid) <= i) lo = mid;
+        else hi = mid;
       }
-    } else {
-      kp = io.k + (first + j) * io.k_stride + static_cast<int64_t>(hk) * io.head_dim;
-      vp = io.v + (first + j) * io.v_stride + static_cast<int64_t>(hk) * io.head_dim;
+      const int2 r = as_rows_of(j, lo);
+      const int t0 = r.x + (i - as_doc_base(r.x, lo)) * AS_KV;
+      if (t0 < r.x) continue;  // only where cu_seqlens is not sorted
+      int dmin = INT_MAX, dmax = -1;
+      for (int t = t0 + lane; t < min(t0 + AS_KV, r.y); t += 32) {
+        const int d = mod.docs[t];
+        if (d >= 0) {
+          dmin = min(dmin, d);
+          dmax = max(dmax, d);
+        }
+      }
+      dmin = __reduce_min_sync(0xffffffffu, dmin);
+      dmax = __reduce_max_sync(0xffffffffu, dmax);
+      if (lane == 0 && t0 < r.y) p.doc_range[i] = make_int2(dmin, dmax);
     }
-    if (on && kp != nullptr) {
-      load4(kp + lane * 4, k);
-      load4(vp + lane * 4, v);
-    } else {
-#pragma unroll
-      for (int e = 0; e < 4; ++e) k[e] = v[e] = 0.f;
-    }
-    float s = q[0] * k[0] + q[1] * k[1] + q[2] * k[2] + q[3] * k[3];
-#pragma unroll
-    for (int x = 16; x > 0; x >>= 1) s += __shfl_xor_sync(0xffffffffu, s, x);
-    s *= mod.scale;
-    if (mod.cap > 0.f) s = mod.cap * tanhf(s / mod.cap);
-    if (mod.slopes != nullptr) s -= mod.slopes[h] * fabsf(static_cast<float>(d));
-    if (mod.bias != nullptr)
-      s += mod.bias[static_cast<int64_t>(h) * (2 * mod.radius + 1) + min(max(d, -mod.radius), mod.radius) + mod.radius];
-    const float m_new = fmaxf(m, s);
-    if (m_new == -INFINITY && s == s) continue;  // nothing seen yet (a NaN score goes on and makes the row NaN)
-    const float keep = expf(m - m_new), p = expf(s - m_new);
-    l = l * keep + p;
-#pragma unroll
-    for (int e = 0; e < 4; ++e) o[e] = o[e] * keep + p * v[e];
-    m = m_new;
+    __syncthreads();
   }
-  if (on) {
-    const float inv = m == -INFINITY ? 0.f : 1.f / l;
-    __nv_bfloat162 a = __floats2bfloat162_rn(o[0] * inv, o[1] * inv), b = __floats2bfloat162_rn(o[2] * inv, o[3] * inv);
-    uint2 u;
-    u.x = *reinterpret_cast<uint32_t*>(&a);
-    u.y = *reinterpret_cast<uint32_t*>(&b);
-    *reinterpret_cast<uint2*>(io.out + t * io.out_stride + static_cast<int64_t>(h) * io.head_dim + lane * 4) = u;
+  if (tid == 0) carry = 0;
+  __syncthreads();
+  for (int base = 0; base < n_entries; base += AS_PLAN_THREADS) {
+    const int e = base + tid;
+    AttnEntry x = {};
+    int doc_lo = 0, doc_hi = INT_MAX;
+    if (e < n_entries) {
+      int lo = 0, hi = j.n_seqs;  // the last sequence whose first entry is <= e: empty ones in front share it
+      while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        if (p.seq_first[mid] <= e) lo = mid;
+        else hi = mid;
+      }
+      const int2 r = as_rows_of(j, lo);
+      const int q0 = (e - p.seq_first[lo]) * tokens_per_entry;
+      x.seq = lo;
+      x.tok0 = r.x + q0;
+      x.n_tok = min(tokens_per_entry, r.y - r.x - q0);
+      x.kv_row0 = r.x;
+      x.kv_len = j.kv_lens == nullptr ? r.y - r.x : min(max(j.kv_lens[lo], 0), j.table_stride * j.page_size);
+      x.pos0 = x.kv_len - (r.y - r.x) + q0;
+      x.prefix = mod.prefix == nullptr ? 0 : min(max(mod.prefix[lo], 0), x.kv_len);
+    }
+    if (mod.docs != nullptr) {  // a warp takes its 32 entries in turn, its lanes look at 32 key tiles at a time
+      for (int who = 0; who < 32; ++who) {
+        const int n_tok = __shfl_sync(0xffffffffu, x.n_tok, who);
+        if (n_tok <= 0) continue;
+        const int seq = __shfl_sync(0xffffffffu, x.seq, who), row0 = __shfl_sync(0xffffffffu, x.kv_row0, who);
+        const int tok0 = __shfl_sync(0xffffffffu, x.tok0, who), tiles = (__shfl_sync(0xffffffffu, x.kv_len, who) + AS_KV - 1) / AS_KV;
+        const int2* range = p.doc_range + as_doc_base(row0, seq);
+        int dmin = INT_MAX, dmax = -1;
+        for (int t = (tok0 - row0) / AS_KV + lane; t <= (tok0 - row0 + n_tok - 1) / AS_KV; t += 32) {
+          dmin = min(dmin, range[t].x);
+          dmax = max(dmax, range[t].y);
+        }
+        dmin = __reduce_min_sync(0xffffffffu, dmin);
+        dmax = __reduce_max_sync(0xffffffffu, dmax);
+        int first = INT_MAX, last = -1;
+        for (int t0 = 0; t0 < tiles; t0 += 32) {
+          bool meets = false;
+          if (t0 + lane < tiles) {
+            const int2 d = range[t0 + lane];
+            meets = d.x <= dmax && d.y >= dmin;
+          }
+          const uint32_t m = __ballot_sync(0xffffffffu, meets);
+          if (m) {
+            first = min(first, t0 + __ffs(m) - 1);
+            last = t0 + 31 - __clz(m);
+          }
+        }
+        if (lane == who) {
+          doc_lo = last < 0 ? 0 : first;
+          doc_hi = last + 1;
+        }
+      }
+    }
+    if (e < n_entries) {
+      // keys that the window of some token reaches, then the tiles of the prefix in front of them
+      const int p1 = x.pos0 + x.n_tok - 1;
+      const int key_lo = static_cast<int>(max(static_cast<int64_t>(x.pos0) - mod.left, int64_t(0)));
+      const int key_hi = static_cast<int>(min(static_cast<int64_t>(p1) + mod.right + 1, static_cast<int64_t>(x.kv_len)));
+      int b0 = 0, b1 = 0, f1 = min((x.prefix + AS_KV - 1) / AS_KV, doc_hi);
+      if (key_hi > key_lo) {
+        b0 = max(key_lo / AS_KV, doc_lo);
+        b1 = max(min((key_hi + AS_KV - 1) / AS_KV, doc_hi), b0);
+      }
+      const int f0 = min(doc_lo, f1);
+      if (b1 == b0) b0 = b1 = f1;  // no window: the prefix alone
+      if (f1 >= b0) {              // the two runs meet
+        b0 = min(b0, f0);
+        b1 = max(b1, f1);
+        f1 = f0;
+      }
+      x.a0 = f0;
+      x.n0 = f1 - f0;
+      x.a1 = b0;
+      x.n = x.n0 + (b1 - b0);
+      if (x.n == 0) {  // nothing visible: one step whose keys are all masked writes the zeros
+        x.a0 = x.a1 = 0;
+        x.n0 = 0;
+        x.n = 1;
+      }
+    }
+    x.before = as_block_sum(x.n, &carry, scratch);
+    if (e < n_entries) p.entry[e] = x;
+  }
+  // Equal parts of all steps; a cut moves to an item's edge that is nearer than 1/16 of a part.
+  const int64_t per_head = carry, total = per_head * j.n_kv_heads;
+  const int slots = static_cast<int>(min(total, static_cast<int64_t>(max_slots)));
+  __syncthreads();
+  if (slots == 0) return;
+  const int64_t slack = total / (16 * static_cast<int64_t>(slots));
+  for (int s = tid; s <= slots; s += AS_PLAN_THREADS) {
+    int64_t at = total / slots * s + total % slots * s / slots;
+    if (s < slots) {
+      int lo = 0, hi = n_entries;
+      while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        if (p.entry[mid].before * j.n_kv_heads <= at) lo = mid;
+        else hi = mid;
+      }
+      const int n = p.entry[lo].n;
+      const int64_t in = at - p.entry[lo].before * j.n_kv_heads;
+      int h = static_cast<int>(in / n), k = static_cast<int>(in % n), e = lo;
+      if (k > 0 && k <= slack && k <= n - k) {
+        at -= k;
+        k = 0;
+      } else if (k > 0 && n - k <= slack) {
+        at += n - k;
+        k = 0;
+        if (++h == j.n_kv_heads) {
+          h = 0;
+          ++e;
+        }
+      }
+      p.slot[s] = AttnSlot{e, h, k, 0};
+    }
+    p.bound[s] = at;
+  }
+  __syncthreads();
+  for (int s = tid; s < slots; s += AS_PLAN_THREADS) p.slot[s].count = static_cast<int>(p.bound[s + 1] - p.bound[s]);
+}
+
+// ---- the attention kernel -----------------------------------------------------------------
+
+template <int D>
+struct AsCfg {
+  static constexpr int BLOCKS = D / 64;
+  static constexpr int TILE = BLOCKS * AS_BLOCK;
+  static constexpr int RING = D == 64 ? 4 : 2;  // key (and value) tiles in flight
+  static constexpr int STAGE_BYTES = 8 * 16 * 128;
+  static constexpr int TABLE_BYTES = 2 * AS_TABLE * 4;
+  static constexpr int BAR_BYTES = 256;
+  static constexpr int SMEM_BYTES = (2 + 2 * RING) * TILE + STAGE_BYTES + TABLE_BYTES + BAR_BYTES + 1024;
+  static constexpr int N_BARS = 4 * RING + 2 * 7;
+  static_assert(N_BARS * 8 + 16 <= BAR_BYTES, "barrier area");
+  static_assert(SMEM_BYTES <= 232448, "shared memory");
+  // Tensor memory columns of stream t. With head_dim 64 P has columns of its own, so the next S may be written as soon as this
+  // one has been read; with 128 P takes the place of S and the next S follows the P V that reads it.
+  static constexpr bool P_APART = D == 64;
+  static __host__ __device__ constexpr uint32_t S(int t) { return t * 128; }
+  static __host__ __device__ constexpr uint32_t O(int t) { return 256 + t * D; }
+  static __host__ __device__ constexpr uint32_t P(int t) { return P_APART ? 384 + t * 64 : t * 128; }
+};
+static constexpr uint32_t AS_TMEM_COLS = 512;
+// Registers: 384 threads are launched with 168 each; the loading and issuing warpgroup gives its share to the two softmax ones.
+static constexpr int AS_REGS_LAUNCH = 168, AS_REGS_SOFTMAX = 208, AS_REGS_OTHER = 88;
+static_assert(2 * AS_REGS_SOFTMAX + AS_REGS_OTHER == 3 * AS_REGS_LAUNCH, "register split");
+
+// The steps of a stream, in order. Every role of the stream walks the same ones.
+struct AsWalk {
+  int left, e, h, k;  // steps left (this one included); entry, key head, key tile of the item
+  bool first;         // first step of a segment (an item, or this stream's part of one)
+  int4 f0, f1, f2;    // the entry
+  __device__ void load(const AttnEntry* entry) {
+    const int4* p = reinterpret_cast<const int4*>(entry + e);
+    f0 = p[0];
+    f1 = p[1];
+    f2 = p[2];
+  }
+  __device__ void start(const AttnPlan& p, int slot) {
+    const int4 s = *reinterpret_cast<const int4*>(p.slot + slot);
+    e = s.x;
+    h = s.y;
+    k = s.z;
+    left = s.w;
+    first = true;
+    if (left > 0) load(p.entry);
+  }
+  __device__ bool last() const { return left == 1 || k == f1.w - 1; }
+  __device__ int key0() const { return (k < f2.y ? f2.x + k : f2.z + k - f2.y) * AS_KV; }
+  __device__ int n_valid() const { return min(max(f1.x - key0(), 0), AS_KV); }
+  __device__ void next(const AttnPlan& p, int n_kv_heads) {
+    first = false;
+    if (++k == f1.w) {
+      k = 0;
+      first = true;
+      if (++h == n_kv_heads) {
+        h = 0;
+        ++e;
+        if (left > 1) load(p.entry);
+      }
+    }
+    --left;
+  }
+};
+
+__device__ __forceinline__ int as_round16(int n) { return max((n + 15) & ~15, 16); }
+
+__device__ __forceinline__ void as_tma_3d(void* dst, const void* tmap, uint64_t* bar, int x, int y, int z) {
+  asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];" ::"r"(
+                   smem_u32(dst)),
+               "l"(reinterpret_cast<uint64_t>(tmap)), "r"(smem_u32(bar)), "r"(x), "r"(y), "r"(z)
+               : "memory");
+}
+__device__ __forceinline__ void as_tma_4d(void* dst, const void* tmap, uint64_t* bar, int x, int y, int z, int w) {
+  asm volatile("cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6}], [%2];" ::"r"(
+                   smem_u32(dst)),
+               "l"(reinterpret_cast<uint64_t>(tmap)), "r"(smem_u32(bar)), "r"(x), "r"(y), "r"(z), "r"(w)
+               : "memory");
+}
+
+// After a failed wait: lets the copies still in flight land before shared memory is released (bounded).
+__device__ __forceinline__ void as_drain(uint64_t* full, uint32_t fills, uint32_t slots) {
+  for (uint32_t i = 0; i < (fills < slots ? fills : slots); ++i) {
+    const uint32_t idx = fills - 1 - i;
+    mbar_wait(&full[idx % slots], (idx / slots) & 1u);
+  }
+}
+
+// Copies the valid rows of a step's key (or value) tile: lane l takes rows (l % 16) * box_rows .. of the 64-column block l / 16.
+template <int D, bool PAGED>
+__device__ __forceinline__ void as_load_tile(const AttnJob& j, const AsWalk& w, const CUtensorMap* tmap, uint8_t* dst, uint64_t* full, int lane) {
+  const int n_valid = w.n_valid();
+  const int boxes = (n_valid + j.box_rows - 1) / j.box_rows;
+  const int r = lane & 15, cb = lane >> 4;
+  const bool mine = r < boxes && cb < AsCfg<D>::BLOCKS;
+  int page = 0, off = 0;
+  const int key = w.key0() + r * j.box_rows;
+  if (PAGED && mine) {
+    const int at = key / j.page_size;
+    off = key - at * j.page_size;
+    page = __ldg(j.page_table + static_cast<int64_t>(w.f0.x) * j.table_stride + at);
+    if (page < 0 || page >= j.n_pages) page = j.n_pages;  // outside the tensor: zeros
+  }
+  if (lane == 0) mbar_arrive_expect_tx(full, boxes * j.box_rows * 128 * AsCfg<D>::BLOCKS);
+  __syncwarp();
+  if (mine) {
+    uint8_t* to = dst + cb * AS_BLOCK + r * j.box_rows * 128;
+    if (PAGED) {
+      if (j.head_first) as_tma_4d(to, tmap, full, cb * 64, w.h, off, page);
+      else as_tma_4d(to, tmap, full, cb * 64, off, w.h, page);
+    } else {
+      as_tma_3d(to, tmap, full, cb * 64, w.h, w.f1.y + key);
+    }
+  }
+}
+
+template <int D, bool PAGED, bool PAIR>
+__global__ void __launch_bounds__(AS_THREADS, 1)
+attn_scored_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constant__ CUtensorMap tmap_k,
+                   const __grid_constant__ CUtensorMap tmap_v, const __grid_constant__ AttnJob j, const __grid_constant__ AttnMod mod,
+                   const __grid_constant__ AttnPlan plan) {
+  using Cfg = AsCfg<D>;
+  constexpr int RING = Cfg::RING;
+  extern __shared__ uint8_t as_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(as_raw) + 1023) & ~uintptr_t(1023));
+  uint8_t* q_s = smem;
+  uint8_t* k_s = q_s + 2 * Cfg::TILE;
+  uint8_t* v_s = k_s + RING * Cfg::TILE;
+  uint8_t* stage_s = v_s + RING * Cfg::TILE;
+  float* table_s = reinterpret_cast<float*>(stage_s + Cfg::STAGE_BYTES);
+  uint64_t* k_full = reinterpret_cast<uint64_t*>(stage_s + Cfg::STAGE_BYTES + Cfg::TABLE_BYTES);
+  uint64_t* k_empty = k_full + RING;
+  uint64_t* v_full = k_empty + RING;
+  uint64_t* v_empty = v_full + RING;
+  uint64_t* q_full = v_empty + RING;  // the following ones per stream
+  uint64_t* q_empty = q_full + 2;
+  uint64_t* s_full = q_empty + 2;     // S of a step is in tensor memory
+  uint64_t* s_read = s_full + 2;      // P_APART: the softmax warps hold it in registers
+  uint64_t* p_full = s_read + 2;      // P of a step is in tensor memory, O may be added to
+  uint64_t* pv_done = p_full + 2;     // P V of a step has finished
+  uint64_t* group_bar = pv_done + 2;  // the four softmax warps of a stream meet
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(group_bar + 2);
+  uint32_t* joins = tmem_slot + 1;    // per stream: this warpgroup joins the parts of the item
+
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0);
+  const int lane = threadIdx.x & 31;
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < RING; ++i) {
+      mbar_init(&k_full[i], 1);
+      mbar_init(&k_empty[i], 1);
+      mbar_init(&v_full[i], 1);
+      mbar_init(&v_empty[i], 1);
+    }
+    for (int t = 0; t < 2; ++t) {
+      mbar_init(&q_full[t], 1);
+      mbar_init(&q_empty[t], 1);
+      mbar_init(&s_full[t], 1);
+      mbar_init(&s_read[t], 4);
+      mbar_init(&p_full[t], 4);
+      mbar_init(&pv_done[t], 1);
+      mbar_init(&group_bar[t], 4);
+    }
+    fence_mbar_init();
+  }
+  if (warp == 8) {
+    tmem_alloc(tmem_slot, AS_TMEM_COLS);
+    tmem_relinquish();
+  }
+  tc_fence_before_sync();
+  __syncthreads();
+  tc_fence_after_sync();
+  const uint32_t tmem_base = *tmem_slot;
+  pdl_wait();  // the plan, and whatever wrote q, k and v
+
+  if (warp >= 8) {
+    setmaxnreg_dec<AS_REGS_OTHER>();
+    if (warp == 8 || warp == 9) {
+      // ---------------- loads: warp 8 Q and K, warp 9 V ----------------
+      const bool is_k = warp == 8;
+      const CUtensorMap* tmap = is_k ? &tmap_k : &tmap_v;
+      uint8_t* ring = is_k ? k_s : v_s;
+      uint64_t* full = is_k ? k_full : v_full;
+      uint64_t* empty = is_k ? k_empty : v_empty;
+      if (lane == 0) {
+        tma_prefetch_desc(tmap);
+        if (is_k) tma_prefetch_desc(&tmap_q);
+      }
+      AsWalk w[2];
+      w[0].start(plan, blockIdx.x);
+      if (PAIR) w[1].left = 0;
+      else w[1].start(plan, blockIdx.x + gridDim.x);
+      int slot = 0;
+      uint32_t phase = 0, fills = 0, q_fills[2] = {0, 0};
+      bool ok = true;
+      while (ok && (w[0].left > 0 || w[1].left > 0)) {
+#pragma unroll
+        for (int t = 0; t < (PAIR ? 1 : 2); ++t) {
+          if (!ok || w[t].left <= 0) continue;
+          if (is_k && w[t].first) {
+#pragma unroll
+            for (int u = t; u < (PAIR ? 2 : t + 1); ++u) {
+              if (ok) ok = __all_sync(0xffffffffu, mbar_wait(&q_empty[u], (q_fills[u] & 1u) ^ 1u));
+              if (ok && lane == 0) {
+                mbar_arrive_expect_tx(&q_full[u], j.group * j.tile_tokens * 128 * Cfg::BLOCKS);
+#pragma unroll
+                for (int b = 0; b < Cfg::BLOCKS; ++b)
+                  as_tma_3d(q_s + u * Cfg::TILE + b * AS_BLOCK, &tmap_q, &q_full[u], b * 64, w[t].h * j.group,
+                            w[t].f0.y + (PAIR ? u * j.tile_tokens : 0));
+              }
+              if (ok) ++q_fills[u];
+            }
+          }
+          if (ok) ok = __all_sync(0xffffffffu, mbar_wait(&empty[slot], phase ^ 1u));
+          if (!ok) break;
+          as_load_tile<D, PAGED>(j, w[t], tmap, ring + slot * Cfg::TILE, &full[slot], lane);
+          ++fills;
+          if (++slot == RING) {
+            slot = 0;
+            phase ^= 1u;
+          }
+          w[t].next(plan, j.n_kv_heads);
+        }
+      }
+      if (is_k) pdl_launch_dependents();
+      if (!ok) {
+        if (lane == 0) atomicExch(plan.status, is_k ? 5 : 8);
+        as_drain(full, fills, RING);
+        if (is_k)
+          for (int u = 0; u < 2; ++u) as_drain(&q_full[u], q_fills[u], 1);
+      }
+    } else if (warp == 10) {
+      // ---------------- matrix instructions: all lanes walk, one elected lane issues ----------------
+      const uint32_t tmem_u = __shfl_sync(0xffffffffu, tmem_base, 0);
+      const uint32_t q_addr = smem_u32(q_s), k_addr = smem_u32(k_s), v_addr = smem_u32(v_s);
+      auto wait_all = [](uint64_t* bar, uint32_t parity) -> bool { return __all_sync(0xffffffffu, mbar_wait(bar, parity)); };
+      AsWalk sw[2], pw[2];  // the next S of each stream, and the next P V
+      sw[0].start(plan, blockIdx.x);
+      sw[1].start(plan, PAIR ? blockIdx.x : blockIdx.x + gridDim.x);
+      pw[0] = sw[0];
+      pw[1] = sw[1];
+      uint32_t q_uses[2] = {0, 0}, n_s[2] = {0, 0}, n_pv[2] = {0, 0};
+      int kslot = 0, vslot = 0;
+      uint32_t kphase = 0, vphase = 0;
+      bool ok = true;
+      // In a pair both streams use the tile of a ring slot, B last; B may have no tokens (the item ends in A's tile).
+      auto has_rows = [&](const AsWalk& w, int t) { return !PAIR || t == 0 || w.f0.z > j.tile_tokens; };
+      auto issue_s = [&](int t) -> bool {
+        AsWalk& w = sw[t];
+        if (w.left <= 0) return true;
+        if (w.first && !wait_all(&q_full[t], q_uses[t]++ & 1u)) return false;
+        if (!wait_all(&k_full[kslot], kphase)) return false;
+        tc_fence_after_sync();
+        const uint32_t idesc = make_idesc_bf16_f32(128, as_round16(w.n_valid()));
+        if (has_rows(w, t)) {
+#pragma unroll
+          for (int k = 0; k < D / 16; ++k) {
+            const uint64_t a = make_kmajor_sw128_desc(q_addr + t * Cfg::TILE + (k / 4) * AS_BLOCK) + 2 * (k % 4);
+            const uint64_t b = make_kmajor_sw128_desc(k_addr + kslot * Cfg::TILE + (k / 4) * AS_BLOCK) + 2 * (k % 4);
+            if (elect_one()) tc_mma_f16(tmem_u + Cfg::S(t), a, b, idesc, k != 0);
+          }
+        }
+        const bool done = !PAIR || t == 1;
+        if (elect_one()) {
+          tc_commit(&s_full[t]);
+          if (done) tc_commit(&k_empty[kslot]);
+          if (w.last()) tc_commit(&q_empty[t]);
+        }
+        if (done && ++kslot == RING) {
+          kslot = 0;
+          kphase ^= 1u;
+        }
+        ++n_s[t];
+        w.next(plan, j.n_kv_heads);
+        return true;
+      };
+      const uint32_t idesc_pv = make_idesc_bf16_f32_b_mn(128, D);
+      auto issue_pv = [&](int t) -> bool {
+        AsWalk& w = pw[t];
+        if (!wait_all(&p_full[t], n_pv[t] & 1u) || !wait_all(&v_full[vslot], vphase)) return false;
+        tc_fence_after_sync();
+        const int n_valid = w.n_valid(), n_eff = as_round16(n_valid);
+        if (n_valid < n_eff && (!PAIR || t == 0)) {
+          // value rows behind the last key: whatever lies there must not meet a zero probability (0 * NaN)
+          uint8_t* tile = v_s + vslot * Cfg::TILE;
+          for (int i = lane; i < (n_eff - n_valid) * 8 * Cfg::BLOCKS; i += 32) {
+            const int b = i / ((n_eff - n_valid) * 8), at = i - b * ((n_eff - n_valid) * 8);
+            *reinterpret_cast<uint4*>(tile + b * AS_BLOCK + n_valid * 128 + at * 16) = make_uint4(0, 0, 0, 0);
+          }
+          fence_proxy_async_smem();
+          __syncwarp();
+        }
+        if (has_rows(w, t)) {
+          const uint64_t v_desc = make_mnmajor_sw128_desc(v_addr + vslot * Cfg::TILE, AS_BLOCK);
+#pragma unroll
+          for (int k = 0; k < AS_KV / 16; ++k)
+            if (k * 16 < n_eff && elect_one())
+              tc_mma_f16_tmem_a(tmem_u + Cfg::O(t), tmem_u + Cfg::P(t) + k * 8, v_desc + k * 128, idesc_pv, !w.first || k != 0);
+        }
+        const bool done = !PAIR || t == 1;
+        if (elect_one()) {
+          tc_commit(&pv_done[t]);
+          if (done) tc_commit(&v_empty[vslot]);
+        }
+        if (done && ++vslot == RING) {
+          vslot = 0;
+          vphase ^= 1u;
+        }
+        ++n_pv[t];
+        w.next(plan, j.n_kv_heads);
+        return true;
+      };
+      ok = issue_s(0) && issue_s(1);
+      while (ok && (pw[0].left > 0 || pw[1].left > 0)) {
+        if (Cfg::P_APART) {
+#pragma unroll
+          for (int t = 0; t < 2; ++t)
+            if (ok && sw[t].left > 0) ok = wait_all(&s_read[t], (n_s[t] - 1) & 1u) && issue_s(t);
+#pragma unroll
+          for (int t = 0; t < 2; ++t)
+            if (ok && pw[t].left > 0) ok = issue_pv(t);
+        } else {
+#pragma unroll
+          for (int t = 0; t < 2; ++t) {
+            if (!ok || pw[t].left <= 0) continue;
+            ok = issue_pv(t);
+            if (ok && sw[t].left > 0) ok = wait_all(&pv_done[t], (n_pv[t] - 1) & 1u) && issue_s(t);
+          }
+        }
+      }
+      if (!ok && lane == 0) atomicExch(plan.status, 7);
+    }
+  } else {
+    // ---------------- softmax: stream t, one row per thread ----------------
+    setmaxnreg_inc<AS_REGS_SOFTMAX>();
+    const int t = warp >> 2, wq = warp & 3, row = wq * 32 + lane;
+    const uint32_t lanes = tmem_base + (static_cast<uint32_t>(wq * 32) << 16);
+    uint8_t* stage = stage_s + warp * (16 * 128);
+    float* table = table_s + t * AS_TABLE;
+    const int group = j.group, g = row % group, row_tok = row / group;
+    const int my_slot = PAIR ? blockIdx.x : blockIdx.x + t * gridDim.x;
+    const int width = 2 * mod.radius + 1;
+    const bool staged = mod.bias != nullptr && group * width <= AS_TABLE;
+    const bool plain = mod.cap == 0.f && mod.slopes == nullptr && mod.bias == nullptr && mod.scale > 0.f;
+    // Scores are kept as the tensor core gives them where nothing but a positive scale follows (the scale is then part of the
+    // exponent's multiply-add), else in log2 units.
+    const float unit = plain ? mod.scale * AS_LOG2E : 1.f;
+    const float scale_log2 = mod.scale * AS_LOG2E;
+    const float cap_in = mod.cap > 0.f ? 2.f * scale_log2 / mod.cap : 0.f, cap_out = mod.cap * AS_LOG2E;
+    AsWalk w;
+    w.start(plan, my_slot);
+    uint32_t step = 0, meetings = 0;
+    bool failed = false;
+    // Bounded barrier of the stream's four softmax warps: one that gave up elsewhere makes the others give up here.
+    auto meet = [&]() {
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&group_bar[t]);
+      if (!mbar_wait(&group_bar[t], meetings++ & 1u)) failed = true;
+      failed = __any_sync(0xffffffffu, failed);
+    };
+    auto part_of = [&](int slot, bool tail) -> int64_t { return (2 * slot + (tail ? 1 : 0)) * (PAIR ? 2 : 1) + (PAIR ? t : 0); };
+    float slope = 0.f;
+    const float* tab = nullptr;
+    float tab_unit = 1.f;
+    while (w.left > 0 && !failed) {
+      // ---- one segment: an item, or this stream's part of one ----
+      const int h = w.h * group + g, k_first = w.k, seg_e = w.e, seg_h = w.h;
+      const int tok0 = w.f0.y + (PAIR ? t * j.tile_tokens : 0);
+      const int n_tok = min(max(w.f0.z - (PAIR ? t * j.tile_tokens : 0), 0), j.tile_tokens);
+      const int n_rows = n_tok * group;
+      const bool active = wq * 32 < n_rows;
+      const bool real = row < n_rows;
+      const int tok = min(tok0 + row_tok, j.n_tokens - 1);
+      const int pos = w.f0.w + (PAIR ? t * j.tile_tokens : 0) + row_tok;
+      const int kv_len = w.f1.x, kv_row0 = w.f1.y, prefix = w.f1.z, n_tiles = w.f1.w;
+      // first and past-the-last visible key of the window of this row
+      const int key_lo = mod.left >= pos ? 0 : pos - mod.left;
+      const int key_hi = mod.right >= kv_len - pos ? kv_len : pos + mod.right + 1;
+      const int doc = mod.docs != nullptr && real ? __ldg(mod.docs + tok) : -1;
+      if (mod.slopes != nullptr) slope = __ldg(mod.slopes + h) * AS_LOG2E;
+      if (mod.bias != nullptr) {
+        if (staged) {
+          meet();  // the previous item's reads are over
+          for (int i = row; i < group * width; i += 128) table[i] = __ldg(mod.bias + static_cast<int64_t>(w.h) * group * width + i) * AS_LOG2E;
+          meet();
+          if (failed) break;
+          tab = table + g * width + mod.radius;
+        } else {
+          tab = mod.bias + static_cast<int64_t>(h) * width + mod.radius;
+          tab_unit = AS_LOG2E;
+        }
+      }
+      float m_ref = -INFINITY, l_run = 0.f;
+      bool first = true, end = false;
+      while (!end) {
+        const int kv0 = w.key0(), n_valid = w.n_valid(), n_chunks = (as_round16(n_valid) + 31) >> 5;
+        end = w.last();
+        if (!mbar_wait(&s_full[t], step & 1u)) failed = true;
+        failed = __any_sync(0xffffffffu, failed);
+        if (failed) break;
+        tc_fence_after_sync();
+        if (active) {
+          uint32_t zr[4][32];  // the score row
+          float mx0 = -INFINITY, mx1 = -INFINITY;
+          tmem_ld_32x32b_x32(lanes + Cfg::S(t), zr[0]);
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            if (q < n_chunks) {
+              // the next 32 scores are on their way while these are worked on
+              tmem_ld_wait_for(zr[q]);
+              if (q < 3 && q + 1 < n_chunks) tmem_ld_32x32b_x32(lanes + Cfg::S(t) + q * 32 + 32, zr[q < 3 ? q + 1 : 3]);
+              const int key = kv0 + q * 32;
+              float y[32];
+#pragma unroll
+              for (int i = 0; i < 32; ++i) y[i] = __uint_as_float(zr[q][i]);
+              if (!plain) {
+                if (mod.cap > 0.f) {
+                  // cap tanh(s / cap) = cap (1 - 2 / (1 + e^(2 s / cap))), in log2 units
+#pragma unroll
+                  for (int i = 0; i < 32; ++i) y[i] = fmaf(-2.f * cap_out, as_rcp(1.f + as_ex2(y[i] * cap_in)), cap_out);
+                } else {
+#pragma unroll
+                  for (int i = 0; i < 32; ++i) y[i] *= scale_log2;
+                }
+                const int d0 = key - pos;
+                if (mod.slopes != nullptr) {
+                  const float f = static_cast<float>(d0);
+#pragma unroll
+                  for (int i = 0; i < 32; ++i) y[i] = fmaf(-slope, fabsf(f + static_cast<float>(i)), y[i]);
+                }
+                if (mod.bias != nullptr) {
+                  if (__all_sync(0xffffffffu, d0 + 31 <= -mod.radius || d0 >= mod.radius)) {
+                    const float b = tab[d0 < 0 ? -mod.radius : mod.radius] * tab_unit;
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) y[i] += b;
+                  } else {
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) y[i] = fmaf(tab[min(max(d0 + i, -mod.radius), mod.radius)], tab_unit, y[i]);
+                  }
+                }
+              }
+              uint32_t seen = (as_below(key_hi - key) & ~as_below(key_lo - key)) | as_below(prefix - key);
+              if (mod.docs != nullptr) {
+                // the keys of each document that some row of the warp belongs to
+                const int key_doc = key + lane < kv_len ? __ldg(mod.docs + kv_row0 + key + lane) : -1;
+                uint32_t same = 0, todo = __ballot_sync(0xffffffffu, doc >= 0);
+                while (todo) {
+                  const int d = __shfl_sync(0xffffffffu, doc, __ffs(todo) - 1);
+                  const uint32_t keys = __ballot_sync(0xffffffffu, key_doc == d);
+                  if (doc == d) same = keys;
+                  todo &= ~__ballot_sync(0xffffffffu, doc == d);
+                }
+                seen &= same;
+              }
+              if (!__all_sync(0xffffffffu, seen == 0xffffffffu)) {
+#pragma unroll
+                for (int i = 0; i < 32; ++i) y[i] = (seen >> i) & 1u ? y[i] : -INFINITY;
+              }
+#pragma unroll
+              for (int i = 0; i < 32; i += 4) {
+                mx0 = as_max3(mx0, y[i], y[i + 1]);
+                mx1 = as_max3(mx1, y[i + 2], y[i + 3]);
+              }
+#pragma unroll
+              for (int i = 0; i < 32; ++i) zr[q][i] = __float_as_uint(y[i]);
+            }
+          }
+          if (Cfg::P_APART) {
+            tc_fence_before_sync();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&s_read[t]);
+          }
+          const float mx = fmaxf(mx0, mx1);
+          // P of the previous step has been read, O is complete up to it
+          if (step > 0 && !mbar_wait(&pv_done[t], (step - 1) & 1u)) failed = true;
+          failed = __any_sync(0xffffffffu, failed);
+          if (failed) break;
+          tc_fence_after_sync();
+          const bool move = mx > m_ref && !((mx - m_ref) * unit <= AS_LAZY);  // also away from -inf
+          if (__any_sync(0xffffffffu, move)) {
+            const float m_new = move ? mx : m_ref;
+            const float alpha = move ? (m_ref == -INFINITY ? 0.f : as_ex2((m_ref - m_new) * unit)) : 1.f;
+            m_ref = m_new;
+            l_run *= alpha;
+            if (!first) {
+#pragma unroll 1
+              for (int c = 0; c < D; c += 16) {
+                uint32_t o[16];
+                tmem_ld_32x32b_x16(lanes + Cfg::O(t) + c, o);
+                tmem_ld_wait_for16(o);
+#pragma unroll
+                for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * alpha);
+                tmem_st_32x32b_x16(lanes + Cfg::O(t) + c, o);
+              }
+            }
+          }
+          const float base = m_ref == -INFINITY ? 0.f : -m_ref * unit;
+          const float2 unit2 = make_float2(unit, unit), base2 = make_float2(base, base);
+          float2 sum = make_float2(0.f, 0.f);
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            if (q < n_chunks) {
+              uint32_t pk[16];
+#pragma unroll
+              for (int i = 0; i < 32; i += 2) {
+                const float2 x = __ffma2_rn(make_float2(__uint_as_float(zr[q][i]), __uint_as_float(zr[q][i + 1])), unit2, base2);
+                const float2 pp = make_float2(as_ex2(x.x), as_ex2(x.y));
+                sum = __fadd2_rn(sum, pp);
+                __nv_bfloat162 b = __floats2bfloat162_rn(pp.x, pp.y);
+                pk[i >> 1] = *reinterpret_cast<uint32_t*>(&b);
+              }
+              tmem_st_32x32b_x16(lanes + Cfg::P(t) + q * 16, pk);
+            }
+          }
+          l_run += sum.x + sum.y;
+          tmem_st_wait();
+          tc_fence_before_sync();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&p_full[t]);
+        } else {
+          // nothing to compute: arrive in step with the warps that do
+          if (Cfg::P_APART && lane == 0) mbar_arrive(&s_read[t]);
+          if (step > 0 && !mbar_wait(&pv_done[t], (step - 1) & 1u)) failed = true;
+          failed = __any_sync(0xffffffffu, failed);
+          if (failed) break;
+          tc_fence_before_sync();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&p_full[t]);
+        }
+        first = false;
+        ++step;
+        w.next(plan, j.n_kv_heads);
+      }
+      if (failed) break;
+      // ---- the segment's rows ----
+      if (!mbar_wait(&pv_done[t], (step - 1) & 1u)) failed = true;
+      failed = __any_sync(0xffffffffu, failed);
+      if (failed) break;
+      tc_fence_after_sync();
+      const int done = (w.e == seg_e && w.h == seg_h) ? w.k : n_tiles;  // tiles of the item up to here
+      if (k_first == 0 && done == n_tiles) {
+        if (active) {
+          const float inv = l_run == 0.f ? 0.f : 1.f / l_run;
+#pragma unroll 1
+          for (int seg = 0; seg < Cfg::BLOCKS; ++seg) {
+#pragma unroll 1
+            for (int part = 0; part < 2; ++part) {
+              uint32_t ra[32];
+              tmem_ld_32x32b_x32(lanes + Cfg::O(t) + seg * 64 + part * 32, ra);
+              tmem_ld_wait_for(ra);
+              // 32 rows x 32 columns (64 bytes) per pass, 16-byte pieces swizzled by row
+#pragma unroll
+              for (int c = 0; c < 4; ++c) {
+                uint4 u;
+                __nv_bfloat162 p0 = __floats2bfloat162_rn(__uint_as_float(ra[8 * c]) * inv, __uint_as_float(ra[8 * c + 1]) * inv);
+                __nv_bfloat162 p1 = __floats2bfloat162_rn(__uint_as_float(ra[8 * c + 2]) * inv, __uint_as_float(ra[8 * c + 3]) * inv);
+                __nv_bfloat162 p2 = __floats2bfloat162_rn(__uint_as_float(ra[8 * c + 4]) * inv, __uint_as_float(ra[8 * c + 5]) * inv);
+                __nv_bfloat162 p3 = __floats2bfloat162_rn(__uint_as_float(ra[8 * c + 6]) * inv, __uint_as_float(ra[8 * c + 7]) * inv);
+                u.x = *reinterpret_cast<uint32_t*>(&p0);
+                u.y = *reinterpret_cast<uint32_t*>(&p1);
+                u.z = *reinterpret_cast<uint32_t*>(&p2);
+                u.w = *reinterpret_cast<uint32_t*>(&p3);
+                if (inv == 0.f) u = make_uint4(0, 0, 0, 0);  // no key seen (the accumulator may hold 0 * NaN)
+                *reinterpret_cast<uint4*>(stage + lane * 64 + ((c ^ ((lane >> 1) & 3)) << 4)) = u;
+              }
+              __syncwarp();
+#pragma unroll
+              for (int i = 0; i < 4; ++i) {
+                const int rl = i * 8 + (lane >> 2), cc = lane & 3, r = wq * 32 + rl;
+                const int col = seg * 64 + part * 32 + cc * 8;
+                if (r < n_rows && col < j.head_dim) {
+                  const uint4 u = *reinterpret_cast<const uint4*>(stage + rl * 64 + ((cc ^ ((rl >> 1) & 3)) << 4));
+                  const int tk = r / group;
+                  *reinterpret_cast<uint4*>(j.out + static_cast<int64_t>(tok0 + tk) * j.out_stride +
+                                            static_cast<int64_t>(seg_h * group + r - tk * group) * j.head_dim + col) = u;
+                }
+              }
+              __syncwarp();
+            }
+          }
+        }
+      } else {
+        // A part: numerators, maximum and denominator go to the workspace. Parts of an item: the one that starts it is the tail of
+        // its slot (odd index), the others are the head of theirs (even).
+        const int64_t id = part_of(my_slot, k_first == 0);
+        if (real) {
+          plan.part_ml[id * plan.rows + row] = make_float2(m_ref == -INFINITY ? -INFINITY : m_ref * unit, l_run);
+        }
+        if (active) {
+          float* dst = plan.part_o + (id * plan.rows + row) * D;
+#pragma unroll 1
+          for (int c = 0; c < D; c += 32) {
+            uint32_t ra[32];
+            tmem_ld_32x32b_x32(lanes + Cfg::O(t) + c, ra);
+            tmem_ld_wait_for(ra);
+            if (real) {
+#pragma unroll
+              for (int i = 0; i < 32; i += 4) *reinterpret_cast<uint4*>(dst + c + i) = make_uint4(ra[i], ra[i + 1], ra[i + 2], ra[i + 3]);
+            }
+          }
+        }
+        // the item's steps, and the slots they lie in
+        const int64_t before = plan.entry[seg_e].before;
+        const int64_t from = before * j.n_kv_heads + static_cast<int64_t>(seg_h) * n_tiles, to = from + n_tiles;
+        int s0 = my_slot, s1 = my_slot;
+        while (plan.bound[s0] > from) --s0;
+        while (plan.bound[s1 + 1] < to) ++s1;
+        __threadfence();
+        meet();
+        if (failed) break;
+        if (row == 0) {
+          const int old = atomicAdd(&plan.counter[2 * s0 + (PAIR ? t : 0)], 1);
+          joins[t] = old == s1 - s0;
+        }
+        meet();
+        if (failed) break;
+        const bool join = joins[t] != 0;
+        if (join) {
+          __threadfence();
+          const int pieces = j.head_dim >> 3;
+          for (int i = row; i < n_rows * pieces; i += 128) {
+            const int r = i / pieces, col = (i - r * pieces) * 8;
+            float top = -INFINITY, l = 0.f, o[8] = {};
+            for (int s = s0; s <= s1; ++s)
+              top = fmaxf(top, __ldcg(&plan.part_ml[part_of(s, s == s0) * plan.rows + r]).x);
+            for (int s = s0; s <= s1; ++s) {
+              const int64_t at = part_of(s, s == s0) * plan.rows + r;
+              const float2 ml = __ldcg(&plan.part_ml[at]);
+              const float f = ml.x == -INFINITY ? (ml.y == ml.y ? 0.f : ml.y) : as_ex2(ml.x - top);
+              const float4 x = __ldcg(reinterpret_cast<const float4*>(plan.part_o + at * D + col));
+              const float4 y = __ldcg(reinterpret_cast<const float4*>(plan.part_o + at * D + col + 4));
+              l = fmaf(f, ml.y, l);
+              o[0] = fmaf(f, x.x, o[0]);
+              o[1] = fmaf(f, x.y, o[1]);
+              o[2] = fmaf(f, x.z, o[2]);
+              o[3] = fmaf(f, x.w, o[3]);
+              o[4] = fmaf(f, y.x, o[4]);
+              o[5] = fmaf(f, y.y, o[5]);
+              o[6] = fmaf(f, y.z, o[6]);
+              o[7] = fmaf(f, y.w, o[7]);
+            }
+            const float inv = l == 0.f ? 0.f : 1.f / l;
+            uint4 u;
+            __nv_bfloat162 p0 = __floats2bfloat162_rn(o[0] * inv, o[1] * inv), p1 = __floats2bfloat162_rn(o[2] * inv, o[3] * inv);
+            __nv_bfloat162 p2 = __floats2bfloat162_rn(o[4] * inv, o[5] * inv), p3 = __floats2bfloat162_rn(o[6] * inv, o[7] * inv);
+            u.x = *reinterpret_cast<uint32_t*>(&p0);
+            u.y = *reinterpret_cast<uint32_t*>(&p1);
+            u.z = *reinterpret_cast<uint32_t*>(&p2);
+            u.w = *reinterpret_cast<uint32_t*>(&p3);
+            if (inv == 0.f) u = make_uint4(0, 0, 0, 0);
+            const int tk = r / group;
+            *reinterpret_cast<uint4*>(j.out + static_cast<int64_t>(tok0 + tk) * j.out_stride +
+                                      static_cast<int64_t>(seg_h * group + r - tk * group) * j.head_dim + col) = u;
+          }
+        }
+        meet();  // joins[t] may be written again
+      }
+      tc_fence_before_sync();  // O has been read: the next segment's first P V may overwrite it
+    }
+    if (failed && lane == 0) atomicExch(plan.status, 4);
+  }
+
+  tc_fence_before_sync();
+  __syncthreads();
+  if (warp == 8) {
+    tc_fence_after_sync();
+    tmem_dealloc(tmem_base, AS_TMEM_COLS);
   }
 }
 
@@ -184,14 +1065,121 @@ static int check_workspace(const void* ws, int64_t have, int64_t want, const cha
   return B200EMB_OK;
 }
 
-template <bool PAGED>
-static int launch_rows(const AttnIo& io, const AttnMod& mod, void* workspace, cudaStream_t s) {
-  const int64_t blocks = (static_cast<int64_t>(io.n_tokens) * io.n_heads + 7) / 8;
-  if (blocks > INT_MAX) return set_error(B200EMB_ERR_UNSUPPORTED, "attention: too many rows");
-  attn_rows_kernel<PAGED><<<static_cast<unsigned>(blocks), 256, 0, s>>>(io, mod, static_cast<int*>(workspace));
-  const cudaError_t e = cudaGetLastError();
+static int as_tile_tokens(int n_heads, int n_kv_heads) { return 128 / (n_heads / n_kv_heads); }
+
+// Carves the workspace (null: only measures it); returns its size.
+static int64_t as_layout(void* workspace, int n_seqs, int n_tokens, int n_heads, int n_kv_heads, int head_dim, AttnPlan* p) {
+  const int64_t seqs = n_seqs, tokens = n_tokens;
+  const int group = n_heads / n_kv_heads, tile = as_tile_tokens(n_heads, n_kv_heads);
+  const int64_t entries = tokens / tile + seqs + 1;
+  const int64_t rows = (tokens < tile ? (tokens > 0 ? tokens : 1) : tile) * group;
+  const int64_t parts = 2 * AS_MAX_SLOTS, dp = head_dim <= 64 ? 64 : 128;
+  int64_t at = 0;
+  auto take = [&](int64_t bytes) {
+    const int64_t mine = at;
+    at += (bytes + AS_ALIGN - 1) / AS_ALIGN * AS_ALIGN;
+    return static_cast<char*>(workspace) + mine;
+  };
+  AttnPlan q = {};
+  q.status = reinterpret_cast<int32_t*>(take(sizeof(int32_t)));
+  q.bound = reinterpret_cast<int64_t*>(take((AS_MAX_SLOTS + 1) * sizeof(int64_t)));
+  q.slot = reinterpret_cast<AttnSlot*>(take(AS_MAX_SLOTS * sizeof(AttnSlot)));
+  q.counter = reinterpret_cast<int32_t*>(take(2 * AS_MAX_SLOTS * sizeof(int32_t)));
+  q.seq_first = reinterpret_cast<int32_t*>(take((seqs + 1) * sizeof(int32_t)));
+  q.doc_range = reinterpret_cast<int2*>(take((tokens / AS_KV + seqs + 1) * sizeof(int2)));
+  q.entry = reinterpret_cast<AttnEntry*>(take(entries * sizeof(AttnEntry)));
+  q.part_ml = reinterpret_cast<float2*>(take(parts * rows * sizeof(float2)));
+  q.part_o = reinterpret_cast<float*>(take(parts * rows * dp * sizeof(float)));
+  q.max_entries = static_cast<int32_t>(entries < INT_MAX ? entries : INT_MAX);
+  q.rows = static_cast<int32_t>(rows);
+  if (p != nullptr) *p = q;
+  return at;
+}
+
+static int as_sm_count(int* out) {
+  int dev = 0;
+  B2_CUDA_CHECK(cudaGetDevice(&dev));
+  B2_CUDA_CHECK(cudaDeviceGetAttribute(out, cudaDevAttrMultiProcessorCount, dev));
+  return B200EMB_OK;
+}
+
+struct AsMaps {
+  CUtensorMap q, k, v;
+};
+
+// Two neighbouring tiles share their keys where sequences have two tiles of rows on average; shorter ones would leave stream B idle.
+static bool as_pair(const AttnJob& j) { return static_cast<int64_t>(j.n_tokens) * j.group >= 256ll * j.n_seqs; }
+
+template <int D, bool PAGED, bool PAIR>
+static int as_launch(const AsMaps& m, const AttnJob& j, const AttnMod& mod, const AttnPlan& plan, int sms, cudaStream_t s) {
+  int64_t grid = sms < AS_MAX_CTAS ? sms : AS_MAX_CTAS;
+  if (!PAGED) {  // no more CTAs than steps there can be
+    const int64_t steps = static_cast<int64_t>(plan.max_entries) * j.n_kv_heads * ((j.n_tokens + AS_KV - 1) / AS_KV);
+    if (steps < grid) grid = steps;
+  }
+  const int slots = static_cast<int>(PAIR ? grid : 2 * grid);
+  cudaError_t e = launch_pdl(attn_plan_kernel, dim3(1), dim3(AS_PLAN_THREADS), 0, s, j, mod, plan, (PAIR ? 2 : 1) * j.tile_tokens, slots);
+  if (e == cudaSuccess)
+    e = launch_pdl(attn_scored_kernel<D, PAGED, PAIR>, dim3(static_cast<unsigned>(grid)), dim3(AS_THREADS), AsCfg<D>::SMEM_BYTES, s, m.q, m.k,
+                   m.v, j, mod, plan);
   if (e != cudaSuccess) return set_error(B200EMB_ERR_CUDA, "attention launch: %s", cudaGetErrorString(e));
   return B200EMB_OK;
+}
+
+template <int D, bool PAGED, bool PAIR>
+static int as_init_one() {
+  cudaFuncAttributes a;
+  B2_CUDA_CHECK(cudaFuncGetAttributes(&a, attn_scored_kernel<D, PAGED, PAIR>));
+  // the register split of the kernel draws on exactly this many: with fewer its softmax warps would wait for good
+  if (a.numRegs != AS_REGS_LAUNCH)
+    return set_error(B200EMB_ERR_CUDA, "attention kernel built with %d registers instead of %d", a.numRegs, AS_REGS_LAUNCH);
+  B2_CUDA_CHECK(cudaFuncSetAttribute(attn_scored_kernel<D, PAGED, PAIR>, cudaFuncAttributeMaxDynamicSharedMemorySize, AsCfg<D>::SMEM_BYTES));
+  return B200EMB_OK;
+}
+
+int attention_scored_init_device() {
+  int rc = as_init_one<64, false, false>();
+  if (!rc) rc = as_init_one<64, false, true>();
+  if (!rc) rc = as_init_one<64, true, false>();
+  if (!rc) rc = as_init_one<64, true, true>();
+  if (!rc) rc = as_init_one<128, false, false>();
+  if (!rc) rc = as_init_one<128, false, true>();
+  if (!rc) rc = as_init_one<128, true, false>();
+  if (!rc) rc = as_init_one<128, true, true>();
+  return rc;
+}
+
+// rows of n heads: [tokens, heads, head_dim] with a row stride
+static int as_map_rows(CUtensorMap* m, const void* base, int n_tokens, int heads, int head_dim, int64_t stride, int box_heads, int box_tokens) {
+  const uint64_t dims[3] = {static_cast<uint64_t>(head_dim), static_cast<uint64_t>(heads), static_cast<uint64_t>(n_tokens)};
+  const uint64_t strides[2] = {static_cast<uint64_t>(head_dim) * 2, static_cast<uint64_t>(stride) * 2};
+  const uint32_t box[3] = {64, static_cast<uint32_t>(box_heads), static_cast<uint32_t>(box_tokens)};
+  return encode_tmap_bf16(m, base, 3, dims, strides, box);
+}
+
+static int as_map_pages(CUtensorMap* m, const void* base, const b200emb_kv_cache& c, bool head_first, int box_rows) {
+  // a dimension of one element may have any stride: give it one the encoder takes
+  const uint64_t ts = static_cast<uint64_t>(c.token_stride) * 2, hs = static_cast<uint64_t>(c.n_kv_heads > 1 ? c.head_stride : c.token_stride) * 2;
+  const uint64_t ps = c.n_pages > 1 ? static_cast<uint64_t>(c.page_stride) * 2 : ts * c.page_size;
+  const uint64_t heads = c.n_kv_heads, page = c.page_size;
+  const uint64_t dims[4] = {static_cast<uint64_t>(c.head_dim), head_first ? heads : page, head_first ? page : heads, static_cast<uint64_t>(c.n_pages)};
+  const uint64_t strides[3] = {head_first ? hs : ts, head_first ? ts : hs, ps};
+  const uint32_t rows = box_rows, box[4] = {64, head_first ? 1u : rows, head_first ? rows : 1u, 1};
+  return encode_tmap_bf16(m, base, 4, dims, strides, box);
+}
+
+template <bool PAGED>
+static int as_dispatch(const AsMaps& m, const AttnJob& j, const AttnMod& mod, void* workspace, cudaStream_t s) {
+  int rc = kernels_init_device();
+  int sms = 0;
+  if (!rc) rc = as_sm_count(&sms);
+  if (rc) return rc;
+  AttnPlan plan;
+  as_layout(workspace, j.n_seqs, j.n_tokens, j.n_heads, j.n_kv_heads, j.head_dim, &plan);
+  const bool pair = as_pair(j);
+  if (j.head_dim <= 64)
+    return pair ? as_launch<64, PAGED, true>(m, j, mod, plan, sms, s) : as_launch<64, PAGED, false>(m, j, mod, plan, sms, s);
+  return pair ? as_launch<128, PAGED, true>(m, j, mod, plan, sms, s) : as_launch<128, PAGED, false>(m, j, mod, plan, sms, s);
 }
 
 }  // namespace b2
@@ -201,7 +1189,7 @@ using namespace b2;
 extern "C" int64_t b200emb_attention_workspace_bytes(int32_t n_seqs, int32_t n_tokens, int32_t n_heads, int32_t n_kv_heads,
                                                      int32_t head_dim) {
   const int rc = check_shape(n_seqs, n_tokens, n_heads, n_kv_heads, head_dim, "attention_workspace_bytes");
-  return rc ? (rc < 0 ? rc : -rc) : AS_ALIGN;
+  return rc ? rc : as_layout(nullptr, n_seqs, n_tokens, n_heads, n_kv_heads, head_dim, nullptr);
 }
 
 extern "C" int b200emb_op_workspace_status(const void* workspace, void* stream) {
@@ -232,22 +1220,23 @@ extern "C" int b200emb_op_attention_scored(const void* q, int64_t q_row_stride, 
   if (!rc && d_cu_seqlens == nullptr) rc = set_error(B200EMB_ERR_INVALID, "%s: null pointer cu_seqlens", who);
   if (!rc) rc = check_workspace(workspace, workspace_bytes, b200emb_attention_workspace_bytes(n_seqs, n_tokens, n_heads, n_kv_heads, head_dim), who);
   if (rc) return rc;
-  AttnIo io = {};
-  io.q = static_cast<const __nv_bfloat16*>(q);
-  io.k = static_cast<const __nv_bfloat16*>(k);
-  io.v = static_cast<const __nv_bfloat16*>(v);
-  io.out = static_cast<__nv_bfloat16*>(out);
-  io.q_stride = q_row_stride;
-  io.k_stride = k_row_stride;
-  io.v_stride = v_row_stride;
-  io.out_stride = out_row_stride;
-  io.cu = d_cu_seqlens;
-  io.n_seqs = n_seqs;
-  io.n_tokens = n_tokens;
-  io.n_heads = n_heads;
-  io.n_kv_heads = n_kv_heads;
-  io.head_dim = head_dim;
-  return launch_rows<false>(io, mod, workspace, reinterpret_cast<cudaStream_t>(stream));
+  AttnJob j = {};
+  j.out = static_cast<__nv_bfloat16*>(out);
+  j.out_stride = out_row_stride;
+  j.cu = d_cu_seqlens;
+  j.n_seqs = n_seqs;
+  j.n_tokens = n_tokens;
+  j.n_heads = n_heads;
+  j.n_kv_heads = n_kv_heads;
+  j.head_dim = head_dim;
+  j.group = n_heads / n_kv_heads;
+  j.tile_tokens = as_tile_tokens(n_heads, n_kv_heads);
+  j.box_rows = AS_PACKED_BOX;
+  AsMaps m;
+  rc = as_map_rows(&m.q, q, n_tokens, n_heads, head_dim, q_row_stride, j.group, j.tile_tokens);
+  if (!rc) rc = as_map_rows(&m.k, k, n_tokens, n_kv_heads, head_dim, k_row_stride, 1, AS_PACKED_BOX);
+  if (!rc) rc = as_map_rows(&m.v, v, n_tokens, n_kv_heads, head_dim, v_row_stride, 1, AS_PACKED_BOX);
+  return rc ? rc : as_dispatch<false>(m, j, mod, workspace, reinterpret_cast<cudaStream_t>(stream));
 }
 
 extern "C" int b200emb_op_attention_paged(const void* q, int64_t q_row_stride, void* out, int64_t out_row_stride,
@@ -275,26 +1264,29 @@ extern "C" int b200emb_op_attention_paged(const void* q, int64_t q_row_stride, v
     rc = check_workspace(workspace, workspace_bytes,
                          b200emb_attention_workspace_bytes(n_seqs, n_tokens, n_heads, cache->n_kv_heads, cache->head_dim), who);
   if (rc) return rc;
-  AttnIo io = {};
-  io.q = static_cast<const __nv_bfloat16*>(q);
-  io.k = static_cast<const __nv_bfloat16*>(cache->k);
-  io.v = static_cast<const __nv_bfloat16*>(cache->v);
-  io.out = static_cast<__nv_bfloat16*>(out);
-  io.q_stride = q_row_stride;
-  io.out_stride = out_row_stride;
-  io.cu = d_cu_seqlens;
-  io.kv_lens = d_kv_lens;
-  io.page_table = cache->page_table;
-  io.page_stride = cache->page_stride;
-  io.token_stride = cache->token_stride;
-  io.head_stride = cache->head_stride;
-  io.n_seqs = n_seqs;
-  io.n_tokens = n_tokens;
-  io.n_heads = n_heads;
-  io.n_kv_heads = cache->n_kv_heads;
-  io.head_dim = cache->head_dim;
-  io.n_pages = cache->n_pages;
-  io.page_size = cache->page_size;
-  io.table_stride = cache->table_stride;
-  return launch_rows<true>(io, mod, workspace, reinterpret_cast<cudaStream_t>(stream));
+  AttnJob j = {};
+  j.out = static_cast<__nv_bfloat16*>(out);
+  j.out_stride = out_row_stride;
+  j.cu = d_cu_seqlens;
+  j.kv_lens = d_kv_lens;
+  j.page_table = cache->page_table;
+  j.n_seqs = n_seqs;
+  j.n_tokens = n_tokens;
+  j.n_heads = n_heads;
+  j.n_kv_heads = cache->n_kv_heads;
+  j.head_dim = cache->head_dim;
+  j.group = n_heads / cache->n_kv_heads;
+  j.tile_tokens = as_tile_tokens(n_heads, cache->n_kv_heads);
+  j.n_pages = cache->n_pages;
+  j.page_size = cache->page_size;
+  j.table_stride = cache->table_stride;
+  j.head_first = cache->head_stride <= cache->token_stride;
+  // rows of one copy: as many as divide both a page and a key tile
+  j.box_rows = AS_KV;
+  while (cache->page_size % j.box_rows != 0) j.box_rows >>= 1;
+  AsMaps m;
+  rc = as_map_rows(&m.q, q, n_tokens, n_heads, cache->head_dim, q_row_stride, j.group, j.tile_tokens);
+  if (!rc) rc = as_map_pages(&m.k, cache->k, *cache, j.head_first != 0, j.box_rows);
+  if (!rc) rc = as_map_pages(&m.v, cache->v, *cache, j.head_first != 0, j.box_rows);
+  return rc ? rc : as_dispatch<true>(m, j, mod, workspace, reinterpret_cast<cudaStream_t>(stream));
 }

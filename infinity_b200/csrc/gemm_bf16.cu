@@ -481,6 +481,24 @@ int make_tmap_bf16_2d(CUtensorMap_st* out, const void* base, uint64_t rows, uint
   return B200EMB_OK;
 }
 
+int encode_tmap_bf16(CUtensorMap_st* out, const void* base, int rank, const uint64_t* dims, const uint64_t* strides, const uint32_t* box) {
+  EncodeTiledFn fn = get_encode_fn();
+  if (fn == nullptr) return set_error(B200EMB_ERR_CUDA, "cuTensorMapEncodeTiled entry point not available");
+  cuuint64_t d[5], st[4];
+  cuuint32_t b[5], es[5];
+  for (int i = 0; i < rank; ++i) {
+    d[i] = dims[i];
+    b[i] = box[i];
+    es[i] = 1;
+    if (i + 1 < rank) st[i] = strides[i];
+  }
+  const CUresult r = fn(out, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, static_cast<cuuint32_t>(rank), const_cast<void*>(base), d, st, b, es,
+                        CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                        CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) return set_error(B200EMB_ERR_CUDA, "cuTensorMapEncodeTiled failed (%d)", (int)r);
+  return B200EMB_OK;
+}
+
 // Row tiles per group of the tile order. Measured on the Qwen2-7B and BERT-large GEMM shapes (group sizes 1 to
 // 32, interleaved runs): 16 is best or within 1 % of the best everywhere; the gate/up GEMM (W = 271 MB) runs
 // 35.2 ms with row-major order and 28.3 ms with 16, the down projection (K = 18944) 17.0 -> 15.7 ms.

@@ -71,6 +71,10 @@ int launch_gemm_bf16(const void* A, const void* W, const float* bias, void* C, i
 int gemm_init_device();
 // TMA descriptor of a bf16 row-major [rows, cols] matrix: box [box_rows x 64 columns], 128-byte swizzle.
 int make_tmap_bf16_2d(::CUtensorMap_st* out, const void* base, uint64_t rows, uint64_t cols, uint32_t box_rows);
+// TMA descriptor of a bf16 tensor of up to 5 dimensions, innermost first: dims in elements, strides of dimensions 1 .. in
+// bytes, 128-byte swizzle (box[0] = 64), zeros outside. Encoded anew each time.
+int encode_tmap_bf16(::CUtensorMap_st* out, const void* base, int rank, const uint64_t* dims, const uint64_t* strides,
+                     const uint32_t* box);
 // Descriptors depend on (address, shape, box, element kind) only, never on the memory's contents, and a forward
 // asks for the same few hundred of them every time (weights, workspace slices): the builders keep the encoded
 // 128 bytes per key and skip the driver call on a repeat. `kind` separates element types / swizzle modes.
@@ -130,6 +134,7 @@ int launch_attention_tc2(const void* qkv, void* out, const AttnTile* d_tiles, in
                          int n_kv_heads, int head_dim, int causal, int sm_count, int* err_flag, cudaStream_t stream);
 int attention_tc_init_device();
 int attention_tc2_init_device();
+int attention_scored_init_device();  // attention with modified scores, packed and paged (attention_scored.cu)
 
 // ---- block-format weight quantisers (quant.cu) ----
 // w bf16 [rows, cols] -> q (packed elements), scales (one byte per block, row-major [rows, cols / block]);
