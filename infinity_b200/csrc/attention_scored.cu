@@ -113,6 +113,8 @@ __device__ __forceinline__ float as_max3(float a, float b, float c) {
   asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
   return d;
 }
+// 1 - 2 / (1 + e^2x)
+__device__ __forceinline__ float as_tanh(float x) { return fmaf(-2.f, as_rcp(1.f + as_ex2(x * (2.f * AS_LOG2E))), 1.f); }
 // 32-bit mask of the x lowest bits, x clamped to 0 .. 32
 __device__ __forceinline__ uint32_t as_below(int x) {
   uint32_t m;
@@ -453,7 +455,24 @@ __device__ __forceinline__ void as_load_tile(const AttnJob& j, const AsWalk& w, 
   }
 }
 
-template <int D, bool PAGED, bool PAIR>
+// What happens to a score before it is masked. The kernel is built for each: a row of 128 scores is worked on in straight-line
+// code, and one body with every branch in it is 120 KB of instructions, which the instruction caches do not hold (7 us a step).
+enum { AS_PLAIN = 0, AS_SLOPES = 1, AS_CAP = 2, AS_ANY = 3 };
+
+// tanh(x) = x (c0 + c1 u + ... + c5 u^5), u = x^2, within 2.5e-7 on [-1, 1]: the odd polynomial with the smallest largest error there
+// (fitted to tanh in 64 bits by reweighted least squares). It spares the two special-function instructions of
+// 1 - 2 / (1 + e^2x) on top of the exponential's own; scores within the cap never leave its range. Two values at a time.
+__device__ __forceinline__ float2 as_tanh_near(float2 x, float2 u) {
+  auto both = [](float c) { return make_float2(c, c); };
+  float2 y = __ffma2_rn(u, both(-0.0028394628316164017f), both(0.01611417345702648f));
+  y = __ffma2_rn(u, y, both(-0.05097285658121109f));
+  y = __ffma2_rn(u, y, both(0.13253524899482727f));
+  y = __ffma2_rn(u, y, both(-0.3332400321960449f));
+  y = __ffma2_rn(u, y, both(0.9999968409538269f));
+  return __fmul2_rn(x, y);
+}
+
+template <int D, bool PAGED, bool PAIR, int MODE>
 __global__ void __launch_bounds__(AS_THREADS, 1)
 attn_scored_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constant__ CUtensorMap tmap_k,
                    const __grid_constant__ CUtensorMap tmap_v, const __grid_constant__ AttnJob j, const __grid_constant__ AttnMod mod,
@@ -678,13 +697,12 @@ attn_scored_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_cons
     const int group = j.group, g = row % group, row_tok = row / group;
     const int my_slot = PAIR ? blockIdx.x : blockIdx.x + t * gridDim.x;
     const int width = 2 * mod.radius + 1;
-    const bool staged = mod.bias != nullptr && group * width <= AS_TABLE;
-    const bool plain = mod.cap == 0.f && mod.slopes == nullptr && mod.bias == nullptr && mod.scale > 0.f;
-    // Scores are kept as the tensor core gives them where nothing but a positive scale follows (the scale is then part of the
-    // exponent's multiply-add), else in log2 units.
-    const float unit = plain ? mod.scale * AS_LOG2E : 1.f;
-    const float scale_log2 = mod.scale * AS_LOG2E;
-    const float cap_in = mod.cap > 0.f ? 2.f * scale_log2 / mod.cap : 0.f, cap_out = mod.cap * AS_LOG2E;
+    const bool staged = MODE == AS_ANY && mod.bias != nullptr && group * width <= AS_TABLE;
+    const float scale_log2 = mod.scale * AS_LOG2E, cap_out = mod.cap * AS_LOG2E;
+    // What a row's values are multiplied by to become exponents of 2: plain scores stay as the tensor core gives them, capped ones are
+    // kept as tanh, the others are in log2 units already.
+    const float unit = MODE == AS_PLAIN ? scale_log2 : MODE == AS_CAP ? cap_out : 1.f;
+    const float cap_in = mod.cap > 0.f ? mod.scale / mod.cap : 0.f;
     AsWalk w;
     w.start(plan, my_slot);
     uint32_t step = 0, meetings = 0;
@@ -715,8 +733,8 @@ attn_scored_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_cons
       const int key_lo = mod.left >= pos ? 0 : pos - mod.left;
       const int key_hi = mod.right >= kv_len - pos ? kv_len : pos + mod.right + 1;
       const int doc = mod.docs != nullptr && real ? __ldg(mod.docs + tok) : -1;
-      if (mod.slopes != nullptr) slope = __ldg(mod.slopes + h) * AS_LOG2E;
-      if (mod.bias != nullptr) {
+      if ((MODE == AS_SLOPES || MODE == AS_ANY) && mod.slopes != nullptr) slope = __ldg(mod.slopes + h) * AS_LOG2E;
+      if (MODE == AS_ANY && mod.bias != nullptr) {
         if (staged) {
           meet();  // the previous item's reads are over
           for (int i = row; i < group * width; i += 128) table[i] = __ldg(mod.bias + static_cast<int64_t>(w.h) * group * width + i) * AS_LOG2E;
@@ -738,6 +756,49 @@ attn_scored_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_cons
         if (failed) break;
         tc_fence_after_sync();
         if (active) {
+          if (MODE == AS_ANY) {
+            // any combination: the scores are rewritten where they are, 32 at a time, and the row is then taken as it is
+#pragma unroll 1
+            for (int q = 0; q < n_chunks; ++q) {
+              uint32_t raw[32];
+              tmem_ld_32x32b_x32(lanes + Cfg::S(t) + q * 32, raw);
+              tmem_ld_wait_for(raw);
+              float y[32];
+#pragma unroll
+              for (int i = 0; i < 32; ++i) y[i] = __uint_as_float(raw[i]);
+              if (mod.cap > 0.f) {
+#pragma unroll
+                for (int i = 0; i < 32; ++i) y[i] = cap_out * as_tanh(y[i] * cap_in);
+              } else {
+#pragma unroll
+                for (int i = 0; i < 32; ++i) y[i] *= scale_log2;
+              }
+              const int d0 = kv0 + q * 32 - pos;
+              if (mod.slopes != nullptr) {
+                const float f = static_cast<float>(d0);
+#pragma unroll
+                for (int i = 0; i < 32; ++i) y[i] = fmaf(-slope, fabsf(f + static_cast<float>(i)), y[i]);
+              }
+              if (mod.bias != nullptr) {
+                if (__all_sync(0xffffffffu, d0 + 31 <= -mod.radius || d0 >= mod.radius)) {
+                  const float b = tab[d0 < 0 ? -mod.radius : mod.radius] * tab_unit;
+#pragma unroll
+                  for (int i = 0; i < 32; ++i) y[i] += b;
+                } else {
+#pragma unroll
+                  for (int i = 0; i < 32; ++i) y[i] = fmaf(tab[min(max(d0 + i, -mod.radius), mod.radius)], tab_unit, y[i]);
+                }
+              }
+              uint32_t half[16];
+#pragma unroll
+              for (int i = 0; i < 16; ++i) half[i] = __float_as_uint(y[i]);
+              tmem_st_32x32b_x16(lanes + Cfg::S(t) + q * 32, half);
+#pragma unroll
+              for (int i = 0; i < 16; ++i) half[i] = __float_as_uint(y[16 + i]);
+              tmem_st_32x32b_x16(lanes + Cfg::S(t) + q * 32 + 16, half);
+            }
+            tmem_st_wait();
+          }
           uint32_t zr[4][32];  // the score row
           float mx0 = -INFINITY, mx1 = -INFINITY;
           tmem_ld_32x32b_x32(lanes + Cfg::S(t), zr[0]);
@@ -748,35 +809,6 @@ attn_scored_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_cons
               tmem_ld_wait_for(zr[q]);
               if (q < 3 && q + 1 < n_chunks) tmem_ld_32x32b_x32(lanes + Cfg::S(t) + q * 32 + 32, zr[q < 3 ? q + 1 : 3]);
               const int key = kv0 + q * 32;
-              float y[32];
-#pragma unroll
-              for (int i = 0; i < 32; ++i) y[i] = __uint_as_float(zr[q][i]);
-              if (!plain) {
-                if (mod.cap > 0.f) {
-                  // cap tanh(s / cap) = cap (1 - 2 / (1 + e^(2 s / cap))), in log2 units
-#pragma unroll
-                  for (int i = 0; i < 32; ++i) y[i] = fmaf(-2.f * cap_out, as_rcp(1.f + as_ex2(y[i] * cap_in)), cap_out);
-                } else {
-#pragma unroll
-                  for (int i = 0; i < 32; ++i) y[i] *= scale_log2;
-                }
-                const int d0 = key - pos;
-                if (mod.slopes != nullptr) {
-                  const float f = static_cast<float>(d0);
-#pragma unroll
-                  for (int i = 0; i < 32; ++i) y[i] = fmaf(-slope, fabsf(f + static_cast<float>(i)), y[i]);
-                }
-                if (mod.bias != nullptr) {
-                  if (__all_sync(0xffffffffu, d0 + 31 <= -mod.radius || d0 >= mod.radius)) {
-                    const float b = tab[d0 < 0 ? -mod.radius : mod.radius] * tab_unit;
-#pragma unroll
-                    for (int i = 0; i < 32; ++i) y[i] += b;
-                  } else {
-#pragma unroll
-                    for (int i = 0; i < 32; ++i) y[i] = fmaf(tab[min(max(d0 + i, -mod.radius), mod.radius)], tab_unit, y[i]);
-                  }
-                }
-              }
               uint32_t seen = (as_below(key_hi - key) & ~as_below(key_lo - key)) | as_below(prefix - key);
               if (mod.docs != nullptr) {
                 // the keys of each document that some row of the warp belongs to
@@ -790,17 +822,67 @@ attn_scored_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_cons
                 }
                 seen &= same;
               }
-              if (!__all_sync(0xffffffffu, seen == 0xffffffffu)) {
+              const bool whole = __all_sync(0xffffffffu, seen == 0xffffffffu || !real);  // rows of no token do not count
+              auto pair_of = [&](int i) { return make_float2(__uint_as_float(zr[q][i]), __uint_as_float(zr[q][i + 1])); };
+              auto put = [&](int i, float2 y) {
+                zr[q][i] = __float_as_uint(y.x);
+                zr[q][i + 1] = __float_as_uint(y.y);
+              };
+              if (MODE == AS_SLOPES) {
+                const int d0 = key - pos;
+                const float f = static_cast<float>(d0);
+                if (__all_sync(0xffffffffu, d0 + 31 <= 0 || d0 >= 0)) {
+                  // all 32 keys on one side of the query: the bias is linear in the key
+                  const float rise = d0 < 0 ? slope : -slope;
+                  const float2 scale2 = make_float2(scale_log2, scale_log2), rise2 = make_float2(2.f * rise, 2.f * rise);
+                  float2 bias2 = make_float2(rise * f, rise * (f + 1.f));
 #pragma unroll
-                for (int i = 0; i < 32; ++i) y[i] = (seen >> i) & 1u ? y[i] : -INFINITY;
+                  for (int i = 0; i < 32; i += 2) {
+                    put(i, __ffma2_rn(pair_of(i), scale2, bias2));
+                    bias2 = __fadd2_rn(bias2, rise2);
+                  }
+                } else {
+#pragma unroll
+                  for (int i = 0; i < 32; ++i)
+                    zr[q][i] = __float_as_uint(fmaf(__uint_as_float(zr[q][i]), scale_log2, -slope * fabsf(f + static_cast<float>(i))));
+                }
+              }
+              if (MODE == AS_CAP) {
+                // Which way the tanh goes is decided by what is seen alone: columns that no key wrote and rows of no token hold whatever
+                // was there before, and results must not depend on it.
+                const float in = real ? cap_in : 0.f;
+                const float2 in2 = make_float2(in, in);
+                if (!whole) {
+#pragma unroll
+                  for (int i = 0; i < 32; ++i)
+                    if (!((seen >> i) & 1u)) zr[q][i] = 0u;
+                }
+                float2 x2[16], u2[16];
+                float far = 0.f;
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                  x2[i] = __fmul2_rn(pair_of(2 * i), in2);
+                  u2[i] = __fmul2_rn(x2[i], x2[i]);
+                  far = as_max3(far, u2[i].x, u2[i].y);
+                }
+                if (__all_sync(0xffffffffu, far <= 1.f)) {
+#pragma unroll
+                  for (int i = 0; i < 16; ++i) put(2 * i, as_tanh_near(x2[i], u2[i]));
+                } else {
+#pragma unroll
+                  for (int i = 0; i < 16; ++i) put(2 * i, make_float2(as_tanh(x2[i].x), as_tanh(x2[i].y)));
+                }
+              }
+              if (!whole) {
+#pragma unroll
+                for (int i = 0; i < 32; ++i)
+                  if (!((seen >> i) & 1u)) zr[q][i] = 0xff800000u;  // -inf
               }
 #pragma unroll
               for (int i = 0; i < 32; i += 4) {
-                mx0 = as_max3(mx0, y[i], y[i + 1]);
-                mx1 = as_max3(mx1, y[i + 2], y[i + 3]);
+                mx0 = as_max3(mx0, __uint_as_float(zr[q][i]), __uint_as_float(zr[q][i + 1]));
+                mx1 = as_max3(mx1, __uint_as_float(zr[q][i + 2]), __uint_as_float(zr[q][i + 3]));
               }
-#pragma unroll
-              for (int i = 0; i < 32; ++i) zr[q][i] = __float_as_uint(y[i]);
             }
           }
           if (Cfg::P_APART) {
@@ -1110,7 +1192,7 @@ struct AsMaps {
 // Two neighbouring tiles share their keys where sequences have two tiles of rows on average; shorter ones would leave stream B idle.
 static bool as_pair(const AttnJob& j) { return static_cast<int64_t>(j.n_tokens) * j.group >= 256ll * j.n_seqs; }
 
-template <int D, bool PAGED, bool PAIR>
+template <int D, bool PAGED, bool PAIR, int MODE>
 static int as_launch(const AsMaps& m, const AttnJob& j, const AttnMod& mod, const AttnPlan& plan, int sms, cudaStream_t s) {
   int64_t grid = sms < AS_MAX_CTAS ? sms : AS_MAX_CTAS;
   if (!PAGED) {  // no more CTAs than steps there can be
@@ -1120,32 +1202,41 @@ static int as_launch(const AsMaps& m, const AttnJob& j, const AttnMod& mod, cons
   const int slots = static_cast<int>(PAIR ? grid : 2 * grid);
   cudaError_t e = launch_pdl(attn_plan_kernel, dim3(1), dim3(AS_PLAN_THREADS), 0, s, j, mod, plan, (PAIR ? 2 : 1) * j.tile_tokens, slots);
   if (e == cudaSuccess)
-    e = launch_pdl(attn_scored_kernel<D, PAGED, PAIR>, dim3(static_cast<unsigned>(grid)), dim3(AS_THREADS), AsCfg<D>::SMEM_BYTES, s, m.q, m.k,
+    e = launch_pdl(attn_scored_kernel<D, PAGED, PAIR, MODE>, dim3(static_cast<unsigned>(grid)), dim3(AS_THREADS), AsCfg<D>::SMEM_BYTES, s, m.q, m.k,
                    m.v, j, mod, plan);
   if (e != cudaSuccess) return set_error(B200EMB_ERR_CUDA, "attention launch: %s", cudaGetErrorString(e));
   return B200EMB_OK;
 }
 
-template <int D, bool PAGED, bool PAIR>
+template <int D, bool PAGED, bool PAIR, int MODE>
 static int as_init_one() {
   cudaFuncAttributes a;
-  B2_CUDA_CHECK(cudaFuncGetAttributes(&a, attn_scored_kernel<D, PAGED, PAIR>));
+  B2_CUDA_CHECK(cudaFuncGetAttributes(&a, attn_scored_kernel<D, PAGED, PAIR, MODE>));
   // the register split of the kernel draws on exactly this many: with fewer its softmax warps would wait for good
   if (a.numRegs != AS_REGS_LAUNCH)
     return set_error(B200EMB_ERR_CUDA, "attention kernel built with %d registers instead of %d", a.numRegs, AS_REGS_LAUNCH);
-  B2_CUDA_CHECK(cudaFuncSetAttribute(attn_scored_kernel<D, PAGED, PAIR>, cudaFuncAttributeMaxDynamicSharedMemorySize, AsCfg<D>::SMEM_BYTES));
+  B2_CUDA_CHECK(cudaFuncSetAttribute(attn_scored_kernel<D, PAGED, PAIR, MODE>, cudaFuncAttributeMaxDynamicSharedMemorySize, AsCfg<D>::SMEM_BYTES));
   return B200EMB_OK;
 }
 
+template <int D, bool PAGED, bool PAIR>
+static int as_init_modes() {
+  int rc = as_init_one<D, PAGED, PAIR, AS_PLAIN>();
+  if (!rc) rc = as_init_one<D, PAGED, PAIR, AS_SLOPES>();
+  if (!rc) rc = as_init_one<D, PAGED, PAIR, AS_CAP>();
+  if (!rc) rc = as_init_one<D, PAGED, PAIR, AS_ANY>();
+  return rc;
+}
+
 int attention_scored_init_device() {
-  int rc = as_init_one<64, false, false>();
-  if (!rc) rc = as_init_one<64, false, true>();
-  if (!rc) rc = as_init_one<64, true, false>();
-  if (!rc) rc = as_init_one<64, true, true>();
-  if (!rc) rc = as_init_one<128, false, false>();
-  if (!rc) rc = as_init_one<128, false, true>();
-  if (!rc) rc = as_init_one<128, true, false>();
-  if (!rc) rc = as_init_one<128, true, true>();
+  int rc = as_init_modes<64, false, false>();
+  if (!rc) rc = as_init_modes<64, false, true>();
+  if (!rc) rc = as_init_modes<64, true, false>();
+  if (!rc) rc = as_init_modes<64, true, true>();
+  if (!rc) rc = as_init_modes<128, false, false>();
+  if (!rc) rc = as_init_modes<128, false, true>();
+  if (!rc) rc = as_init_modes<128, true, false>();
+  if (!rc) rc = as_init_modes<128, true, true>();
   return rc;
 }
 
@@ -1168,6 +1259,15 @@ static int as_map_pages(CUtensorMap* m, const void* base, const b200emb_kv_cache
   return encode_tmap_bf16(m, base, 4, dims, strides, box);
 }
 
+template <int D, bool PAGED, bool PAIR>
+static int as_launch_mode(const AsMaps& m, const AttnJob& j, const AttnMod& mod, const AttnPlan& plan, int sms, cudaStream_t s) {
+  const bool up = mod.scale > 0.f;  // the plain row maximum is that of the scaled scores
+  if (mod.cap == 0.f && mod.slopes == nullptr && mod.bias == nullptr && up) return as_launch<D, PAGED, PAIR, AS_PLAIN>(m, j, mod, plan, sms, s);
+  if (mod.cap == 0.f && mod.slopes != nullptr) return as_launch<D, PAGED, PAIR, AS_SLOPES>(m, j, mod, plan, sms, s);
+  if (mod.cap > 0.f && mod.slopes == nullptr && mod.bias == nullptr) return as_launch<D, PAGED, PAIR, AS_CAP>(m, j, mod, plan, sms, s);
+  return as_launch<D, PAGED, PAIR, AS_ANY>(m, j, mod, plan, sms, s);
+}
+
 template <bool PAGED>
 static int as_dispatch(const AsMaps& m, const AttnJob& j, const AttnMod& mod, void* workspace, cudaStream_t s) {
   int rc = kernels_init_device();
@@ -1178,8 +1278,8 @@ static int as_dispatch(const AsMaps& m, const AttnJob& j, const AttnMod& mod, vo
   as_layout(workspace, j.n_seqs, j.n_tokens, j.n_heads, j.n_kv_heads, j.head_dim, &plan);
   const bool pair = as_pair(j);
   if (j.head_dim <= 64)
-    return pair ? as_launch<64, PAGED, true>(m, j, mod, plan, sms, s) : as_launch<64, PAGED, false>(m, j, mod, plan, sms, s);
-  return pair ? as_launch<128, PAGED, true>(m, j, mod, plan, sms, s) : as_launch<128, PAGED, false>(m, j, mod, plan, sms, s);
+    return pair ? as_launch_mode<64, PAGED, true>(m, j, mod, plan, sms, s) : as_launch_mode<64, PAGED, false>(m, j, mod, plan, sms, s);
+  return pair ? as_launch_mode<128, PAGED, true>(m, j, mod, plan, sms, s) : as_launch_mode<128, PAGED, false>(m, j, mod, plan, sms, s);
 }
 
 }  // namespace b2
