@@ -16,9 +16,11 @@
 // neighbouring tiles of the same item row and share every key and value tile ("pair"); otherwise each walks its own part.
 // Per step of a stream:
 //   S = Q K^T     tcgen05.mma 128 x N x 16 (N = valid keys rounded up to 16), fp32 in tensor memory
-//   softmax       128 threads, one row each: the whole score row is read into registers, modified and masked there, and reduced to
-//                 its maximum; the reference of the exponentials moves only when the maximum passes it by 2^8
-//                 (probabilities then stay below 2^8, sums far inside fp32), which is when O is rescaled
+//   softmax       128 threads, one row each, in one pass over the row: a score becomes its exponential against the row's reference
+//                 at once. The reference is a guess (the first 32 scores of the row's first step) and is only replaced, by the exact
+//                 maximum and a second pass, when a step's sum leaves 2^-60 .. 2^60: numerators and denominator share its
+//                 scale, and fp32 sums and bf16 probabilities keep their relative precision anywhere in between. Capped scores
+//                 lie within +-cap and need no reference at all.
 //   O += P V      P rounded to bf16 (the tensor core's operand type; half a step of 2^-8 per probability) in tensor memory, V as an MN-major
 //                 shared-memory operand
 // Warps: 0-3 softmax A, 4-7 softmax B, 8 loads Q and K, 9 loads V, 10 issues the matrix instructions, 11 idle (it completes the
@@ -50,7 +52,9 @@ static constexpr int AS_BLOCK = 128 * 64 * 2;      // 128 rows x 64 columns, 128
 static constexpr int AS_PACKED_BOX = 32;           // rows of one copy of a packed key tile: short sequences copy few rows
 static constexpr int AS_TABLE = 2048;              // floats of a stream's staged bias tables
 static constexpr float AS_LOG2E = 1.4426950408889634f;
-static constexpr float AS_LAZY = 8.f;              // the softmax reference moves when the maximum passes it by 2^AS_LAZY
+static constexpr float AS_LAZY = 8.f;              // AS_ANY: the reference moves when a maximum passes it by 2^AS_LAZY
+static constexpr float AS_SUM_LOW = 0x1p-60f, AS_SUM_HIGH = 0x1p60f;  // sums that keep the reference, see above
+static constexpr float AS_CAP_LOW = 0x1p-7f, AS_CAP_HIGH = 80.f;      // cap * log2(e) that AS_CAP serves: 2^+-80 keeps fp32 sums in range
 
 struct AttnMod {
   float scale, cap;
@@ -65,7 +69,7 @@ struct AttnMod {
 struct __align__(16) AttnEntry {
   int32_t seq, tok0, n_tok, pos0;     // first row of q and out, tokens, position of the first
   int32_t kv_len, kv_row0, prefix, n; // keys; packed: first row of k and v; visible prefix; key tiles visited
-  int32_t a0, n0, a1, pad;            // visited tiles: a0 .. a0 + n0 - 1, then a1 ..
+  int32_t a0, n0, a1, near;           // visited tiles: a0 .. a0 + n0 - 1, then the run from a1, tile a1 + near first, down, then up
   int64_t before;                     // tiles of the entries in front (per key head)
   int64_t pad2;
 };
@@ -111,6 +115,11 @@ __device__ __forceinline__ float as_rcp(float x) {
 __device__ __forceinline__ float as_max3(float a, float b, float c) {
   float d;
   asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
+__device__ __forceinline__ float as_max3_abs(float a, float b, float c) {  // max(|a|, |b|, |c|)
+  float d;
+  asm("max.abs.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
   return d;
 }
 // 1 - 2 / (1 + e^2x)
@@ -294,6 +303,7 @@ attn_plan_kernel(const AttnJob j, const AttnMod mod, const AttnPlan p, int token
       x.n0 = f1 - f0;
       x.a1 = b0;
       x.n = x.n0 + (b1 - b0);
+      if (mod.slopes != nullptr) x.near = min(max(p1 / AS_KV - b0, 0), max(b1 - b0 - 1, 0));
       if (x.n == 0) {  // nothing visible: one step whose keys are all masked writes the zeros
         x.a0 = x.a1 = 0;
         x.n0 = 0;
@@ -387,7 +397,12 @@ struct AsWalk {
     if (left > 0) load(p.entry);
   }
   __device__ bool last() const { return left == 1 || k == f1.w - 1; }
-  __device__ int key0() const { return (k < f2.y ? f2.x + k : f2.z + k - f2.y) * AS_KV; }
+  // With a bias that falls with the distance the run starts at the queries' own tile and moves away from it, so that the first
+  // reference of a row serves all steps; otherwise near is 0 and the run is taken in order.
+  __device__ int key0() const {
+    const int i = k - f2.y;
+    return (i < 0 ? f2.x + k : f2.z + (i <= f2.w ? f2.w - i : i)) * AS_KV;
+  }
   __device__ int n_valid() const { return min(max(f1.x - key0(), 0), AS_KV); }
   __device__ void next(const AttnPlan& p, int n_kv_heads) {
     first = false;
@@ -418,6 +433,38 @@ __device__ __forceinline__ void as_tma_4d(void* dst, const void* tmap, uint64_t*
                "l"(reinterpret_cast<uint64_t>(tmap)), "r"(smem_u32(bar)), "r"(x), "r"(y), "r"(z), "r"(w)
                : "memory");
 }
+
+// One look at a barrier: whether the phase of this parity is over.
+__device__ __forceinline__ bool as_test(uint64_t* bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n"
+      " .reg .pred p;\n"
+      " mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n"
+      " selp.u32 %0, 1, 0, p;\n"
+      "}\n"
+      : "=r"(ok)
+      : "r"(smem_u32(bar)), "r"(parity)
+      : "memory");
+  return ok != 0;
+}
+
+// Bound of a loop that looks at several barriers in turn: false when nothing has moved for WAIT_LIMIT_NS. Every lane asks; the
+// warp gives up together.
+struct AsPatience {
+  uint32_t idle = 0;
+  unsigned long long since = 0;
+  __device__ bool go_on(bool moved) {
+    if (moved) {
+      idle = 0;
+      return true;
+    }
+    if ((++idle & 0xffu) != 0u) return true;
+    const unsigned long long now = globaltimer_ns();
+    if (idle == 0x100u) since = now;
+    return __all_sync(0xffffffffu, now - since <= WAIT_LIMIT_NS) != 0;
+  }
+};
 
 // After a failed wait: lets the copies still in flight land before shared memory is released (bounded).
 __device__ __forceinline__ void as_drain(uint64_t* full, uint32_t fills, uint32_t slots) {
@@ -461,16 +508,29 @@ enum { AS_PLAIN = 0, AS_SLOPES = 1, AS_CAP = 2, AS_ANY = 3 };
 
 // tanh(x) = x (c0 + c1 u + ... + c5 u^5), u = x^2, within 2.5e-7 on [-1, 1]: the odd polynomial with the smallest largest error there
 // (fitted to tanh in 64 bits by reweighted least squares). It spares the two special-function instructions of
-// 1 - 2 / (1 + e^2x) on top of the exponential's own; scores within the cap never leave its range. Two values at a time.
-__device__ __forceinline__ float2 as_tanh_near(float2 x, float2 u) {
-  auto both = [](float c) { return make_float2(c, c); };
-  float2 y = __ffma2_rn(u, both(-0.0028394628316164017f), both(0.01611417345702648f));
-  y = __ffma2_rn(u, y, both(-0.05097285658121109f));
-  y = __ffma2_rn(u, y, both(0.13253524899482727f));
-  y = __ffma2_rn(u, y, both(-0.3332400321960449f));
-  y = __ffma2_rn(u, y, both(0.9999968409538269f));
-  return __fmul2_rn(x, y);
-}
+// 1 - 2 / (1 + e^2x) on top of the exponential's own; scores within the cap never leave its range. Two values at a time;
+// c tanh(v / c) is formed with c^-2k folded into the coefficients (AS_CAP_LOW .. AS_CAP_HIGH keeps them in fp32's range).
+struct AsTanh {
+  float2 c[6];
+  __device__ explicit AsTanh(float cap) {
+    const float f = 1.f / (cap * cap);
+    const float c0[6] = {0.9999968409538269f, -0.3332400321960449f, 0.13253524899482727f, -0.05097285658121109f, 0.01611417345702648f, -0.0028394628316164017f};
+    float g = 1.f;
+#pragma unroll
+    for (int i = 0; i < 6; ++i) {
+      c[i] = make_float2(c0[i] * g, c0[i] * g);
+      g *= f;
+    }
+  }
+  __device__ float2 operator()(float2 v, float2 w) const {
+    float2 y = __ffma2_rn(w, c[5], c[4]);
+    y = __ffma2_rn(w, y, c[3]);
+    y = __ffma2_rn(w, y, c[2]);
+    y = __ffma2_rn(w, y, c[1]);
+    y = __ffma2_rn(w, y, c[0]);
+    return __fmul2_rn(v, y);
+  }
+};
 
 template <int D, bool PAGED, bool PAIR, int MODE>
 __global__ void __launch_bounds__(AS_THREADS, 1)
@@ -479,6 +539,8 @@ attn_scored_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_cons
                    const __grid_constant__ AttnPlan plan) {
   using Cfg = AsCfg<D>;
   constexpr int RING = Cfg::RING;
+  // A stream's own tiles in flight, so that neither stream waits for the other's; a pair has one ring.
+  constexpr uint32_t SLOTS = PAIR ? RING : RING / 2;
   extern __shared__ uint8_t as_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(as_raw) + 1023) & ~uintptr_t(1023));
   uint8_t* q_s = smem;
@@ -505,9 +567,9 @@ attn_scored_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_cons
   if (threadIdx.x == 0) {
     for (int i = 0; i < RING; ++i) {
       mbar_init(&k_full[i], 1);
-      mbar_init(&k_empty[i], 1);
+      mbar_init(&k_empty[i], PAIR ? 2 : 1);  // a tile is read by both streams of a pair
       mbar_init(&v_full[i], 1);
-      mbar_init(&v_empty[i], 1);
+      mbar_init(&v_empty[i], PAIR ? 2 : 1);
     }
     for (int t = 0; t < 2; ++t) {
       mbar_init(&q_full[t], 1);
@@ -547,42 +609,46 @@ attn_scored_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_cons
       w[0].start(plan, blockIdx.x);
       if (PAIR) w[1].left = 0;
       else w[1].start(plan, blockIdx.x + gridDim.x);
-      int slot = 0;
-      uint32_t phase = 0, fills = 0, q_fills[2] = {0, 0};
+      uint32_t fills[2] = {0, 0}, q_fills[2] = {0, 0};
+      AsPatience patience;
       bool ok = true;
+      // whichever stream has room takes its next step
       while (ok && (w[0].left > 0 || w[1].left > 0)) {
+        bool moved = false;
 #pragma unroll
         for (int t = 0; t < (PAIR ? 1 : 2); ++t) {
-          if (!ok || w[t].left <= 0) continue;
+          if (w[t].left <= 0) continue;
+          const uint32_t slot = t * SLOTS + fills[t] % SLOTS;
+          bool ready = as_test(&empty[slot], ((fills[t] / SLOTS) & 1u) ^ 1u);
+          if (is_k && w[t].first) {
+#pragma unroll
+            for (int u = t; u < (PAIR ? 2 : t + 1); ++u) ready = ready && as_test(&q_empty[u], (q_fills[u] & 1u) ^ 1u);
+          }
+          if (!__all_sync(0xffffffffu, ready)) continue;
+          moved = true;
           if (is_k && w[t].first) {
 #pragma unroll
             for (int u = t; u < (PAIR ? 2 : t + 1); ++u) {
-              if (ok) ok = __all_sync(0xffffffffu, mbar_wait(&q_empty[u], (q_fills[u] & 1u) ^ 1u));
-              if (ok && lane == 0) {
+              if (lane == 0) {
                 mbar_arrive_expect_tx(&q_full[u], j.group * j.tile_tokens * 128 * Cfg::BLOCKS);
 #pragma unroll
                 for (int b = 0; b < Cfg::BLOCKS; ++b)
                   as_tma_3d(q_s + u * Cfg::TILE + b * AS_BLOCK, &tmap_q, &q_full[u], b * 64, w[t].h * j.group,
                             w[t].f0.y + (PAIR ? u * j.tile_tokens : 0));
               }
-              if (ok) ++q_fills[u];
+              ++q_fills[u];
             }
           }
-          if (ok) ok = __all_sync(0xffffffffu, mbar_wait(&empty[slot], phase ^ 1u));
-          if (!ok) break;
           as_load_tile<D, PAGED>(j, w[t], tmap, ring + slot * Cfg::TILE, &full[slot], lane);
-          ++fills;
-          if (++slot == RING) {
-            slot = 0;
-            phase ^= 1u;
-          }
+          ++fills[t];
           w[t].next(plan, j.n_kv_heads);
         }
+        ok = patience.go_on(moved);
       }
       if (is_k) pdl_launch_dependents();
       if (!ok) {
         if (lane == 0) atomicExch(plan.status, is_k ? 5 : 8);
-        as_drain(full, fills, RING);
+        for (int t = 0; t < (PAIR ? 1 : 2); ++t) as_drain(&full[t * SLOTS], fills[t], SLOTS);
         if (is_k)
           for (int u = 0; u < 2; ++u) as_drain(&q_full[u], q_fills[u], 1);
       }
@@ -590,100 +656,84 @@ attn_scored_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_cons
       // ---------------- matrix instructions: all lanes walk, one elected lane issues ----------------
       const uint32_t tmem_u = __shfl_sync(0xffffffffu, tmem_base, 0);
       const uint32_t q_addr = smem_u32(q_s), k_addr = smem_u32(k_s), v_addr = smem_u32(v_s);
-      auto wait_all = [](uint64_t* bar, uint32_t parity) -> bool { return __all_sync(0xffffffffu, mbar_wait(bar, parity)); };
       AsWalk sw[2], pw[2];  // the next S of each stream, and the next P V
       sw[0].start(plan, blockIdx.x);
       sw[1].start(plan, PAIR ? blockIdx.x : blockIdx.x + gridDim.x);
       pw[0] = sw[0];
       pw[1] = sw[1];
-      uint32_t q_uses[2] = {0, 0}, n_s[2] = {0, 0}, n_pv[2] = {0, 0};
-      int kslot = 0, vslot = 0;
-      uint32_t kphase = 0, vphase = 0;
-      bool ok = true;
-      // In a pair both streams use the tile of a ring slot, B last; B may have no tokens (the item ends in A's tile).
-      auto has_rows = [&](const AsWalk& w, int t) { return !PAIR || t == 0 || w.f0.z > j.tile_tokens; };
-      auto issue_s = [&](int t) -> bool {
-        AsWalk& w = sw[t];
-        if (w.left <= 0) return true;
-        if (w.first && !wait_all(&q_full[t], q_uses[t]++ & 1u)) return false;
-        if (!wait_all(&k_full[kslot], kphase)) return false;
-        tc_fence_after_sync();
-        const uint32_t idesc = make_idesc_bf16_f32(128, as_round16(w.n_valid()));
-        if (has_rows(w, t)) {
-#pragma unroll
-          for (int k = 0; k < D / 16; ++k) {
-            const uint64_t a = make_kmajor_sw128_desc(q_addr + t * Cfg::TILE + (k / 4) * AS_BLOCK) + 2 * (k % 4);
-            const uint64_t b = make_kmajor_sw128_desc(k_addr + kslot * Cfg::TILE + (k / 4) * AS_BLOCK) + 2 * (k % 4);
-            if (elect_one()) tc_mma_f16(tmem_u + Cfg::S(t), a, b, idesc, k != 0);
-          }
-        }
-        const bool done = !PAIR || t == 1;
-        if (elect_one()) {
-          tc_commit(&s_full[t]);
-          if (done) tc_commit(&k_empty[kslot]);
-          if (w.last()) tc_commit(&q_empty[t]);
-        }
-        if (done && ++kslot == RING) {
-          kslot = 0;
-          kphase ^= 1u;
-        }
-        ++n_s[t];
-        w.next(plan, j.n_kv_heads);
-        return true;
-      };
+      uint32_t q_uses[2] = {0, 0}, n_s[2] = {0, 0}, n_pv[2] = {0, 0}, zeroed = 0;
       const uint32_t idesc_pv = make_idesc_bf16_f32_b_mn(128, D);
-      auto issue_pv = [&](int t) -> bool {
-        AsWalk& w = pw[t];
-        if (!wait_all(&p_full[t], n_pv[t] & 1u) || !wait_all(&v_full[vslot], vphase)) return false;
-        tc_fence_after_sync();
-        const int n_valid = w.n_valid(), n_eff = as_round16(n_valid);
-        if (n_valid < n_eff && (!PAIR || t == 0)) {
-          // value rows behind the last key: whatever lies there must not meet a zero probability (0 * NaN)
-          uint8_t* tile = v_s + vslot * Cfg::TILE;
-          for (int i = lane; i < (n_eff - n_valid) * 8 * Cfg::BLOCKS; i += 32) {
-            const int b = i / ((n_eff - n_valid) * 8), at = i - b * ((n_eff - n_valid) * 8);
-            *reinterpret_cast<uint4*>(tile + b * AS_BLOCK + n_valid * 128 + at * 16) = make_uint4(0, 0, 0, 0);
-          }
-          fence_proxy_async_smem();
-          __syncwarp();
-        }
-        if (has_rows(w, t)) {
-          const uint64_t v_desc = make_mnmajor_sw128_desc(v_addr + vslot * Cfg::TILE, AS_BLOCK);
-#pragma unroll
-          for (int k = 0; k < AS_KV / 16; ++k)
-            if (k * 16 < n_eff && elect_one())
-              tc_mma_f16_tmem_a(tmem_u + Cfg::O(t), tmem_u + Cfg::P(t) + k * 8, v_desc + k * 128, idesc_pv, !w.first || k != 0);
-        }
-        const bool done = !PAIR || t == 1;
-        if (elect_one()) {
-          tc_commit(&pv_done[t]);
-          if (done) tc_commit(&v_empty[vslot]);
-        }
-        if (done && ++vslot == RING) {
-          vslot = 0;
-          vphase ^= 1u;
-        }
-        ++n_pv[t];
-        w.next(plan, j.n_kv_heads);
-        return true;
-      };
-      ok = issue_s(0) && issue_s(1);
+      // In a pair stream B may have no tokens (the item ends in A's tile): its steps are then only counted.
+      auto has_rows = [&](const AsWalk& w, int t) { return !PAIR || t == 0 || w.f0.z > j.tile_tokens; };
+      AsPatience patience;
+      bool ok = true;
+      // whichever stream's operands are there goes next
       while (ok && (pw[0].left > 0 || pw[1].left > 0)) {
-        if (Cfg::P_APART) {
+        bool moved = false;
 #pragma unroll
-          for (int t = 0; t < 2; ++t)
-            if (ok && sw[t].left > 0) ok = wait_all(&s_read[t], (n_s[t] - 1) & 1u) && issue_s(t);
+        for (int t = 0; t < 2; ++t) {
+          const uint32_t pv_slot = (PAIR ? 0 : t * SLOTS) + n_pv[t] % SLOTS;
+          if (n_pv[t] < n_s[t] &&
+              __all_sync(0xffffffffu, as_test(&p_full[t], n_pv[t] & 1u) && as_test(&v_full[pv_slot], (n_pv[t] / SLOTS) & 1u))) {
+            AsWalk& w = pw[t];
+            tc_fence_after_sync();
+            const int n_valid = w.n_valid(), n_eff = as_round16(n_valid);
+            if (n_valid < n_eff && (!PAIR || n_pv[t] >= zeroed)) {
+              // value rows behind the last key: whatever lies there must not meet a zero probability (0 * NaN)
+              uint8_t* tile = v_s + pv_slot * Cfg::TILE;
+              for (int i = lane; i < (n_eff - n_valid) * 8 * Cfg::BLOCKS; i += 32) {
+                const int b = i / ((n_eff - n_valid) * 8), at = i - b * ((n_eff - n_valid) * 8);
+                *reinterpret_cast<uint4*>(tile + b * AS_BLOCK + n_valid * 128 + at * 16) = make_uint4(0, 0, 0, 0);
+              }
+              fence_proxy_async_smem();
+              __syncwarp();
+              zeroed = n_pv[t] + 1;
+            }
+            if (has_rows(w, t)) {
+              const uint64_t v_desc = make_mnmajor_sw128_desc(v_addr + pv_slot * Cfg::TILE, AS_BLOCK);
 #pragma unroll
-          for (int t = 0; t < 2; ++t)
-            if (ok && pw[t].left > 0) ok = issue_pv(t);
-        } else {
+              for (int k = 0; k < AS_KV / 16; ++k)
+                if (k * 16 < n_eff && elect_one())
+                  tc_mma_f16_tmem_a(tmem_u + Cfg::O(t), tmem_u + Cfg::P(t) + k * 8, v_desc + k * 128, idesc_pv, !w.first || k != 0);
+            }
+            if (elect_one()) {
+              tc_commit(&pv_done[t]);
+              tc_commit(&v_empty[pv_slot]);
+            }
+            ++n_pv[t];
+            w.next(plan, j.n_kv_heads);
+            moved = true;
+          }
+          // S of the next step: its columns are free once the softmax has read the last one (P apart) or P V has read the P that took
+          // their place
+          const uint32_t s_slot = (PAIR ? 0 : t * SLOTS) + n_s[t] % SLOTS;
+          if (sw[t].left > 0 && (Cfg::P_APART || n_pv[t] == n_s[t]) &&
+              __all_sync(0xffffffffu, (n_s[t] == 0 || as_test(Cfg::P_APART ? &s_read[t] : &pv_done[t], (n_s[t] - 1) & 1u)) &&
+                                          as_test(&k_full[s_slot], (n_s[t] / SLOTS) & 1u) &&
+                                          (!sw[t].first || as_test(&q_full[t], q_uses[t] & 1u)))) {
+            AsWalk& w = sw[t];
+            if (w.first) ++q_uses[t];
+            tc_fence_after_sync();
+            const uint32_t idesc = make_idesc_bf16_f32(128, as_round16(w.n_valid()));
+            if (has_rows(w, t)) {
 #pragma unroll
-          for (int t = 0; t < 2; ++t) {
-            if (!ok || pw[t].left <= 0) continue;
-            ok = issue_pv(t);
-            if (ok && sw[t].left > 0) ok = wait_all(&pv_done[t], (n_pv[t] - 1) & 1u) && issue_s(t);
+              for (int k = 0; k < D / 16; ++k) {
+                const uint64_t a = make_kmajor_sw128_desc(q_addr + t * Cfg::TILE + (k / 4) * AS_BLOCK) + 2 * (k % 4);
+                const uint64_t b = make_kmajor_sw128_desc(k_addr + s_slot * Cfg::TILE + (k / 4) * AS_BLOCK) + 2 * (k % 4);
+                if (elect_one()) tc_mma_f16(tmem_u + Cfg::S(t), a, b, idesc, k != 0);
+              }
+            }
+            if (elect_one()) {
+              tc_commit(&s_full[t]);
+              tc_commit(&k_empty[s_slot]);
+              if (w.last()) tc_commit(&q_empty[t]);
+            }
+            ++n_s[t];
+            w.next(plan, j.n_kv_heads);
+            moved = true;
           }
         }
+        ok = patience.go_on(moved);
       }
       if (!ok && lane == 0) atomicExch(plan.status, 7);
     }
@@ -694,15 +744,17 @@ attn_scored_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_cons
     const uint32_t lanes = tmem_base + (static_cast<uint32_t>(wq * 32) << 16);
     uint8_t* stage = stage_s + warp * (16 * 128);
     float* table = table_s + t * AS_TABLE;
-    const int group = j.group, g = row % group, row_tok = row / group;
+    const int group = j.group, group_inv = (65536 + group - 1) / group;  // r / group = r * group_inv >> 16 for r, group <= 128
+    const int row_tok = (row * group_inv) >> 16, g = row - row_tok * group;
     const int my_slot = PAIR ? blockIdx.x : blockIdx.x + t * gridDim.x;
     const int width = 2 * mod.radius + 1;
     const bool staged = MODE == AS_ANY && mod.bias != nullptr && group * width <= AS_TABLE;
     const float scale_log2 = mod.scale * AS_LOG2E, cap_out = mod.cap * AS_LOG2E;
-    // What a row's values are multiplied by to become exponents of 2: plain scores stay as the tensor core gives them, capped ones are
-    // kept as tanh, the others are in log2 units already.
-    const float unit = MODE == AS_PLAIN ? scale_log2 : MODE == AS_CAP ? cap_out : 1.f;
     const float cap_in = mod.cap > 0.f ? mod.scale / mod.cap : 0.f;
+    const float cap_far = mod.cap > 0.f ? fabsf(mod.cap / mod.scale) : 0.f;
+    const float2 scale2 = make_float2(scale_log2, scale_log2);
+    // exponent of a capped score v = scale_log2 * s: cap_out tanh(v / cap_out) = v * tanh_poly(v^2), see as_tanh_near
+    const AsTanh tanh_near(MODE == AS_CAP ? cap_out : 1.f);
     AsWalk w;
     w.start(plan, my_slot);
     uint32_t step = 0, meetings = 0;
@@ -746,7 +798,7 @@ attn_scored_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_cons
           tab_unit = AS_LOG2E;
         }
       }
-      float m_ref = -INFINITY, l_run = 0.f;
+      float ref = 0.f, l_run = 0.f;  // reference (log2 units) and sum of the exponentials against it
       bool first = true, end = false;
       while (!end) {
         const int kv0 = w.key0(), n_valid = w.n_valid(), n_chunks = (as_round16(n_valid) + 31) >> 5;
@@ -756,30 +808,51 @@ attn_scored_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_cons
         if (failed) break;
         tc_fence_after_sync();
         if (active) {
-          if (MODE == AS_ANY) {
-            // any combination: the scores are rewritten where they are, 32 at a time, and the row is then taken as it is
+          // keys that all rows of the warp see need no masks; rows of no token do not count
+          const bool full = mod.docs == nullptr && __all_sync(0xffffffffu, !real || (key_lo <= kv0 && key_hi >= kv0 + AS_KV));
+          auto seen_of = [&](int key) -> uint32_t {
+            uint32_t seen = (as_below(key_hi - key) & ~as_below(key_lo - key)) | as_below(prefix - key);
+            if (mod.docs != nullptr) {
+              // the keys of each document that some row of the warp belongs to
+              const int key_doc = key + lane < kv_len ? __ldg(mod.docs + kv_row0 + key + lane) : -1;
+              uint32_t same = 0, todo = __ballot_sync(0xffffffffu, doc >= 0);
+              while (todo) {
+                const int d = __shfl_sync(0xffffffffu, doc, __ffs(todo) - 1);
+                const uint32_t keys = __ballot_sync(0xffffffffu, key_doc == d);
+                if (doc == d) same = keys;
+                todo &= ~__ballot_sync(0xffffffffu, doc == d);
+              }
+              seen &= same;
+            }
+            return seen;
+          };
+          // The exact maximum (log2 units) of the row's visible scores of this step, 32 keys at a time. With AS_ANY and AS_CAP the
+          // modified and masked scores take the place of the raw ones.
+          auto exact_max = [&]() -> float {
+            float mx = -INFINITY;
 #pragma unroll 1
             for (int q = 0; q < n_chunks; ++q) {
               uint32_t raw[32];
               tmem_ld_32x32b_x32(lanes + Cfg::S(t) + q * 32, raw);
+              const int key = kv0 + q * 32, d0 = key - pos;
+              const uint32_t seen = full ? 0xffffffffu : seen_of(key);
               tmem_ld_wait_for(raw);
               float y[32];
 #pragma unroll
               for (int i = 0; i < 32; ++i) y[i] = __uint_as_float(raw[i]);
-              if (mod.cap > 0.f) {
+              if (MODE == AS_CAP || (MODE == AS_ANY && mod.cap > 0.f)) {
 #pragma unroll
                 for (int i = 0; i < 32; ++i) y[i] = cap_out * as_tanh(y[i] * cap_in);
               } else {
 #pragma unroll
                 for (int i = 0; i < 32; ++i) y[i] *= scale_log2;
               }
-              const int d0 = kv0 + q * 32 - pos;
-              if (mod.slopes != nullptr) {
+              if (MODE == AS_SLOPES || (MODE == AS_ANY && mod.slopes != nullptr)) {
                 const float f = static_cast<float>(d0);
 #pragma unroll
                 for (int i = 0; i < 32; ++i) y[i] = fmaf(-slope, fabsf(f + static_cast<float>(i)), y[i]);
               }
-              if (mod.bias != nullptr) {
+              if (MODE == AS_ANY && mod.bias != nullptr) {
                 if (__all_sync(0xffffffffu, d0 + 31 <= -mod.radius || d0 >= mod.radius)) {
                   const float b = tab[d0 < 0 ? -mod.radius : mod.radius] * tab_unit;
 #pragma unroll
@@ -789,150 +862,178 @@ attn_scored_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_cons
                   for (int i = 0; i < 32; ++i) y[i] = fmaf(tab[min(max(d0 + i, -mod.radius), mod.radius)], tab_unit, y[i]);
                 }
               }
-              uint32_t half[16];
 #pragma unroll
-              for (int i = 0; i < 16; ++i) half[i] = __float_as_uint(y[i]);
-              tmem_st_32x32b_x16(lanes + Cfg::S(t) + q * 32, half);
-#pragma unroll
-              for (int i = 0; i < 16; ++i) half[i] = __float_as_uint(y[16 + i]);
-              tmem_st_32x32b_x16(lanes + Cfg::S(t) + q * 32 + 16, half);
-            }
-            tmem_st_wait();
-          }
-          uint32_t zr[4][32];  // the score row
-          float mx0 = -INFINITY, mx1 = -INFINITY;
-          tmem_ld_32x32b_x32(lanes + Cfg::S(t), zr[0]);
-#pragma unroll
-          for (int q = 0; q < 4; ++q) {
-            if (q < n_chunks) {
-              // the next 32 scores are on their way while these are worked on
-              tmem_ld_wait_for(zr[q]);
-              if (q < 3 && q + 1 < n_chunks) tmem_ld_32x32b_x32(lanes + Cfg::S(t) + q * 32 + 32, zr[q < 3 ? q + 1 : 3]);
-              const int key = kv0 + q * 32;
-              uint32_t seen = (as_below(key_hi - key) & ~as_below(key_lo - key)) | as_below(prefix - key);
-              if (mod.docs != nullptr) {
-                // the keys of each document that some row of the warp belongs to
-                const int key_doc = key + lane < kv_len ? __ldg(mod.docs + kv_row0 + key + lane) : -1;
-                uint32_t same = 0, todo = __ballot_sync(0xffffffffu, doc >= 0);
-                while (todo) {
-                  const int d = __shfl_sync(0xffffffffu, doc, __ffs(todo) - 1);
-                  const uint32_t keys = __ballot_sync(0xffffffffu, key_doc == d);
-                  if (doc == d) same = keys;
-                  todo &= ~__ballot_sync(0xffffffffu, doc == d);
-                }
-                seen &= same;
+              for (int i = 0; i < 32; ++i) {
+                if (!((seen >> i) & 1u)) y[i] = -INFINITY;
+                mx = fmaxf(mx, y[i]);
               }
-              const bool whole = __all_sync(0xffffffffu, seen == 0xffffffffu || !real);  // rows of no token do not count
-              auto pair_of = [&](int i) { return make_float2(__uint_as_float(zr[q][i]), __uint_as_float(zr[q][i + 1])); };
-              auto put = [&](int i, float2 y) {
-                zr[q][i] = __float_as_uint(y.x);
-                zr[q][i + 1] = __float_as_uint(y.y);
-              };
-              if (MODE == AS_SLOPES) {
-                const int d0 = key - pos;
-                const float f = static_cast<float>(d0);
-                if (__all_sync(0xffffffffu, d0 + 31 <= 0 || d0 >= 0)) {
-                  // all 32 keys on one side of the query: the bias is linear in the key
-                  const float rise = d0 < 0 ? slope : -slope;
-                  const float2 scale2 = make_float2(scale_log2, scale_log2), rise2 = make_float2(2.f * rise, 2.f * rise);
-                  float2 bias2 = make_float2(rise * f, rise * (f + 1.f));
+              if (MODE == AS_ANY || MODE == AS_CAP) {
+                uint32_t half[16];
+#pragma unroll
+                for (int i = 0; i < 16; ++i) half[i] = __float_as_uint(y[i]);
+                tmem_st_32x32b_x16(lanes + Cfg::S(t) + q * 32, half);
+#pragma unroll
+                for (int i = 0; i < 16; ++i) half[i] = __float_as_uint(y[16 + i]);
+                tmem_st_32x32b_x16(lanes + Cfg::S(t) + q * 32 + 16, half);
+              }
+            }
+            if (MODE == AS_ANY || MODE == AS_CAP) tmem_st_wait();
+            return mx;
+          };
+          float alpha = 1.f;
+          // The reference moves to the larger of this step's maximum and the logarithm of the sum so far (which may lie far below the
+          // old reference, where that was a bad guess).
+          auto move_to = [&](float mx) {
+            const float so_far = l_run > 0.f ? ref + __log2f(l_run) : -INFINITY;
+            const float m = fmaxf(mx, so_far);
+            if (m == -INFINITY) return;
+            const float a = l_run > 0.f ? as_ex2(ref - m) : l_run;  // nothing summed: 0, and NaN stays NaN
+            alpha *= a;
+            l_run *= a;
+            ref = m;
+          };
+          if (MODE == AS_ANY) {
+            const float mx = exact_max();
+            if (first || mx > ref + AS_LAZY || !(l_run > 0.f)) move_to(mx);
+          }
+          uint32_t pk[4][16];  // the row's probabilities, two to a register
+          float total;
+#pragma unroll 1
+          for (bool again = false;; again = true) {
+            uint32_t zr[2][32], any_seen = full ? 1u : 0u;
+            float2 sum = make_float2(0.f, 0.f);
+            float far = 0.f;
+            tmem_ld_32x32b_x32(lanes + Cfg::S(t), zr[0]);
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+              if (q < n_chunks) {
+                // the next 32 scores are on their way while these are worked on
+                uint32_t(&z)[32] = zr[q & 1];
+                const int key = kv0 + q * 32;
+                uint32_t seen = 0xffffffffu;
+                bool whole = true;
+                if (MODE != AS_ANY && !full) {
+                  seen = seen_of(key);
+                  any_seen |= seen;
+                  whole = __all_sync(0xffffffffu, seen == 0xffffffffu || !real);
+                }
+                tmem_ld_wait_for(z);
+                if (q + 1 < 4 && q + 1 < n_chunks) tmem_ld_32x32b_x32(lanes + Cfg::S(t) + q * 32 + 32, zr[(q + 1) & 1]);
+                auto two = [&](int i) { return make_float2(__uint_as_float(z[i]), __uint_as_float(z[i + 1])); };
+                if ((MODE == AS_PLAIN || MODE == AS_SLOPES) && q == 0 && first && !again) {
+                  // first guess of the reference: these scores, at the bias of the step's nearest key
+                  float m0 = -INFINITY, m1 = -INFINITY;
 #pragma unroll
                   for (int i = 0; i < 32; i += 2) {
-                    put(i, __ffma2_rn(pair_of(i), scale2, bias2));
-                    bias2 = __fadd2_rn(bias2, rise2);
+                    m0 = fmaxf(m0, (seen >> i) & 1u ? __uint_as_float(z[i]) : -INFINITY);
+                    m1 = fmaxf(m1, (seen >> (i + 1)) & 1u ? __uint_as_float(z[i + 1]) : -INFINITY);
                   }
-                } else {
-#pragma unroll
-                  for (int i = 0; i < 32; ++i)
-                    zr[q][i] = __float_as_uint(fmaf(__uint_as_float(zr[q][i]), scale_log2, -slope * fabsf(f + static_cast<float>(i))));
+                  ref = fmaxf(m0, m1) * scale_log2;
+                  if (MODE == AS_SLOPES) ref -= slope * static_cast<float>(max(max(kv0 - pos, pos - (kv0 + n_valid - 1)), 0));
+                  if (ref == -INFINITY) ref = 0.f;  // none of them is visible
                 }
-              }
-              if (MODE == AS_CAP) {
-                // Which way the tanh goes is decided by what is seen alone: columns that no key wrote and rows of no token hold whatever
-                // was there before, and results must not depend on it.
-                const float in = real ? cap_in : 0.f;
-                const float2 in2 = make_float2(in, in);
+                // exponents against the reference
+                float2 e2[16];
+                if (MODE == AS_PLAIN) {
+                  const float2 base2 = make_float2(-ref, -ref);
+#pragma unroll
+                  for (int i = 0; i < 16; ++i) e2[i] = __ffma2_rn(two(2 * i), scale2, base2);
+                } else if (MODE == AS_ANY) {
+                  const float2 base2 = make_float2(-ref, -ref);
+#pragma unroll
+                  for (int i = 0; i < 16; ++i) e2[i] = __fadd2_rn(two(2 * i), base2);
+                } else if (MODE == AS_SLOPES) {
+                  const int d0 = key - pos;
+                  const float f = static_cast<float>(d0);
+                  if (__all_sync(0xffffffffu, d0 + 31 <= 0 || d0 >= 0 || !real)) {
+                    // all 32 keys on one side of the query: the bias is linear in the key
+                    const float rise = d0 < 0 ? slope : -slope;
+                    const float2 rise2 = make_float2(2.f * rise, 2.f * rise);
+                    float2 bias2 = make_float2(fmaf(rise, f, -ref), fmaf(rise, f + 1.f, -ref));
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) {
+                      e2[i] = __ffma2_rn(two(2 * i), scale2, bias2);
+                      bias2 = __fadd2_rn(bias2, rise2);
+                    }
+                  } else {
+#pragma unroll
+                    for (int i = 0; i < 16; ++i)
+                      e2[i] = __ffma2_rn(two(2 * i), scale2, make_float2(fmaf(-slope, fabsf(f + static_cast<float>(2 * i)), -ref),
+                                                                          fmaf(-slope, fabsf(f + static_cast<float>(2 * i + 1)), -ref)));
+                  }
+                } else if (again) {  // rewritten with the tanh that holds everywhere
+#pragma unroll
+                  for (int i = 0; i < 16; ++i) e2[i] = two(2 * i);
+                } else {
+                  float top = 0.f;
+                  if (whole) {
+#pragma unroll
+                    for (int i = 0; i < 32; i += 2) top = as_max3_abs(top, __uint_as_float(z[i]), __uint_as_float(z[i + 1]));
+                  } else {
+                    // what no key wrote must not decide the way the tanh goes
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) top = fmaxf(top, (seen >> i) & 1u ? fabsf(__uint_as_float(z[i])) : 0.f);
+                  }
+                  far = fmaxf(far, top);
+#pragma unroll
+                  for (int i = 0; i < 16; ++i) {
+                    const float2 v = __fmul2_rn(two(2 * i), scale2);
+                    e2[i] = tanh_near(v, __fmul2_rn(v, v));
+                  }
+                }
                 if (!whole) {
 #pragma unroll
-                  for (int i = 0; i < 32; ++i)
-                    if (!((seen >> i) & 1u)) zr[q][i] = 0u;
+                  for (int i = 0; i < 16; ++i) {
+                    if (!((seen >> (2 * i)) & 1u)) e2[i].x = -INFINITY;
+                    if (!((seen >> (2 * i + 1)) & 1u)) e2[i].y = -INFINITY;
+                  }
                 }
-                float2 x2[16], u2[16];
-                float far = 0.f;
 #pragma unroll
                 for (int i = 0; i < 16; ++i) {
-                  x2[i] = __fmul2_rn(pair_of(2 * i), in2);
-                  u2[i] = __fmul2_rn(x2[i], x2[i]);
-                  far = as_max3(far, u2[i].x, u2[i].y);
+                  const float2 p2 = make_float2(as_ex2(e2[i].x), as_ex2(e2[i].y));
+                  sum = __fadd2_rn(sum, p2);
+                  __nv_bfloat162 b = __floats2bfloat162_rn(p2.x, p2.y);
+                  pk[q][i] = *reinterpret_cast<uint32_t*>(&b);
                 }
-                if (__all_sync(0xffffffffu, far <= 1.f)) {
-#pragma unroll
-                  for (int i = 0; i < 16; ++i) put(2 * i, as_tanh_near(x2[i], u2[i]));
-                } else {
-#pragma unroll
-                  for (int i = 0; i < 16; ++i) put(2 * i, make_float2(as_tanh(x2[i].x), as_tanh(x2[i].y)));
-                }
-              }
-              if (!whole) {
-#pragma unroll
-                for (int i = 0; i < 32; ++i)
-                  if (!((seen >> i) & 1u)) zr[q][i] = 0xff800000u;  // -inf
-              }
-#pragma unroll
-              for (int i = 0; i < 32; i += 4) {
-                mx0 = as_max3(mx0, __uint_as_float(zr[q][i]), __uint_as_float(zr[q][i + 1]));
-                mx1 = as_max3(mx1, __uint_as_float(zr[q][i + 2]), __uint_as_float(zr[q][i + 3]));
               }
             }
+            total = sum.x + sum.y;
+            if (MODE == AS_ANY || again) break;
+            if (MODE == AS_CAP) {  // a score beyond the cap, outside the polynomial's range
+              if (!__any_sync(0xffffffffu, real && far > cap_far)) break;
+              exact_max();
+              continue;
+            }
+            const bool bad = real && any_seen != 0u && !(l_run + total >= AS_SUM_LOW && total <= AS_SUM_HIGH);
+            if (!__any_sync(0xffffffffu, bad)) break;
+            const float mx = exact_max();
+            if (bad) move_to(mx);
           }
           if (Cfg::P_APART) {
             tc_fence_before_sync();
             __syncwarp();
             if (lane == 0) mbar_arrive(&s_read[t]);
           }
-          const float mx = fmaxf(mx0, mx1);
+          l_run += total;
           // P of the previous step has been read, O is complete up to it
           if (step > 0 && !mbar_wait(&pv_done[t], (step - 1) & 1u)) failed = true;
           failed = __any_sync(0xffffffffu, failed);
           if (failed) break;
           tc_fence_after_sync();
-          const bool move = mx > m_ref && !((mx - m_ref) * unit <= AS_LAZY);  // also away from -inf
-          if (__any_sync(0xffffffffu, move)) {
-            const float m_new = move ? mx : m_ref;
-            const float alpha = move ? (m_ref == -INFINITY ? 0.f : as_ex2((m_ref - m_new) * unit)) : 1.f;
-            m_ref = m_new;
-            l_run *= alpha;
-            if (!first) {
+          if (!first && __any_sync(0xffffffffu, alpha != 1.f)) {
 #pragma unroll 1
-              for (int c = 0; c < D; c += 16) {
-                uint32_t o[16];
-                tmem_ld_32x32b_x16(lanes + Cfg::O(t) + c, o);
-                tmem_ld_wait_for16(o);
+            for (int c = 0; c < D; c += 16) {
+              uint32_t o[16];
+              tmem_ld_32x32b_x16(lanes + Cfg::O(t) + c, o);
+              tmem_ld_wait_for16(o);
 #pragma unroll
-                for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * alpha);
-                tmem_st_32x32b_x16(lanes + Cfg::O(t) + c, o);
-              }
+              for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * alpha);
+              tmem_st_32x32b_x16(lanes + Cfg::O(t) + c, o);
             }
           }
-          const float base = m_ref == -INFINITY ? 0.f : -m_ref * unit;
-          const float2 unit2 = make_float2(unit, unit), base2 = make_float2(base, base);
-          float2 sum = make_float2(0.f, 0.f);
 #pragma unroll
-          for (int q = 0; q < 4; ++q) {
-            if (q < n_chunks) {
-              uint32_t pk[16];
-#pragma unroll
-              for (int i = 0; i < 32; i += 2) {
-                const float2 x = __ffma2_rn(make_float2(__uint_as_float(zr[q][i]), __uint_as_float(zr[q][i + 1])), unit2, base2);
-                const float2 pp = make_float2(as_ex2(x.x), as_ex2(x.y));
-                sum = __fadd2_rn(sum, pp);
-                __nv_bfloat162 b = __floats2bfloat162_rn(pp.x, pp.y);
-                pk[i >> 1] = *reinterpret_cast<uint32_t*>(&b);
-              }
-              tmem_st_32x32b_x16(lanes + Cfg::P(t) + q * 16, pk);
-            }
-          }
-          l_run += sum.x + sum.y;
+          for (int q = 0; q < 4; ++q)
+            if (q < n_chunks) tmem_st_32x32b_x16(lanes + Cfg::P(t) + q * 16, pk[q]);
           tmem_st_wait();
           tc_fence_before_sync();
           __syncwarp();
@@ -990,7 +1091,7 @@ attn_scored_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_cons
                 const int col = seg * 64 + part * 32 + cc * 8;
                 if (r < n_rows && col < j.head_dim) {
                   const uint4 u = *reinterpret_cast<const uint4*>(stage + rl * 64 + ((cc ^ ((rl >> 1) & 3)) << 4));
-                  const int tk = r / group;
+                  const int tk = (r * group_inv) >> 16;
                   *reinterpret_cast<uint4*>(j.out + static_cast<int64_t>(tok0 + tk) * j.out_stride +
                                             static_cast<int64_t>(seg_h * group + r - tk * group) * j.head_dim + col) = u;
                 }
@@ -1004,10 +1105,11 @@ attn_scored_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_cons
         // its slot (odd index), the others are the head of theirs (even).
         const int64_t id = part_of(my_slot, k_first == 0);
         if (real) {
-          plan.part_ml[id * plan.rows + row] = make_float2(m_ref == -INFINITY ? -INFINITY : m_ref * unit, l_run);
+          plan.part_ml[id * plan.rows + row] = make_float2(ref, l_run);
         }
         if (active) {
-          float* dst = plan.part_o + (id * plan.rows + row) * D;
+          // four columns of all rows lie together: neighbouring lanes write neighbouring 16 bytes
+          float* dst = plan.part_o + (id * (D / 4) * plan.rows + row) * 4;
 #pragma unroll 1
           for (int c = 0; c < D; c += 32) {
             uint32_t ra[32];
@@ -1015,7 +1117,8 @@ attn_scored_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_cons
             tmem_ld_wait_for(ra);
             if (real) {
 #pragma unroll
-              for (int i = 0; i < 32; i += 4) *reinterpret_cast<uint4*>(dst + c + i) = make_uint4(ra[i], ra[i + 1], ra[i + 2], ra[i + 3]);
+              for (int i = 0; i < 32; i += 4)
+                *reinterpret_cast<uint4*>(dst + static_cast<int64_t>((c + i) / 4) * plan.rows * 4) = make_uint4(ra[i], ra[i + 1], ra[i + 2], ra[i + 3]);
             }
           }
         }
@@ -1039,16 +1142,20 @@ attn_scored_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_cons
           __threadfence();
           const int pieces = j.head_dim >> 3;
           for (int i = row; i < n_rows * pieces; i += 128) {
-            const int r = i / pieces, col = (i - r * pieces) * 8;
+            const int piece = i / n_rows, r = i - piece * n_rows, col = piece * 8;
             float top = -INFINITY, l = 0.f, o[8] = {};
-            for (int s = s0; s <= s1; ++s)
-              top = fmaxf(top, __ldcg(&plan.part_ml[part_of(s, s == s0) * plan.rows + r]).x);
             for (int s = s0; s <= s1; ++s) {
-              const int64_t at = part_of(s, s == s0) * plan.rows + r;
-              const float2 ml = __ldcg(&plan.part_ml[at]);
-              const float f = ml.x == -INFINITY ? (ml.y == ml.y ? 0.f : ml.y) : as_ex2(ml.x - top);
-              const float4 x = __ldcg(reinterpret_cast<const float4*>(plan.part_o + at * D + col));
-              const float4 y = __ldcg(reinterpret_cast<const float4*>(plan.part_o + at * D + col + 4));
+              const float2 ml = __ldcg(&plan.part_ml[part_of(s, s == s0) * plan.rows + r]);
+              if (ml.y > 0.f) top = fmaxf(top, ml.x + __log2f(ml.y));  // a reference alone may be far from its sum
+            }
+#pragma unroll 2
+            for (int s = s0; s <= s1; ++s) {
+              const int64_t id2 = part_of(s, s == s0);
+              const float2 ml = __ldcg(&plan.part_ml[id2 * plan.rows + r]);
+              const float f = ml.y > 0.f ? as_ex2(ml.x - top) : ml.y;  // nothing seen: 0, and NaN stays NaN
+              const float* src = plan.part_o + ((id2 * (D / 4) + 2 * piece) * plan.rows + r) * 4;
+              const float4 x = __ldcg(reinterpret_cast<const float4*>(src));
+              const float4 y = __ldcg(reinterpret_cast<const float4*>(src + static_cast<int64_t>(plan.rows) * 4));
               l = fmaf(f, ml.y, l);
               o[0] = fmaf(f, x.x, o[0]);
               o[1] = fmaf(f, x.y, o[1]);
@@ -1068,7 +1175,7 @@ attn_scored_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_cons
             u.z = *reinterpret_cast<uint32_t*>(&p2);
             u.w = *reinterpret_cast<uint32_t*>(&p3);
             if (inv == 0.f) u = make_uint4(0, 0, 0, 0);
-            const int tk = r / group;
+            const int tk = (r * group_inv) >> 16;
             *reinterpret_cast<uint4*>(j.out + static_cast<int64_t>(tok0 + tk) * j.out_stride +
                                       static_cast<int64_t>(seg_h * group + r - tk * group) * j.head_dim + col) = u;
           }
@@ -1264,7 +1371,9 @@ static int as_launch_mode(const AsMaps& m, const AttnJob& j, const AttnMod& mod,
   const bool up = mod.scale > 0.f;  // the plain row maximum is that of the scaled scores
   if (mod.cap == 0.f && mod.slopes == nullptr && mod.bias == nullptr && up) return as_launch<D, PAGED, PAIR, AS_PLAIN>(m, j, mod, plan, sms, s);
   if (mod.cap == 0.f && mod.slopes != nullptr) return as_launch<D, PAGED, PAIR, AS_SLOPES>(m, j, mod, plan, sms, s);
-  if (mod.cap > 0.f && mod.slopes == nullptr && mod.bias == nullptr) return as_launch<D, PAGED, PAIR, AS_CAP>(m, j, mod, plan, sms, s);
+  const float cap = mod.cap * AS_LOG2E;
+  if (cap >= AS_CAP_LOW && cap <= AS_CAP_HIGH && mod.slopes == nullptr && mod.bias == nullptr)
+    return as_launch<D, PAGED, PAIR, AS_CAP>(m, j, mod, plan, sms, s);
   return as_launch<D, PAGED, PAIR, AS_ANY>(m, j, mod, plan, sms, s);
 }
 
