@@ -14,17 +14,16 @@
 // A CTA (one per SM) runs two streams, A and B, each with its own 128-row tile, softmax warpgroup and tensor-memory
 // accumulators, so that one stream's exponentials run under the other's matrix products. With long queries the two streams take
 // neighbouring tiles of the same item row and share every key and value tile ("pair"); otherwise each walks its own part.
-// Per step of a stream:
+// Per step of a stream (128 keys with head_dim up to 64, 64 with more):
 //   S = Q K^T     tcgen05.mma 128 x N x 16 (N = valid keys rounded up to 16), fp32 in tensor memory
 //   softmax       128 threads, one row each, in one pass over the row: a score becomes its exponential against the row's reference
-//                 at once. The reference is a guess (the first 32 scores of the row's first step) and is only replaced, by the exact
-//                 maximum and a second pass, when a step's sum leaves 2^-60 .. 2^60: numerators and denominator share its
+//                 at once. The reference is a guess (from the first 32 scores of the row's first step) and is only replaced, by the
+//                 exact maximum and a second pass, when a sum leaves 2^-60 .. 2^60: numerators and denominator share its
 //                 scale, and fp32 sums and bf16 probabilities keep their relative precision anywhere in between. Capped scores
 //                 lie within +-cap and need no reference at all.
 //   O += P V      P rounded to bf16 (the tensor core's operand type; half a step of 2^-8 per probability) in tensor memory, V as an MN-major
 //                 shared-memory operand
-// Warps: 0-3 softmax A, 4-7 softmax B, 8 loads Q and K, 9 loads V, 10 issues the matrix instructions, 11 idle (it completes the
-// warpgroup whose registers go to the softmax warps).
+// Warps: 0-3 softmax A, 4-7 softmax B, 8 loads Q and K, 9 loads V, 10 issues the matrix instructions.
 #include <cuda.h>
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
@@ -45,12 +44,13 @@ static constexpr int AS_MAX_GROUP = 128;
 static constexpr int64_t AS_ALIGN = 256;
 static constexpr int AS_MAX_CTAS = 160;
 static constexpr int AS_MAX_SLOTS = 2 * AS_MAX_CTAS;
-static constexpr int AS_THREADS = 384;
+static constexpr int AS_SOFTMAX_WARPS = 8, AS_K_WARP = 8, AS_V_WARP = 9, AS_MMA_WARP = 10;
+static constexpr int AS_THREADS = 11 * 32;
 static constexpr int AS_PLAN_THREADS = 1024;
-static constexpr int AS_KV = 128;                  // keys of a step
-static constexpr int AS_BLOCK = 128 * 64 * 2;      // 128 rows x 64 columns, 128-byte swizzle
+static constexpr int AS_STAGE = 16 * 64;           // output staging of a warp: 16 rows of 64 bytes
+static constexpr uint32_t AS_TMEM_COLS = 512;
 static constexpr int AS_PACKED_BOX = 32;           // rows of one copy of a packed key tile: short sequences copy few rows
-static constexpr int AS_TABLE = 2048;              // floats of a stream's staged bias tables
+static constexpr int AS_TABLE = 1024;              // floats of a stream's staged bias tables
 static constexpr float AS_LOG2E = 1.4426950408889634f;
 static constexpr float AS_LAZY = 8.f;              // AS_ANY: the reference moves when a maximum passes it by 2^AS_LAZY
 static constexpr float AS_SUM_LOW = 0x1p-60f, AS_SUM_HIGH = 0x1p60f;  // sums that keep the reference, see above
@@ -85,7 +85,7 @@ struct AttnPlan {  // views into the workspace
   AttnSlot* slot;        // [slots]
   int32_t* counter;      // [2 * slots] finished parts of the item that starts in a slot (PAIR: per stream)
   int32_t* seq_first;    // [n_seqs + 1] first entry of a sequence
-  int2* doc_range;       // [n_tokens / 128 + n_seqs + 1] smallest and largest document of a key tile
+  int2* doc_range;       // [n_tokens / keys of a tile + n_seqs + 1] smallest and largest document of a key tile
   AttnEntry* entry;
   float2* part_ml;       // [2 * slots * streams][rows] maximum (log2 units) and denominator
   float* part_o;         // [...][rows][Dp]
@@ -168,11 +168,11 @@ __device__ int64_t as_block_sum(int64_t v, int64_t* carry, int64_t* scratch) {
   return base + x - v;
 }
 
-// First key tile record of sequence s: (first token / 128) + s never runs into the next sequence's.
-__device__ __forceinline__ int as_doc_base(int first, int s) { return first / AS_KV + s; }
+// First key tile record of sequence s: (first token / kv) + s never runs into the next sequence's.
+__device__ __forceinline__ int as_doc_base(int first, int s, int kv) { return first / kv + s; }
 
 __global__ void __launch_bounds__(AS_PLAN_THREADS, 1)
-attn_plan_kernel(const AttnJob j, const AttnMod mod, const AttnPlan p, int tokens_per_entry, int max_slots) {
+attn_plan_kernel(const AttnJob j, const AttnMod mod, const AttnPlan p, int tokens_per_entry, int max_slots, int kv) {
   __shared__ int64_t scratch[32];
   __shared__ int64_t carry;
   pdl_launch_dependents();
@@ -200,20 +200,20 @@ attn_plan_kernel(const AttnJob j, const AttnMod mod, const AttnPlan p, int token
   if (tid == 0) p.seq_first[j.n_seqs] = n_entries;
   __syncthreads();
   if (mod.docs != nullptr) {
-    // documents of every 128-token tile (tokens of no document left out)
-    const int records = j.n_tokens / AS_KV + j.n_seqs;
+    // documents of every key tile (tokens of no document left out)
+    const int records = j.n_tokens / kv + j.n_seqs;
     for (int i = warp; i < records; i += AS_PLAN_THREADS / 32) {
       int lo = 0, hi = j.n_seqs;
       while (hi - lo > 1) {
         const int mid = (lo + hi) >> 1;
-        if (as_doc_base(as_rows_of(j, mid).x, mid) <= i) lo = mid;
+        if (as_doc_base(as_rows_of(j, mid).x, mid, kv) <= i) lo = mid;
         else hi = mid;
       }
       const int2 r = as_rows_of(j, lo);
-      const int t0 = r.x + (i - as_doc_base(r.x, lo)) * AS_KV;
+      const int t0 = r.x + (i - as_doc_base(r.x, lo, kv)) * kv;
       if (t0 < r.x) continue;  // only where cu_seqlens is not sorted
       int dmin = INT_MAX, dmax = -1;
-      for (int t = t0 + lane; t < min(t0 + AS_KV, r.y); t += 32) {
+      for (int t = t0 + lane; t < min(t0 + kv, r.y); t += 32) {
         const int d = mod.docs[t];
         if (d >= 0) {
           dmin = min(dmin, d);
@@ -254,10 +254,10 @@ attn_plan_kernel(const AttnJob j, const AttnMod mod, const AttnPlan p, int token
         const int n_tok = __shfl_sync(0xffffffffu, x.n_tok, who);
         if (n_tok <= 0) continue;
         const int seq = __shfl_sync(0xffffffffu, x.seq, who), row0 = __shfl_sync(0xffffffffu, x.kv_row0, who);
-        const int tok0 = __shfl_sync(0xffffffffu, x.tok0, who), tiles = (__shfl_sync(0xffffffffu, x.kv_len, who) + AS_KV - 1) / AS_KV;
-        const int2* range = p.doc_range + as_doc_base(row0, seq);
+        const int tok0 = __shfl_sync(0xffffffffu, x.tok0, who), tiles = (__shfl_sync(0xffffffffu, x.kv_len, who) + kv - 1) / kv;
+        const int2* range = p.doc_range + as_doc_base(row0, seq, kv);
         int dmin = INT_MAX, dmax = -1;
-        for (int t = (tok0 - row0) / AS_KV + lane; t <= (tok0 - row0 + n_tok - 1) / AS_KV; t += 32) {
+        for (int t = (tok0 - row0) / kv + lane; t <= (tok0 - row0 + n_tok - 1) / kv; t += 32) {
           dmin = min(dmin, range[t].x);
           dmax = max(dmax, range[t].y);
         }
@@ -287,10 +287,10 @@ attn_plan_kernel(const AttnJob j, const AttnMod mod, const AttnPlan p, int token
       const int p1 = x.pos0 + x.n_tok - 1;
       const int key_lo = static_cast<int>(max(static_cast<int64_t>(x.pos0) - mod.left, int64_t(0)));
       const int key_hi = static_cast<int>(min(static_cast<int64_t>(p1) + mod.right + 1, static_cast<int64_t>(x.kv_len)));
-      int b0 = 0, b1 = 0, f1 = min((x.prefix + AS_KV - 1) / AS_KV, doc_hi);
+      int b0 = 0, b1 = 0, f1 = min((x.prefix + kv - 1) / kv, doc_hi);
       if (key_hi > key_lo) {
-        b0 = max(key_lo / AS_KV, doc_lo);
-        b1 = max(min((key_hi + AS_KV - 1) / AS_KV, doc_hi), b0);
+        b0 = max(key_lo / kv, doc_lo);
+        b1 = max(min((key_hi + kv - 1) / kv, doc_hi), b0);
       }
       const int f0 = min(doc_lo, f1);
       if (b1 == b0) b0 = b1 = f1;  // no window: the prefix alone
@@ -303,7 +303,7 @@ attn_plan_kernel(const AttnJob j, const AttnMod mod, const AttnPlan p, int token
       x.n0 = f1 - f0;
       x.a1 = b0;
       x.n = x.n0 + (b1 - b0);
-      if (mod.slopes != nullptr) x.near = min(max(p1 / AS_KV - b0, 0), max(b1 - b0 - 1, 0));
+      if (mod.slopes != nullptr) x.near = min(max(p1 / kv - b0, 0), max(b1 - b0 - 1, 0));
       if (x.n == 0) {  // nothing visible: one step whose keys are all masked writes the zeros
         x.a0 = x.a1 = 0;
         x.n0 = 0;
@@ -355,28 +355,30 @@ attn_plan_kernel(const AttnJob j, const AttnMod mod, const AttnPlan p, int token
 template <int D>
 struct AsCfg {
   static constexpr int BLOCKS = D / 64;
-  static constexpr int TILE = BLOCKS * AS_BLOCK;
-  static constexpr int RING = D == 64 ? 4 : 2;  // key (and value) tiles in flight
-  static constexpr int STAGE_BYTES = 8 * 16 * 128;
+  // Keys of a step. With head_dim 128 the accumulators take half of tensor memory; steps of 64 keys leave room for two score
+  // buffers a stream, so that the next scores are there before the softmax has finished these.
+  static constexpr int KV = D == 64 ? 128 : 64;
+  static constexpr int Q_BLOCK = 128 * 128, Q_TILE = BLOCKS * Q_BLOCK;     // rows of 64 columns, 128-byte swizzle
+  static constexpr int KV_BLOCK = KV * 128, KV_TILE = BLOCKS * KV_BLOCK;  // 16 KB either way
+  static constexpr int RING = 4;  // key (and value) tiles in flight
+  static constexpr int STAGE_BYTES = AS_SOFTMAX_WARPS * AS_STAGE;
   static constexpr int TABLE_BYTES = 2 * AS_TABLE * 4;
-  static constexpr int BAR_BYTES = 256;
-  static constexpr int SMEM_BYTES = (2 + 2 * RING) * TILE + STAGE_BYTES + TABLE_BYTES + BAR_BYTES + 1024;
-  static constexpr int N_BARS = 4 * RING + 2 * 7;
+  static constexpr int BAR_BYTES = 384;
+  static constexpr int SMEM_BYTES = 2 * Q_TILE + 2 * RING * KV_TILE + STAGE_BYTES + TABLE_BYTES + BAR_BYTES + 1024;
+  static constexpr int N_BARS = 4 * RING + 2 * 10;
   static_assert(N_BARS * 8 + 16 <= BAR_BYTES, "barrier area");
   static_assert(SMEM_BYTES <= 232448, "shared memory");
-  // Tensor memory columns of stream t. With head_dim 64 P has columns of its own, so the next S may be written as soon as this
-  // one has been read; with 128 P takes the place of S and the next S follows the P V that reads it.
-  static constexpr bool P_APART = D == 64;
-  static __host__ __device__ constexpr uint32_t S(int t) { return t * 128; }
+  // Tensor memory of stream t. head_dim 64: one score buffer of 128 columns, P beside it (the next S may be written as soon as
+  // this one has been read). 128: two score buffers of 64 columns, P in the place of its own S.
+  static constexpr int S_BUFS = D == 64 ? 1 : 2;
+  static __host__ __device__ constexpr uint32_t S(int t, int b) { return t * 128 + b * 64; }
   static __host__ __device__ constexpr uint32_t O(int t) { return 256 + t * D; }
-  static __host__ __device__ constexpr uint32_t P(int t) { return P_APART ? 384 + t * 64 : t * 128; }
+  static __host__ __device__ constexpr uint32_t P(int t, int b) { return D == 64 ? 384 + t * 64 : S(t, b); }
+  static constexpr int CHUNKS = KV / 32;
 };
-static constexpr uint32_t AS_TMEM_COLS = 512;
-// Registers: 384 threads are launched with 168 each; the loading and issuing warpgroup gives its share to the two softmax ones.
-static constexpr int AS_REGS_LAUNCH = 168, AS_REGS_SOFTMAX = 208, AS_REGS_OTHER = 88;
-static_assert(2 * AS_REGS_SOFTMAX + AS_REGS_OTHER == 3 * AS_REGS_LAUNCH, "register split");
 
 // The steps of a stream, in order. Every role of the stream walks the same ones.
+template <int KV>
 struct AsWalk {
   int left, e, h, k;  // steps left (this one included); entry, key head, key tile of the item
   bool first;         // first step of a segment (an item, or this stream's part of one)
@@ -401,9 +403,9 @@ struct AsWalk {
   // reference of a row serves all steps; otherwise near is 0 and the run is taken in order.
   __device__ int key0() const {
     const int i = k - f2.y;
-    return (i < 0 ? f2.x + k : f2.z + (i <= f2.w ? f2.w - i : i)) * AS_KV;
+    return (i < 0 ? f2.x + k : f2.z + (i <= f2.w ? f2.w - i : i)) * KV;
   }
-  __device__ int n_valid() const { return min(max(f1.x - key0(), 0), AS_KV); }
+  __device__ int n_valid() const { return min(max(f1.x - key0(), 0), KV); }
   __device__ void next(const AttnPlan& p, int n_kv_heads) {
     first = false;
     if (++k == f1.w) {
@@ -476,7 +478,8 @@ __device__ __forceinline__ void as_drain(uint64_t* full, uint32_t fills, uint32_
 
 // Copies the valid rows of a step's key (or value) tile: lane l takes rows (l % 16) * box_rows .. of the 64-column block l / 16.
 template <int D, bool PAGED>
-__device__ __forceinline__ void as_load_tile(const AttnJob& j, const AsWalk& w, const CUtensorMap* tmap, uint8_t* dst, uint64_t* full, int lane) {
+__device__ __forceinline__ void as_load_tile(const AttnJob& j, const AsWalk<AsCfg<D>::KV>& w, const CUtensorMap* tmap, uint8_t* dst,
+                                             uint64_t* full, int lane) {
   const int n_valid = w.n_valid();
   const int boxes = (n_valid + j.box_rows - 1) / j.box_rows;
   const int r = lane & 15, cb = lane >> 4;
@@ -492,7 +495,7 @@ __device__ __forceinline__ void as_load_tile(const AttnJob& j, const AsWalk& w, 
   if (lane == 0) mbar_arrive_expect_tx(full, boxes * j.box_rows * 128 * AsCfg<D>::BLOCKS);
   __syncwarp();
   if (mine) {
-    uint8_t* to = dst + cb * AS_BLOCK + r * j.box_rows * 128;
+    uint8_t* to = dst + cb * AsCfg<D>::KV_BLOCK + r * j.box_rows * 128;
     if (PAGED) {
       if (j.head_first) as_tma_4d(to, tmap, full, cb * 64, w.h, off, page);
       else as_tma_4d(to, tmap, full, cb * 64, off, w.h, page);
@@ -502,7 +505,7 @@ __device__ __forceinline__ void as_load_tile(const AttnJob& j, const AsWalk& w, 
   }
 }
 
-// What happens to a score before it is masked. The kernel is built for each: a row of 128 scores is worked on in straight-line
+// What happens to a score before it is masked. The kernel is built for each: a row of scores is worked on in straight-line
 // code, and one body with every branch in it is 120 KB of instructions, which the instruction caches do not hold (7 us a step).
 enum { AS_PLAIN = 0, AS_SLOPES = 1, AS_CAP = 2, AS_ANY = 3 };
 
@@ -538,15 +541,15 @@ attn_scored_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_cons
                    const __grid_constant__ CUtensorMap tmap_v, const __grid_constant__ AttnJob j, const __grid_constant__ AttnMod mod,
                    const __grid_constant__ AttnPlan plan) {
   using Cfg = AsCfg<D>;
-  constexpr int RING = Cfg::RING;
+  constexpr int RING = Cfg::RING, KV = Cfg::KV, S_BUFS = Cfg::S_BUFS;
   // A stream's own tiles in flight, so that neither stream waits for the other's; a pair has one ring.
   constexpr uint32_t SLOTS = PAIR ? RING : RING / 2;
   extern __shared__ uint8_t as_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(as_raw) + 1023) & ~uintptr_t(1023));
   uint8_t* q_s = smem;
-  uint8_t* k_s = q_s + 2 * Cfg::TILE;
-  uint8_t* v_s = k_s + RING * Cfg::TILE;
-  uint8_t* stage_s = v_s + RING * Cfg::TILE;
+  uint8_t* k_s = q_s + 2 * Cfg::Q_TILE;
+  uint8_t* v_s = k_s + RING * Cfg::KV_TILE;
+  uint8_t* stage_s = v_s + RING * Cfg::KV_TILE;
   float* table_s = reinterpret_cast<float*>(stage_s + Cfg::STAGE_BYTES);
   uint64_t* k_full = reinterpret_cast<uint64_t*>(stage_s + Cfg::STAGE_BYTES + Cfg::TABLE_BYTES);
   uint64_t* k_empty = k_full + RING;
@@ -554,13 +557,13 @@ attn_scored_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_cons
   uint64_t* v_empty = v_full + RING;
   uint64_t* q_full = v_empty + RING;  // the following ones per stream
   uint64_t* q_empty = q_full + 2;
-  uint64_t* s_full = q_empty + 2;     // S of a step is in tensor memory
-  uint64_t* s_read = s_full + 2;      // P_APART: the softmax warps hold it in registers
-  uint64_t* p_full = s_read + 2;      // P of a step is in tensor memory, O may be added to
-  uint64_t* pv_done = p_full + 2;     // P V of a step has finished
-  uint64_t* group_bar = pv_done + 2;  // the four softmax warps of a stream meet
+  uint64_t* s_full = q_empty + 2;     // [stream][buffer] S of a step is in tensor memory
+  uint64_t* p_full = s_full + 4;      // [stream][buffer] P of a step is in tensor memory, O may be added to
+  uint64_t* pv_done = p_full + 4;     // [stream][buffer] P V of a step has finished
+  uint64_t* s_read = pv_done + 4;     // one score buffer: the softmax warps hold its scores in registers
+  uint64_t* group_bar = s_read + 2;   // the softmax warps of a stream meet
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(group_bar + 2);
-  uint32_t* joins = tmem_slot + 1;    // per stream: this warpgroup joins the parts of the item
+  uint32_t* joins = tmem_slot + 1;                                          // per stream: these warps join the parts of the item
 
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0);
   const int lane = threadIdx.x & 31;
@@ -574,15 +577,17 @@ attn_scored_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_cons
     for (int t = 0; t < 2; ++t) {
       mbar_init(&q_full[t], 1);
       mbar_init(&q_empty[t], 1);
-      mbar_init(&s_full[t], 1);
-      mbar_init(&s_read[t], 4);
-      mbar_init(&p_full[t], 4);
-      mbar_init(&pv_done[t], 1);
-      mbar_init(&group_bar[t], 4);
+      for (int b = 0; b < 2; ++b) {
+        mbar_init(&s_full[2 * t + b], 1);
+        mbar_init(&p_full[2 * t + b], AS_SOFTMAX_WARPS / 2);
+        mbar_init(&pv_done[2 * t + b], 1);
+      }
+      mbar_init(&s_read[t], AS_SOFTMAX_WARPS / 2);
+      mbar_init(&group_bar[t], AS_SOFTMAX_WARPS / 2);
     }
     fence_mbar_init();
   }
-  if (warp == 8) {
+  if (warp == AS_MMA_WARP) {
     tmem_alloc(tmem_slot, AS_TMEM_COLS);
     tmem_relinquish();
   }
@@ -592,157 +597,156 @@ attn_scored_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_cons
   const uint32_t tmem_base = *tmem_slot;
   pdl_wait();  // the plan, and whatever wrote q, k and v
 
-  if (warp >= 8) {
-    setmaxnreg_dec<AS_REGS_OTHER>();
-    if (warp == 8 || warp == 9) {
-      // ---------------- loads: warp 8 Q and K, warp 9 V ----------------
-      const bool is_k = warp == 8;
-      const CUtensorMap* tmap = is_k ? &tmap_k : &tmap_v;
-      uint8_t* ring = is_k ? k_s : v_s;
-      uint64_t* full = is_k ? k_full : v_full;
-      uint64_t* empty = is_k ? k_empty : v_empty;
-      if (lane == 0) {
-        tma_prefetch_desc(tmap);
-        if (is_k) tma_prefetch_desc(&tmap_q);
-      }
-      AsWalk w[2];
-      w[0].start(plan, blockIdx.x);
-      if (PAIR) w[1].left = 0;
-      else w[1].start(plan, blockIdx.x + gridDim.x);
-      uint32_t fills[2] = {0, 0}, q_fills[2] = {0, 0};
-      AsPatience patience;
-      bool ok = true;
-      // whichever stream has room takes its next step
-      while (ok && (w[0].left > 0 || w[1].left > 0)) {
-        bool moved = false;
-#pragma unroll
-        for (int t = 0; t < (PAIR ? 1 : 2); ++t) {
-          if (w[t].left <= 0) continue;
-          const uint32_t slot = t * SLOTS + fills[t] % SLOTS;
-          bool ready = as_test(&empty[slot], ((fills[t] / SLOTS) & 1u) ^ 1u);
-          if (is_k && w[t].first) {
-#pragma unroll
-            for (int u = t; u < (PAIR ? 2 : t + 1); ++u) ready = ready && as_test(&q_empty[u], (q_fills[u] & 1u) ^ 1u);
-          }
-          if (!__all_sync(0xffffffffu, ready)) continue;
-          moved = true;
-          if (is_k && w[t].first) {
-#pragma unroll
-            for (int u = t; u < (PAIR ? 2 : t + 1); ++u) {
-              if (lane == 0) {
-                mbar_arrive_expect_tx(&q_full[u], j.group * j.tile_tokens * 128 * Cfg::BLOCKS);
-#pragma unroll
-                for (int b = 0; b < Cfg::BLOCKS; ++b)
-                  as_tma_3d(q_s + u * Cfg::TILE + b * AS_BLOCK, &tmap_q, &q_full[u], b * 64, w[t].h * j.group,
-                            w[t].f0.y + (PAIR ? u * j.tile_tokens : 0));
-              }
-              ++q_fills[u];
-            }
-          }
-          as_load_tile<D, PAGED>(j, w[t], tmap, ring + slot * Cfg::TILE, &full[slot], lane);
-          ++fills[t];
-          w[t].next(plan, j.n_kv_heads);
-        }
-        ok = patience.go_on(moved);
-      }
-      if (is_k) pdl_launch_dependents();
-      if (!ok) {
-        if (lane == 0) atomicExch(plan.status, is_k ? 5 : 8);
-        for (int t = 0; t < (PAIR ? 1 : 2); ++t) as_drain(&full[t * SLOTS], fills[t], SLOTS);
-        if (is_k)
-          for (int u = 0; u < 2; ++u) as_drain(&q_full[u], q_fills[u], 1);
-      }
-    } else if (warp == 10) {
-      // ---------------- matrix instructions: all lanes walk, one elected lane issues ----------------
-      const uint32_t tmem_u = __shfl_sync(0xffffffffu, tmem_base, 0);
-      const uint32_t q_addr = smem_u32(q_s), k_addr = smem_u32(k_s), v_addr = smem_u32(v_s);
-      AsWalk sw[2], pw[2];  // the next S of each stream, and the next P V
-      sw[0].start(plan, blockIdx.x);
-      sw[1].start(plan, PAIR ? blockIdx.x : blockIdx.x + gridDim.x);
-      pw[0] = sw[0];
-      pw[1] = sw[1];
-      uint32_t q_uses[2] = {0, 0}, n_s[2] = {0, 0}, n_pv[2] = {0, 0}, zeroed = 0;
-      const uint32_t idesc_pv = make_idesc_bf16_f32_b_mn(128, D);
-      // In a pair stream B may have no tokens (the item ends in A's tile): its steps are then only counted.
-      auto has_rows = [&](const AsWalk& w, int t) { return !PAIR || t == 0 || w.f0.z > j.tile_tokens; };
-      AsPatience patience;
-      bool ok = true;
-      // whichever stream's operands are there goes next
-      while (ok && (pw[0].left > 0 || pw[1].left > 0)) {
-        bool moved = false;
-#pragma unroll
-        for (int t = 0; t < 2; ++t) {
-          const uint32_t pv_slot = (PAIR ? 0 : t * SLOTS) + n_pv[t] % SLOTS;
-          if (n_pv[t] < n_s[t] &&
-              __all_sync(0xffffffffu, as_test(&p_full[t], n_pv[t] & 1u) && as_test(&v_full[pv_slot], (n_pv[t] / SLOTS) & 1u))) {
-            AsWalk& w = pw[t];
-            tc_fence_after_sync();
-            const int n_valid = w.n_valid(), n_eff = as_round16(n_valid);
-            if (n_valid < n_eff && (!PAIR || n_pv[t] >= zeroed)) {
-              // value rows behind the last key: whatever lies there must not meet a zero probability (0 * NaN)
-              uint8_t* tile = v_s + pv_slot * Cfg::TILE;
-              for (int i = lane; i < (n_eff - n_valid) * 8 * Cfg::BLOCKS; i += 32) {
-                const int b = i / ((n_eff - n_valid) * 8), at = i - b * ((n_eff - n_valid) * 8);
-                *reinterpret_cast<uint4*>(tile + b * AS_BLOCK + n_valid * 128 + at * 16) = make_uint4(0, 0, 0, 0);
-              }
-              fence_proxy_async_smem();
-              __syncwarp();
-              zeroed = n_pv[t] + 1;
-            }
-            if (has_rows(w, t)) {
-              const uint64_t v_desc = make_mnmajor_sw128_desc(v_addr + pv_slot * Cfg::TILE, AS_BLOCK);
-#pragma unroll
-              for (int k = 0; k < AS_KV / 16; ++k)
-                if (k * 16 < n_eff && elect_one())
-                  tc_mma_f16_tmem_a(tmem_u + Cfg::O(t), tmem_u + Cfg::P(t) + k * 8, v_desc + k * 128, idesc_pv, !w.first || k != 0);
-            }
-            if (elect_one()) {
-              tc_commit(&pv_done[t]);
-              tc_commit(&v_empty[pv_slot]);
-            }
-            ++n_pv[t];
-            w.next(plan, j.n_kv_heads);
-            moved = true;
-          }
-          // S of the next step: its columns are free once the softmax has read the last one (P apart) or P V has read the P that took
-          // their place
-          const uint32_t s_slot = (PAIR ? 0 : t * SLOTS) + n_s[t] % SLOTS;
-          if (sw[t].left > 0 && (Cfg::P_APART || n_pv[t] == n_s[t]) &&
-              __all_sync(0xffffffffu, (n_s[t] == 0 || as_test(Cfg::P_APART ? &s_read[t] : &pv_done[t], (n_s[t] - 1) & 1u)) &&
-                                          as_test(&k_full[s_slot], (n_s[t] / SLOTS) & 1u) &&
-                                          (!sw[t].first || as_test(&q_full[t], q_uses[t] & 1u)))) {
-            AsWalk& w = sw[t];
-            if (w.first) ++q_uses[t];
-            tc_fence_after_sync();
-            const uint32_t idesc = make_idesc_bf16_f32(128, as_round16(w.n_valid()));
-            if (has_rows(w, t)) {
-#pragma unroll
-              for (int k = 0; k < D / 16; ++k) {
-                const uint64_t a = make_kmajor_sw128_desc(q_addr + t * Cfg::TILE + (k / 4) * AS_BLOCK) + 2 * (k % 4);
-                const uint64_t b = make_kmajor_sw128_desc(k_addr + s_slot * Cfg::TILE + (k / 4) * AS_BLOCK) + 2 * (k % 4);
-                if (elect_one()) tc_mma_f16(tmem_u + Cfg::S(t), a, b, idesc, k != 0);
-              }
-            }
-            if (elect_one()) {
-              tc_commit(&s_full[t]);
-              tc_commit(&k_empty[s_slot]);
-              if (w.last()) tc_commit(&q_empty[t]);
-            }
-            ++n_s[t];
-            w.next(plan, j.n_kv_heads);
-            moved = true;
-          }
-        }
-        ok = patience.go_on(moved);
-      }
-      if (!ok && lane == 0) atomicExch(plan.status, 7);
+  if (warp == AS_K_WARP || warp == AS_V_WARP) {
+    // ---------------- loads: Q and K, V ----------------
+    const bool is_k = warp == AS_K_WARP;
+    const CUtensorMap* tmap = is_k ? &tmap_k : &tmap_v;
+    uint8_t* ring = is_k ? k_s : v_s;
+    uint64_t* full = is_k ? k_full : v_full;
+    uint64_t* empty = is_k ? k_empty : v_empty;
+    if (lane == 0) {
+      tma_prefetch_desc(tmap);
+      if (is_k) tma_prefetch_desc(&tmap_q);
     }
+    AsWalk<KV> w[2];
+    w[0].start(plan, blockIdx.x);
+    if (PAIR) w[1].left = 0;
+    else w[1].start(plan, blockIdx.x + gridDim.x);
+    uint32_t fills[2] = {0, 0}, q_fills[2] = {0, 0};
+    AsPatience patience;
+    bool ok = true;
+    // whichever stream has room takes its next step
+    while (ok && (w[0].left > 0 || w[1].left > 0)) {
+      bool moved = false;
+#pragma unroll
+      for (int t = 0; t < (PAIR ? 1 : 2); ++t) {
+        if (w[t].left <= 0) continue;
+        const uint32_t slot = t * SLOTS + fills[t] % SLOTS;
+        bool ready = as_test(&empty[slot], ((fills[t] / SLOTS) & 1u) ^ 1u);
+        if (is_k && w[t].first) {
+#pragma unroll
+          for (int u = t; u < (PAIR ? 2 : t + 1); ++u) ready = ready && as_test(&q_empty[u], (q_fills[u] & 1u) ^ 1u);
+        }
+        if (!__all_sync(0xffffffffu, ready)) continue;
+        moved = true;
+        if (is_k && w[t].first) {
+#pragma unroll
+          for (int u = t; u < (PAIR ? 2 : t + 1); ++u) {
+            if (lane == 0) {
+              mbar_arrive_expect_tx(&q_full[u], j.group * j.tile_tokens * 128 * Cfg::BLOCKS);
+#pragma unroll
+              for (int b = 0; b < Cfg::BLOCKS; ++b)
+                as_tma_3d(q_s + u * Cfg::Q_TILE + b * Cfg::Q_BLOCK, &tmap_q, &q_full[u], b * 64, w[t].h * j.group,
+                          w[t].f0.y + (PAIR ? u * j.tile_tokens : 0));
+            }
+            ++q_fills[u];
+          }
+        }
+        as_load_tile<D, PAGED>(j, w[t], tmap, ring + slot * Cfg::KV_TILE, &full[slot], lane);
+        ++fills[t];
+        w[t].next(plan, j.n_kv_heads);
+      }
+      ok = patience.go_on(moved);
+    }
+    if (is_k) pdl_launch_dependents();
+    if (!ok) {
+      if (lane == 0) atomicExch(plan.status, is_k ? 5 : 8);
+      for (int t = 0; t < (PAIR ? 1 : 2); ++t) as_drain(&full[t * SLOTS], fills[t], SLOTS);
+      if (is_k)
+        for (int u = 0; u < 2; ++u) as_drain(&q_full[u], q_fills[u], 1);
+    }
+  } else if (warp == AS_MMA_WARP) {
+    // ---------------- matrix instructions: all lanes walk, one elected lane issues ----------------
+    const uint32_t tmem_u = __shfl_sync(0xffffffffu, tmem_base, 0);
+    const uint32_t q_addr = smem_u32(q_s), k_addr = smem_u32(k_s), v_addr = smem_u32(v_s);
+    AsWalk<KV> sw[2], pw[2];  // the next S of each stream, and the next P V
+    sw[0].start(plan, blockIdx.x);
+    sw[1].start(plan, PAIR ? blockIdx.x : blockIdx.x + gridDim.x);
+    pw[0] = sw[0];
+    pw[1] = sw[1];
+    uint32_t q_uses[2] = {0, 0}, n_s[2] = {0, 0}, n_pv[2] = {0, 0}, pv_over[2] = {0, 0}, zeroed = 0;
+    const uint32_t idesc_pv = make_idesc_bf16_f32_b_mn(128, D);
+    // In a pair stream B may have no tokens (the item ends in A's tile): its steps are then only counted.
+    auto has_rows = [&](const AsWalk<KV>& w, int t) { return !PAIR || t == 0 || w.f0.z > j.tile_tokens; };
+    AsPatience patience;
+    bool ok = true;
+    // whichever stream's operands are there goes next
+    while (ok && (pw[0].left > 0 || pw[1].left > 0)) {
+      bool moved = false;
+#pragma unroll
+      for (int t = 0; t < 2; ++t) {
+        if (S_BUFS == 2 && pv_over[t] < n_pv[t] && __all_sync(0xffffffffu, as_test(&pv_done[2 * t + pv_over[t] % S_BUFS], (pv_over[t] / S_BUFS) & 1u))) {
+          ++pv_over[t];
+          moved = true;
+        }
+        const uint32_t pv_slot = (PAIR ? 0 : t * SLOTS) + n_pv[t] % SLOTS, pv_buf = n_pv[t] % S_BUFS;
+        if (n_pv[t] < n_s[t] && (S_BUFS == 1 || pv_over[t] == n_pv[t]) &&
+            __all_sync(0xffffffffu, as_test(&p_full[2 * t + pv_buf], (n_pv[t] / S_BUFS) & 1u) && as_test(&v_full[pv_slot], (n_pv[t] / SLOTS) & 1u))) {
+          AsWalk<KV>& w = pw[t];
+          tc_fence_after_sync();
+          const int n_valid = w.n_valid(), n_eff = as_round16(n_valid);
+          if (n_valid < n_eff && (!PAIR || n_pv[t] >= zeroed)) {
+            // value rows behind the last key: whatever lies there must not meet a zero probability (0 * NaN)
+            uint8_t* tile = v_s + pv_slot * Cfg::KV_TILE;
+            for (int i = lane; i < (n_eff - n_valid) * 8 * Cfg::BLOCKS; i += 32) {
+              const int b = i / ((n_eff - n_valid) * 8), at = i - b * ((n_eff - n_valid) * 8);
+              *reinterpret_cast<uint4*>(tile + b * Cfg::KV_BLOCK + n_valid * 128 + at * 16) = make_uint4(0, 0, 0, 0);
+            }
+            fence_proxy_async_smem();
+            __syncwarp();
+            zeroed = n_pv[t] + 1;
+          }
+          if (has_rows(w, t)) {
+            const uint64_t v_desc = make_mnmajor_sw128_desc(v_addr + pv_slot * Cfg::KV_TILE, Cfg::KV_BLOCK);
+#pragma unroll
+            for (int k = 0; k < KV / 16; ++k)
+              if (k * 16 < n_eff && elect_one())
+                tc_mma_f16_tmem_a(tmem_u + Cfg::O(t), tmem_u + Cfg::P(t, pv_buf) + k * 8, v_desc + k * 128, idesc_pv, !w.first || k != 0);
+          }
+          if (elect_one()) {
+            tc_commit(&pv_done[2 * t + pv_buf]);
+            tc_commit(&v_empty[pv_slot]);
+          }
+          ++n_pv[t];
+          w.next(plan, j.n_kv_heads);
+          moved = true;
+        }
+        // S of the next step: its columns are free once the softmax has read the last scores there (one buffer), or P V has read the P
+        // that took their place (two buffers: the step before the last)
+        const uint32_t s_slot = (PAIR ? 0 : t * SLOTS) + n_s[t] % SLOTS, s_buf = n_s[t] % S_BUFS;
+        if (sw[t].left > 0 && (S_BUFS == 1 || n_s[t] < pv_over[t] + 2) &&
+            __all_sync(0xffffffffu, (S_BUFS == 2 || n_s[t] == 0 || as_test(&s_read[t], (n_s[t] - 1) & 1u)) &&
+                                        as_test(&k_full[s_slot], (n_s[t] / SLOTS) & 1u) && (!sw[t].first || as_test(&q_full[t], q_uses[t] & 1u)))) {
+          AsWalk<KV>& w = sw[t];
+          if (w.first) ++q_uses[t];
+          tc_fence_after_sync();
+          const uint32_t idesc = make_idesc_bf16_f32(128, as_round16(w.n_valid()));
+          if (has_rows(w, t)) {
+#pragma unroll
+            for (int k = 0; k < D / 16; ++k) {
+              const uint64_t a = make_kmajor_sw128_desc(q_addr + t * Cfg::Q_TILE + (k / 4) * Cfg::Q_BLOCK) + 2 * (k % 4);
+              const uint64_t b = make_kmajor_sw128_desc(k_addr + s_slot * Cfg::KV_TILE + (k / 4) * Cfg::KV_BLOCK) + 2 * (k % 4);
+              if (elect_one()) tc_mma_f16(tmem_u + Cfg::S(t, s_buf), a, b, idesc, k != 0);
+            }
+          }
+          if (elect_one()) {
+            tc_commit(&s_full[2 * t + s_buf]);
+            tc_commit(&k_empty[s_slot]);
+            if (w.last()) tc_commit(&q_empty[t]);
+          }
+          ++n_s[t];
+          w.next(plan, j.n_kv_heads);
+          moved = true;
+        }
+      }
+      ok = patience.go_on(moved);
+    }
+    if (!ok && lane == 0) atomicExch(plan.status, 7);
   } else {
     // ---------------- softmax: stream t, one row per thread ----------------
-    setmaxnreg_inc<AS_REGS_SOFTMAX>();
     const int t = warp >> 2, wq = warp & 3, row = wq * 32 + lane;
     const uint32_t lanes = tmem_base + (static_cast<uint32_t>(wq * 32) << 16);
-    uint8_t* stage = stage_s + warp * (16 * 128);
+    uint8_t* stage = stage_s + warp * AS_STAGE;
     float* table = table_s + t * AS_TABLE;
     const int group = j.group, group_inv = (65536 + group - 1) / group;  // r / group = r * group_inv >> 16 for r, group <= 128
     const int row_tok = (row * group_inv) >> 16, g = row - row_tok * group;
@@ -753,19 +757,22 @@ attn_scored_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_cons
     const float cap_in = mod.cap > 0.f ? mod.scale / mod.cap : 0.f;
     const float cap_far = mod.cap > 0.f ? fabsf(mod.cap / mod.scale) : 0.f;
     const float2 scale2 = make_float2(scale_log2, scale_log2);
-    // exponent of a capped score v = scale_log2 * s: cap_out tanh(v / cap_out) = v * tanh_poly(v^2), see as_tanh_near
+    // exponent of a capped score v = scale_log2 * s: cap_out tanh(v / cap_out), see AsTanh
     const AsTanh tanh_near(MODE == AS_CAP ? cap_out : 1.f);
-    AsWalk w;
+    AsWalk<KV> w;
     w.start(plan, my_slot);
     uint32_t step = 0, meetings = 0;
     bool failed = false;
-    // Bounded barrier of the stream's four softmax warps: one that gave up elsewhere makes the others give up here.
+    // Bounded barrier of the stream's softmax warps: one that gave up elsewhere makes the others give up here.
     auto meet = [&]() {
       __syncwarp();
       if (lane == 0) mbar_arrive(&group_bar[t]);
       if (!mbar_wait(&group_bar[t], meetings++ & 1u)) failed = true;
       failed = __any_sync(0xffffffffu, failed);
     };
+    // P V of step s, one of the last two. A barrier is told by its parity alone, so each of two score buffers has its own: of the P V
+    // of two steps before, the scores of step s + 1 have already told.
+    auto pv_wait = [&](uint32_t s) { return mbar_wait(&pv_done[2 * t + s % S_BUFS], (s / S_BUFS) & 1u); };
     auto part_of = [&](int slot, bool tail) -> int64_t { return (2 * slot + (tail ? 1 : 0)) * (PAIR ? 2 : 1) + (PAIR ? t : 0); };
     float slope = 0.f;
     const float* tab = nullptr;
@@ -789,7 +796,9 @@ attn_scored_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_cons
       if (MODE == AS_ANY && mod.bias != nullptr) {
         if (staged) {
           meet();  // the previous item's reads are over
-          for (int i = row; i < group * width; i += 128) table[i] = __ldg(mod.bias + static_cast<int64_t>(w.h) * group * width + i) * AS_LOG2E;
+          if (failed) break;
+          for (int i = row; i < group * width; i += 128)
+            table[i] = __ldg(mod.bias + static_cast<int64_t>(w.h) * group * width + i) * AS_LOG2E;
           meet();
           if (failed) break;
           tab = table + g * width + mod.radius;
@@ -798,18 +807,20 @@ attn_scored_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_cons
           tab_unit = AS_LOG2E;
         }
       }
-      float ref = 0.f, l_run = 0.f;  // reference (log2 units) and sum of the exponentials against it
+      float ref = 0.f, l_run = 0.f;  // reference (log2 units), and the sum of the exponentials against it
       bool first = true, end = false;
       while (!end) {
-        const int kv0 = w.key0(), n_valid = w.n_valid(), n_chunks = (as_round16(n_valid) + 31) >> 5;
+        const int kv0 = w.key0(), n_valid = w.n_valid(), buf = step % S_BUFS;
+        const int n_chunks = (as_round16(n_valid) + 31) >> 5;
         end = w.last();
-        if (!mbar_wait(&s_full[t], step & 1u)) failed = true;
+        if (!mbar_wait(&s_full[2 * t + buf], (step / S_BUFS) & 1u)) failed = true;
         failed = __any_sync(0xffffffffu, failed);
         if (failed) break;
         tc_fence_after_sync();
         if (active) {
+          const uint32_t s_at = lanes + Cfg::S(t, buf);
           // keys that all rows of the warp see need no masks; rows of no token do not count
-          const bool full = mod.docs == nullptr && __all_sync(0xffffffffu, !real || (key_lo <= kv0 && key_hi >= kv0 + AS_KV));
+          const bool full = mod.docs == nullptr && __all_sync(0xffffffffu, !real || (key_lo <= kv0 && key_hi >= kv0 + KV));
           auto seen_of = [&](int key) -> uint32_t {
             uint32_t seen = (as_below(key_hi - key) & ~as_below(key_lo - key)) | as_below(prefix - key);
             if (mod.docs != nullptr) {
@@ -826,14 +837,14 @@ attn_scored_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_cons
             }
             return seen;
           };
-          // The exact maximum (log2 units) of the row's visible scores of this step, 32 keys at a time. With AS_ANY and AS_CAP the
+          // The exact maximum (log2 units) of the row's visible scores in this step, 32 keys at a time. With AS_ANY and AS_CAP the
           // modified and masked scores take the place of the raw ones.
           auto exact_max = [&]() -> float {
             float mx = -INFINITY;
 #pragma unroll 1
             for (int q = 0; q < n_chunks; ++q) {
               uint32_t raw[32];
-              tmem_ld_32x32b_x32(lanes + Cfg::S(t) + q * 32, raw);
+              tmem_ld_32x32b_x32(s_at + q * 32, raw);
               const int key = kv0 + q * 32, d0 = key - pos;
               const uint32_t seen = full ? 0xffffffffu : seen_of(key);
               tmem_ld_wait_for(raw);
@@ -871,54 +882,49 @@ attn_scored_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_cons
                 uint32_t half[16];
 #pragma unroll
                 for (int i = 0; i < 16; ++i) half[i] = __float_as_uint(y[i]);
-                tmem_st_32x32b_x16(lanes + Cfg::S(t) + q * 32, half);
+                tmem_st_32x32b_x16(s_at + q * 32, half);
 #pragma unroll
                 for (int i = 0; i < 16; ++i) half[i] = __float_as_uint(y[16 + i]);
-                tmem_st_32x32b_x16(lanes + Cfg::S(t) + q * 32 + 16, half);
+                tmem_st_32x32b_x16(s_at + q * 32 + 16, half);
               }
             }
             if (MODE == AS_ANY || MODE == AS_CAP) tmem_st_wait();
             return mx;
           };
-          float alpha = 1.f;
-          // The reference moves to the larger of this step's maximum and the logarithm of the sum so far (which may lie far below the
-          // old reference, where that was a bad guess).
-          auto move_to = [&](float mx) {
+          float alpha = 1.f, mx = -INFINITY;
+          // The reference moves to the larger of the step's maximum and the logarithm of the sum so far (which lies far below the old
+          // reference where that was a bad guess).
+          auto move_reference = [&]() {
             const float so_far = l_run > 0.f ? ref + __log2f(l_run) : -INFINITY;
             const float m = fmaxf(mx, so_far);
-            if (m == -INFINITY) return;
-            const float a = l_run > 0.f ? as_ex2(ref - m) : l_run;  // nothing summed: 0, and NaN stays NaN
-            alpha *= a;
-            l_run *= a;
-            ref = m;
+            if (m != -INFINITY) {
+              const float a = l_run > 0.f ? as_ex2(ref - m) : l_run;  // nothing summed: 0, and NaN stays NaN
+              alpha *= a;
+              l_run *= a;
+              ref = m;
+            }
           };
-          if (MODE == AS_ANY) {
-            const float mx = exact_max();
-            if (first || mx > ref + AS_LAZY || !(l_run > 0.f)) move_to(mx);
-          }
-          uint32_t pk[4][16];  // the row's probabilities, two to a register
-          float total;
-#pragma unroll 1
-          for (bool again = false;; again = true) {
-            uint32_t zr[2][32], any_seen = full ? 1u : 0u;
+          uint32_t pk[Cfg::CHUNKS][16];  // the row's probabilities, two to a register
+          float total = 0.f, far = 0.f;
+          uint32_t any_seen = 0;
+          bool again = false;
+          auto pass = [&]() {
+            any_seen = full ? 1u : 0u;
             float2 sum = make_float2(0.f, 0.f);
-            float far = 0.f;
-            tmem_ld_32x32b_x32(lanes + Cfg::S(t), zr[0]);
 #pragma unroll
-            for (int q = 0; q < 4; ++q) {
+            for (int q = 0; q < Cfg::CHUNKS; ++q) {
               if (q < n_chunks) {
-                // the next 32 scores are on their way while these are worked on
-                uint32_t(&z)[32] = zr[q & 1];
+                uint32_t z[32];
+                tmem_ld_32x32b_x32(s_at + q * 32, z);
                 const int key = kv0 + q * 32;
                 uint32_t seen = 0xffffffffu;
                 bool whole = true;
-                if (MODE != AS_ANY && !full) {
+                if (!full) {
                   seen = seen_of(key);
                   any_seen |= seen;
                   whole = __all_sync(0xffffffffu, seen == 0xffffffffu || !real);
                 }
                 tmem_ld_wait_for(z);
-                if (q + 1 < 4 && q + 1 < n_chunks) tmem_ld_32x32b_x32(lanes + Cfg::S(t) + q * 32 + 32, zr[(q + 1) & 1]);
                 auto two = [&](int i) { return make_float2(__uint_as_float(z[i]), __uint_as_float(z[i + 1])); };
                 if ((MODE == AS_PLAIN || MODE == AS_SLOPES) && q == 0 && first && !again) {
                   // first guess of the reference: these scores, at the bias of the step's nearest key
@@ -938,7 +944,7 @@ attn_scored_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_cons
                   const float2 base2 = make_float2(-ref, -ref);
 #pragma unroll
                   for (int i = 0; i < 16; ++i) e2[i] = __ffma2_rn(two(2 * i), scale2, base2);
-                } else if (MODE == AS_ANY) {
+                } else if (MODE == AS_ANY || (MODE == AS_CAP && again)) {
                   const float2 base2 = make_float2(-ref, -ref);
 #pragma unroll
                   for (int i = 0; i < 16; ++i) e2[i] = __fadd2_rn(two(2 * i), base2);
@@ -961,9 +967,6 @@ attn_scored_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_cons
                       e2[i] = __ffma2_rn(two(2 * i), scale2, make_float2(fmaf(-slope, fabsf(f + static_cast<float>(2 * i)), -ref),
                                                                           fmaf(-slope, fabsf(f + static_cast<float>(2 * i + 1)), -ref)));
                   }
-                } else if (again) {  // rewritten with the tanh that holds everywhere
-#pragma unroll
-                  for (int i = 0; i < 16; ++i) e2[i] = two(2 * i);
                 } else {
                   float top = 0.f;
                   if (whole) {
@@ -998,29 +1001,40 @@ attn_scored_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_cons
               }
             }
             total = sum.x + sum.y;
+          };
+          if (MODE == AS_ANY) mx = exact_max();
+          if (MODE == AS_ANY && (first || mx > ref + AS_LAZY || !(l_run > 0.f))) move_reference();
+#pragma unroll 1
+          while (true) {
+            pass();
             if (MODE == AS_ANY || again) break;
-            if (MODE == AS_CAP) {  // a score beyond the cap, outside the polynomial's range
+            again = true;
+            if (MODE == AS_CAP) {
+              // a score beyond the cap is outside the polynomial's range: the tanh that holds everywhere, in place
               if (!__any_sync(0xffffffffu, real && far > cap_far)) break;
               exact_max();
-              continue;
+            } else {
+              const bool bad = real && any_seen != 0u && !(l_run + total >= AS_SUM_LOW && total <= AS_SUM_HIGH);
+              if (!__any_sync(0xffffffffu, bad)) break;
+              mx = exact_max();
+              if (bad) move_reference();
             }
-            const bool bad = real && any_seen != 0u && !(l_run + total >= AS_SUM_LOW && total <= AS_SUM_HIGH);
-            if (!__any_sync(0xffffffffu, bad)) break;
-            const float mx = exact_max();
-            if (bad) move_to(mx);
           }
-          if (Cfg::P_APART) {
+          if (S_BUFS == 1) {
             tc_fence_before_sync();
             __syncwarp();
             if (lane == 0) mbar_arrive(&s_read[t]);
           }
           l_run += total;
-          // P of the previous step has been read, O is complete up to it
-          if (step > 0 && !mbar_wait(&pv_done[t], (step - 1) & 1u)) failed = true;
-          failed = __any_sync(0xffffffffu, failed);
-          if (failed) break;
-          tc_fence_after_sync();
-          if (!first && __any_sync(0xffffffffu, alpha != 1.f)) {
+          const bool rescale = !first && __any_sync(0xffffffffu, alpha != 1.f);
+          if (step > 0 && (S_BUFS == 1 || rescale)) {
+            // the previous step's P has been read, O is complete up to it
+            if (!pv_wait(step - 1)) failed = true;
+            failed = __any_sync(0xffffffffu, failed);
+            if (failed) break;
+            tc_fence_after_sync();
+          }
+          if (rescale) {
 #pragma unroll 1
             for (int c = 0; c < D; c += 16) {
               uint32_t o[16];
@@ -1032,21 +1046,23 @@ attn_scored_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_cons
             }
           }
 #pragma unroll
-          for (int q = 0; q < 4; ++q)
-            if (q < n_chunks) tmem_st_32x32b_x16(lanes + Cfg::P(t) + q * 16, pk[q]);
+          for (int q = 0; q < Cfg::CHUNKS; ++q)
+            if (q < n_chunks) tmem_st_32x32b_x16(lanes + Cfg::P(t, buf) + q * 16, pk[q]);
           tmem_st_wait();
           tc_fence_before_sync();
           __syncwarp();
-          if (lane == 0) mbar_arrive(&p_full[t]);
+          if (lane == 0) mbar_arrive(&p_full[2 * t + buf]);
         } else {
           // nothing to compute: arrive in step with the warps that do
-          if (Cfg::P_APART && lane == 0) mbar_arrive(&s_read[t]);
-          if (step > 0 && !mbar_wait(&pv_done[t], (step - 1) & 1u)) failed = true;
-          failed = __any_sync(0xffffffffu, failed);
-          if (failed) break;
+          if (S_BUFS == 1) {
+            if (lane == 0) mbar_arrive(&s_read[t]);
+            if (step > 0 && !pv_wait(step - 1)) failed = true;
+            failed = __any_sync(0xffffffffu, failed);
+            if (failed) break;
+          }
           tc_fence_before_sync();
           __syncwarp();
-          if (lane == 0) mbar_arrive(&p_full[t]);
+          if (lane == 0) mbar_arrive(&p_full[2 * t + buf]);
         }
         first = false;
         ++step;
@@ -1054,7 +1070,7 @@ attn_scored_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_cons
       }
       if (failed) break;
       // ---- the segment's rows ----
-      if (!mbar_wait(&pv_done[t], (step - 1) & 1u)) failed = true;
+      if (!pv_wait(step - 1)) failed = true;
       failed = __any_sync(0xffffffffu, failed);
       if (failed) break;
       tc_fence_after_sync();
@@ -1063,37 +1079,39 @@ attn_scored_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_cons
         if (active) {
           const float inv = l_run == 0.f ? 0.f : 1.f / l_run;
 #pragma unroll 1
-          for (int seg = 0; seg < Cfg::BLOCKS; ++seg) {
-#pragma unroll 1
-            for (int part = 0; part < 2; ++part) {
-              uint32_t ra[32];
-              tmem_ld_32x32b_x32(lanes + Cfg::O(t) + seg * 64 + part * 32, ra);
-              tmem_ld_wait_for(ra);
-              // 32 rows x 32 columns (64 bytes) per pass, 16-byte pieces swizzled by row
+          for (int c = 0; c < D && c < j.head_dim; c += 32) {
+            uint32_t ra[32];
+            tmem_ld_32x32b_x32(lanes + Cfg::O(t) + c, ra);
+            tmem_ld_wait_for(ra);
+            // 32 columns (64 bytes) of 16 rows at a time through shared memory, 16-byte pieces swizzled by row
 #pragma unroll
-              for (int c = 0; c < 4; ++c) {
-                uint4 u;
-                __nv_bfloat162 p0 = __floats2bfloat162_rn(__uint_as_float(ra[8 * c]) * inv, __uint_as_float(ra[8 * c + 1]) * inv);
-                __nv_bfloat162 p1 = __floats2bfloat162_rn(__uint_as_float(ra[8 * c + 2]) * inv, __uint_as_float(ra[8 * c + 3]) * inv);
-                __nv_bfloat162 p2 = __floats2bfloat162_rn(__uint_as_float(ra[8 * c + 4]) * inv, __uint_as_float(ra[8 * c + 5]) * inv);
-                __nv_bfloat162 p3 = __floats2bfloat162_rn(__uint_as_float(ra[8 * c + 6]) * inv, __uint_as_float(ra[8 * c + 7]) * inv);
-                u.x = *reinterpret_cast<uint32_t*>(&p0);
-                u.y = *reinterpret_cast<uint32_t*>(&p1);
-                u.z = *reinterpret_cast<uint32_t*>(&p2);
-                u.w = *reinterpret_cast<uint32_t*>(&p3);
-                if (inv == 0.f) u = make_uint4(0, 0, 0, 0);  // no key seen (the accumulator may hold 0 * NaN)
-                *reinterpret_cast<uint4*>(stage + lane * 64 + ((c ^ ((lane >> 1) & 3)) << 4)) = u;
+            for (int half = 0; half < 2; ++half) {
+              if ((lane >> 4) == half) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                  uint4 x;
+                  __nv_bfloat162 p0 = __floats2bfloat162_rn(__uint_as_float(ra[8 * i]) * inv, __uint_as_float(ra[8 * i + 1]) * inv);
+                  __nv_bfloat162 p1 = __floats2bfloat162_rn(__uint_as_float(ra[8 * i + 2]) * inv, __uint_as_float(ra[8 * i + 3]) * inv);
+                  __nv_bfloat162 p2 = __floats2bfloat162_rn(__uint_as_float(ra[8 * i + 4]) * inv, __uint_as_float(ra[8 * i + 5]) * inv);
+                  __nv_bfloat162 p3 = __floats2bfloat162_rn(__uint_as_float(ra[8 * i + 6]) * inv, __uint_as_float(ra[8 * i + 7]) * inv);
+                  x.x = *reinterpret_cast<uint32_t*>(&p0);
+                  x.y = *reinterpret_cast<uint32_t*>(&p1);
+                  x.z = *reinterpret_cast<uint32_t*>(&p2);
+                  x.w = *reinterpret_cast<uint32_t*>(&p3);
+                  if (inv == 0.f) x = make_uint4(0, 0, 0, 0);  // no key seen (the accumulator may hold 0 * NaN)
+                  *reinterpret_cast<uint4*>(stage + (lane & 15) * 64 + ((i ^ ((lane >> 1) & 3)) << 4)) = x;
+                }
               }
               __syncwarp();
 #pragma unroll
-              for (int i = 0; i < 4; ++i) {
-                const int rl = i * 8 + (lane >> 2), cc = lane & 3, r = wq * 32 + rl;
-                const int col = seg * 64 + part * 32 + cc * 8;
+              for (int i = 0; i < 2; ++i) {
+                const int rl = i * 8 + (lane >> 2), cc = lane & 3, r = wq * 32 + half * 16 + rl;
+                const int col = c + cc * 8;
                 if (r < n_rows && col < j.head_dim) {
-                  const uint4 u = *reinterpret_cast<const uint4*>(stage + rl * 64 + ((cc ^ ((rl >> 1) & 3)) << 4));
+                  const uint4 x = *reinterpret_cast<const uint4*>(stage + rl * 64 + ((cc ^ ((rl >> 1) & 3)) << 4));
                   const int tk = (r * group_inv) >> 16;
                   *reinterpret_cast<uint4*>(j.out + static_cast<int64_t>(tok0 + tk) * j.out_stride +
-                                            static_cast<int64_t>(seg_h * group + r - tk * group) * j.head_dim + col) = u;
+                                            static_cast<int64_t>(seg_h * group + r - tk * group) * j.head_dim + col) = x;
                 }
               }
               __syncwarp();
@@ -1101,17 +1119,15 @@ attn_scored_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_cons
           }
         }
       } else {
-        // A part: numerators, maximum and denominator go to the workspace. Parts of an item: the one that starts it is the tail of
+        // A part: numerators, reference and denominator go to the workspace. Parts of an item: the one that starts it is the tail of
         // its slot (odd index), the others are the head of theirs (even).
         const int64_t id = part_of(my_slot, k_first == 0);
-        if (real) {
-          plan.part_ml[id * plan.rows + row] = make_float2(ref, l_run);
-        }
+        if (real) plan.part_ml[id * plan.rows + row] = make_float2(ref, l_run);
         if (active) {
           // four columns of all rows lie together: neighbouring lanes write neighbouring 16 bytes
           float* dst = plan.part_o + (id * (D / 4) * plan.rows + row) * 4;
 #pragma unroll 1
-          for (int c = 0; c < D; c += 32) {
+          for (int c = 0; c < D && c < j.head_dim; c += 32) {
             uint32_t ra[32];
             tmem_ld_32x32b_x32(lanes + Cfg::O(t) + c, ra);
             tmem_ld_wait_for(ra);
@@ -1167,17 +1183,17 @@ attn_scored_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_cons
               o[7] = fmaf(f, y.w, o[7]);
             }
             const float inv = l == 0.f ? 0.f : 1.f / l;
-            uint4 u;
+            uint4 x;
             __nv_bfloat162 p0 = __floats2bfloat162_rn(o[0] * inv, o[1] * inv), p1 = __floats2bfloat162_rn(o[2] * inv, o[3] * inv);
             __nv_bfloat162 p2 = __floats2bfloat162_rn(o[4] * inv, o[5] * inv), p3 = __floats2bfloat162_rn(o[6] * inv, o[7] * inv);
-            u.x = *reinterpret_cast<uint32_t*>(&p0);
-            u.y = *reinterpret_cast<uint32_t*>(&p1);
-            u.z = *reinterpret_cast<uint32_t*>(&p2);
-            u.w = *reinterpret_cast<uint32_t*>(&p3);
-            if (inv == 0.f) u = make_uint4(0, 0, 0, 0);
+            x.x = *reinterpret_cast<uint32_t*>(&p0);
+            x.y = *reinterpret_cast<uint32_t*>(&p1);
+            x.z = *reinterpret_cast<uint32_t*>(&p2);
+            x.w = *reinterpret_cast<uint32_t*>(&p3);
+            if (inv == 0.f) x = make_uint4(0, 0, 0, 0);
             const int tk = (r * group_inv) >> 16;
             *reinterpret_cast<uint4*>(j.out + static_cast<int64_t>(tok0 + tk) * j.out_stride +
-                                      static_cast<int64_t>(seg_h * group + r - tk * group) * j.head_dim + col) = u;
+                                      static_cast<int64_t>(seg_h * group + r - tk * group) * j.head_dim + col) = x;
           }
         }
         meet();  // joins[t] may be written again
@@ -1189,7 +1205,7 @@ attn_scored_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_cons
 
   tc_fence_before_sync();
   __syncthreads();
-  if (warp == 8) {
+  if (warp == AS_MMA_WARP) {
     tc_fence_after_sync();
     tmem_dealloc(tmem_base, AS_TMEM_COLS);
   }
@@ -1275,7 +1291,7 @@ static int64_t as_layout(void* workspace, int n_seqs, int n_tokens, int n_heads,
   q.slot = reinterpret_cast<AttnSlot*>(take(AS_MAX_SLOTS * sizeof(AttnSlot)));
   q.counter = reinterpret_cast<int32_t*>(take(2 * AS_MAX_SLOTS * sizeof(int32_t)));
   q.seq_first = reinterpret_cast<int32_t*>(take((seqs + 1) * sizeof(int32_t)));
-  q.doc_range = reinterpret_cast<int2*>(take((tokens / AS_KV + seqs + 1) * sizeof(int2)));
+  q.doc_range = reinterpret_cast<int2*>(take((tokens / 64 + seqs + 1) * sizeof(int2)));
   q.entry = reinterpret_cast<AttnEntry*>(take(entries * sizeof(AttnEntry)));
   q.part_ml = reinterpret_cast<float2*>(take(parts * rows * sizeof(float2)));
   q.part_o = reinterpret_cast<float*>(take(parts * rows * dp * sizeof(float)));
@@ -1303,11 +1319,11 @@ template <int D, bool PAGED, bool PAIR, int MODE>
 static int as_launch(const AsMaps& m, const AttnJob& j, const AttnMod& mod, const AttnPlan& plan, int sms, cudaStream_t s) {
   int64_t grid = sms < AS_MAX_CTAS ? sms : AS_MAX_CTAS;
   if (!PAGED) {  // no more CTAs than steps there can be
-    const int64_t steps = static_cast<int64_t>(plan.max_entries) * j.n_kv_heads * ((j.n_tokens + AS_KV - 1) / AS_KV);
+    const int64_t steps = static_cast<int64_t>(plan.max_entries) * j.n_kv_heads * ((j.n_tokens + AsCfg<D>::KV - 1) / AsCfg<D>::KV);
     if (steps < grid) grid = steps;
   }
   const int slots = static_cast<int>(PAIR ? grid : 2 * grid);
-  cudaError_t e = launch_pdl(attn_plan_kernel, dim3(1), dim3(AS_PLAN_THREADS), 0, s, j, mod, plan, (PAIR ? 2 : 1) * j.tile_tokens, slots);
+  cudaError_t e = launch_pdl(attn_plan_kernel, dim3(1), dim3(AS_PLAN_THREADS), 0, s, j, mod, plan, (PAIR ? 2 : 1) * j.tile_tokens, slots, AsCfg<D>::KV);
   if (e == cudaSuccess)
     e = launch_pdl(attn_scored_kernel<D, PAGED, PAIR, MODE>, dim3(static_cast<unsigned>(grid)), dim3(AS_THREADS), AsCfg<D>::SMEM_BYTES, s, m.q, m.k,
                    m.v, j, mod, plan);
@@ -1317,11 +1333,6 @@ static int as_launch(const AsMaps& m, const AttnJob& j, const AttnMod& mod, cons
 
 template <int D, bool PAGED, bool PAIR, int MODE>
 static int as_init_one() {
-  cudaFuncAttributes a;
-  B2_CUDA_CHECK(cudaFuncGetAttributes(&a, attn_scored_kernel<D, PAGED, PAIR, MODE>));
-  // the register split of the kernel draws on exactly this many: with fewer its softmax warps would wait for good
-  if (a.numRegs != AS_REGS_LAUNCH)
-    return set_error(B200EMB_ERR_CUDA, "attention kernel built with %d registers instead of %d", a.numRegs, AS_REGS_LAUNCH);
   B2_CUDA_CHECK(cudaFuncSetAttribute(attn_scored_kernel<D, PAGED, PAIR, MODE>, cudaFuncAttributeMaxDynamicSharedMemorySize, AsCfg<D>::SMEM_BYTES));
   return B200EMB_OK;
 }
@@ -1491,7 +1502,7 @@ extern "C" int b200emb_op_attention_paged(const void* q, int64_t q_row_stride, v
   j.table_stride = cache->table_stride;
   j.head_first = cache->head_stride <= cache->token_stride;
   // rows of one copy: as many as divide both a page and a key tile
-  j.box_rows = AS_KV;
+  j.box_rows = cache->head_dim <= 64 ? AsCfg<64>::KV : AsCfg<128>::KV;
   while (cache->page_size % j.box_rows != 0) j.box_rows >>= 1;
   AsMaps m;
   rc = as_map_rows(&m.q, q, n_tokens, n_heads, cache->head_dim, q_row_stride, j.group, j.tile_tokens);
