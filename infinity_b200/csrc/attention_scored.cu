@@ -52,7 +52,6 @@ static constexpr uint32_t AS_TMEM_COLS = 512;
 static constexpr int AS_PACKED_BOX = 32;           // rows of one copy of a packed key tile: short sequences copy few rows
 static constexpr int AS_TABLE = 1024;              // floats of a stream's staged bias tables
 static constexpr float AS_LOG2E = 1.4426950408889634f;
-static constexpr float AS_LAZY = 8.f;              // AS_ANY: the reference moves when a maximum passes it by 2^AS_LAZY
 static constexpr float AS_SUM_LOW = 0x1p-60f, AS_SUM_HIGH = 0x1p60f;  // sums that keep the reference, see above
 static constexpr float AS_CAP_LOW = 0x1p-7f, AS_CAP_HIGH = 80.f;      // cap * log2(e) that AS_CAP serves: 2^+-80 keeps fp32 sums in range
 
@@ -373,7 +372,8 @@ struct AsCfg {
   static constexpr int S_BUFS = D == 64 ? 1 : 2;
   static __host__ __device__ constexpr uint32_t S(int t, int b) { return t * 128 + b * 64; }
   static __host__ __device__ constexpr uint32_t O(int t) { return 256 + t * D; }
-  static __host__ __device__ constexpr uint32_t P(int t, int b) { return D == 64 ? 384 + t * 64 : S(t, b); }
+  // P of the 32 keys of chunk q: 16 columns, with two score buffers the first of the chunk's own 32
+  static __host__ __device__ constexpr uint32_t P(int t, int b, int q) { return D == 64 ? 384 + t * 64 + q * 16 : S(t, b) + q * 32; }
   static constexpr int CHUNKS = KV / 32;
 };
 
@@ -701,7 +701,7 @@ attn_scored_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_cons
 #pragma unroll
             for (int k = 0; k < KV / 16; ++k)
               if (k * 16 < n_eff && elect_one())
-                tc_mma_f16_tmem_a(tmem_u + Cfg::O(t), tmem_u + Cfg::P(t, pv_buf) + k * 8, v_desc + k * 128, idesc_pv, !w.first || k != 0);
+                tc_mma_f16_tmem_a(tmem_u + Cfg::O(t), tmem_u + Cfg::P(t, pv_buf, k / 2) + (k % 2) * 8, v_desc + k * 128, idesc_pv, !w.first || k != 0);
           }
           if (elect_one()) {
             tc_commit(&pv_done[2 * t + pv_buf]);
@@ -837,33 +837,122 @@ attn_scored_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_cons
             }
             return seen;
           };
-          // The exact maximum (log2 units) of the row's visible scores in this step, 32 keys at a time. With AS_ANY and AS_CAP the
-          // modified and masked scores take the place of the raw ones.
-          auto exact_max = [&]() -> float {
-            float mx = -INFINITY;
+          // O and what this step has already put into P follow a reference that has moved (by whole powers of two: nothing is rounded).
+          auto rescale = [&](float alpha, int q) {
+            if (!__any_sync(0xffffffffu, alpha != 1.f)) return;
+            if (!first) {
+              // the previous step's P has been read, O is complete up to it
+              if (!pv_wait(step - 1)) failed = true;
+              tc_fence_after_sync();
 #pragma unroll 1
-            for (int q = 0; q < n_chunks; ++q) {
-              uint32_t raw[32];
-              tmem_ld_32x32b_x32(s_at + q * 32, raw);
-              const int key = kv0 + q * 32, d0 = key - pos;
-              const uint32_t seen = full ? 0xffffffffu : seen_of(key);
-              tmem_ld_wait_for(raw);
-              float y[32];
+              for (int c = 0; c < D; c += 16) {
+                uint32_t o[16];
+                tmem_ld_32x32b_x16(lanes + Cfg::O(t) + c, o);
+                tmem_ld_wait_for16(o);
 #pragma unroll
-              for (int i = 0; i < 32; ++i) y[i] = __uint_as_float(raw[i]);
-              if (MODE == AS_CAP || (MODE == AS_ANY && mod.cap > 0.f)) {
+                for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * alpha);
+                tmem_st_32x32b_x16(lanes + Cfg::O(t) + c, o);
+              }
+            }
+            tmem_st_wait();
+#pragma unroll 1
+            for (int c = 0; c < q; ++c) {
+              uint32_t o[16];
+              tmem_ld_32x32b_x16(lanes + Cfg::P(t, buf, 0) + c * (Cfg::P(0, 0, 1) - Cfg::P(0, 0, 0)), o);
+              tmem_ld_wait_for16(o);
 #pragma unroll
-                for (int i = 0; i < 32; ++i) y[i] = cap_out * as_tanh(y[i] * cap_in);
+              for (int i = 0; i < 16; ++i) {
+                const float2 x = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&o[i]));
+                const __nv_bfloat162 b = __floats2bfloat162_rn(x.x * alpha, x.y * alpha);
+                o[i] = *reinterpret_cast<const uint32_t*>(&b);
+              }
+              tmem_st_32x32b_x16(lanes + Cfg::P(t, buf, 0) + c * (Cfg::P(0, 0, 1) - Cfg::P(0, 0, 0)), o);
+            }
+            tmem_st_wait();
+          };
+          // 32 scores of the row, z, become probabilities
+          auto chunk = [&](uint32_t(&z)[32], int q) {
+            const int key = kv0 + q * 32;
+            uint32_t seen = 0xffffffffu;
+            bool whole = true;
+            if (!full) {
+              seen = seen_of(key);
+              whole = __all_sync(0xffffffffu, seen == 0xffffffffu || !real);
+            }
+            auto two = [&](int i) { return make_float2(__uint_as_float(z[2 * i]), __uint_as_float(z[2 * i + 1])); };
+            const bool guess = MODE != AS_CAP && first && q == 0;  // the segment's first scores set the reference
+            float raw_max = -INFINITY;
+            if (MODE == AS_SLOPES && guess) {
+#pragma unroll
+              for (int i = 0; i < 32; ++i) raw_max = fmaxf(raw_max, (seen >> i) & 1u ? __uint_as_float(z[i]) * scale_log2 : -INFINITY);
+            }
+            // exponents against the reference
+            float2 e2[16];
+            if (MODE == AS_PLAIN) {
+              const float2 base2 = make_float2(-ref, -ref);
+#pragma unroll
+              for (int i = 0; i < 16; ++i) e2[i] = __ffma2_rn(two(i), scale2, base2);
+            } else if (MODE == AS_SLOPES) {
+              const int d0 = key - pos;
+              const float f = static_cast<float>(d0);
+              if (__all_sync(0xffffffffu, d0 + 31 <= 0 || d0 >= 0 || !real)) {
+                // all 32 keys on one side of the query: the bias is linear in the key
+                const float rise = d0 < 0 ? slope : -slope;
+                const float2 rise2 = make_float2(2.f * rise, 2.f * rise);
+                float2 bias2 = make_float2(fmaf(rise, f, -ref), fmaf(rise, f + 1.f, -ref));
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                  e2[i] = __ffma2_rn(two(i), scale2, bias2);
+                  bias2 = __fadd2_rn(bias2, rise2);
+                }
               } else {
 #pragma unroll
-                for (int i = 0; i < 32; ++i) y[i] *= scale_log2;
+                for (int i = 0; i < 16; ++i)
+                  e2[i] = __ffma2_rn(two(i), scale2, make_float2(fmaf(-slope, fabsf(f + static_cast<float>(2 * i)), -ref),
+                                                                 fmaf(-slope, fabsf(f + static_cast<float>(2 * i + 1)), -ref)));
               }
-              if (MODE == AS_SLOPES || (MODE == AS_ANY && mod.slopes != nullptr)) {
+            } else if (MODE == AS_CAP) {
+              // Which way the tanh goes is decided by what is seen alone: columns that no key wrote and rows of no token hold whatever was
+              // there before, and results must not depend on it.
+              float top = 0.f;
+              if (whole) {
+#pragma unroll
+                for (int i = 0; i < 32; i += 2) top = as_max3_abs(top, __uint_as_float(z[i]), __uint_as_float(z[i + 1]));
+              } else {
+#pragma unroll
+                for (int i = 0; i < 32; ++i) top = fmaxf(top, (seen >> i) & 1u ? fabsf(__uint_as_float(z[i])) : 0.f);
+              }
+              if (__all_sync(0xffffffffu, top <= cap_far || !real)) {
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                  const float2 v = __fmul2_rn(two(i), scale2);
+                  e2[i] = tanh_near(v, __fmul2_rn(v, v));
+                }
+              } else {
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                  const float2 v = two(i);
+                  e2[i] = make_float2(cap_out * as_tanh(v.x * cap_in), cap_out * as_tanh(v.y * cap_in));
+                }
+              }
+            } else {
+              float y[32];
+#pragma unroll
+              for (int i = 0; i < 32; ++i) y[i] = __uint_as_float(z[i]);
+              if (mod.cap > 0.f) {
+#pragma unroll
+                for (int i = 0; i < 32; ++i) y[i] = fmaf(cap_out, as_tanh(y[i] * cap_in), -ref);
+              } else {
+#pragma unroll
+                for (int i = 0; i < 32; ++i) y[i] = fmaf(y[i], scale_log2, -ref);
+              }
+              const int d0 = key - pos;
+              if (mod.slopes != nullptr) {
                 const float f = static_cast<float>(d0);
 #pragma unroll
                 for (int i = 0; i < 32; ++i) y[i] = fmaf(-slope, fabsf(f + static_cast<float>(i)), y[i]);
               }
-              if (MODE == AS_ANY && mod.bias != nullptr) {
+              if (mod.bias != nullptr) {
                 if (__all_sync(0xffffffffu, d0 + 31 <= -mod.radius || d0 >= mod.radius)) {
                   const float b = tab[d0 < 0 ? -mod.radius : mod.radius] * tab_unit;
 #pragma unroll
@@ -874,180 +963,93 @@ attn_scored_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_cons
                 }
               }
 #pragma unroll
-              for (int i = 0; i < 32; ++i) {
-                if (!((seen >> i) & 1u)) y[i] = -INFINITY;
-                mx = fmaxf(mx, y[i]);
-              }
-              if (MODE == AS_ANY || MODE == AS_CAP) {
-                uint32_t half[16];
+              for (int i = 0; i < 16; ++i) e2[i] = make_float2(y[2 * i], y[2 * i + 1]);
+            }
+            if (!whole) {
 #pragma unroll
-                for (int i = 0; i < 16; ++i) half[i] = __float_as_uint(y[i]);
-                tmem_st_32x32b_x16(s_at + q * 32, half);
-#pragma unroll
-                for (int i = 0; i < 16; ++i) half[i] = __float_as_uint(y[16 + i]);
-                tmem_st_32x32b_x16(s_at + q * 32 + 16, half);
+              for (int i = 0; i < 16; ++i) {
+                if (!((seen >> (2 * i)) & 1u)) e2[i].x = -INFINITY;
+                if (!((seen >> (2 * i + 1)) & 1u)) e2[i].y = -INFINITY;
               }
             }
-            if (MODE == AS_ANY || MODE == AS_CAP) tmem_st_wait();
-            return mx;
-          };
-          float alpha = 1.f, mx = -INFINITY;
-          // The reference moves to the larger of the step's maximum and the logarithm of the sum so far (which lies far below the old
-          // reference where that was a bad guess).
-          auto move_reference = [&]() {
-            const float so_far = l_run > 0.f ? ref + __log2f(l_run) : -INFINITY;
-            const float m = fmaxf(mx, so_far);
-            if (m != -INFINITY) {
-              const float a = l_run > 0.f ? as_ex2(ref - m) : l_run;  // nothing summed: 0, and NaN stays NaN
-              alpha *= a;
-              l_run *= a;
-              ref = m;
+            uint32_t pk[16];
+            float total;
+            auto exponentials = [&]() {
+              float2 sum = make_float2(0.f, 0.f), sum1 = make_float2(0.f, 0.f);
+#pragma unroll
+              for (int i = 0; i < 16; i += 2) {
+                const float2 a = make_float2(as_ex2(e2[i].x), as_ex2(e2[i].y)), b = make_float2(as_ex2(e2[i + 1].x), as_ex2(e2[i + 1].y));
+                sum = __fadd2_rn(sum, a);
+                sum1 = __fadd2_rn(sum1, b);
+                const __nv_bfloat162 ha = __floats2bfloat162_rn(a.x, a.y), hb = __floats2bfloat162_rn(b.x, b.y);
+                pk[i] = *reinterpret_cast<const uint32_t*>(&ha);
+                pk[i + 1] = *reinterpret_cast<const uint32_t*>(&hb);
+              }
+              total = (sum.x + sum1.x) + (sum.y + sum1.y);
+            };
+            // The reference moves to the larger of these scores and the logarithm of the sum so far (which lies far below it where the
+            // reference was a bad guess), by a whole number.
+            auto move = [&](float mx) -> float {
+              const float so_far = l_run > 0.f ? __log2f(l_run) : -INFINITY;
+              const float by = ceilf(fmaxf(mx, so_far));
+              if (by == -INFINITY) return 1.f;
+              const float alpha = l_run > 0.f ? as_ex2(-by) : l_run;  // nothing summed: 0, and NaN stays NaN
+              l_run *= alpha;
+              ref += by;
+#pragma unroll
+              for (int i = 0; i < 16; ++i) e2[i] = __fadd2_rn(e2[i], make_float2(-by, -by));
+              return alpha;
+            };
+            auto highest = [&]() -> float {
+              float m0 = -INFINITY, m1 = -INFINITY;
+#pragma unroll
+              for (int i = 0; i < 16; i += 2) {
+                m0 = as_max3(m0, e2[i].x, e2[i].y);
+                m1 = as_max3(m1, e2[i + 1].x, e2[i + 1].y);
+              }
+              return fmaxf(m0, m1);
+            };
+            if (guess) {
+              // with slopes at the bias of the step's nearest key, which later scores will not exceed by much
+              if (MODE == AS_SLOPES) raw_max -= slope * static_cast<float>(max(max(kv0 - pos, pos - (kv0 + n_valid - 1)), 0));
+              move(MODE == AS_SLOPES ? raw_max : highest());
             }
-          };
-          uint32_t pk[Cfg::CHUNKS][16];  // the row's probabilities, two to a register
-          float total = 0.f, far = 0.f;
-          uint32_t any_seen = 0;
-          bool again = false;
-          auto pass = [&]() {
-            any_seen = full ? 1u : 0u;
-            float2 sum = make_float2(0.f, 0.f);
-#pragma unroll
-            for (int q = 0; q < Cfg::CHUNKS; ++q) {
-              if (q < n_chunks) {
-                uint32_t z[32];
-                tmem_ld_32x32b_x32(s_at + q * 32, z);
-                const int key = kv0 + q * 32;
-                uint32_t seen = 0xffffffffu;
-                bool whole = true;
-                if (!full) {
-                  seen = seen_of(key);
-                  any_seen |= seen;
-                  whole = __all_sync(0xffffffffu, seen == 0xffffffffu || !real);
-                }
-                tmem_ld_wait_for(z);
-                auto two = [&](int i) { return make_float2(__uint_as_float(z[i]), __uint_as_float(z[i + 1])); };
-                if ((MODE == AS_PLAIN || MODE == AS_SLOPES) && q == 0 && first && !again) {
-                  // first guess of the reference: these scores, at the bias of the step's nearest key
-                  float m0 = -INFINITY, m1 = -INFINITY;
-#pragma unroll
-                  for (int i = 0; i < 32; i += 2) {
-                    m0 = fmaxf(m0, (seen >> i) & 1u ? __uint_as_float(z[i]) : -INFINITY);
-                    m1 = fmaxf(m1, (seen >> (i + 1)) & 1u ? __uint_as_float(z[i + 1]) : -INFINITY);
-                  }
-                  ref = fmaxf(m0, m1) * scale_log2;
-                  if (MODE == AS_SLOPES) ref -= slope * static_cast<float>(max(max(kv0 - pos, pos - (kv0 + n_valid - 1)), 0));
-                  if (ref == -INFINITY) ref = 0.f;  // none of them is visible
-                }
-                // exponents against the reference
-                float2 e2[16];
-                if (MODE == AS_PLAIN) {
-                  const float2 base2 = make_float2(-ref, -ref);
-#pragma unroll
-                  for (int i = 0; i < 16; ++i) e2[i] = __ffma2_rn(two(2 * i), scale2, base2);
-                } else if (MODE == AS_ANY || (MODE == AS_CAP && again)) {
-                  const float2 base2 = make_float2(-ref, -ref);
-#pragma unroll
-                  for (int i = 0; i < 16; ++i) e2[i] = __fadd2_rn(two(2 * i), base2);
-                } else if (MODE == AS_SLOPES) {
-                  const int d0 = key - pos;
-                  const float f = static_cast<float>(d0);
-                  if (__all_sync(0xffffffffu, d0 + 31 <= 0 || d0 >= 0 || !real)) {
-                    // all 32 keys on one side of the query: the bias is linear in the key
-                    const float rise = d0 < 0 ? slope : -slope;
-                    const float2 rise2 = make_float2(2.f * rise, 2.f * rise);
-                    float2 bias2 = make_float2(fmaf(rise, f, -ref), fmaf(rise, f + 1.f, -ref));
-#pragma unroll
-                    for (int i = 0; i < 16; ++i) {
-                      e2[i] = __ffma2_rn(two(2 * i), scale2, bias2);
-                      bias2 = __fadd2_rn(bias2, rise2);
-                    }
-                  } else {
-#pragma unroll
-                    for (int i = 0; i < 16; ++i)
-                      e2[i] = __ffma2_rn(two(2 * i), scale2, make_float2(fmaf(-slope, fabsf(f + static_cast<float>(2 * i)), -ref),
-                                                                          fmaf(-slope, fabsf(f + static_cast<float>(2 * i + 1)), -ref)));
-                  }
-                } else {
-                  float top = 0.f;
-                  if (whole) {
-#pragma unroll
-                    for (int i = 0; i < 32; i += 2) top = as_max3_abs(top, __uint_as_float(z[i]), __uint_as_float(z[i + 1]));
-                  } else {
-                    // what no key wrote must not decide the way the tanh goes
-#pragma unroll
-                    for (int i = 0; i < 32; ++i) top = fmaxf(top, (seen >> i) & 1u ? fabsf(__uint_as_float(z[i])) : 0.f);
-                  }
-                  far = fmaxf(far, top);
-#pragma unroll
-                  for (int i = 0; i < 16; ++i) {
-                    const float2 v = __fmul2_rn(two(2 * i), scale2);
-                    e2[i] = tanh_near(v, __fmul2_rn(v, v));
-                  }
-                }
-                if (!whole) {
-#pragma unroll
-                  for (int i = 0; i < 16; ++i) {
-                    if (!((seen >> (2 * i)) & 1u)) e2[i].x = -INFINITY;
-                    if (!((seen >> (2 * i + 1)) & 1u)) e2[i].y = -INFINITY;
-                  }
-                }
-#pragma unroll
-                for (int i = 0; i < 16; ++i) {
-                  const float2 p2 = make_float2(as_ex2(e2[i].x), as_ex2(e2[i].y));
-                  sum = __fadd2_rn(sum, p2);
-                  __nv_bfloat162 b = __floats2bfloat162_rn(p2.x, p2.y);
-                  pk[q][i] = *reinterpret_cast<uint32_t*>(&b);
-                }
+            exponentials();
+            if (MODE != AS_CAP) {
+              const bool bad = real && seen != 0u && !(l_run + total >= AS_SUM_LOW && total <= AS_SUM_HIGH);
+              if (__any_sync(0xffffffffu, bad)) {
+                float alpha = 1.f;
+                const float mx = highest();
+                if (bad) alpha = move(mx);
+                rescale(alpha, q);
+                exponentials();
               }
             }
-            total = sum.x + sum.y;
+            l_run += total;
+            if (S_BUFS == 1 && q == 0 && step > 0) {
+              // the previous step's P has been read
+              if (!pv_wait(step - 1)) failed = true;
+              tc_fence_after_sync();
+            }
+            tmem_st_32x32b_x16(lanes + Cfg::P(t, buf, 0) + q * (Cfg::P(0, 0, 1) - Cfg::P(0, 0, 0)), pk);
           };
-          if (MODE == AS_ANY) mx = exact_max();
-          if (MODE == AS_ANY && (first || mx > ref + AS_LAZY || !(l_run > 0.f))) move_reference();
+          uint32_t za[32], zb[32];
+          tmem_ld_32x32b_x32(s_at, za);
 #pragma unroll 1
-          while (true) {
-            pass();
-            if (MODE == AS_ANY || again) break;
-            again = true;
-            if (MODE == AS_CAP) {
-              // a score beyond the cap is outside the polynomial's range: the tanh that holds everywhere, in place
-              if (!__any_sync(0xffffffffu, real && far > cap_far)) break;
-              exact_max();
-            } else {
-              const bool bad = real && any_seen != 0u && !(l_run + total >= AS_SUM_LOW && total <= AS_SUM_HIGH);
-              if (!__any_sync(0xffffffffu, bad)) break;
-              mx = exact_max();
-              if (bad) move_reference();
+          for (int q = 0; q < n_chunks; q += 2) {
+            // the next 32 scores are on their way while these are worked on
+            tmem_ld_wait_for(za);
+            if (q + 1 < n_chunks) tmem_ld_32x32b_x32(s_at + q * 32 + 32, zb);
+            chunk(za, q);
+            if (q + 1 < n_chunks) {
+              tmem_ld_wait_for(zb);
+              if (q + 2 < n_chunks) tmem_ld_32x32b_x32(s_at + q * 32 + 64, za);
+              chunk(zb, q + 1);
             }
           }
-          if (S_BUFS == 1) {
-            tc_fence_before_sync();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&s_read[t]);
-          }
-          l_run += total;
-          const bool rescale = !first && __any_sync(0xffffffffu, alpha != 1.f);
-          if (step > 0 && (S_BUFS == 1 || rescale)) {
-            // the previous step's P has been read, O is complete up to it
-            if (!pv_wait(step - 1)) failed = true;
-            failed = __any_sync(0xffffffffu, failed);
-            if (failed) break;
-            tc_fence_after_sync();
-          }
-          if (rescale) {
-#pragma unroll 1
-            for (int c = 0; c < D; c += 16) {
-              uint32_t o[16];
-              tmem_ld_32x32b_x16(lanes + Cfg::O(t) + c, o);
-              tmem_ld_wait_for16(o);
-#pragma unroll
-              for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * alpha);
-              tmem_st_32x32b_x16(lanes + Cfg::O(t) + c, o);
-            }
-          }
-#pragma unroll
-          for (int q = 0; q < Cfg::CHUNKS; ++q)
-            if (q < n_chunks) tmem_st_32x32b_x16(lanes + Cfg::P(t, buf) + q * 16, pk[q]);
+          failed = __any_sync(0xffffffffu, failed);
+          if (failed) break;
+          if (S_BUFS == 1 && lane == 0) mbar_arrive(&s_read[t]);  // every lane's scores have been waited for
           tmem_st_wait();
           tc_fence_before_sync();
           __syncwarp();
