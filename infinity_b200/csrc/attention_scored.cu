@@ -18,12 +18,12 @@
 //   S = Q K^T     tcgen05.mma 128 x N x 16 (N = valid keys rounded up to 16), fp32 in tensor memory
 //   softmax       128 threads, one row each, in one pass over the row: a score becomes its exponential against the row's reference
 //                 at once. The reference is a guess (from the first 32 scores of the row's first step) and is only replaced, by the
-//                 exact maximum and a second pass, when a sum leaves 2^-60 .. 2^60: numerators and denominator share its
+//                 exact maximum and a second pass, when the sum leaves 2^-60 .. 2^80: numerators and denominator share its
 //                 scale, and fp32 sums and bf16 probabilities keep their relative precision anywhere in between. Capped scores
 //                 lie within +-cap and need no reference at all.
 //   O += P V      P rounded to bf16 (the tensor core's operand type; half a step of 2^-8 per probability) in tensor memory, V as an MN-major
 //                 shared-memory operand
-// Warps: 0-3 softmax A, 4-7 softmax B, 8 loads Q and K, 9 loads V, 10 issues the matrix instructions.
+// Warps: 0-3 softmax A, 4-7 softmax B, 8 loads Q and K, 9 loads V, 10 and 11 issue the matrix instructions of A and B.
 #include <cuda.h>
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
@@ -44,15 +44,16 @@ static constexpr int AS_MAX_GROUP = 128;
 static constexpr int64_t AS_ALIGN = 256;
 static constexpr int AS_MAX_CTAS = 160;
 static constexpr int AS_MAX_SLOTS = 2 * AS_MAX_CTAS;
-static constexpr int AS_SOFTMAX_WARPS = 8, AS_K_WARP = 8, AS_V_WARP = 9, AS_MMA_WARP = 10;
-static constexpr int AS_THREADS = 11 * 32;
+static constexpr int AS_SOFTMAX_WARPS = 8, AS_K_WARP = 8, AS_V_WARP = 9, AS_MMA_WARP = 10;  // and 11: one a stream
+static constexpr int AS_THREADS = 12 * 32;
 static constexpr int AS_PLAN_THREADS = 1024;
 static constexpr int AS_STAGE = 16 * 64;           // output staging of a warp: 16 rows of 64 bytes
 static constexpr uint32_t AS_TMEM_COLS = 512;
+static constexpr int AS_COLD = 12;                 // words of a softmax warp's values that only an item's ends need
 static constexpr int AS_PACKED_BOX = 32;           // rows of one copy of a packed key tile: short sequences copy few rows
 static constexpr int AS_TABLE = 1024;              // floats of a stream's staged bias tables
 static constexpr float AS_LOG2E = 1.4426950408889634f;
-static constexpr float AS_SUM_LOW = 0x1p-60f, AS_SUM_HIGH = 0x1p60f;  // sums that keep the reference, see above
+static constexpr float AS_SUM_LOW = 0x1p-60f, AS_SUM_HIGH = 0x1p80f;  // sums that keep the reference, see above
 static constexpr float AS_CAP_LOW = 0x1p-7f, AS_CAP_HIGH = 80.f;      // cap * log2(e) that AS_CAP serves: 2^+-80 keeps fp32 sums in range
 
 struct AttnMod {
@@ -97,7 +98,7 @@ struct AttnJob {
   const int32_t* cu;
   const int32_t* kv_lens;
   const int32_t* page_table;
-  int n_seqs, n_tokens, n_heads, n_kv_heads, head_dim, group, tile_tokens;
+  int n_seqs, n_tokens, n_heads, n_kv_heads, head_dim, group, group_inv, tile_tokens;  // r / group = r * group_inv >> 16 for r, group <= 128
   int n_pages, page_size, table_stride, box_rows, head_first;
 };
 
@@ -363,7 +364,8 @@ struct AsCfg {
   static constexpr int STAGE_BYTES = AS_SOFTMAX_WARPS * AS_STAGE;
   static constexpr int TABLE_BYTES = 2 * AS_TABLE * 4;
   static constexpr int BAR_BYTES = 384;
-  static constexpr int SMEM_BYTES = 2 * Q_TILE + 2 * RING * KV_TILE + STAGE_BYTES + TABLE_BYTES + BAR_BYTES + 1024;
+  static constexpr int COLD_BYTES = AS_SOFTMAX_WARPS * AS_COLD * 4;
+  static constexpr int SMEM_BYTES = 2 * Q_TILE + 2 * RING * KV_TILE + STAGE_BYTES + TABLE_BYTES + BAR_BYTES + COLD_BYTES + 1024;
   static constexpr int N_BARS = 4 * RING + 2 * 10;
   static_assert(N_BARS * 8 + 16 <= BAR_BYTES, "barrier area");
   static_assert(SMEM_BYTES <= 232448, "shared memory");
@@ -461,6 +463,7 @@ struct AsPatience {
       idle = 0;
       return true;
     }
+    __nanosleep(40);  // leaves the issue slots to the warps that have work
     if ((++idle & 0xffu) != 0u) return true;
     const unsigned long long now = globaltimer_ns();
     if (idle == 0x100u) since = now;
@@ -655,112 +658,113 @@ attn_scored_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_cons
       if (is_k)
         for (int u = 0; u < 2; ++u) as_drain(&q_full[u], q_fills[u], 1);
     }
-  } else if (warp == AS_MMA_WARP) {
-    // ---------------- matrix instructions: all lanes walk, one elected lane issues ----------------
+  } else if (warp >= AS_MMA_WARP) {
+    // ---------------- matrix instructions of stream t: all lanes walk, one elected lane issues ----------------
+    // (a warp for each stream: one warp that looks at both streams' barriers in turn answers each some hundred cycles later)
+    const int t = warp - AS_MMA_WARP;
     const uint32_t tmem_u = __shfl_sync(0xffffffffu, tmem_base, 0);
-    const uint32_t q_addr = smem_u32(q_s), k_addr = smem_u32(k_s), v_addr = smem_u32(v_s);
-    AsWalk<KV> sw[2], pw[2];  // the next S of each stream, and the next P V
-    sw[0].start(plan, blockIdx.x);
-    sw[1].start(plan, PAIR ? blockIdx.x : blockIdx.x + gridDim.x);
-    pw[0] = sw[0];
-    pw[1] = sw[1];
-    uint32_t q_uses[2] = {0, 0}, n_s[2] = {0, 0}, n_pv[2] = {0, 0}, pv_over[2] = {0, 0}, zeroed = 0;
+    const uint32_t q_addr = smem_u32(q_s) + t * Cfg::Q_TILE, k_addr = smem_u32(k_s), v_addr = smem_u32(v_s);
+    const uint32_t ring0 = PAIR ? 0 : t * SLOTS;
+    AsWalk<KV> sw, pw;  // the next S, and the next P V
+    sw.start(plan, PAIR ? blockIdx.x : blockIdx.x + t * gridDim.x);
+    pw = sw;
+    uint32_t q_uses = 0, n_s = 0, n_pv = 0;
     const uint32_t idesc_pv = make_idesc_bf16_f32_b_mn(128, D);
     // In a pair stream B may have no tokens (the item ends in A's tile): its steps are then only counted.
-    auto has_rows = [&](const AsWalk<KV>& w, int t) { return !PAIR || t == 0 || w.f0.z > j.tile_tokens; };
-    AsPatience patience;
-    bool ok = true;
-    // whichever stream's operands are there goes next
-    while (ok && (pw[0].left > 0 || pw[1].left > 0)) {
-      bool moved = false;
+    auto has_rows = [&](const AsWalk<KV>& w) { return !PAIR || t == 0 || w.f0.z > j.tile_tokens; };
+    auto wait_all = [](uint64_t* bar, uint32_t parity) -> bool { return __all_sync(0xffffffffu, mbar_wait(bar, parity)); };
+    auto issue_s = [&]() -> bool {
+      const uint32_t slot = ring0 + n_s % SLOTS, buf = n_s % S_BUFS;
+      if (sw.first && !wait_all(&q_full[t], q_uses++ & 1u)) return false;
+      if (!wait_all(&k_full[slot], (n_s / SLOTS) & 1u)) return false;
+      tc_fence_after_sync();
+      const uint32_t idesc = make_idesc_bf16_f32(128, as_round16(sw.n_valid()));
+      if (has_rows(sw)) {
 #pragma unroll
-      for (int t = 0; t < 2; ++t) {
-        if (S_BUFS == 2 && pv_over[t] < n_pv[t] && __all_sync(0xffffffffu, as_test(&pv_done[2 * t + pv_over[t] % S_BUFS], (pv_over[t] / S_BUFS) & 1u))) {
-          ++pv_over[t];
-          moved = true;
-        }
-        const uint32_t pv_slot = (PAIR ? 0 : t * SLOTS) + n_pv[t] % SLOTS, pv_buf = n_pv[t] % S_BUFS;
-        if (n_pv[t] < n_s[t] && (S_BUFS == 1 || pv_over[t] == n_pv[t]) &&
-            __all_sync(0xffffffffu, as_test(&p_full[2 * t + pv_buf], (n_pv[t] / S_BUFS) & 1u) && as_test(&v_full[pv_slot], (n_pv[t] / SLOTS) & 1u))) {
-          AsWalk<KV>& w = pw[t];
-          tc_fence_after_sync();
-          const int n_valid = w.n_valid(), n_eff = as_round16(n_valid);
-          if (n_valid < n_eff && (!PAIR || n_pv[t] >= zeroed)) {
-            // value rows behind the last key: whatever lies there must not meet a zero probability (0 * NaN)
-            uint8_t* tile = v_s + pv_slot * Cfg::KV_TILE;
-            for (int i = lane; i < (n_eff - n_valid) * 8 * Cfg::BLOCKS; i += 32) {
-              const int b = i / ((n_eff - n_valid) * 8), at = i - b * ((n_eff - n_valid) * 8);
-              *reinterpret_cast<uint4*>(tile + b * Cfg::KV_BLOCK + n_valid * 128 + at * 16) = make_uint4(0, 0, 0, 0);
-            }
-            fence_proxy_async_smem();
-            __syncwarp();
-            zeroed = n_pv[t] + 1;
-          }
-          if (has_rows(w, t)) {
-            const uint64_t v_desc = make_mnmajor_sw128_desc(v_addr + pv_slot * Cfg::KV_TILE, Cfg::KV_BLOCK);
-#pragma unroll
-            for (int k = 0; k < KV / 16; ++k)
-              if (k * 16 < n_eff && elect_one())
-                tc_mma_f16_tmem_a(tmem_u + Cfg::O(t), tmem_u + Cfg::P(t, pv_buf, k / 2) + (k % 2) * 8, v_desc + k * 128, idesc_pv, !w.first || k != 0);
-          }
-          if (elect_one()) {
-            tc_commit(&pv_done[2 * t + pv_buf]);
-            tc_commit(&v_empty[pv_slot]);
-          }
-          ++n_pv[t];
-          w.next(plan, j.n_kv_heads);
-          moved = true;
-        }
-        // S of the next step: its columns are free once the softmax has read the last scores there (one buffer), or P V has read the P
-        // that took their place (two buffers: the step before the last)
-        const uint32_t s_slot = (PAIR ? 0 : t * SLOTS) + n_s[t] % SLOTS, s_buf = n_s[t] % S_BUFS;
-        if (sw[t].left > 0 && (S_BUFS == 1 || n_s[t] < pv_over[t] + 2) &&
-            __all_sync(0xffffffffu, (S_BUFS == 2 || n_s[t] == 0 || as_test(&s_read[t], (n_s[t] - 1) & 1u)) &&
-                                        as_test(&k_full[s_slot], (n_s[t] / SLOTS) & 1u) && (!sw[t].first || as_test(&q_full[t], q_uses[t] & 1u)))) {
-          AsWalk<KV>& w = sw[t];
-          if (w.first) ++q_uses[t];
-          tc_fence_after_sync();
-          const uint32_t idesc = make_idesc_bf16_f32(128, as_round16(w.n_valid()));
-          if (has_rows(w, t)) {
-#pragma unroll
-            for (int k = 0; k < D / 16; ++k) {
-              const uint64_t a = make_kmajor_sw128_desc(q_addr + t * Cfg::Q_TILE + (k / 4) * Cfg::Q_BLOCK) + 2 * (k % 4);
-              const uint64_t b = make_kmajor_sw128_desc(k_addr + s_slot * Cfg::KV_TILE + (k / 4) * Cfg::KV_BLOCK) + 2 * (k % 4);
-              if (elect_one()) tc_mma_f16(tmem_u + Cfg::S(t, s_buf), a, b, idesc, k != 0);
-            }
-          }
-          if (elect_one()) {
-            tc_commit(&s_full[2 * t + s_buf]);
-            tc_commit(&k_empty[s_slot]);
-            if (w.last()) tc_commit(&q_empty[t]);
-          }
-          ++n_s[t];
-          w.next(plan, j.n_kv_heads);
-          moved = true;
+        for (int k = 0; k < D / 16; ++k) {
+          const uint64_t a = make_kmajor_sw128_desc(q_addr + (k / 4) * Cfg::Q_BLOCK) + 2 * (k % 4);
+          const uint64_t b = make_kmajor_sw128_desc(k_addr + slot * Cfg::KV_TILE + (k / 4) * Cfg::KV_BLOCK) + 2 * (k % 4);
+          if (elect_one()) tc_mma_f16(tmem_u + t * (Cfg::S(1, 0) - Cfg::S(0, 0)) + buf * (Cfg::S(0, 1) - Cfg::S(0, 0)), a, b, idesc, k != 0);
         }
       }
-      ok = patience.go_on(moved);
+      if (elect_one()) {
+        tc_commit(&s_full[2 * t + buf]);
+        tc_commit(&k_empty[slot]);
+        if (sw.last()) tc_commit(&q_empty[t]);
+      }
+      ++n_s;
+      sw.next(plan, j.n_kv_heads);
+      return true;
+    };
+    auto issue_pv = [&]() -> bool {
+      const uint32_t slot = ring0 + n_pv % SLOTS, buf = n_pv % S_BUFS;
+      if (!wait_all(&v_full[slot], (n_pv / SLOTS) & 1u)) return false;
+      const int n_valid = pw.n_valid(), n_eff = as_round16(n_valid);
+      if (n_valid < n_eff) {
+        // value rows behind the last key: whatever lies there must not meet a zero probability (0 * NaN). In a pair both warps write
+        // these zeros, each before its own instructions.
+        uint8_t* tile = v_s + slot * Cfg::KV_TILE;
+        for (int i = lane; i < (n_eff - n_valid) * 8 * Cfg::BLOCKS; i += 32) {
+          const int b = i / ((n_eff - n_valid) * 8), at = i - b * ((n_eff - n_valid) * 8);
+          *reinterpret_cast<uint4*>(tile + b * Cfg::KV_BLOCK + n_valid * 128 + at * 16) = make_uint4(0, 0, 0, 0);
+        }
+        fence_proxy_async_smem();
+        __syncwarp();
+      }
+      if (!wait_all(&p_full[2 * t + buf], (n_pv / S_BUFS) & 1u)) return false;
+      tc_fence_after_sync();
+      if (has_rows(pw)) {
+        const uint64_t v_desc = make_mnmajor_sw128_desc(v_addr + slot * Cfg::KV_TILE, Cfg::KV_BLOCK);
+        const uint32_t p_at = tmem_u + t * (Cfg::P(1, 0, 0) - Cfg::P(0, 0, 0)) + buf * (Cfg::P(0, 1, 0) - Cfg::P(0, 0, 0)) + Cfg::P(0, 0, 0);
+#pragma unroll
+        for (int k = 0; k < KV / 16; ++k)
+          if (k * 16 < n_eff && elect_one())
+            tc_mma_f16_tmem_a(tmem_u + Cfg::O(0) + t * (Cfg::O(1) - Cfg::O(0)), p_at + Cfg::P(0, 0, k / 2) - Cfg::P(0, 0, 0) + (k % 2) * 8, v_desc + k * 128,
+                              idesc_pv, !pw.first || k != 0);
+      }
+      if (elect_one()) {
+        tc_commit(&pv_done[2 * t + buf]);
+        tc_commit(&v_empty[slot]);
+      }
+      ++n_pv;
+      pw.next(plan, j.n_kv_heads);
+      return true;
+    };
+    bool ok = true;
+    for (int i = 0; i < S_BUFS; ++i)
+      if (ok && sw.left > 0) ok = issue_s();
+    while (ok && pw.left > 0) {
+      // One score buffer: the next S goes there as soon as the softmax has read it, P V follows. Two: P V reads the P that took the
+      // place of its S, then the S after the next may follow.
+      if (S_BUFS == 1 && sw.left > 0) ok = wait_all(&s_read[t], (n_s - 1) & 1u) && issue_s();
+      if (ok) ok = issue_pv();
+      if (S_BUFS == 2 && ok && sw.left > 0) ok = wait_all(&pv_done[2 * t + (n_pv - 1) % S_BUFS], ((n_pv - 1) / S_BUFS) & 1u) && issue_s();
     }
     if (!ok && lane == 0) atomicExch(plan.status, 7);
   } else {
     // ---------------- softmax: stream t, one row per thread ----------------
+    // Registers are what limits this role: what only the ends of a segment need lies in shared memory in between.
     const int t = warp >> 2, wq = warp & 3, row = wq * 32 + lane;
     const uint32_t lanes = tmem_base + (static_cast<uint32_t>(wq * 32) << 16);
-    uint8_t* stage = stage_s + warp * AS_STAGE;
+    enum { C_LEFT, C_E, C_H, C_K, C_TOK0, C_NTOK, C_KVROW0, C_PREFIX, C_N };
+    volatile int* cold = reinterpret_cast<volatile int*>(smem + Cfg::SMEM_BYTES - 1024 - Cfg::COLD_BYTES) + warp * AS_COLD;
     float* table = table_s + t * AS_TABLE;
-    const int group = j.group, group_inv = (65536 + group - 1) / group;  // r / group = r * group_inv >> 16 for r, group <= 128
-    const int row_tok = (row * group_inv) >> 16, g = row - row_tok * group;
+    const int row_tok = (row * j.group_inv) >> 16, g = row - row_tok * j.group;
     const int my_slot = PAIR ? blockIdx.x : blockIdx.x + t * gridDim.x;
-    const int width = 2 * mod.radius + 1;
-    const bool staged = MODE == AS_ANY && mod.bias != nullptr && group * width <= AS_TABLE;
     const float scale_log2 = mod.scale * AS_LOG2E, cap_out = mod.cap * AS_LOG2E;
     const float cap_in = mod.cap > 0.f ? mod.scale / mod.cap : 0.f;
     const float cap_far = mod.cap > 0.f ? fabsf(mod.cap / mod.scale) : 0.f;
     const float2 scale2 = make_float2(scale_log2, scale_log2);
     // exponent of a capped score v = scale_log2 * s: cap_out tanh(v / cap_out), see AsTanh
     const AsTanh tanh_near(MODE == AS_CAP ? cap_out : 1.f);
-    AsWalk<KV> w;
-    w.start(plan, my_slot);
+    if (lane == 0) {
+      const int4 s = *reinterpret_cast<const int4*>(plan.slot + my_slot);
+      cold[C_E] = s.x;
+      cold[C_H] = s.y;
+      cold[C_K] = s.z;
+      cold[C_LEFT] = s.w;
+    }
+    __syncwarp();
     uint32_t step = 0, meetings = 0;
     bool failed = false;
     // Bounded barrier of the stream's softmax warps: one that gave up elsewhere makes the others give up here.
@@ -777,55 +781,89 @@ attn_scored_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_cons
     float slope = 0.f;
     const float* tab = nullptr;
     float tab_unit = 1.f;
-    while (w.left > 0 && !failed) {
+    while (cold[C_LEFT] > 0 && !failed) {
       // ---- one segment: an item, or this stream's part of one ----
-      const int h = w.h * group + g, k_first = w.k, seg_e = w.e, seg_h = w.h;
-      const int tok0 = w.f0.y + (PAIR ? t * j.tile_tokens : 0);
-      const int n_tok = min(max(w.f0.z - (PAIR ? t * j.tile_tokens : 0), 0), j.tile_tokens);
-      const int n_rows = n_tok * group;
-      const bool active = wq * 32 < n_rows;
-      const bool real = row < n_rows;
-      const int tok = min(tok0 + row_tok, j.n_tokens - 1);
-      const int pos = w.f0.w + (PAIR ? t * j.tile_tokens : 0) + row_tok;
-      const int kv_len = w.f1.x, kv_row0 = w.f1.y, prefix = w.f1.z, n_tiles = w.f1.w;
-      // first and past-the-last visible key of the window of this row
-      const int key_lo = mod.left >= pos ? 0 : pos - mod.left;
-      const int key_hi = mod.right >= kv_len - pos ? kv_len : pos + mod.right + 1;
-      const int doc = mod.docs != nullptr && real ? __ldg(mod.docs + tok) : -1;
-      if ((MODE == AS_SLOPES || MODE == AS_ANY) && mod.slopes != nullptr) slope = __ldg(mod.slopes + h) * AS_LOG2E;
-      if (MODE == AS_ANY && mod.bias != nullptr) {
-        if (staged) {
-          meet();  // the previous item's reads are over
-          if (failed) break;
-          for (int i = row; i < group * width; i += 128)
-            table[i] = __ldg(mod.bias + static_cast<int64_t>(w.h) * group * width + i) * AS_LOG2E;
-          meet();
-          if (failed) break;
-          tab = table + g * width + mod.radius;
-        } else {
-          tab = mod.bias + static_cast<int64_t>(h) * width + mod.radius;
-          tab_unit = AS_LOG2E;
+      int i_k, i_end, run0, run_n0, run1, run_near, kv_len, pos, n_rows;
+      {
+        const int h = cold[C_H];
+        const int4* entry = reinterpret_cast<const int4*>(plan.entry + cold[C_E]);
+        const int4 f0 = entry[0], f1 = entry[1], f2 = entry[2];
+        const int skip = PAIR ? t * j.tile_tokens : 0, n_tok = min(max(f0.z - skip, 0), j.tile_tokens);
+        i_k = cold[C_K];
+        i_end = min(f1.w, i_k + cold[C_LEFT]);
+        run0 = f2.x;
+        run_n0 = f2.y;
+        run1 = f2.z;
+        run_near = f2.w;
+        kv_len = f1.x;
+        pos = f0.w + skip + row_tok;
+        n_rows = n_tok * j.group;
+        __syncwarp();
+        if (lane == 0) {
+          cold[C_TOK0] = f0.y + skip;
+          cold[C_NTOK] = n_tok;
+          cold[C_KVROW0] = f1.y;
+          cold[C_PREFIX] = f1.z;
+          cold[C_N] = f1.w;
+        }
+        __syncwarp();
+        if ((MODE == AS_SLOPES || MODE == AS_ANY) && mod.slopes != nullptr) slope = __ldg(mod.slopes + h * j.group + g) * AS_LOG2E;
+        if (MODE == AS_ANY && mod.bias != nullptr) {
+          const int width = 2 * mod.radius + 1, n = j.group * width;
+          if (n <= AS_TABLE) {
+            meet();  // the previous item's reads are over
+            if (failed) break;
+            for (int i = row; i < n; i += 128) table[i] = __ldg(mod.bias + static_cast<int64_t>(h) * n + i) * AS_LOG2E;
+            meet();
+            if (failed) break;
+            tab = table + g * width + mod.radius;
+          } else {
+            tab = mod.bias + static_cast<int64_t>(h * j.group + g) * width + mod.radius;
+            tab_unit = AS_LOG2E;
+          }
         }
       }
+      const bool active = wq * 32 < n_rows, real = row < n_rows;
+      const int doc = mod.docs != nullptr && real ? __ldg(mod.docs + cold[C_TOK0] + row_tok) : -1;
+      // first and past-the-last visible key of the window of this row
+      auto key_lo = [&]() { return mod.left >= pos ? 0 : pos - mod.left; };
+      auto key_hi = [&]() { return mod.right >= kv_len - pos ? kv_len : pos + mod.right + 1; };
+      // what holds for all rows of the warp (rows of no token do not count)
+      const uint32_t real_rows = __ballot_sync(0xffffffffu, real);
+      const int all_lo = __reduce_max_sync(0xffffffffu, real ? key_lo() : INT_MIN), all_hi = __reduce_min_sync(0xffffffffu, real ? key_hi() : INT_MAX);
+      const int pos_first = __reduce_min_sync(0xffffffffu, real ? pos : INT_MAX), pos_last = __reduce_max_sync(0xffffffffu, real ? pos : INT_MIN);
+      const int one_doc = __reduce_min_sync(0xffffffffu, real ? doc : INT_MAX) == __reduce_max_sync(0xffffffffu, real ? doc : -1)
+                              ? __reduce_max_sync(0xffffffffu, real ? doc : -1) : -1;  // the document of all rows, or -1
+      auto key0_of = [&](int k) {  // as AsWalk::key0
+        const int i = k - run_n0;
+        return (i < 0 ? run0 + k : run1 + (i <= run_near ? run_near - i : i)) * KV;
+      };
       float ref = 0.f, l_run = 0.f;  // reference (log2 units), and the sum of the exponentials against it
-      bool first = true, end = false;
-      while (!end) {
-        const int kv0 = w.key0(), n_valid = w.n_valid(), buf = step % S_BUFS;
-        const int n_chunks = (as_round16(n_valid) + 31) >> 5;
-        end = w.last();
-        if (!mbar_wait(&s_full[2 * t + buf], (step / S_BUFS) & 1u)) failed = true;
-        failed = __any_sync(0xffffffffu, failed);
-        if (failed) break;
+      bool first = true;
+      int kv0 = key0_of(i_k);
+      for (; i_k < i_end; ++i_k) {
+        const int buf = step % S_BUFS, n_valid = min(max(kv_len - kv0, 0), KV), n_rem = as_round16(n_valid);
+        const int next_kv0 = key0_of(i_k + 1);
+        int key_docs[KV / 32];  // documents of the step's keys, lane l's of 32 l' + l
+        if (mod.docs != nullptr) {
+#pragma unroll
+          for (int q = 0; q < KV / 32; ++q) {
+            const int key = kv0 + q * 32 + lane;
+            key_docs[q] = key < kv_len ? __ldg(mod.docs + cold[C_KVROW0] + key) : -1;
+          }
+        }
+        if (!mbar_wait(&s_full[2 * t + buf], (step / S_BUFS) & 1u)) failed = true;  // looked at below, once a step
         tc_fence_after_sync();
         if (active) {
           const uint32_t s_at = lanes + Cfg::S(t, buf);
-          // keys that all rows of the warp see need no masks; rows of no token do not count
-          const bool full = mod.docs == nullptr && __all_sync(0xffffffffu, !real || (key_lo <= kv0 && key_hi >= kv0 + KV));
-          auto seen_of = [&](int key) -> uint32_t {
-            uint32_t seen = (as_below(key_hi - key) & ~as_below(key_lo - key)) | as_below(prefix - key);
+          auto seen_of = [&](int q) -> uint32_t {
+            const int key = kv0 + q * 32;
+            uint32_t seen = (as_below(key_hi() - key) & ~as_below(key_lo() - key)) | as_below(cold[C_PREFIX] - key);
             if (mod.docs != nullptr) {
               // the keys of each document that some row of the warp belongs to
-              const int key_doc = key + lane < kv_len ? __ldg(mod.docs + kv_row0 + key + lane) : -1;
+              int key_doc = key_docs[0];
+#pragma unroll
+              for (int i = 1; i < KV / 32; ++i) key_doc = q == i ? key_docs[i] : key_doc;
               uint32_t same = 0, todo = __ballot_sync(0xffffffffu, doc >= 0);
               while (todo) {
                 const int d = __shfl_sync(0xffffffffu, doc, __ffs(todo) - 1);
@@ -870,182 +908,198 @@ attn_scored_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_cons
             }
             tmem_st_wait();
           };
-          // 32 scores of the row, z, become probabilities
-          auto chunk = [&](uint32_t(&z)[32], int q) {
-            const int key = kv0 + q * 32;
-            uint32_t seen = 0xffffffffu;
-            bool whole = true;
-            if (!full) {
-              seen = seen_of(key);
-              whole = __all_sync(0xffffffffu, seen == 0xffffffffu || !real);
+          // 64 scores of the row become probabilities
+#pragma unroll 1
+          for (int c = 0; c < KV && c < n_rem; c += 64) {
+            const bool both = c + 32 < n_rem;
+            const int key = kv0 + c;
+            bool whole = all_lo <= key && all_hi >= key + 64;  // no masks
+            if (mod.docs != nullptr && whole) {
+              const int q = c / 32;
+              int d0 = key_docs[0], d1 = key_docs[1];
+#pragma unroll
+              for (int i = 2; i < KV / 32; i += 2) {
+                d0 = q == i ? key_docs[i] : d0;
+                d1 = q == i ? key_docs[i + 1] : d1;
+              }
+              whole = one_doc >= 0 && __all_sync(0xffffffffu, d0 == one_doc && d1 == one_doc);
             }
-            auto two = [&](int i) { return make_float2(__uint_as_float(z[2 * i]), __uint_as_float(z[2 * i + 1])); };
-            const bool guess = MODE != AS_CAP && first && q == 0;  // the segment's first scores set the reference
-            float raw_max = -INFINITY;
-            if (MODE == AS_SLOPES && guess) {
-#pragma unroll
-              for (int i = 0; i < 32; ++i) raw_max = fmaxf(raw_max, (seen >> i) & 1u ? __uint_as_float(z[i]) * scale_log2 : -INFINITY);
-            }
-            // exponents against the reference
-            float2 e2[16];
-            if (MODE == AS_PLAIN) {
-              const float2 base2 = make_float2(-ref, -ref);
-#pragma unroll
-              for (int i = 0; i < 16; ++i) e2[i] = __ffma2_rn(two(i), scale2, base2);
-            } else if (MODE == AS_SLOPES) {
-              const int d0 = key - pos;
-              const float f = static_cast<float>(d0);
-              if (__all_sync(0xffffffffu, d0 + 31 <= 0 || d0 >= 0 || !real)) {
-                // all 32 keys on one side of the query: the bias is linear in the key
-                const float rise = d0 < 0 ? slope : -slope;
-                const float2 rise2 = make_float2(2.f * rise, 2.f * rise);
-                float2 bias2 = make_float2(fmaf(rise, f, -ref), fmaf(rise, f + 1.f, -ref));
-#pragma unroll
-                for (int i = 0; i < 16; ++i) {
-                  e2[i] = __ffma2_rn(two(i), scale2, bias2);
-                  bias2 = __fadd2_rn(bias2, rise2);
-                }
-              } else {
-#pragma unroll
-                for (int i = 0; i < 16; ++i)
-                  e2[i] = __ffma2_rn(two(i), scale2, make_float2(fmaf(-slope, fabsf(f + static_cast<float>(2 * i)), -ref),
-                                                                 fmaf(-slope, fabsf(f + static_cast<float>(2 * i + 1)), -ref)));
-              }
-            } else if (MODE == AS_CAP) {
-              // Which way the tanh goes is decided by what is seen alone: columns that no key wrote and rows of no token hold whatever was
-              // there before, and results must not depend on it.
-              float top = 0.f;
-              if (whole) {
-#pragma unroll
-                for (int i = 0; i < 32; i += 2) top = as_max3_abs(top, __uint_as_float(z[i]), __uint_as_float(z[i + 1]));
-              } else {
-#pragma unroll
-                for (int i = 0; i < 32; ++i) top = fmaxf(top, (seen >> i) & 1u ? fabsf(__uint_as_float(z[i])) : 0.f);
-              }
-              if (__all_sync(0xffffffffu, top <= cap_far || !real)) {
-#pragma unroll
-                for (int i = 0; i < 16; ++i) {
-                  const float2 v = __fmul2_rn(two(i), scale2);
-                  e2[i] = tanh_near(v, __fmul2_rn(v, v));
-                }
-              } else {
-#pragma unroll
-                for (int i = 0; i < 16; ++i) {
-                  const float2 v = two(i);
-                  e2[i] = make_float2(cap_out * as_tanh(v.x * cap_in), cap_out * as_tanh(v.y * cap_in));
-                }
-              }
-            } else {
-              float y[32];
-#pragma unroll
-              for (int i = 0; i < 32; ++i) y[i] = __uint_as_float(z[i]);
-              if (mod.cap > 0.f) {
-#pragma unroll
-                for (int i = 0; i < 32; ++i) y[i] = fmaf(cap_out, as_tanh(y[i] * cap_in), -ref);
-              } else {
-#pragma unroll
-                for (int i = 0; i < 32; ++i) y[i] = fmaf(y[i], scale_log2, -ref);
-              }
-              const int d0 = key - pos;
-              if (mod.slopes != nullptr) {
-                const float f = static_cast<float>(d0);
-#pragma unroll
-                for (int i = 0; i < 32; ++i) y[i] = fmaf(-slope, fabsf(f + static_cast<float>(i)), y[i]);
-              }
-              if (mod.bias != nullptr) {
-                if (__all_sync(0xffffffffu, d0 + 31 <= -mod.radius || d0 >= mod.radius)) {
-                  const float b = tab[d0 < 0 ? -mod.radius : mod.radius] * tab_unit;
-#pragma unroll
-                  for (int i = 0; i < 32; ++i) y[i] += b;
-                } else {
-#pragma unroll
-                  for (int i = 0; i < 32; ++i) y[i] = fmaf(tab[min(max(d0 + i, -mod.radius), mod.radius)], tab_unit, y[i]);
-                }
-              }
-#pragma unroll
-              for (int i = 0; i < 16; ++i) e2[i] = make_float2(y[2 * i], y[2 * i + 1]);
-            }
+            uint32_t seen[2] = {0xffffffffu, 0xffffffffu};
             if (!whole) {
+              seen[0] = seen_of(c / 32);
+              seen[1] = both ? seen_of(c / 32 + 1) : 0u;
+            }
+            uint32_t pk[2][16];
+            float total;
+            // Normally once. A row whose sum leaves its range moves its reference, and the scores, still where they were, are taken again.
+            bool moves = MODE != AS_CAP && first && c == 0 && real;  // the segment's first scores set the reference
+            bool again = false;
+#pragma unroll 1
+            while (true) {
+            uint32_t z[2][32];
+            tmem_ld_32x32b_x32(s_at + c, z[0]);
+            if (both) tmem_ld_32x32b_x32(s_at + c + 32, z[1]);
+            const bool guess = MODE != AS_CAP && first && c == 0 && !again;
+            tmem_ld_wait_for(z[0]);
+            tmem_ld_wait_for(z[1]);
+            float2 e2[2][16];  // exponents against the reference
+            float raw_max = -INFINITY;
 #pragma unroll
-              for (int i = 0; i < 16; ++i) {
-                if (!((seen >> (2 * i)) & 1u)) e2[i].x = -INFINITY;
-                if (!((seen >> (2 * i + 1)) & 1u)) e2[i].y = -INFINITY;
+            for (int g2 = 0; g2 < 2; ++g2) {
+              if (g2 == 0 || both) {
+                const int key32 = key + g2 * 32;
+                auto two = [&](int i) { return make_float2(__uint_as_float(z[g2][2 * i]), __uint_as_float(z[g2][2 * i + 1])); };
+                if (MODE == AS_SLOPES && guess) {
+#pragma unroll
+                  for (int i = 0; i < 32; ++i) raw_max = fmaxf(raw_max, (seen[g2] >> i) & 1u ? __uint_as_float(z[g2][i]) * scale_log2 : -INFINITY);
+                }
+                if (MODE == AS_PLAIN) {
+                  const float2 base2 = make_float2(-ref, -ref);
+#pragma unroll
+                  for (int i = 0; i < 16; ++i) e2[g2][i] = __ffma2_rn(two(i), scale2, base2);
+                } else if (MODE == AS_SLOPES) {
+                  const float f = static_cast<float>(key32 - pos);
+                  if (key32 + 31 <= pos_first || key32 >= pos_last) {
+                    // all 32 keys on one side of the queries: the bias is linear in the key
+                    const float rise = key32 < pos_last ? slope : -slope;
+                    const float2 rise2 = make_float2(2.f * rise, 2.f * rise);
+                    float2 bias2 = make_float2(fmaf(rise, f, -ref), fmaf(rise, f + 1.f, -ref));
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) {
+                      e2[g2][i] = __ffma2_rn(two(i), scale2, bias2);
+                      bias2 = __fadd2_rn(bias2, rise2);
+                    }
+                  } else {
+#pragma unroll
+                    for (int i = 0; i < 16; ++i)
+                      e2[g2][i] = __ffma2_rn(two(i), scale2, make_float2(fmaf(-slope, fabsf(f + static_cast<float>(2 * i)), -ref),
+                                                                         fmaf(-slope, fabsf(f + static_cast<float>(2 * i + 1)), -ref)));
+                  }
+                } else if (MODE == AS_CAP) {
+                  // Which way the tanh goes is decided by what is seen alone: columns that no key wrote and rows of no token hold whatever
+                  // was there before, and results must not depend on it.
+                  float top = 0.f;
+                  if (whole) {
+#pragma unroll
+                    for (int i = 0; i < 32; i += 2) top = as_max3_abs(top, __uint_as_float(z[g2][i]), __uint_as_float(z[g2][i + 1]));
+                  } else {
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) top = fmaxf(top, (seen[g2] >> i) & 1u ? fabsf(__uint_as_float(z[g2][i])) : 0.f);
+                  }
+                  if ((__ballot_sync(0xffffffffu, top > cap_far) & real_rows) == 0u) {
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) {
+                      const float2 v = __fmul2_rn(two(i), scale2);
+                      e2[g2][i] = tanh_near(v, __fmul2_rn(v, v));
+                    }
+                  } else {
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) {
+                      const float2 v = two(i);
+                      e2[g2][i] = make_float2(cap_out * as_tanh(v.x * cap_in), cap_out * as_tanh(v.y * cap_in));
+                    }
+                  }
+                } else {
+                  float y[32];
+#pragma unroll
+                  for (int i = 0; i < 32; ++i) y[i] = __uint_as_float(z[g2][i]);
+                  if (mod.cap > 0.f) {
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) y[i] = fmaf(cap_out, as_tanh(y[i] * cap_in), -ref);
+                  } else {
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) y[i] = fmaf(y[i], scale_log2, -ref);
+                  }
+                  const int d0 = key32 - pos;
+                  if (mod.slopes != nullptr) {
+                    const float f = static_cast<float>(d0);
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) y[i] = fmaf(-slope, fabsf(f + static_cast<float>(i)), y[i]);
+                  }
+                  if (mod.bias != nullptr) {
+                    if (key32 + 31 - pos_first <= -mod.radius || key32 - pos_last >= mod.radius) {
+                      const float b = tab[key32 < pos_last ? -mod.radius : mod.radius] * tab_unit;
+#pragma unroll
+                      for (int i = 0; i < 32; ++i) y[i] += b;
+                    } else {
+#pragma unroll
+                      for (int i = 0; i < 32; ++i) y[i] = fmaf(tab[min(max(d0 + i, -mod.radius), mod.radius)], tab_unit, y[i]);
+                    }
+                  }
+#pragma unroll
+                  for (int i = 0; i < 16; ++i) e2[g2][i] = make_float2(y[2 * i], y[2 * i + 1]);
+                }
+                if (!whole) {
+#pragma unroll
+                  for (int i = 0; i < 16; ++i) {
+                    if (!((seen[g2] >> (2 * i)) & 1u)) e2[g2][i].x = -INFINITY;
+                    if (!((seen[g2] >> (2 * i + 1)) & 1u)) e2[g2][i].y = -INFINITY;
+                  }
+                }
               }
             }
-            uint32_t pk[16];
-            float total;
-            auto exponentials = [&]() {
-              float2 sum = make_float2(0.f, 0.f), sum1 = make_float2(0.f, 0.f);
+            if (MODE != AS_CAP && (guess || again)) {
+              // The reference moves to the larger of these scores and the logarithm of the sum so far (which lies far below it where the
+              // reference was a bad guess), by a whole number. With slopes the first guess takes the bias of the step's nearest key, which
+              // later scores will not exceed by much.
+              float mx = raw_max - (MODE == AS_SLOPES ? slope * static_cast<float>(max(max(kv0 - pos, pos - (kv0 + n_valid - 1)), 0)) : 0.f);
+              if (MODE != AS_SLOPES || again) {
+                float m1 = -INFINITY;
+                mx = -INFINITY;
 #pragma unroll
-              for (int i = 0; i < 16; i += 2) {
-                const float2 a = make_float2(as_ex2(e2[i].x), as_ex2(e2[i].y)), b = make_float2(as_ex2(e2[i + 1].x), as_ex2(e2[i + 1].y));
-                sum = __fadd2_rn(sum, a);
-                sum1 = __fadd2_rn(sum1, b);
-                const __nv_bfloat162 ha = __floats2bfloat162_rn(a.x, a.y), hb = __floats2bfloat162_rn(b.x, b.y);
-                pk[i] = *reinterpret_cast<const uint32_t*>(&ha);
-                pk[i + 1] = *reinterpret_cast<const uint32_t*>(&hb);
+                for (int i = 0; i < 16; ++i) mx = as_max3(mx, e2[0][i].x, e2[0][i].y);
+                if (both) {
+#pragma unroll
+                  for (int i = 0; i < 16; ++i) m1 = as_max3(m1, e2[1][i].x, e2[1][i].y);
+                }
+                mx = fmaxf(mx, m1);
               }
-              total = (sum.x + sum1.x) + (sum.y + sum1.y);
-            };
-            // The reference moves to the larger of these scores and the logarithm of the sum so far (which lies far below it where the
-            // reference was a bad guess), by a whole number.
-            auto move = [&](float mx) -> float {
-              const float so_far = l_run > 0.f ? __log2f(l_run) : -INFINITY;
-              const float by = ceilf(fmaxf(mx, so_far));
-              if (by == -INFINITY) return 1.f;
-              const float alpha = l_run > 0.f ? as_ex2(-by) : l_run;  // nothing summed: 0, and NaN stays NaN
+              float by = ceilf(fmaxf(mx, l_run > 0.f ? __log2f(l_run) : -INFINITY));
+              if (!moves || by == -INFINITY) by = 0.f;
+              const float alpha = l_run > 0.f ? as_ex2(-by) : by != 0.f ? l_run : 1.f;  // nothing summed: 0, and NaN stays NaN
               l_run *= alpha;
               ref += by;
 #pragma unroll
-              for (int i = 0; i < 16; ++i) e2[i] = __fadd2_rn(e2[i], make_float2(-by, -by));
-              return alpha;
-            };
-            auto highest = [&]() -> float {
-              float m0 = -INFINITY, m1 = -INFINITY;
+              for (int i = 0; i < 32; ++i) e2[i >> 4][i & 15] = __fadd2_rn(e2[i >> 4][i & 15], make_float2(-by, -by));
+              if (again) rescale(alpha, c / 32);
+            }
+            float2 sum = make_float2(0.f, 0.f), sum1 = make_float2(0.f, 0.f);
 #pragma unroll
-              for (int i = 0; i < 16; i += 2) {
-                m0 = as_max3(m0, e2[i].x, e2[i].y);
-                m1 = as_max3(m1, e2[i + 1].x, e2[i + 1].y);
-              }
-              return fmaxf(m0, m1);
-            };
-            if (guess) {
-              // with slopes at the bias of the step's nearest key, which later scores will not exceed by much
-              if (MODE == AS_SLOPES) raw_max -= slope * static_cast<float>(max(max(kv0 - pos, pos - (kv0 + n_valid - 1)), 0));
-              move(MODE == AS_SLOPES ? raw_max : highest());
-            }
-            exponentials();
-            if (MODE != AS_CAP) {
-              const bool bad = real && seen != 0u && !(l_run + total >= AS_SUM_LOW && total <= AS_SUM_HIGH);
-              if (__any_sync(0xffffffffu, bad)) {
-                float alpha = 1.f;
-                const float mx = highest();
-                if (bad) alpha = move(mx);
-                rescale(alpha, q);
-                exponentials();
+            for (int g2 = 0; g2 < 2; ++g2) {
+              if (g2 == 0 || both) {
+#pragma unroll
+                for (int i = 0; i < 16; i += 2) {
+                  const float2 a = make_float2(as_ex2(e2[g2][i].x), as_ex2(e2[g2][i].y)), b = make_float2(as_ex2(e2[g2][i + 1].x), as_ex2(e2[g2][i + 1].y));
+                  sum = __fadd2_rn(sum, a);
+                  sum1 = __fadd2_rn(sum1, b);
+                  const __nv_bfloat162 ha = __floats2bfloat162_rn(a.x, a.y), hb = __floats2bfloat162_rn(b.x, b.y);
+                  pk[g2][i] = *reinterpret_cast<const uint32_t*>(&ha);
+                  pk[g2][i + 1] = *reinterpret_cast<const uint32_t*>(&hb);
+                }
               }
             }
+            total = (sum.x + sum1.x) + (sum.y + sum1.y);
+            if (again) break;
+            // one vote a step: sums out of range, and waits that gave up
+            const float sum_now = l_run + total;
+            bool bad = MODE != AS_CAP && !(sum_now >= AS_SUM_LOW && sum_now <= AS_SUM_HIGH);
+            if (!whole) bad = bad && (seen[0] | seen[1]) != 0u;
+            if ((__ballot_sync(0xffffffffu, bad || failed) & real_rows) == 0u) break;
+            failed = __any_sync(0xffffffffu, failed);
+            if (failed) break;
+            moves = bad && real;
+            again = true;
+            }
+            if (failed) break;
             l_run += total;
-            if (S_BUFS == 1 && q == 0 && step > 0) {
+            if (S_BUFS == 1 && c == 0 && step > 0) {
               // the previous step's P has been read
               if (!pv_wait(step - 1)) failed = true;
               tc_fence_after_sync();
             }
-            tmem_st_32x32b_x16(lanes + Cfg::P(t, buf, 0) + q * (Cfg::P(0, 0, 1) - Cfg::P(0, 0, 0)), pk);
-          };
-          uint32_t za[32], zb[32];
-          tmem_ld_32x32b_x32(s_at, za);
-#pragma unroll 1
-          for (int q = 0; q < n_chunks; q += 2) {
-            // the next 32 scores are on their way while these are worked on
-            tmem_ld_wait_for(za);
-            if (q + 1 < n_chunks) tmem_ld_32x32b_x32(s_at + q * 32 + 32, zb);
-            chunk(za, q);
-            if (q + 1 < n_chunks) {
-              tmem_ld_wait_for(zb);
-              if (q + 2 < n_chunks) tmem_ld_32x32b_x32(s_at + q * 32 + 64, za);
-              chunk(zb, q + 1);
-            }
+            const uint32_t p_at = lanes + Cfg::P(t, buf, 0) + (c / 32) * (Cfg::P(0, 0, 1) - Cfg::P(0, 0, 0));
+            tmem_st_32x32b_x16(p_at, pk[0]);
+            if (both) tmem_st_32x32b_x16(p_at + (Cfg::P(0, 0, 1) - Cfg::P(0, 0, 0)), pk[1]);
           }
           failed = __any_sync(0xffffffffu, failed);
           if (failed) break;
@@ -1068,7 +1122,7 @@ attn_scored_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_cons
         }
         first = false;
         ++step;
-        w.next(plan, j.n_kv_heads);
+        kv0 = next_kv0;
       }
       if (failed) break;
       // ---- the segment's rows ----
@@ -1076,8 +1130,9 @@ attn_scored_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_cons
       failed = __any_sync(0xffffffffu, failed);
       if (failed) break;
       tc_fence_after_sync();
-      const int done = (w.e == seg_e && w.h == seg_h) ? w.k : n_tiles;  // tiles of the item up to here
-      if (k_first == 0 && done == n_tiles) {
+      const int k_first = cold[C_K], n_tiles = cold[C_N], seg_h = cold[C_H], seg_e = cold[C_E], tok0 = cold[C_TOK0];
+      if (k_first == 0 && i_end == n_tiles) {
+        uint8_t* stage = stage_s + warp * AS_STAGE;
         if (active) {
           const float inv = l_run == 0.f ? 0.f : 1.f / l_run;
 #pragma unroll 1
@@ -1111,9 +1166,9 @@ attn_scored_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_cons
                 const int col = c + cc * 8;
                 if (r < n_rows && col < j.head_dim) {
                   const uint4 x = *reinterpret_cast<const uint4*>(stage + rl * 64 + ((cc ^ ((rl >> 1) & 3)) << 4));
-                  const int tk = (r * group_inv) >> 16;
+                  const int tk = (r * j.group_inv) >> 16;
                   *reinterpret_cast<uint4*>(j.out + static_cast<int64_t>(tok0 + tk) * j.out_stride +
-                                            static_cast<int64_t>(seg_h * group + r - tk * group) * j.head_dim + col) = x;
+                                            static_cast<int64_t>(seg_h * j.group + r - tk * j.group) * j.head_dim + col) = x;
                 }
               }
               __syncwarp();
@@ -1193,14 +1248,23 @@ attn_scored_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_cons
             x.z = *reinterpret_cast<uint32_t*>(&p2);
             x.w = *reinterpret_cast<uint32_t*>(&p3);
             if (inv == 0.f) x = make_uint4(0, 0, 0, 0);
-            const int tk = (r * group_inv) >> 16;
+            const int tk = (r * j.group_inv) >> 16;
             *reinterpret_cast<uint4*>(j.out + static_cast<int64_t>(tok0 + tk) * j.out_stride +
-                                      static_cast<int64_t>(seg_h * group + r - tk * group) * j.head_dim + col) = x;
+                                      static_cast<int64_t>(seg_h * j.group + r - tk * j.group) * j.head_dim + col) = x;
           }
         }
         meet();  // joins[t] may be written again
       }
       tc_fence_before_sync();  // O has been read: the next segment's first P V may overwrite it
+      __syncwarp();
+      if (lane == 0) {
+        cold[C_LEFT] -= i_end - k_first;
+        const bool over = i_end == n_tiles, head_over = over && seg_h + 1 == j.n_kv_heads;
+        cold[C_K] = over ? 0 : i_end;
+        cold[C_H] = head_over ? 0 : seg_h + (over ? 1 : 0);
+        cold[C_E] = seg_e + (head_over ? 1 : 0);
+      }
+      __syncwarp();
     }
     if (failed && lane == 0) atomicExch(plan.status, 4);
   }
@@ -1452,6 +1516,7 @@ extern "C" int b200emb_op_attention_scored(const void* q, int64_t q_row_stride, 
   j.n_kv_heads = n_kv_heads;
   j.head_dim = head_dim;
   j.group = n_heads / n_kv_heads;
+  j.group_inv = (65536 + j.group - 1) / j.group;
   j.tile_tokens = as_tile_tokens(n_heads, n_kv_heads);
   j.box_rows = AS_PACKED_BOX;
   AsMaps m;
@@ -1498,6 +1563,7 @@ extern "C" int b200emb_op_attention_paged(const void* q, int64_t q_row_stride, v
   j.n_kv_heads = cache->n_kv_heads;
   j.head_dim = cache->head_dim;
   j.group = n_heads / cache->n_kv_heads;
+  j.group_inv = (65536 + j.group - 1) / j.group;
   j.tile_tokens = as_tile_tokens(n_heads, cache->n_kv_heads);
   j.n_pages = cache->n_pages;
   j.page_size = cache->page_size;
