@@ -14,7 +14,7 @@
 // A CTA (one per SM) runs two streams, A and B, each with its own 128-row tile, softmax warpgroup and tensor-memory
 // accumulators, so that one stream's exponentials run under the other's matrix products. With long queries the two streams take
 // neighbouring tiles of the same item row and share every key and value tile ("pair"); otherwise each walks its own part.
-// Per step of a stream (128 keys with head_dim up to 64, 64 with more):
+// Per step of a stream, 64 keys:
 //   S = Q K^T     tcgen05.mma 128 x N x 16 (N = valid keys rounded up to 16), fp32 in tensor memory
 //   softmax       128 threads, one row each, in one pass over the row: a score becomes its exponential against the row's reference
 //                 at once. The reference is a guess (from the first 32 scores of the row's first step) and is only replaced, by the
@@ -355,28 +355,24 @@ attn_plan_kernel(const AttnJob j, const AttnMod mod, const AttnPlan p, int token
 template <int D>
 struct AsCfg {
   static constexpr int BLOCKS = D / 64;
-  // Keys of a step. With head_dim 128 the accumulators take half of tensor memory; steps of 64 keys leave room for two score
-  // buffers a stream, so that the next scores are there before the softmax has finished these.
-  static constexpr int KV = D == 64 ? 128 : 64;
+  // Keys of a step. Steps of 64 leave room in tensor memory for two score buffers a stream, so that the next scores are there
+  // before the softmax has finished these.
+  static constexpr int KV = 64;
   static constexpr int Q_BLOCK = 128 * 128, Q_TILE = BLOCKS * Q_BLOCK;     // rows of 64 columns, 128-byte swizzle
-  static constexpr int KV_BLOCK = KV * 128, KV_TILE = BLOCKS * KV_BLOCK;  // 16 KB either way
-  static constexpr int RING = 4;  // key (and value) tiles in flight
+  static constexpr int KV_BLOCK = KV * 128, KV_TILE = BLOCKS * KV_BLOCK;
+  static constexpr int RING = D == 64 ? 8 : 4;  // key (and value) tiles in flight: 64 KB of each
   static constexpr int STAGE_BYTES = AS_SOFTMAX_WARPS * AS_STAGE;
   static constexpr int TABLE_BYTES = 2 * AS_TABLE * 4;
-  static constexpr int BAR_BYTES = 384;
+  static constexpr int BAR_BYTES = 512;
   static constexpr int COLD_BYTES = AS_SOFTMAX_WARPS * AS_COLD * 4;
   static constexpr int SMEM_BYTES = 2 * Q_TILE + 2 * RING * KV_TILE + STAGE_BYTES + TABLE_BYTES + BAR_BYTES + COLD_BYTES + 1024;
-  static constexpr int N_BARS = 4 * RING + 2 * 10;
+  static constexpr int N_BARS = 4 * RING + 2 * 9;
   static_assert(N_BARS * 8 + 16 <= BAR_BYTES, "barrier area");
   static_assert(SMEM_BYTES <= 232448, "shared memory");
-  // Tensor memory of stream t. head_dim 64: one score buffer of 128 columns, P beside it (the next S may be written as soon as
-  // this one has been read). 128: two score buffers of 64 columns, P in the place of its own S.
-  static constexpr int S_BUFS = D == 64 ? 1 : 2;
+  // Tensor memory of stream t: two score buffers of 64 columns, the accumulators, and P of a buffer's chunk of 32 keys in the first 16
+  // of the chunk's own 32 columns.
   static __host__ __device__ constexpr uint32_t S(int t, int b) { return t * 128 + b * 64; }
   static __host__ __device__ constexpr uint32_t O(int t) { return 256 + t * D; }
-  // P of the 32 keys of chunk q: 16 columns, with two score buffers the first of the chunk's own 32
-  static __host__ __device__ constexpr uint32_t P(int t, int b, int q) { return D == 64 ? 384 + t * 64 + q * 16 : S(t, b) + q * 32; }
-  static constexpr int CHUNKS = KV / 32;
 };
 
 // The steps of a stream, in order. Every role of the stream walks the same ones.
@@ -544,7 +540,7 @@ attn_scored_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_cons
                    const __grid_constant__ CUtensorMap tmap_v, const __grid_constant__ AttnJob j, const __grid_constant__ AttnMod mod,
                    const __grid_constant__ AttnPlan plan) {
   using Cfg = AsCfg<D>;
-  constexpr int RING = Cfg::RING, KV = Cfg::KV, S_BUFS = Cfg::S_BUFS;
+  constexpr int RING = Cfg::RING, KV = Cfg::KV;
   // A stream's own tiles in flight, so that neither stream waits for the other's; a pair has one ring.
   constexpr uint32_t SLOTS = PAIR ? RING : RING / 2;
   extern __shared__ uint8_t as_raw[];
@@ -563,8 +559,7 @@ attn_scored_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_cons
   uint64_t* s_full = q_empty + 2;     // [stream][buffer] S of a step is in tensor memory
   uint64_t* p_full = s_full + 4;      // [stream][buffer] P of a step is in tensor memory, O may be added to
   uint64_t* pv_done = p_full + 4;     // [stream][buffer] P V of a step has finished
-  uint64_t* s_read = pv_done + 4;     // one score buffer: the softmax warps hold its scores in registers
-  uint64_t* group_bar = s_read + 2;   // the softmax warps of a stream meet
+  uint64_t* group_bar = pv_done + 4;  // the softmax warps of a stream meet
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(group_bar + 2);
   uint32_t* joins = tmem_slot + 1;                                          // per stream: these warps join the parts of the item
 
@@ -585,7 +580,6 @@ attn_scored_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_cons
         mbar_init(&p_full[2 * t + b], AS_SOFTMAX_WARPS / 2);
         mbar_init(&pv_done[2 * t + b], 1);
       }
-      mbar_init(&s_read[t], AS_SOFTMAX_WARPS / 2);
       mbar_init(&group_bar[t], AS_SOFTMAX_WARPS / 2);
     }
     fence_mbar_init();
@@ -674,7 +668,7 @@ attn_scored_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_cons
     auto has_rows = [&](const AsWalk<KV>& w) { return !PAIR || t == 0 || w.f0.z > j.tile_tokens; };
     auto wait_all = [](uint64_t* bar, uint32_t parity) -> bool { return __all_sync(0xffffffffu, mbar_wait(bar, parity)); };
     auto issue_s = [&]() -> bool {
-      const uint32_t slot = ring0 + n_s % SLOTS, buf = n_s % S_BUFS;
+      const uint32_t slot = ring0 + n_s % SLOTS, buf = n_s % 2;
       if (sw.first && !wait_all(&q_full[t], q_uses++ & 1u)) return false;
       if (!wait_all(&k_full[slot], (n_s / SLOTS) & 1u)) return false;
       tc_fence_after_sync();
@@ -684,7 +678,7 @@ attn_scored_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_cons
         for (int k = 0; k < D / 16; ++k) {
           const uint64_t a = make_kmajor_sw128_desc(q_addr + (k / 4) * Cfg::Q_BLOCK) + 2 * (k % 4);
           const uint64_t b = make_kmajor_sw128_desc(k_addr + slot * Cfg::KV_TILE + (k / 4) * Cfg::KV_BLOCK) + 2 * (k % 4);
-          if (elect_one()) tc_mma_f16(tmem_u + t * (Cfg::S(1, 0) - Cfg::S(0, 0)) + buf * (Cfg::S(0, 1) - Cfg::S(0, 0)), a, b, idesc, k != 0);
+          if (elect_one()) tc_mma_f16(tmem_u + t * Cfg::S(1, 0) + buf * Cfg::S(0, 1), a, b, idesc, k != 0);
         }
       }
       if (elect_one()) {
@@ -697,7 +691,7 @@ attn_scored_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_cons
       return true;
     };
     auto issue_pv = [&]() -> bool {
-      const uint32_t slot = ring0 + n_pv % SLOTS, buf = n_pv % S_BUFS;
+      const uint32_t slot = ring0 + n_pv % SLOTS, buf = n_pv % 2;
       if (!wait_all(&v_full[slot], (n_pv / SLOTS) & 1u)) return false;
       const int n_valid = pw.n_valid(), n_eff = as_round16(n_valid);
       if (n_valid < n_eff) {
@@ -711,15 +705,15 @@ attn_scored_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_cons
         fence_proxy_async_smem();
         __syncwarp();
       }
-      if (!wait_all(&p_full[2 * t + buf], (n_pv / S_BUFS) & 1u)) return false;
+      if (!wait_all(&p_full[2 * t + buf], (n_pv / 2) & 1u)) return false;
       tc_fence_after_sync();
       if (has_rows(pw)) {
         const uint64_t v_desc = make_mnmajor_sw128_desc(v_addr + slot * Cfg::KV_TILE, Cfg::KV_BLOCK);
-        const uint32_t p_at = tmem_u + t * (Cfg::P(1, 0, 0) - Cfg::P(0, 0, 0)) + buf * (Cfg::P(0, 1, 0) - Cfg::P(0, 0, 0)) + Cfg::P(0, 0, 0);
+        const uint32_t p_at = tmem_u + t * Cfg::S(1, 0) + buf * Cfg::S(0, 1);
 #pragma unroll
         for (int k = 0; k < KV / 16; ++k)
           if (k * 16 < n_eff && elect_one())
-            tc_mma_f16_tmem_a(tmem_u + Cfg::O(0) + t * (Cfg::O(1) - Cfg::O(0)), p_at + Cfg::P(0, 0, k / 2) - Cfg::P(0, 0, 0) + (k % 2) * 8, v_desc + k * 128,
+            tc_mma_f16_tmem_a(tmem_u + Cfg::O(0) + t * (Cfg::O(1) - Cfg::O(0)), p_at + (k / 2) * 32 + (k % 2) * 8, v_desc + k * 128,
                               idesc_pv, !pw.first || k != 0);
       }
       if (elect_one()) {
@@ -731,14 +725,12 @@ attn_scored_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_cons
       return true;
     };
     bool ok = true;
-    for (int i = 0; i < S_BUFS; ++i)
+    for (int i = 0; i < 2; ++i)
       if (ok && sw.left > 0) ok = issue_s();
     while (ok && pw.left > 0) {
-      // One score buffer: the next S goes there as soon as the softmax has read it, P V follows. Two: P V reads the P that took the
-      // place of its S, then the S after the next may follow.
-      if (S_BUFS == 1 && sw.left > 0) ok = wait_all(&s_read[t], (n_s - 1) & 1u) && issue_s();
-      if (ok) ok = issue_pv();
-      if (S_BUFS == 2 && ok && sw.left > 0) ok = wait_all(&pv_done[2 * t + (n_pv - 1) % S_BUFS], ((n_pv - 1) / S_BUFS) & 1u) && issue_s();
+      // P V reads the P that took the place of its scores, then the scores of the step after the next may go there
+      ok = issue_pv();
+      if (ok && sw.left > 0) ok = wait_all(&pv_done[2 * t + (n_pv - 1) % 2], ((n_pv - 1) / 2) & 1u) && issue_s();
     }
     if (!ok && lane == 0) atomicExch(plan.status, 7);
   } else {
@@ -776,7 +768,7 @@ attn_scored_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_cons
     };
     // P V of step s, one of the last two. A barrier is told by its parity alone, so each of two score buffers has its own: of the P V
     // of two steps before, the scores of step s + 1 have already told.
-    auto pv_wait = [&](uint32_t s) { return mbar_wait(&pv_done[2 * t + s % S_BUFS], (s / S_BUFS) & 1u); };
+    auto pv_wait = [&](uint32_t s) { return mbar_wait(&pv_done[2 * t + s % 2], (s / 2) & 1u); };
     auto part_of = [&](int slot, bool tail) -> int64_t { return (2 * slot + (tail ? 1 : 0)) * (PAIR ? 2 : 1) + (PAIR ? t : 0); };
     float slope = 0.f;
     const float* tab = nullptr;
@@ -824,7 +816,7 @@ attn_scored_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_cons
         }
       }
       const bool active = wq * 32 < n_rows, real = row < n_rows;
-      const int doc = mod.docs != nullptr && real ? __ldg(mod.docs + cold[C_TOK0] + row_tok) : -1;
+      const int doc = MODE == AS_ANY && mod.docs != nullptr && real ? __ldg(mod.docs + cold[C_TOK0] + row_tok) : -1;
       // first and past-the-last visible key of the window of this row
       auto key_lo = [&]() { return mod.left >= pos ? 0 : pos - mod.left; };
       auto key_hi = [&]() { return mod.right >= kv_len - pos ? kv_len : pos + mod.right + 1; };
@@ -832,8 +824,11 @@ attn_scored_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_cons
       const uint32_t real_rows = __ballot_sync(0xffffffffu, real);
       const int all_lo = __reduce_max_sync(0xffffffffu, real ? key_lo() : INT_MIN), all_hi = __reduce_min_sync(0xffffffffu, real ? key_hi() : INT_MAX);
       const int pos_first = __reduce_min_sync(0xffffffffu, real ? pos : INT_MAX), pos_last = __reduce_max_sync(0xffffffffu, real ? pos : INT_MIN);
-      const int one_doc = __reduce_min_sync(0xffffffffu, real ? doc : INT_MAX) == __reduce_max_sync(0xffffffffu, real ? doc : -1)
-                              ? __reduce_max_sync(0xffffffffu, real ? doc : -1) : -1;  // the document of all rows, or -1
+      int one_doc = -1;  // the document of all rows, or -1
+      if (MODE == AS_ANY && mod.docs != nullptr) {
+        const int least = __reduce_min_sync(0xffffffffu, real ? doc : INT_MAX), most = __reduce_max_sync(0xffffffffu, real ? doc : -1);
+        one_doc = least == most ? most : -1;
+      }
       auto key0_of = [&](int k) {  // as AsWalk::key0
         const int i = k - run_n0;
         return (i < 0 ? run0 + k : run1 + (i <= run_near ? run_near - i : i)) * KV;
@@ -842,28 +837,29 @@ attn_scored_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_cons
       bool first = true;
       int kv0 = key0_of(i_k);
       for (; i_k < i_end; ++i_k) {
-        const int buf = step % S_BUFS, n_valid = min(max(kv_len - kv0, 0), KV), n_rem = as_round16(n_valid);
+        const int buf = step % 2, n_valid = min(max(kv_len - kv0, 0), KV), n_rem = as_round16(n_valid);
         const int next_kv0 = key0_of(i_k + 1);
-        int key_docs[KV / 32];  // documents of the step's keys, lane l's of 32 l' + l
-        if (mod.docs != nullptr) {
+        int key_docs[KV / 32] = {};  // documents of the step's keys, lane l's of 32 l' + l
+        if (MODE == AS_ANY && mod.docs != nullptr) {
 #pragma unroll
           for (int q = 0; q < KV / 32; ++q) {
             const int key = kv0 + q * 32 + lane;
             key_docs[q] = key < kv_len ? __ldg(mod.docs + cold[C_KVROW0] + key) : -1;
           }
         }
-        if (!mbar_wait(&s_full[2 * t + buf], (step / S_BUFS) & 1u)) failed = true;  // looked at below, once a step
+        if (!mbar_wait(&s_full[2 * t + buf], (step / 2) & 1u)) failed = true;  // looked at below, once a step
         tc_fence_after_sync();
         if (active) {
-          const uint32_t s_at = lanes + Cfg::S(t, buf);
+          const uint32_t s_at = lanes + t * Cfg::S(1, 0) + buf * Cfg::S(0, 1);
+          bool whole = all_lo <= kv0 && all_hi >= kv0 + KV;  // no masks
+          if (MODE == AS_ANY && mod.docs != nullptr && whole)
+            whole = one_doc >= 0 && __all_sync(0xffffffffu, key_docs[0] == one_doc && key_docs[1] == one_doc);
           auto seen_of = [&](int q) -> uint32_t {
             const int key = kv0 + q * 32;
             uint32_t seen = (as_below(key_hi() - key) & ~as_below(key_lo() - key)) | as_below(cold[C_PREFIX] - key);
-            if (mod.docs != nullptr) {
+            if (MODE == AS_ANY && mod.docs != nullptr) {
               // the keys of each document that some row of the warp belongs to
-              int key_doc = key_docs[0];
-#pragma unroll
-              for (int i = 1; i < KV / 32; ++i) key_doc = q == i ? key_docs[i] : key_doc;
+              const int key_doc = key_docs[q];
               uint32_t same = 0, todo = __ballot_sync(0xffffffffu, doc >= 0);
               while (todo) {
                 const int d = __shfl_sync(0xffffffffu, doc, __ffs(todo) - 1);
@@ -875,71 +871,99 @@ attn_scored_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_cons
             }
             return seen;
           };
-          // O and what this step has already put into P follow a reference that has moved (by whole powers of two: nothing is rounded).
-          auto rescale = [&](float alpha, int q) {
-            if (!__any_sync(0xffffffffu, alpha != 1.f)) return;
-            if (!first) {
-              // the previous step's P has been read, O is complete up to it
-              if (!pv_wait(step - 1)) failed = true;
-              tc_fence_after_sync();
+          // O follows a reference that has moved (by a whole power of two: nothing is rounded)
+          auto rescale = [&](float alpha) {
+            if (first || !__any_sync(0xffffffffu, alpha != 1.f)) return;
+            if (!pv_wait(step - 1)) failed = true;
+            tc_fence_after_sync();
 #pragma unroll 1
-              for (int c = 0; c < D; c += 16) {
-                uint32_t o[16];
-                tmem_ld_32x32b_x16(lanes + Cfg::O(t) + c, o);
-                tmem_ld_wait_for16(o);
-#pragma unroll
-                for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * alpha);
-                tmem_st_32x32b_x16(lanes + Cfg::O(t) + c, o);
-              }
-            }
-            tmem_st_wait();
-#pragma unroll 1
-            for (int c = 0; c < q; ++c) {
+            for (int c = 0; c < D; c += 16) {
               uint32_t o[16];
-              tmem_ld_32x32b_x16(lanes + Cfg::P(t, buf, 0) + c * (Cfg::P(0, 0, 1) - Cfg::P(0, 0, 0)), o);
+              tmem_ld_32x32b_x16(lanes + Cfg::O(t) + c, o);
               tmem_ld_wait_for16(o);
 #pragma unroll
-              for (int i = 0; i < 16; ++i) {
-                const float2 x = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&o[i]));
-                const __nv_bfloat162 b = __floats2bfloat162_rn(x.x * alpha, x.y * alpha);
-                o[i] = *reinterpret_cast<const uint32_t*>(&b);
-              }
-              tmem_st_32x32b_x16(lanes + Cfg::P(t, buf, 0) + c * (Cfg::P(0, 0, 1) - Cfg::P(0, 0, 0)), o);
+              for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * alpha);
+              tmem_st_32x32b_x16(lanes + Cfg::O(t) + c, o);
             }
             tmem_st_wait();
           };
-          // 64 scores of the row become probabilities
-#pragma unroll 1
-          for (int c = 0; c < KV && c < n_rem; c += 64) {
-            const bool both = c + 32 < n_rem;
-            const int key = kv0 + c;
-            bool whole = all_lo <= key && all_hi >= key + 64;  // no masks
-            if (mod.docs != nullptr && whole) {
-              const int q = c / 32;
-              int d0 = key_docs[0], d1 = key_docs[1];
+          uint32_t pk[2][16];  // the row's probabilities, two to a register
+          float total;
+          auto exponentials = [&](const float2 (&e2)[2][16], bool both) {
+            float2 sum = make_float2(0.f, 0.f), sum1 = make_float2(0.f, 0.f);
 #pragma unroll
-              for (int i = 2; i < KV / 32; i += 2) {
-                d0 = q == i ? key_docs[i] : d0;
-                d1 = q == i ? key_docs[i + 1] : d1;
+            for (int g2 = 0; g2 < 2; ++g2) {
+              if (g2 == 0 || both) {
+#pragma unroll
+                for (int i = 0; i < 16; i += 2) {
+                  const float2 a = make_float2(as_ex2(e2[g2][i].x), as_ex2(e2[g2][i].y)), b = make_float2(as_ex2(e2[g2][i + 1].x), as_ex2(e2[g2][i + 1].y));
+                  sum = __fadd2_rn(sum, a);
+                  sum1 = __fadd2_rn(sum1, b);
+                  const __nv_bfloat162 ha = __floats2bfloat162_rn(a.x, a.y), hb = __floats2bfloat162_rn(b.x, b.y);
+                  pk[g2][i] = *reinterpret_cast<const uint32_t*>(&ha);
+                  pk[g2][i + 1] = *reinterpret_cast<const uint32_t*>(&hb);
+                }
               }
-              whole = one_doc >= 0 && __all_sync(0xffffffffu, d0 == one_doc && d1 == one_doc);
             }
+            total = (sum.x + sum1.x) + (sum.y + sum1.y);
+          };
+          // Most steps: every row sees all 64 keys, the reference stands, nothing is asked of a score one by one. What does not fit
+          // (a sum out of range, a score beyond the cap, a wait that gave up) is taken again below, from the same scores.
+          bool done = false;
+          if (MODE != AS_ANY && whole && (MODE == AS_CAP || !first) && (MODE != AS_SLOPES || kv0 + KV <= pos_first || kv0 > pos_last)) {
+            uint32_t z[2][32];
+            tmem_ld_32x32b_x32(s_at, z[0]);
+            tmem_ld_32x32b_x32(s_at + 32, z[1]);
+            tmem_ld_wait_for(z[0]);
+            tmem_ld_wait_for(z[1]);
+            float2 e2[2][16];
+            auto two = [&](int g2, int i) { return make_float2(__uint_as_float(z[g2][2 * i]), __uint_as_float(z[g2][2 * i + 1])); };
+            bool odd = failed;
+            if (MODE == AS_PLAIN) {
+              const float2 base2 = make_float2(-ref, -ref);
+#pragma unroll
+              for (int i = 0; i < 32; ++i) e2[i >> 4][i & 15] = __ffma2_rn(two(i >> 4, i & 15), scale2, base2);
+            } else if (MODE == AS_SLOPES) {
+              const float f = static_cast<float>(kv0 - pos), rise = kv0 < pos_first ? slope : -slope;
+              const float2 rise2 = make_float2(2.f * rise, 2.f * rise);
+              float2 bias2 = make_float2(fmaf(rise, f, -ref), fmaf(rise, f + 1.f, -ref));
+#pragma unroll
+              for (int i = 0; i < 32; ++i) {
+                e2[i >> 4][i & 15] = __ffma2_rn(two(i >> 4, i & 15), scale2, bias2);
+                bias2 = __fadd2_rn(bias2, rise2);
+              }
+            } else {
+              float top = 0.f;
+#pragma unroll
+              for (int i = 0; i < 64; i += 2) top = as_max3_abs(top, __uint_as_float(z[i >> 5][i & 31]), __uint_as_float(z[i >> 5][(i & 31) + 1]));
+              odd = odd || top > cap_far;
+#pragma unroll
+              for (int i = 0; i < 32; ++i) {
+                const float2 v = __fmul2_rn(two(i >> 4, i & 15), scale2);
+                e2[i >> 4][i & 15] = tanh_near(v, __fmul2_rn(v, v));
+              }
+            }
+            exponentials(e2, true);
+            const float sum_now = l_run + total;
+            if (MODE != AS_CAP) odd = odd || !(sum_now >= AS_SUM_LOW && sum_now <= AS_SUM_HIGH);
+            done = (__ballot_sync(0xffffffffu, odd) & real_rows) == 0u;
+          }
+          if (!done) {
+            const bool both = n_rem > 32;
             uint32_t seen[2] = {0xffffffffu, 0xffffffffu};
             if (!whole) {
-              seen[0] = seen_of(c / 32);
-              seen[1] = both ? seen_of(c / 32 + 1) : 0u;
+              seen[0] = seen_of(0);
+              seen[1] = both ? seen_of(1) : 0u;
             }
-            uint32_t pk[2][16];
-            float total;
             // Normally once. A row whose sum leaves its range moves its reference, and the scores, still where they were, are taken again.
-            bool moves = MODE != AS_CAP && first && c == 0 && real;  // the segment's first scores set the reference
+            bool moves = MODE != AS_CAP && first && real;  // the segment's first scores set the reference
             bool again = false;
 #pragma unroll 1
             while (true) {
             uint32_t z[2][32];
-            tmem_ld_32x32b_x32(s_at + c, z[0]);
-            if (both) tmem_ld_32x32b_x32(s_at + c + 32, z[1]);
-            const bool guess = MODE != AS_CAP && first && c == 0 && !again;
+            tmem_ld_32x32b_x32(s_at, z[0]);
+            if (both) tmem_ld_32x32b_x32(s_at + 32, z[1]);
+            const bool guess = MODE != AS_CAP && first && !again;
             tmem_ld_wait_for(z[0]);
             tmem_ld_wait_for(z[1]);
             float2 e2[2][16];  // exponents against the reference
@@ -947,7 +971,7 @@ attn_scored_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_cons
 #pragma unroll
             for (int g2 = 0; g2 < 2; ++g2) {
               if (g2 == 0 || both) {
-                const int key32 = key + g2 * 32;
+                const int key32 = kv0 + g2 * 32;
                 auto two = [&](int i) { return make_float2(__uint_as_float(z[g2][2 * i]), __uint_as_float(z[g2][2 * i + 1])); };
                 if (MODE == AS_SLOPES && guess) {
 #pragma unroll
@@ -1061,24 +1085,9 @@ attn_scored_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_cons
               ref += by;
 #pragma unroll
               for (int i = 0; i < 32; ++i) e2[i >> 4][i & 15] = __fadd2_rn(e2[i >> 4][i & 15], make_float2(-by, -by));
-              if (again) rescale(alpha, c / 32);
+              if (again) rescale(alpha);
             }
-            float2 sum = make_float2(0.f, 0.f), sum1 = make_float2(0.f, 0.f);
-#pragma unroll
-            for (int g2 = 0; g2 < 2; ++g2) {
-              if (g2 == 0 || both) {
-#pragma unroll
-                for (int i = 0; i < 16; i += 2) {
-                  const float2 a = make_float2(as_ex2(e2[g2][i].x), as_ex2(e2[g2][i].y)), b = make_float2(as_ex2(e2[g2][i + 1].x), as_ex2(e2[g2][i + 1].y));
-                  sum = __fadd2_rn(sum, a);
-                  sum1 = __fadd2_rn(sum1, b);
-                  const __nv_bfloat162 ha = __floats2bfloat162_rn(a.x, a.y), hb = __floats2bfloat162_rn(b.x, b.y);
-                  pk[g2][i] = *reinterpret_cast<const uint32_t*>(&ha);
-                  pk[g2][i + 1] = *reinterpret_cast<const uint32_t*>(&hb);
-                }
-              }
-            }
-            total = (sum.x + sum1.x) + (sum.y + sum1.y);
+            exponentials(e2, both);
             if (again) break;
             // one vote a step: sums out of range, and waits that gave up
             const float sum_now = l_run + total;
@@ -1091,31 +1100,18 @@ attn_scored_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_cons
             again = true;
             }
             if (failed) break;
-            l_run += total;
-            if (S_BUFS == 1 && c == 0 && step > 0) {
-              // the previous step's P has been read
-              if (!pv_wait(step - 1)) failed = true;
-              tc_fence_after_sync();
-            }
-            const uint32_t p_at = lanes + Cfg::P(t, buf, 0) + (c / 32) * (Cfg::P(0, 0, 1) - Cfg::P(0, 0, 0));
-            tmem_st_32x32b_x16(p_at, pk[0]);
-            if (both) tmem_st_32x32b_x16(p_at + (Cfg::P(0, 0, 1) - Cfg::P(0, 0, 0)), pk[1]);
           }
-          failed = __any_sync(0xffffffffu, failed);
-          if (failed) break;
-          if (S_BUFS == 1 && lane == 0) mbar_arrive(&s_read[t]);  // every lane's scores have been waited for
+          l_run += total;
+          tmem_st_32x32b_x16(s_at, pk[0]);
+          if (n_rem > 32) tmem_st_32x32b_x16(s_at + 32, pk[1]);
           tmem_st_wait();
           tc_fence_before_sync();
           __syncwarp();
           if (lane == 0) mbar_arrive(&p_full[2 * t + buf]);
         } else {
           // nothing to compute: arrive in step with the warps that do
-          if (S_BUFS == 1) {
-            if (lane == 0) mbar_arrive(&s_read[t]);
-            if (step > 0 && !pv_wait(step - 1)) failed = true;
-            failed = __any_sync(0xffffffffu, failed);
-            if (failed) break;
-          }
+          failed = __any_sync(0xffffffffu, failed);
+          if (failed) break;
           tc_fence_before_sync();
           __syncwarp();
           if (lane == 0) mbar_arrive(&p_full[2 * t + buf]);
@@ -1445,8 +1441,8 @@ static int as_map_pages(CUtensorMap* m, const void* base, const b200emb_kv_cache
 
 template <int D, bool PAGED, bool PAIR>
 static int as_launch_mode(const AsMaps& m, const AttnJob& j, const AttnMod& mod, const AttnPlan& plan, int sms, cudaStream_t s) {
-  const bool up = mod.scale > 0.f;  // the plain row maximum is that of the scaled scores
-  if (mod.cap == 0.f && mod.slopes == nullptr && mod.bias == nullptr && up) return as_launch<D, PAGED, PAIR, AS_PLAIN>(m, j, mod, plan, sms, s);
+  if (mod.docs != nullptr) return as_launch<D, PAGED, PAIR, AS_ANY>(m, j, mod, plan, sms, s);
+  if (mod.cap == 0.f && mod.slopes == nullptr && mod.bias == nullptr) return as_launch<D, PAGED, PAIR, AS_PLAIN>(m, j, mod, plan, sms, s);
   if (mod.cap == 0.f && mod.slopes != nullptr) return as_launch<D, PAGED, PAIR, AS_SLOPES>(m, j, mod, plan, sms, s);
   const float cap = mod.cap * AS_LOG2E;
   if (cap >= AS_CAP_LOW && cap <= AS_CAP_HIGH && mod.slopes == nullptr && mod.bias == nullptr)
@@ -1570,7 +1566,7 @@ extern "C" int b200emb_op_attention_paged(const void* q, int64_t q_row_stride, v
   j.table_stride = cache->table_stride;
   j.head_first = cache->head_stride <= cache->token_stride;
   // rows of one copy: as many as divide both a page and a key tile
-  j.box_rows = cache->head_dim <= 64 ? AsCfg<64>::KV : AsCfg<128>::KV;
+  j.box_rows = AsCfg<128>::KV;
   while (cache->page_size % j.box_rows != 0) j.box_rows >>= 1;
   AsMaps m;
   rc = as_map_rows(&m.q, q, n_tokens, n_heads, cache->head_dim, q_row_stride, j.group, j.tile_tokens);
