@@ -46,7 +46,10 @@ static constexpr int AS_MAX_CTAS = 160;
 static constexpr int AS_MAX_SLOTS = 2 * AS_MAX_CTAS;
 static constexpr int AS_SOFTMAX_WARPS = 8, AS_K_WARP = 8, AS_V_WARP = 9, AS_MMA_WARP = 10;  // and 11: one a stream
 static constexpr int AS_THREADS = 12 * 32;
-static constexpr int AS_PLAN_THREADS = 1024;
+static constexpr int AS_PLAN_THREADS = 1024, AS_PLAN_CACHE = 1024;  // entries whose prefix sums the planner keeps in shared memory
+// What an item costs beside its steps, in steps (its loads, first scores, output): measured on 16 sequences of causal attention,
+// where slots of short items took 2.7 us an item longer than equal slots of long ones at 1.45 us a step.
+static constexpr int AS_ITEM_STEPS = 2;
 static constexpr int AS_STAGE = 16 * 64;           // output staging of a warp: 16 rows of 64 bytes
 static constexpr uint32_t AS_TMEM_COLS = 512;
 static constexpr int AS_COLD = 12;                 // words of a softmax warp's values that only an item's ends need
@@ -70,8 +73,8 @@ struct __align__(16) AttnEntry {
   int32_t seq, tok0, n_tok, pos0;     // first row of q and out, tokens, position of the first
   int32_t kv_len, kv_row0, prefix, n; // keys; packed: first row of k and v; visible prefix; key tiles visited
   int32_t a0, n0, a1, near;           // visited tiles: a0 .. a0 + n0 - 1, then the run from a1, tile a1 + near first, down, then up
-  int64_t before;                     // tiles of the entries in front (per key head)
-  int64_t pad2;
+  int64_t before;                     // key tiles of the entries in front (per key head)
+  int64_t cost;                       // the same with AS_ITEM_STEPS more for each entry
 };
 static_assert(sizeof(AttnEntry) == 64, "entry layout");
 
@@ -151,7 +154,7 @@ __device__ int64_t as_block_sum(int64_t v, int64_t* carry, int64_t* scratch) {
   if (lane == 31) scratch[warp] = x;
   __syncthreads();
   if (warp == 0) {
-    int64_t w = scratch[lane];
+    int64_t w = lane < (blockDim.x >> 5) ? scratch[lane] : 0;
 #pragma unroll
     for (int d = 1; d < 32; d <<= 1) {
       const int64_t y = __shfl_up_sync(0xffffffffu, w, d);
@@ -175,6 +178,8 @@ __global__ void __launch_bounds__(AS_PLAN_THREADS, 1)
 attn_plan_kernel(const AttnJob j, const AttnMod mod, const AttnPlan p, int tokens_per_entry, int max_slots, int kv) {
   __shared__ int64_t scratch[32];
   __shared__ int64_t carry;
+  __shared__ int64_t steps_of[AS_PLAN_CACHE];  // AttnEntry::before
+  __shared__ int64_t cuts[AS_MAX_SLOTS + 1];
   pdl_launch_dependents();
   pdl_wait();
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -182,11 +187,11 @@ attn_plan_kernel(const AttnJob j, const AttnMod mod, const AttnPlan p, int token
     *p.status = 0;
     carry = 0;
   }
-  for (int i = tid; i < 2 * max_slots; i += AS_PLAN_THREADS) p.counter[i] = 0;
-  for (int i = tid; i < max_slots; i += AS_PLAN_THREADS) p.slot[i] = AttnSlot{0, 0, 0, 0};
+  for (int i = tid; i < 2 * max_slots; i += static_cast<int>(blockDim.x)) p.counter[i] = 0;
+  for (int i = tid; i < max_slots; i += static_cast<int>(blockDim.x)) p.slot[i] = AttnSlot{0, 0, 0, 0};
   __syncthreads();
   // entries of each sequence
-  for (int base = 0; base < j.n_seqs; base += AS_PLAN_THREADS) {
+  for (int base = 0; base < j.n_seqs; base += static_cast<int>(blockDim.x)) {
     const int s = base + tid;
     int count = 0;
     if (s < j.n_seqs) {
@@ -202,7 +207,7 @@ attn_plan_kernel(const AttnJob j, const AttnMod mod, const AttnPlan p, int token
   if (mod.docs != nullptr) {
     // documents of every key tile (tokens of no document left out)
     const int records = j.n_tokens / kv + j.n_seqs;
-    for (int i = warp; i < records; i += AS_PLAN_THREADS / 32) {
+    for (int i = warp; i < records; i += (blockDim.x >> 5)) {
       int lo = 0, hi = j.n_seqs;
       while (hi - lo > 1) {
         const int mid = (lo + hi) >> 1;
@@ -228,7 +233,7 @@ attn_plan_kernel(const AttnJob j, const AttnMod mod, const AttnPlan p, int token
   }
   if (tid == 0) carry = 0;
   __syncthreads();
-  for (int base = 0; base < n_entries; base += AS_PLAN_THREADS) {
+  for (int base = 0; base < n_entries; base += static_cast<int>(blockDim.x)) {
     const int e = base + tid;
     AttnEntry x = {};
     int doc_lo = 0, doc_hi = INT_MAX;
@@ -311,43 +316,77 @@ attn_plan_kernel(const AttnJob j, const AttnMod mod, const AttnPlan p, int token
       }
     }
     x.before = as_block_sum(x.n, &carry, scratch);
-    if (e < n_entries) p.entry[e] = x;
+    x.cost = x.before + static_cast<int64_t>(AS_ITEM_STEPS) * e;
+    if (e < n_entries) {
+      p.entry[e] = x;
+      if (e < AS_PLAN_CACHE) steps_of[e] = x.before;
+    }
   }
-  // Equal parts of all steps; a cut moves to an item's edge that is nearer than 1/16 of a part.
-  const int64_t per_head = carry, total = per_head * j.n_kv_heads;
+  // Parts of equal cost; a cut moves to an item's edge that is nearer than 1/16 of a part.
+  const int heads = j.n_kv_heads;
+  const int64_t total = carry * heads, total_cost = (carry + static_cast<int64_t>(AS_ITEM_STEPS) * n_entries) * heads;
   const int slots = static_cast<int>(min(total, static_cast<int64_t>(max_slots)));
   __syncthreads();
   if (slots == 0) return;
-  const int64_t slack = total / (16 * static_cast<int64_t>(slots));
-  for (int s = tid; s <= slots; s += AS_PLAN_THREADS) {
-    int64_t at = total / slots * s + total % slots * s / slots;
-    if (s < slots) {
-      int lo = 0, hi = n_entries;
-      while (hi - lo > 1) {
-        const int mid = (lo + hi) >> 1;
-        if (p.entry[mid].before * j.n_kv_heads <= at) lo = mid;
-        else hi = mid;
-      }
-      const int n = p.entry[lo].n;
-      const int64_t in = at - p.entry[lo].before * j.n_kv_heads;
-      int h = static_cast<int>(in / n), k = static_cast<int>(in % n), e = lo;
-      if (k > 0 && k <= slack && k <= n - k) {
-        at -= k;
-        k = 0;
-      } else if (k > 0 && n - k <= slack) {
-        at += n - k;
-        k = 0;
-        if (++h == j.n_kv_heads) {
-          h = 0;
-          ++e;
-        }
-      }
-      p.slot[s] = AttnSlot{e, h, k, 0};
+  auto before_of = [&](int e) { return e < AS_PLAN_CACHE ? steps_of[e] : p.entry[e].before; };
+  auto last_entry = [&](int64_t at, int extra) {  // the last entry that starts at or before `at`, with `extra` steps for each in front
+    int lo = 0, hi = n_entries;
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) >> 1;
+      if ((before_of(mid) + static_cast<int64_t>(extra) * mid) * heads <= at) lo = mid;
+      else hi = mid;
     }
-    p.bound[s] = at;
+    return lo;
+  };
+  auto tiles_of = [&](int e) { return static_cast<int>((e + 1 < n_entries ? before_of(e + 1) : carry) - before_of(e)); };
+  const int64_t slack = total_cost / (16 * static_cast<int64_t>(slots));
+  for (int s = tid; s <= slots; s += static_cast<int>(blockDim.x)) {
+    int64_t cut = total;
+    if (s < slots) {
+      const int64_t at = total_cost / slots * s + total_cost % slots * s / slots;
+      const int e = last_entry(at, AS_ITEM_STEPS), n = tiles_of(e);
+      const int64_t in = at - (before_of(e) + static_cast<int64_t>(AS_ITEM_STEPS) * e) * heads;
+      const int h = static_cast<int>(in / (n + AS_ITEM_STEPS));
+      int k = min(max(static_cast<int>(in - static_cast<int64_t>(h) * (n + AS_ITEM_STEPS)) - AS_ITEM_STEPS / 2, 0), n);
+      if (k <= slack && k <= n - k) k = 0;
+      else if (n - k <= slack) k = n;
+      cut = before_of(e) * heads + static_cast<int64_t>(h) * n + k;
+    }
+    cuts[s] = cut - s;
   }
   __syncthreads();
-  for (int s = tid; s < slots; s += AS_PLAN_THREADS) p.slot[s].count = static_cast<int>(p.bound[s + 1] - p.bound[s]);
+  // every part has a step: the running maximum of (cut - number) makes the cuts strictly ascending, the end bounds them
+  if (warp == 0) {
+    const int per = (slots + 32) / 32;
+    int64_t top = INT64_MIN;
+    for (int i = 0; i < per; ++i)
+      if (lane * per + i <= slots) top = max(top, cuts[lane * per + i]);
+    int64_t front = top;
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+      const int64_t y = __shfl_up_sync(0xffffffffu, front, d);
+      if (lane >= d) front = max(front, y);
+    }
+    front = __shfl_up_sync(0xffffffffu, front, 1);
+    if (lane == 0) front = INT64_MIN;
+    for (int i = 0; i < per; ++i) {
+      const int s = lane * per + i;
+      if (s <= slots) {
+        front = max(front, cuts[s]);
+        cuts[s] = min(front + s, total - (slots - s));
+      }
+    }
+  }
+  __syncthreads();
+  for (int s = tid; s <= slots; s += static_cast<int>(blockDim.x)) {
+    const int64_t cut = cuts[s];
+    p.bound[s] = cut;
+    if (s < slots) {
+      const int e = last_entry(cut, 0), n = tiles_of(e);
+      const int64_t in = cut - before_of(e) * heads;
+      p.slot[s] = AttnSlot{e, static_cast<int>(in / n), static_cast<int>(in % n), static_cast<int>(cuts[s + 1] - cut)};
+    }
+  }
 }
 
 // ---- the attention kernel -----------------------------------------------------------------
@@ -361,12 +400,13 @@ struct AsCfg {
   static constexpr int Q_BLOCK = 128 * 128, Q_TILE = BLOCKS * Q_BLOCK;     // rows of 64 columns, 128-byte swizzle
   static constexpr int KV_BLOCK = KV * 128, KV_TILE = BLOCKS * KV_BLOCK;
   static constexpr int RING = D == 64 ? 8 : 4;  // key (and value) tiles in flight: 64 KB of each
+  static constexpr int Q_BUFS = D == 64 ? 2 : 1;  // query tiles of a stream
   static constexpr int STAGE_BYTES = AS_SOFTMAX_WARPS * AS_STAGE;
   static constexpr int TABLE_BYTES = 2 * AS_TABLE * 4;
   static constexpr int BAR_BYTES = 512;
   static constexpr int COLD_BYTES = AS_SOFTMAX_WARPS * AS_COLD * 4;
-  static constexpr int SMEM_BYTES = 2 * Q_TILE + 2 * RING * KV_TILE + STAGE_BYTES + TABLE_BYTES + BAR_BYTES + COLD_BYTES + 1024;
-  static constexpr int N_BARS = 4 * RING + 2 * 9;
+  static constexpr int SMEM_BYTES = 2 * Q_BUFS * Q_TILE + 2 * RING * KV_TILE + STAGE_BYTES + TABLE_BYTES + BAR_BYTES + COLD_BYTES + 1024;
+  static constexpr int N_BARS = 4 * RING + 4 * 2 + 2 * 7;
   static_assert(N_BARS * 8 + 16 <= BAR_BYTES, "barrier area");
   static_assert(SMEM_BYTES <= 232448, "shared memory");
   // Tensor memory of stream t: two score buffers of 64 columns, the accumulators, and P of a buffer's chunk of 32 keys in the first 16
@@ -541,12 +581,13 @@ attn_scored_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_cons
                    const __grid_constant__ AttnPlan plan) {
   using Cfg = AsCfg<D>;
   constexpr int RING = Cfg::RING, KV = Cfg::KV;
+  constexpr uint32_t Q_BUFS = Cfg::Q_BUFS;
   // A stream's own tiles in flight, so that neither stream waits for the other's; a pair has one ring.
   constexpr uint32_t SLOTS = PAIR ? RING : RING / 2;
   extern __shared__ uint8_t as_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(as_raw) + 1023) & ~uintptr_t(1023));
   uint8_t* q_s = smem;
-  uint8_t* k_s = q_s + 2 * Cfg::Q_TILE;
+  uint8_t* k_s = q_s + 2 * Cfg::Q_BUFS * Cfg::Q_TILE;
   uint8_t* v_s = k_s + RING * Cfg::KV_TILE;
   uint8_t* stage_s = v_s + RING * Cfg::KV_TILE;
   float* table_s = reinterpret_cast<float*>(stage_s + Cfg::STAGE_BYTES);
@@ -554,9 +595,9 @@ attn_scored_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_cons
   uint64_t* k_empty = k_full + RING;
   uint64_t* v_full = k_empty + RING;
   uint64_t* v_empty = v_full + RING;
-  uint64_t* q_full = v_empty + RING;  // the following ones per stream
-  uint64_t* q_empty = q_full + 2;
-  uint64_t* s_full = q_empty + 2;     // [stream][buffer] S of a step is in tensor memory
+  uint64_t* q_full = v_empty + RING;  // the following ones per stream: [stream][buffer]
+  uint64_t* q_empty = q_full + 4;
+  uint64_t* s_full = q_empty + 4;     // [stream][buffer] S of a step is in tensor memory
   uint64_t* p_full = s_full + 4;      // [stream][buffer] P of a step is in tensor memory, O may be added to
   uint64_t* pv_done = p_full + 4;     // [stream][buffer] P V of a step has finished
   uint64_t* group_bar = pv_done + 4;  // the softmax warps of a stream meet
@@ -573,9 +614,9 @@ attn_scored_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_cons
       mbar_init(&v_empty[i], PAIR ? 2 : 1);
     }
     for (int t = 0; t < 2; ++t) {
-      mbar_init(&q_full[t], 1);
-      mbar_init(&q_empty[t], 1);
       for (int b = 0; b < 2; ++b) {
+        mbar_init(&q_full[2 * t + b], 1);
+        mbar_init(&q_empty[2 * t + b], 1);
         mbar_init(&s_full[2 * t + b], 1);
         mbar_init(&p_full[2 * t + b], AS_SOFTMAX_WARPS / 2);
         mbar_init(&pv_done[2 * t + b], 1);
@@ -622,7 +663,7 @@ attn_scored_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_cons
         bool ready = as_test(&empty[slot], ((fills[t] / SLOTS) & 1u) ^ 1u);
         if (is_k && w[t].first) {
 #pragma unroll
-          for (int u = t; u < (PAIR ? 2 : t + 1); ++u) ready = ready && as_test(&q_empty[u], (q_fills[u] & 1u) ^ 1u);
+          for (int u = t; u < (PAIR ? 2 : t + 1); ++u) ready = ready && as_test(&q_empty[2 * u + q_fills[u] % Q_BUFS], ((q_fills[u] / Q_BUFS) & 1u) ^ 1u);
         }
         if (!__all_sync(0xffffffffu, ready)) continue;
         moved = true;
@@ -630,10 +671,11 @@ attn_scored_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_cons
 #pragma unroll
           for (int u = t; u < (PAIR ? 2 : t + 1); ++u) {
             if (lane == 0) {
-              mbar_arrive_expect_tx(&q_full[u], j.group * j.tile_tokens * 128 * Cfg::BLOCKS);
+              const uint32_t qb = q_fills[u] % Q_BUFS;
+              mbar_arrive_expect_tx(&q_full[2 * u + qb], j.group * j.tile_tokens * 128 * Cfg::BLOCKS);
 #pragma unroll
               for (int b = 0; b < Cfg::BLOCKS; ++b)
-                as_tma_3d(q_s + u * Cfg::Q_TILE + b * Cfg::Q_BLOCK, &tmap_q, &q_full[u], b * 64, w[t].h * j.group,
+                as_tma_3d(q_s + (u * Q_BUFS + qb) * Cfg::Q_TILE + b * Cfg::Q_BLOCK, &tmap_q, &q_full[2 * u + qb], b * 64, w[t].h * j.group,
                           w[t].f0.y + (PAIR ? u * j.tile_tokens : 0));
             }
             ++q_fills[u];
@@ -650,14 +692,14 @@ attn_scored_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_cons
       if (lane == 0) atomicExch(plan.status, is_k ? 5 : 8);
       for (int t = 0; t < (PAIR ? 1 : 2); ++t) as_drain(&full[t * SLOTS], fills[t], SLOTS);
       if (is_k)
-        for (int u = 0; u < 2; ++u) as_drain(&q_full[u], q_fills[u], 1);
+        for (int u = 0; u < 2; ++u) as_drain(&q_full[2 * u], q_fills[u], Q_BUFS);
     }
   } else if (warp >= AS_MMA_WARP) {
     // ---------------- matrix instructions of stream t: all lanes walk, one elected lane issues ----------------
     // (a warp for each stream: one warp that looks at both streams' barriers in turn answers each some hundred cycles later)
     const int t = warp - AS_MMA_WARP;
     const uint32_t tmem_u = __shfl_sync(0xffffffffu, tmem_base, 0);
-    const uint32_t q_addr = smem_u32(q_s) + t * Cfg::Q_TILE, k_addr = smem_u32(k_s), v_addr = smem_u32(v_s);
+    const uint32_t q_addr = smem_u32(q_s) + t * Q_BUFS * Cfg::Q_TILE, k_addr = smem_u32(k_s), v_addr = smem_u32(v_s);
     const uint32_t ring0 = PAIR ? 0 : t * SLOTS;
     AsWalk<KV> sw, pw;  // the next S, and the next P V
     sw.start(plan, PAIR ? blockIdx.x : blockIdx.x + t * gridDim.x);
@@ -669,14 +711,18 @@ attn_scored_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_cons
     auto wait_all = [](uint64_t* bar, uint32_t parity) -> bool { return __all_sync(0xffffffffu, mbar_wait(bar, parity)); };
     auto issue_s = [&]() -> bool {
       const uint32_t slot = ring0 + n_s % SLOTS, buf = n_s % 2;
-      if (sw.first && !wait_all(&q_full[t], q_uses++ & 1u)) return false;
+      if (sw.first) {
+        if (!wait_all(&q_full[2 * t + q_uses % Q_BUFS], (q_uses / Q_BUFS) & 1u)) return false;
+        ++q_uses;
+      }
+      const uint32_t qb = (q_uses - 1) % Q_BUFS;
       if (!wait_all(&k_full[slot], (n_s / SLOTS) & 1u)) return false;
       tc_fence_after_sync();
       const uint32_t idesc = make_idesc_bf16_f32(128, as_round16(sw.n_valid()));
       if (has_rows(sw)) {
 #pragma unroll
         for (int k = 0; k < D / 16; ++k) {
-          const uint64_t a = make_kmajor_sw128_desc(q_addr + (k / 4) * Cfg::Q_BLOCK) + 2 * (k % 4);
+          const uint64_t a = make_kmajor_sw128_desc(q_addr + qb * Cfg::Q_TILE + (k / 4) * Cfg::Q_BLOCK) + 2 * (k % 4);
           const uint64_t b = make_kmajor_sw128_desc(k_addr + slot * Cfg::KV_TILE + (k / 4) * Cfg::KV_BLOCK) + 2 * (k % 4);
           if (elect_one()) tc_mma_f16(tmem_u + t * Cfg::S(1, 0) + buf * Cfg::S(0, 1), a, b, idesc, k != 0);
         }
@@ -684,7 +730,7 @@ attn_scored_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_cons
       if (elect_one()) {
         tc_commit(&s_full[2 * t + buf]);
         tc_commit(&k_empty[slot]);
-        if (sw.last()) tc_commit(&q_empty[t]);
+        if (sw.last()) tc_commit(&q_empty[2 * t + qb]);
       }
       ++n_s;
       sw.next(plan, j.n_kv_heads);
@@ -773,6 +819,12 @@ attn_scored_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_cons
     float slope = 0.f;
     const float* tab = nullptr;
     float tab_unit = 1.f;
+    // every head's slope, for the whole launch (the tables of a bias are not in use then)
+    const bool slopes_here = MODE == AS_SLOPES && j.n_heads <= 2 * AS_TABLE;
+    if (slopes_here) {
+      for (int i = row; i < j.n_heads; i += 128) table_s[i] = __ldg(mod.slopes + i) * AS_LOG2E;  // both streams write the same
+      meet();
+    }
     while (cold[C_LEFT] > 0 && !failed) {
       // ---- one segment: an item, or this stream's part of one ----
       int i_k, i_end, run0, run_n0, run1, run_near, kv_len, pos, n_rows;
@@ -799,7 +851,8 @@ attn_scored_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_cons
           cold[C_N] = f1.w;
         }
         __syncwarp();
-        if ((MODE == AS_SLOPES || MODE == AS_ANY) && mod.slopes != nullptr) slope = __ldg(mod.slopes + h * j.group + g) * AS_LOG2E;
+        if ((MODE == AS_SLOPES || MODE == AS_ANY) && mod.slopes != nullptr)
+          slope = slopes_here ? table_s[h * j.group + g] : __ldg(mod.slopes + h * j.group + g) * AS_LOG2E;
         if (MODE == AS_ANY && mod.bias != nullptr) {
           const int width = 2 * mod.radius + 1, n = j.group * width;
           if (n <= AS_TABLE) {
@@ -1197,18 +1250,18 @@ attn_scored_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_cons
         int s0 = my_slot, s1 = my_slot;
         while (plan.bound[s0] > from) --s0;
         while (plan.bound[s1 + 1] < to) ++s1;
-        __threadfence();
-        meet();
+        meet();  // the part is written; one fence publishes what the barrier has gathered
         if (failed) break;
         if (row == 0) {
+          __threadfence();
           const int old = atomicAdd(&plan.counter[2 * s0 + (PAIR ? t : 0)], 1);
+          __threadfence();
           joins[t] = old == s1 - s0;
         }
         meet();
         if (failed) break;
         const bool join = joins[t] != 0;
         if (join) {
-          __threadfence();
           const int pieces = j.head_dim >> 3;
           for (int i = row; i < n_rows * pieces; i += 128) {
             const int piece = i / n_rows, r = i - piece * n_rows, col = piece * 8;
@@ -1385,7 +1438,9 @@ static int as_launch(const AsMaps& m, const AttnJob& j, const AttnMod& mod, cons
     if (steps < grid) grid = steps;
   }
   const int slots = static_cast<int>(PAIR ? grid : 2 * grid);
-  cudaError_t e = launch_pdl(attn_plan_kernel, dim3(1), dim3(AS_PLAN_THREADS), 0, s, j, mod, plan, (PAIR ? 2 : 1) * j.tile_tokens, slots, AsCfg<D>::KV);
+  // few entries are planned by fewer threads: their barriers are what it takes
+  const int threads = plan.max_entries <= 256 && j.n_seqs <= 256 ? 256 : AS_PLAN_THREADS;
+  cudaError_t e = launch_pdl(attn_plan_kernel, dim3(1), dim3(threads), 0, s, j, mod, plan, (PAIR ? 2 : 1) * j.tile_tokens, slots, AsCfg<D>::KV);
   if (e == cudaSuccess)
     e = launch_pdl(attn_scored_kernel<D, PAGED, PAIR, MODE>, dim3(static_cast<unsigned>(grid)), dim3(AS_THREADS), AsCfg<D>::SMEM_BYTES, s, m.q, m.k,
                    m.v, j, mod, plan);
