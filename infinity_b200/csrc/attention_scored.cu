@@ -204,10 +204,19 @@ attn_plan_kernel(const AttnJob j, const AttnMod mod, const AttnPlan p, int token
   const int n_entries = static_cast<int>(min(carry, static_cast<int64_t>(p.max_entries)));
   if (tid == 0) p.seq_first[j.n_seqs] = n_entries;
   __syncthreads();
+  auto sequence_of_entry = [&](int e) {  // the last sequence whose first entry is <= e: empty ones in front share it
+    int lo = 0, hi = j.n_seqs;
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) >> 1;
+      if (p.seq_first[mid] <= e) lo = mid;
+      else hi = mid;
+    }
+    return lo;
+  };
   if (mod.docs != nullptr) {
-    // documents of every key tile (tokens of no document left out)
+    // documents of every key tile (tokens of no document left out), a warp a tile
     const int records = j.n_tokens / kv + j.n_seqs;
-    for (int i = warp; i < records; i += (blockDim.x >> 5)) {
+    for (int i = warp; i < records; i += static_cast<int>(blockDim.x) >> 5) {
       int lo = 0, hi = j.n_seqs;
       while (hi - lo > 1) {
         const int mid = (lo + hi) >> 1;
@@ -230,6 +239,38 @@ attn_plan_kernel(const AttnJob j, const AttnMod mod, const AttnPlan p, int token
       if (lane == 0 && t0 < r.y) p.doc_range[i] = make_int2(dmin, dmax);
     }
     __syncthreads();
+    // first and past-the-last key tile whose documents meet an entry's (kept in its record), a warp an entry, 32 key tiles at a time
+    for (int e = warp; e < n_entries; e += static_cast<int>(blockDim.x) >> 5) {
+      const int s = sequence_of_entry(e);
+      const int2 r = as_rows_of(j, s);
+      const int q0 = (e - p.seq_first[s]) * tokens_per_entry, tiles = (r.y - r.x + kv - 1) / kv;
+      const int2* range = p.doc_range + as_doc_base(r.x, s, kv);
+      int dmin = INT_MAX, dmax = -1;
+      for (int t = q0 / kv + lane; t <= min(q0 + tokens_per_entry, r.y - r.x) / kv && t < tiles; t += 32) {
+        dmin = min(dmin, range[t].x);
+        dmax = max(dmax, range[t].y);
+      }
+      dmin = __reduce_min_sync(0xffffffffu, dmin);
+      dmax = __reduce_max_sync(0xffffffffu, dmax);
+      int first = INT_MAX, last = -1;
+      for (int t0 = 0; t0 < tiles; t0 += 32) {
+        bool meets = false;
+        if (t0 + lane < tiles) {
+          const int2 d = range[t0 + lane];
+          meets = d.x <= dmax && d.y >= dmin;
+        }
+        const uint32_t m = __ballot_sync(0xffffffffu, meets);
+        if (m) {
+          first = min(first, t0 + __ffs(m) - 1);
+          last = t0 + 31 - __clz(m);
+        }
+      }
+      if (lane == 0) {
+        p.entry[e].a0 = last < 0 ? 0 : first;
+        p.entry[e].n0 = last + 1;
+      }
+    }
+    __syncthreads();
   }
   if (tid == 0) carry = 0;
   __syncthreads();
@@ -238,12 +279,7 @@ attn_plan_kernel(const AttnJob j, const AttnMod mod, const AttnPlan p, int token
     AttnEntry x = {};
     int doc_lo = 0, doc_hi = INT_MAX;
     if (e < n_entries) {
-      int lo = 0, hi = j.n_seqs;  // the last sequence whose first entry is <= e: empty ones in front share it
-      while (hi - lo > 1) {
-        const int mid = (lo + hi) >> 1;
-        if (p.seq_first[mid] <= e) lo = mid;
-        else hi = mid;
-      }
+      const int lo = sequence_of_entry(e);
       const int2 r = as_rows_of(j, lo);
       const int q0 = (e - p.seq_first[lo]) * tokens_per_entry;
       x.seq = lo;
@@ -253,38 +289,9 @@ attn_plan_kernel(const AttnJob j, const AttnMod mod, const AttnPlan p, int token
       x.kv_len = j.kv_lens == nullptr ? r.y - r.x : min(max(j.kv_lens[lo], 0), j.table_stride * j.page_size);
       x.pos0 = x.kv_len - (r.y - r.x) + q0;
       x.prefix = mod.prefix == nullptr ? 0 : min(max(mod.prefix[lo], 0), x.kv_len);
-    }
-    if (mod.docs != nullptr) {  // a warp takes its 32 entries in turn, its lanes look at 32 key tiles at a time
-      for (int who = 0; who < 32; ++who) {
-        const int n_tok = __shfl_sync(0xffffffffu, x.n_tok, who);
-        if (n_tok <= 0) continue;
-        const int seq = __shfl_sync(0xffffffffu, x.seq, who), row0 = __shfl_sync(0xffffffffu, x.kv_row0, who);
-        const int tok0 = __shfl_sync(0xffffffffu, x.tok0, who), tiles = (__shfl_sync(0xffffffffu, x.kv_len, who) + kv - 1) / kv;
-        const int2* range = p.doc_range + as_doc_base(row0, seq, kv);
-        int dmin = INT_MAX, dmax = -1;
-        for (int t = (tok0 - row0) / kv + lane; t <= (tok0 - row0 + n_tok - 1) / kv; t += 32) {
-          dmin = min(dmin, range[t].x);
-          dmax = max(dmax, range[t].y);
-        }
-        dmin = __reduce_min_sync(0xffffffffu, dmin);
-        dmax = __reduce_max_sync(0xffffffffu, dmax);
-        int first = INT_MAX, last = -1;
-        for (int t0 = 0; t0 < tiles; t0 += 32) {
-          bool meets = false;
-          if (t0 + lane < tiles) {
-            const int2 d = range[t0 + lane];
-            meets = d.x <= dmax && d.y >= dmin;
-          }
-          const uint32_t m = __ballot_sync(0xffffffffu, meets);
-          if (m) {
-            first = min(first, t0 + __ffs(m) - 1);
-            last = t0 + 31 - __clz(m);
-          }
-        }
-        if (lane == who) {
-          doc_lo = last < 0 ? 0 : first;
-          doc_hi = last + 1;
-        }
+      if (mod.docs != nullptr) {
+        doc_lo = p.entry[e].a0;
+        doc_hi = p.entry[e].n0;
       }
     }
     if (e < n_entries) {
@@ -889,17 +896,17 @@ attn_scored_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_cons
       float ref = 0.f, l_run = 0.f;  // reference (log2 units), and the sum of the exponentials against it
       bool first = true;
       int kv0 = key0_of(i_k);
+      int next_docs[2] = {-1, -1};  // documents of a step's keys, lane l's of l and 32 + l: asked for a step ahead
+      auto docs_of = [&](int key) {
+#pragma unroll
+        for (int q = 0; q < 2; ++q) next_docs[q] = key + q * 32 + lane < kv_len ? __ldg(mod.docs + cold[C_KVROW0] + key + q * 32 + lane) : -1;
+      };
+      if (MODE == AS_ANY && mod.docs != nullptr) docs_of(kv0);
       for (; i_k < i_end; ++i_k) {
         const int buf = step % 2, n_valid = min(max(kv_len - kv0, 0), KV), n_rem = as_round16(n_valid);
-        const int next_kv0 = key0_of(i_k + 1);
-        int key_docs[KV / 32] = {};  // documents of the step's keys, lane l's of 32 l' + l
-        if (MODE == AS_ANY && mod.docs != nullptr) {
-#pragma unroll
-          for (int q = 0; q < KV / 32; ++q) {
-            const int key = kv0 + q * 32 + lane;
-            key_docs[q] = key < kv_len ? __ldg(mod.docs + cold[C_KVROW0] + key) : -1;
-          }
-        }
+        const int next_kv0 = i_k + 1 < i_end ? key0_of(i_k + 1) : 0;
+        int key_docs[2] = {next_docs[0], next_docs[1]};
+        if (MODE == AS_ANY && mod.docs != nullptr) docs_of(next_kv0);
         if (!mbar_wait(&s_full[2 * t + buf], (step / 2) & 1u)) failed = true;  // looked at below, once a step
         tc_fence_after_sync();
         if (active) {
@@ -912,7 +919,7 @@ attn_scored_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_cons
             uint32_t seen = (as_below(key_hi() - key) & ~as_below(key_lo() - key)) | as_below(cold[C_PREFIX] - key);
             if (MODE == AS_ANY && mod.docs != nullptr) {
               // the keys of each document that some row of the warp belongs to
-              const int key_doc = key_docs[q];
+              const int key_doc = q == 0 ? key_docs[0] : key_docs[1];
               uint32_t same = 0, todo = __ballot_sync(0xffffffffu, doc >= 0);
               while (todo) {
                 const int d = __shfl_sync(0xffffffffu, doc, __ffs(todo) - 1);
@@ -924,46 +931,91 @@ attn_scored_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_cons
             }
             return seen;
           };
-          // O follows a reference that has moved (by a whole power of two: nothing is rounded)
-          auto rescale = [&](float alpha) {
-            if (first || !__any_sync(0xffffffffu, alpha != 1.f)) return;
-            if (!pv_wait(step - 1)) failed = true;
-            tc_fence_after_sync();
+          // O, and P of the first 32 keys when the second are at work, follow a reference that has moved (by a whole power of two: nothing
+          // is rounded)
+          auto rescale = [&](float alpha, bool p_too) {
+            if (!__any_sync(0xffffffffu, alpha != 1.f)) return;
+            if (!first) {
+              if (!pv_wait(step - 1)) failed = true;
+              tc_fence_after_sync();
 #pragma unroll 1
-            for (int c = 0; c < D; c += 16) {
-              uint32_t o[16];
-              tmem_ld_32x32b_x16(lanes + Cfg::O(t) + c, o);
-              tmem_ld_wait_for16(o);
+              for (int c = 0; c < D; c += 16) {
+                uint32_t o[16];
+                tmem_ld_32x32b_x16(lanes + Cfg::O(t) + c, o);
+                tmem_ld_wait_for16(o);
 #pragma unroll
-              for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * alpha);
-              tmem_st_32x32b_x16(lanes + Cfg::O(t) + c, o);
-            }
-            tmem_st_wait();
-          };
-          uint32_t pk[2][16];  // the row's probabilities, two to a register
-          float total;
-          auto exponentials = [&](const float2 (&e2)[2][16], bool both) {
-            float2 sum = make_float2(0.f, 0.f), sum1 = make_float2(0.f, 0.f);
-#pragma unroll
-            for (int g2 = 0; g2 < 2; ++g2) {
-              if (g2 == 0 || both) {
-#pragma unroll
-                for (int i = 0; i < 16; i += 2) {
-                  const float2 a = make_float2(as_ex2(e2[g2][i].x), as_ex2(e2[g2][i].y)), b = make_float2(as_ex2(e2[g2][i + 1].x), as_ex2(e2[g2][i + 1].y));
-                  sum = __fadd2_rn(sum, a);
-                  sum1 = __fadd2_rn(sum1, b);
-                  const __nv_bfloat162 ha = __floats2bfloat162_rn(a.x, a.y), hb = __floats2bfloat162_rn(b.x, b.y);
-                  pk[g2][i] = *reinterpret_cast<const uint32_t*>(&ha);
-                  pk[g2][i + 1] = *reinterpret_cast<const uint32_t*>(&hb);
-                }
+                for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * alpha);
+                tmem_st_32x32b_x16(lanes + Cfg::O(t) + c, o);
               }
             }
-            total = (sum.x + sum1.x) + (sum.y + sum1.y);
+            tmem_st_wait();
+            if (p_too) {
+              uint32_t o[16];
+              tmem_ld_32x32b_x16(s_at, o);
+              tmem_ld_wait_for16(o);
+#pragma unroll
+              for (int i = 0; i < 16; ++i) {
+                const float2 x = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&o[i]));
+                const __nv_bfloat162 h2 = __floats2bfloat162_rn(x.x * alpha, x.y * alpha);
+                o[i] = *reinterpret_cast<const uint32_t*>(&h2);
+              }
+              tmem_st_32x32b_x16(s_at, o);
+              tmem_st_wait();
+            }
+          };
+          // probabilities of 32 keys, two to a register, and their sum
+          auto exponentials = [&](const float2 (&e2)[16], uint32_t (&pk)[16]) -> float {
+            float2 sum = make_float2(0.f, 0.f), sum1 = make_float2(0.f, 0.f);
+#pragma unroll
+            for (int i = 0; i < 16; i += 2) {
+              const float2 a = make_float2(as_ex2(e2[i].x), as_ex2(e2[i].y)), b = make_float2(as_ex2(e2[i + 1].x), as_ex2(e2[i + 1].y));
+              sum = __fadd2_rn(sum, a);
+              sum1 = __fadd2_rn(sum1, b);
+              const __nv_bfloat162 ha = __floats2bfloat162_rn(a.x, a.y), hb = __floats2bfloat162_rn(b.x, b.y);
+              pk[i] = *reinterpret_cast<const uint32_t*>(&ha);
+              pk[i + 1] = *reinterpret_cast<const uint32_t*>(&hb);
+            }
+            return (sum.x + sum1.x) + (sum.y + sum1.y);
+          };
+          // AS_ANY: 32 scores into exponents against the reference
+          auto any_scores = [&](const uint32_t (&z)[32], int key32, float2 (&e2)[16]) {
+            float y[32];
+#pragma unroll
+            for (int i = 0; i < 32; ++i) y[i] = __uint_as_float(z[i]);
+            if (mod.cap > 0.f) {
+#pragma unroll
+              for (int i = 0; i < 32; ++i) y[i] = fmaf(cap_out, as_tanh(y[i] * cap_in), -ref);
+            } else {
+#pragma unroll
+              for (int i = 0; i < 32; ++i) y[i] = fmaf(y[i], scale_log2, -ref);
+            }
+            const int d0 = key32 - pos;
+            if (mod.slopes != nullptr) {
+              const float f = static_cast<float>(d0);
+#pragma unroll
+              for (int i = 0; i < 32; ++i) y[i] = fmaf(-slope, fabsf(f + static_cast<float>(i)), y[i]);
+            }
+            if (mod.bias != nullptr) {
+              if (key32 + 31 - pos_first <= -mod.radius || key32 - pos_last >= mod.radius) {  // beyond the table for all rows
+                const float b = tab[key32 < pos_last ? -mod.radius : mod.radius] * tab_unit;
+#pragma unroll
+                for (int i = 0; i < 32; ++i) y[i] += b;
+              } else if (key32 - pos_last >= -mod.radius && key32 + 31 - pos_first <= mod.radius && real) {  // inside for all rows
+                const float* from = tab + d0;
+#pragma unroll
+                for (int i = 0; i < 32; ++i) y[i] = fmaf(from[i], tab_unit, y[i]);
+              } else {
+#pragma unroll
+                for (int i = 0; i < 32; ++i) y[i] = fmaf(tab[min(max(d0 + i, -mod.radius), mod.radius)], tab_unit, y[i]);
+              }
+            }
+#pragma unroll
+            for (int i = 0; i < 16; ++i) e2[i] = make_float2(y[2 * i], y[2 * i + 1]);
           };
           // Most steps: every row sees all 64 keys, the reference stands, nothing is asked of a score one by one. What does not fit
           // (a sum out of range, a score beyond the cap, a wait that gave up) is taken again below, from the same scores.
           bool done = false;
-          if (MODE != AS_ANY && whole && (MODE == AS_CAP || !first) && (MODE != AS_SLOPES || kv0 + KV <= pos_first || kv0 > pos_last)) {
+          if (whole && (MODE == AS_CAP || !first) && (MODE != AS_SLOPES || kv0 + KV <= pos_first || kv0 > pos_last)) {
             uint32_t z[2][32];
             tmem_ld_32x32b_x32(s_at, z[0]);
             tmem_ld_32x32b_x32(s_at + 32, z[1]);
@@ -985,6 +1037,9 @@ attn_scored_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_cons
                 e2[i >> 4][i & 15] = __ffma2_rn(two(i >> 4, i & 15), scale2, bias2);
                 bias2 = __fadd2_rn(bias2, rise2);
               }
+            } else if (MODE == AS_ANY) {
+              any_scores(z[0], kv0, e2[0]);
+              any_scores(z[1], kv0 + 32, e2[1]);
             } else {
               float top = 0.f;
 #pragma unroll
@@ -996,167 +1051,115 @@ attn_scored_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_cons
                 e2[i >> 4][i & 15] = tanh_near(v, __fmul2_rn(v, v));
               }
             }
-            exponentials(e2, true);
+            uint32_t pk[2][16];
+            float total = exponentials(e2[0], pk[0]);
+            total += exponentials(e2[1], pk[1]);
             const float sum_now = l_run + total;
             if (MODE != AS_CAP) odd = odd || !(sum_now >= AS_SUM_LOW && sum_now <= AS_SUM_HIGH);
             done = (__ballot_sync(0xffffffffu, odd) & real_rows) == 0u;
-          }
-          if (!done) {
-            const bool both = n_rem > 32;
-            uint32_t seen[2] = {0xffffffffu, 0xffffffffu};
-            if (!whole) {
-              seen[0] = seen_of(0);
-              seen[1] = both ? seen_of(1) : 0u;
+            if (done) {
+              l_run = sum_now;
+              tmem_st_32x32b_x16(s_at, pk[0]);
+              tmem_st_32x32b_x16(s_at + 32, pk[1]);
             }
-            // Normally once. A row whose sum leaves its range moves its reference, and the scores, still where they were, are taken again.
-            bool moves = MODE != AS_CAP && first && real;  // the segment's first scores set the reference
+          }
+          // 32 keys at a time: masks, the segment's first scores, references that move. (Kept small in registers: what spills from here is
+          // a trip to L2 each, shared memory has taken all of L1.)
+#pragma unroll 1
+          for (int q = 0; !done && q * 32 < n_rem; ++q) {
+            const int key32 = kv0 + q * 32;
+            uint32_t seen = 0xffffffffu;
+            if (!whole) seen = seen_of(q);
+            bool moves = MODE != AS_CAP && first && q == 0 && real;  // the segment's first scores set the reference
             bool again = false;
+            float total;
+            uint32_t pk[16];
 #pragma unroll 1
             while (true) {
-            uint32_t z[2][32];
-            tmem_ld_32x32b_x32(s_at, z[0]);
-            if (both) tmem_ld_32x32b_x32(s_at + 32, z[1]);
-            const bool guess = MODE != AS_CAP && first && !again;
-            tmem_ld_wait_for(z[0]);
-            tmem_ld_wait_for(z[1]);
-            float2 e2[2][16];  // exponents against the reference
-            float raw_max = -INFINITY;
+              uint32_t z[32];
+              tmem_ld_32x32b_x32(s_at + q * 32, z);
+              tmem_ld_wait_for(z);
+              const bool guess = MODE != AS_CAP && first && q == 0 && !again;
+              float2 e2[16];  // exponents against the reference
+              float mx = -INFINITY;
+              auto two = [&](int i) { return make_float2(__uint_as_float(z[2 * i]), __uint_as_float(z[2 * i + 1])); };
+              if (MODE == AS_SLOPES && guess) {
+                // the first guess takes the bias of the step's nearest key, which later scores will not exceed by much
 #pragma unroll
-            for (int g2 = 0; g2 < 2; ++g2) {
-              if (g2 == 0 || both) {
-                const int key32 = kv0 + g2 * 32;
-                auto two = [&](int i) { return make_float2(__uint_as_float(z[g2][2 * i]), __uint_as_float(z[g2][2 * i + 1])); };
-                if (MODE == AS_SLOPES && guess) {
+                for (int i = 0; i < 32; ++i) mx = fmaxf(mx, (seen >> i) & 1u ? __uint_as_float(z[i]) * scale_log2 : -INFINITY);
+                mx -= slope * static_cast<float>(max(max(kv0 - pos, pos - (kv0 + n_valid - 1)), 0));
+              }
+              if (MODE == AS_PLAIN) {
+                const float2 base2 = make_float2(-ref, -ref);
 #pragma unroll
-                  for (int i = 0; i < 32; ++i) raw_max = fmaxf(raw_max, (seen[g2] >> i) & 1u ? __uint_as_float(z[g2][i]) * scale_log2 : -INFINITY);
-                }
-                if (MODE == AS_PLAIN) {
-                  const float2 base2 = make_float2(-ref, -ref);
+                for (int i = 0; i < 16; ++i) e2[i] = __ffma2_rn(two(i), scale2, base2);
+              } else if (MODE == AS_SLOPES) {
+                const float f = static_cast<float>(key32 - pos);
 #pragma unroll
-                  for (int i = 0; i < 16; ++i) e2[g2][i] = __ffma2_rn(two(i), scale2, base2);
-                } else if (MODE == AS_SLOPES) {
-                  const float f = static_cast<float>(key32 - pos);
-                  if (key32 + 31 <= pos_first || key32 >= pos_last) {
-                    // all 32 keys on one side of the queries: the bias is linear in the key
-                    const float rise = key32 < pos_last ? slope : -slope;
-                    const float2 rise2 = make_float2(2.f * rise, 2.f * rise);
-                    float2 bias2 = make_float2(fmaf(rise, f, -ref), fmaf(rise, f + 1.f, -ref));
+                for (int i = 0; i < 16; ++i)
+                  e2[i] = __ffma2_rn(two(i), scale2, make_float2(fmaf(-slope, fabsf(f + static_cast<float>(2 * i)), -ref),
+                                                                 fmaf(-slope, fabsf(f + static_cast<float>(2 * i + 1)), -ref)));
+              } else if (MODE == AS_CAP) {
+                // Which way the tanh goes is decided by what is seen alone: columns that no key wrote and rows of no token hold whatever was
+                // there before, and results must not depend on it.
+                float top = 0.f;
 #pragma unroll
-                    for (int i = 0; i < 16; ++i) {
-                      e2[g2][i] = __ffma2_rn(two(i), scale2, bias2);
-                      bias2 = __fadd2_rn(bias2, rise2);
-                    }
-                  } else {
-#pragma unroll
-                    for (int i = 0; i < 16; ++i)
-                      e2[g2][i] = __ffma2_rn(two(i), scale2, make_float2(fmaf(-slope, fabsf(f + static_cast<float>(2 * i)), -ref),
-                                                                         fmaf(-slope, fabsf(f + static_cast<float>(2 * i + 1)), -ref)));
-                  }
-                } else if (MODE == AS_CAP) {
-                  // Which way the tanh goes is decided by what is seen alone: columns that no key wrote and rows of no token hold whatever
-                  // was there before, and results must not depend on it.
-                  float top = 0.f;
-                  if (whole) {
-#pragma unroll
-                    for (int i = 0; i < 32; i += 2) top = as_max3_abs(top, __uint_as_float(z[g2][i]), __uint_as_float(z[g2][i + 1]));
-                  } else {
-#pragma unroll
-                    for (int i = 0; i < 32; ++i) top = fmaxf(top, (seen[g2] >> i) & 1u ? fabsf(__uint_as_float(z[g2][i])) : 0.f);
-                  }
-                  if ((__ballot_sync(0xffffffffu, top > cap_far) & real_rows) == 0u) {
-#pragma unroll
-                    for (int i = 0; i < 16; ++i) {
-                      const float2 v = __fmul2_rn(two(i), scale2);
-                      e2[g2][i] = tanh_near(v, __fmul2_rn(v, v));
-                    }
-                  } else {
-#pragma unroll
-                    for (int i = 0; i < 16; ++i) {
-                      const float2 v = two(i);
-                      e2[g2][i] = make_float2(cap_out * as_tanh(v.x * cap_in), cap_out * as_tanh(v.y * cap_in));
-                    }
-                  }
-                } else {
-                  float y[32];
-#pragma unroll
-                  for (int i = 0; i < 32; ++i) y[i] = __uint_as_float(z[g2][i]);
-                  if (mod.cap > 0.f) {
-#pragma unroll
-                    for (int i = 0; i < 32; ++i) y[i] = fmaf(cap_out, as_tanh(y[i] * cap_in), -ref);
-                  } else {
-#pragma unroll
-                    for (int i = 0; i < 32; ++i) y[i] = fmaf(y[i], scale_log2, -ref);
-                  }
-                  const int d0 = key32 - pos;
-                  if (mod.slopes != nullptr) {
-                    const float f = static_cast<float>(d0);
-#pragma unroll
-                    for (int i = 0; i < 32; ++i) y[i] = fmaf(-slope, fabsf(f + static_cast<float>(i)), y[i]);
-                  }
-                  if (mod.bias != nullptr) {
-                    if (key32 + 31 - pos_first <= -mod.radius || key32 - pos_last >= mod.radius) {
-                      const float b = tab[key32 < pos_last ? -mod.radius : mod.radius] * tab_unit;
-#pragma unroll
-                      for (int i = 0; i < 32; ++i) y[i] += b;
-                    } else {
-#pragma unroll
-                      for (int i = 0; i < 32; ++i) y[i] = fmaf(tab[min(max(d0 + i, -mod.radius), mod.radius)], tab_unit, y[i]);
-                    }
-                  }
-#pragma unroll
-                  for (int i = 0; i < 16; ++i) e2[g2][i] = make_float2(y[2 * i], y[2 * i + 1]);
-                }
-                if (!whole) {
+                for (int i = 0; i < 32; ++i) top = fmaxf(top, (seen >> i) & 1u ? fabsf(__uint_as_float(z[i])) : 0.f);
+                if ((__ballot_sync(0xffffffffu, top > cap_far) & real_rows) == 0u) {
 #pragma unroll
                   for (int i = 0; i < 16; ++i) {
-                    if (!((seen[g2] >> (2 * i)) & 1u)) e2[g2][i].x = -INFINITY;
-                    if (!((seen[g2] >> (2 * i + 1)) & 1u)) e2[g2][i].y = -INFINITY;
+                    const float2 v = __fmul2_rn(two(i), scale2);
+                    e2[i] = tanh_near(v, __fmul2_rn(v, v));
+                  }
+                } else {
+#pragma unroll
+                  for (int i = 0; i < 16; ++i) {
+                    const float2 v = two(i);
+                    e2[i] = make_float2(cap_out * as_tanh(v.x * cap_in), cap_out * as_tanh(v.y * cap_in));
                   }
                 }
+              } else {
+                any_scores(z, key32, e2);
               }
-            }
-            if (MODE != AS_CAP && (guess || again)) {
-              // The reference moves to the larger of these scores and the logarithm of the sum so far (which lies far below it where the
-              // reference was a bad guess), by a whole number. With slopes the first guess takes the bias of the step's nearest key, which
-              // later scores will not exceed by much.
-              float mx = raw_max - (MODE == AS_SLOPES ? slope * static_cast<float>(max(max(kv0 - pos, pos - (kv0 + n_valid - 1)), 0)) : 0.f);
-              if (MODE != AS_SLOPES || again) {
-                float m1 = -INFINITY;
-                mx = -INFINITY;
+              if (!whole) {
 #pragma unroll
-                for (int i = 0; i < 16; ++i) mx = as_max3(mx, e2[0][i].x, e2[0][i].y);
-                if (both) {
-#pragma unroll
-                  for (int i = 0; i < 16; ++i) m1 = as_max3(m1, e2[1][i].x, e2[1][i].y);
+                for (int i = 0; i < 16; ++i) {
+                  if (!((seen >> (2 * i)) & 1u)) e2[i].x = -INFINITY;
+                  if (!((seen >> (2 * i + 1)) & 1u)) e2[i].y = -INFINITY;
                 }
-                mx = fmaxf(mx, m1);
               }
-              float by = ceilf(fmaxf(mx, l_run > 0.f ? __log2f(l_run) : -INFINITY));
-              if (!moves || by == -INFINITY) by = 0.f;
-              const float alpha = l_run > 0.f ? as_ex2(-by) : by != 0.f ? l_run : 1.f;  // nothing summed: 0, and NaN stays NaN
-              l_run *= alpha;
-              ref += by;
+              if (MODE != AS_CAP && (guess || again)) {
+                // The reference moves to the larger of these scores and the logarithm of the sum so far (which lies far below it where the
+                // reference was a bad guess), by a whole number.
+                if (MODE != AS_SLOPES || again) {
 #pragma unroll
-              for (int i = 0; i < 32; ++i) e2[i >> 4][i & 15] = __fadd2_rn(e2[i >> 4][i & 15], make_float2(-by, -by));
-              if (again) rescale(alpha);
+                  for (int i = 0; i < 16; ++i) mx = as_max3(mx, e2[i].x, e2[i].y);
+                }
+                float by = ceilf(fmaxf(mx, l_run > 0.f ? __log2f(l_run) : -INFINITY));
+                if (!moves || by == -INFINITY) by = 0.f;
+                const float alpha = l_run > 0.f ? as_ex2(-by) : by != 0.f ? l_run : 1.f;  // nothing summed: 0, and NaN stays NaN
+                l_run *= alpha;
+                ref += by;
+#pragma unroll
+                for (int i = 0; i < 16; ++i) e2[i] = __fadd2_rn(e2[i], make_float2(-by, -by));
+                if (again) rescale(alpha, q != 0);
+              }
+              total = exponentials(e2, pk);
+              if (again) break;
+              // sums out of range, and waits that gave up
+              const float sum_now = l_run + total;
+              const bool bad = MODE != AS_CAP && seen != 0u && !(sum_now >= AS_SUM_LOW && sum_now <= AS_SUM_HIGH);
+              if ((__ballot_sync(0xffffffffu, bad || failed) & real_rows) == 0u) break;
+              failed = __any_sync(0xffffffffu, failed);
+              if (failed) break;
+              moves = bad && real;
+              again = true;
             }
-            exponentials(e2, both);
-            if (again) break;
-            // one vote a step: sums out of range, and waits that gave up
-            const float sum_now = l_run + total;
-            bool bad = MODE != AS_CAP && !(sum_now >= AS_SUM_LOW && sum_now <= AS_SUM_HIGH);
-            if (!whole) bad = bad && (seen[0] | seen[1]) != 0u;
-            if ((__ballot_sync(0xffffffffu, bad || failed) & real_rows) == 0u) break;
-            failed = __any_sync(0xffffffffu, failed);
             if (failed) break;
-            moves = bad && real;
-            again = true;
-            }
-            if (failed) break;
+            l_run += total;
+            tmem_st_32x32b_x16(s_at + q * 32, pk);
           }
-          l_run += total;
-          tmem_st_32x32b_x16(s_at, pk[0]);
-          if (n_rem > 32) tmem_st_32x32b_x16(s_at + 32, pk[1]);
+          if (failed) break;
           tmem_st_wait();
           tc_fence_before_sync();
           __syncwarp();
@@ -1428,7 +1431,9 @@ struct AsMaps {
 };
 
 // Two neighbouring tiles share their keys where sequences have two tiles of rows on average; shorter ones would leave stream B idle.
-static bool as_pair(const AttnJob& j) { return static_cast<int64_t>(j.n_tokens) * j.group >= 256ll * j.n_seqs; }
+// Documents keep each tile to its own few keys. (8 sequences of 2048, causal, 28/4 heads of 128: 404 us in pairs, 423 without; 192 of 8 to
+// 512, 16 heads of 64: 219 and 193.)
+static bool as_pair(const AttnJob& j, const AttnMod& mod) { return mod.docs == nullptr && static_cast<int64_t>(j.n_tokens) * j.group >= 256ll * j.n_seqs; }
 
 template <int D, bool PAGED, bool PAIR, int MODE>
 static int as_launch(const AsMaps& m, const AttnJob& j, const AttnMod& mod, const AttnPlan& plan, int sms, cudaStream_t s) {
@@ -1513,7 +1518,7 @@ static int as_dispatch(const AsMaps& m, const AttnJob& j, const AttnMod& mod, vo
   if (rc) return rc;
   AttnPlan plan;
   as_layout(workspace, j.n_seqs, j.n_tokens, j.n_heads, j.n_kv_heads, j.head_dim, &plan);
-  const bool pair = as_pair(j);
+  const bool pair = as_pair(j, mod);
   if (j.head_dim <= 64)
     return pair ? as_launch_mode<64, PAGED, true>(m, j, mod, plan, sms, s) : as_launch_mode<64, PAGED, false>(m, j, mod, plan, sms, s);
   return pair ? as_launch_mode<128, PAGED, true>(m, j, mod, plan, sms, s) : as_launch_mode<128, PAGED, false>(m, j, mod, plan, sms, s);
