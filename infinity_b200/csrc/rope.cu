@@ -14,7 +14,7 @@
 namespace b2 {
 
 static constexpr int ROPE_MAX_PAIRS = 128;
-static constexpr int ROPE_THREADS = 256;
+static constexpr int ROPE_MAX_THREADS = 128;
 
 struct RopeParams {
   double w[ROPE_MAX_PAIRS];  // angle per position of pair i
@@ -40,15 +40,22 @@ struct RopeJob {
   const int32_t* page_table;
   int64_t page_stride, token_stride, head_stride;
   int n_pages, page_size, n_kv_heads, table_stride;
+  // set at launch, for the chosen V
+  int n_rot_heads, first_head, rot_items, per_head, turned, items;
 };
 
-// Sequence of token t: the last s with cu[s] <= t (empty sequences share a start; the last of them owns the token).
+// Sequence of token t: the last s with cu[s] <= t (empty sequences share a start; the last of them owns the token). The warp looks
+// at 32 starts at a time: two dependent reads for up to 1024 sequences.
 __device__ __forceinline__ int sequence_of(const int32_t* __restrict__ cu, int n_seqs, int t) {
-  int lo = 0, hi = n_seqs;
-  while (hi - lo > 1) {
-    const int mid = (lo + hi) >> 1;
-    if (__ldg(cu + mid) <= t) lo = mid;
-    else hi = mid;
+  const int lane = threadIdx.x & 31;
+  int lo = 0, n = n_seqs;
+  while (n > 1) {
+    const int step = (n + 31) / 32;
+    const bool in = lane * step < n;
+    const int below = __popc(__ballot_sync(0xffffffffu, in && __ldg(cu + lo + lane * step) <= t));
+    const int at = max(below - 1, 0) * step;
+    lo += at;
+    n = min(step, n - at);
   }
   return lo;
 }
@@ -79,12 +86,45 @@ union Pack {
   __device__ Pack() {}
 };
 
-// One block per token. An item is V elements of the interleaved layout or of the part that passes through, or V
-// elements of the first half together with the V they pair with.
+// One block per token. An item is V elements of the interleaved layout or of a part that passes through, or V elements of the
+// first half together with the V they pair with. A thread asks for its item before the block works out its position and angles, so that
+// the row is on its way meanwhile. Reading and writing the row once is all the kernel cannot do without; what bounds it is instructions
+// (76 % of the issue slots with 512 threads a block), so a block is small: the search, the angles and the barrier are paid by every
+// warp of it. 19 506 tokens of 32 heads of 128, half of each turned (320 MB, 49 us at the copy rate): 62 us with 64 or 128 threads, 66 with
+// 256, 80 with 512; 94 us where 256 threads read after the angles; 111 us and more with blocks that stay and ask a token ahead. Keys and
+// values of 8 483 tokens into their pages (156 MB, 24 us): 37 us.
 template <int V, bool APPEND>
-__global__ void __launch_bounds__(ROPE_THREADS) rope_kernel_op(const __grid_constant__ RopeParams p, const __grid_constant__ RopeJob j) {
+__global__ void __launch_bounds__(ROPE_MAX_THREADS) rope_kernel_op(const __grid_constant__ RopeParams p, const __grid_constant__ RopeJob j) {
   __shared__ float2 cs[ROPE_MAX_PAIRS];
+  using T = typename Vec<V>::T;
   const int t = blockIdx.x;
+  const int hd = j.head_dim;
+  const int turned = j.turned, items = j.items;  // items of heads that turn, and with those of the values
+  const __nv_bfloat16* row = j.x + static_cast<int64_t>(t) * j.x_stride;
+  Pack<V> a, b;
+  int head = 0, e = 0, kind = 0;  // head of the row, first element of it, and 0 copied, 1 interleaved, 2 halves
+  auto fetch = [&](int w) {
+    if (APPEND && w >= turned) {
+      const int vecs = hd / V;
+      head = (w - turned) / vecs;
+      e = (w - turned - head * vecs) * V;
+      head += j.n_rot_heads;
+      kind = 0;
+    } else {
+      head = w / j.per_head;
+      const int g = w - head * j.per_head;
+      head += j.first_head;
+      const bool turns = g < j.rot_items;
+      e = turns ? g * V : 2 * p.n_pairs + (g - j.rot_items) * V;
+      kind = !turns ? 0 : p.interleaved ? 1 : 2;
+    }
+    const __nv_bfloat16* src = row + static_cast<int64_t>(head) * hd + e;
+    a.raw = *reinterpret_cast<const T*>(src);
+    if (kind == 2) b.raw = *reinterpret_cast<const T*>(src + p.n_pairs);
+    if (V == 1 && kind == 1 && (e & 1) == 0) b.raw = *reinterpret_cast<const T*>(src + 1);
+  };
+  if (threadIdx.x < items) fetch(threadIdx.x);
+
   int pos, seq = 0;
   if (!APPEND && j.positions != nullptr) {
     pos = __ldg(j.positions + t);
@@ -95,22 +135,6 @@ __global__ void __launch_bounds__(ROPE_THREADS) rope_kernel_op(const __grid_cons
     if (APPEND) pos = __ldg(j.pos_start + seq) - (end - first) + (t - first);
     else pos = (j.pos_start != nullptr ? __ldg(j.pos_start + seq) : 0) + (t - first);
   }
-  for (int i = threadIdx.x; i < p.n_pairs; i += ROPE_THREADS) {
-    const double a = static_cast<double>(pos) * p.w[i];
-    const double turns = rint(a * 0.15915494309189535);         // 1 / (2 pi)
-    double r = fma(-turns, 6.283185307179586, a);                // 2 pi, high part
-    r = fma(-turns, 2.4492935982947064e-16, r);                  // and what the high part leaves
-    float s, c;
-    sincosf(static_cast<float>(r), &s, &c);
-    cs[i] = make_float2(c * p.magnitude, s * p.magnitude * p.sign);
-  }
-  __syncthreads();
-
-  const int hd = j.head_dim, rot = 2 * p.n_pairs;
-  const int rot_items = p.interleaved ? rot / V : p.n_pairs / V;
-  const int per_head = rot_items + (hd - rot) / V;
-  const int n_rot_heads = j.n_out_heads + (APPEND ? j.n_kv_heads : 0);
-  const int first_head = (APPEND && j.q_out == nullptr) ? j.n_out_heads : 0;
   // the page slot of this token; a slot that does not exist is not written
   int64_t slot = -1;
   if (APPEND && pos >= 0 && pos / j.page_size < j.table_stride) {
@@ -118,59 +142,52 @@ __global__ void __launch_bounds__(ROPE_THREADS) rope_kernel_op(const __grid_cons
     if (page >= 0 && page < j.n_pages)
       slot = static_cast<int64_t>(page) * j.page_stride + static_cast<int64_t>(pos % j.page_size) * j.token_stride;
   }
-  const __nv_bfloat16* row = j.x + static_cast<int64_t>(t) * j.x_stride;
-  using T = typename Vec<V>::T;
-  for (int w = threadIdx.x; w < (n_rot_heads - first_head) * per_head; w += ROPE_THREADS) {
-    const int h = first_head + w / per_head, g = w % per_head;
-    const __nv_bfloat16* src = row + static_cast<int64_t>(h) * hd;
-    __nv_bfloat16* dst;
-    if (!APPEND || h < j.n_out_heads) dst = j.q_out + static_cast<int64_t>(t) * j.q_stride + static_cast<int64_t>(h) * hd;
-    else if (slot >= 0) dst = j.k + slot + (h - j.n_out_heads) * j.head_stride;
-    else continue;
-    if (g >= rot_items) {  // passes through
-      const int e = rot + (g - rot_items) * V;
-      *reinterpret_cast<T*>(dst + e) = *reinterpret_cast<const T*>(src + e);
-    } else if (p.interleaved) {
-      if constexpr (V > 1) {
-        Pack<V> a;
-        a.raw = *reinterpret_cast<const T*>(src + g * V);
-#pragma unroll
-        for (int e = 0; e < V; e += 2) {
-          const float2 c = cs[g * (V / 2) + (e >> 1)];
-          const float u = __bfloat162float(a.e[e]), v = __bfloat162float(a.e[e + 1]);
-          a.e[e] = __float2bfloat16_rn(u * c.x - v * c.y);
-          a.e[e + 1] = __float2bfloat16_rn(v * c.x + u * c.y);
-        }
-        *reinterpret_cast<T*>(dst + g * V) = a.raw;
-      } else if ((g & 1) == 0) {
-        const float2 c = cs[g >> 1];
-        const float u = __bfloat162float(src[g]), v = __bfloat162float(src[g + 1]);
-        dst[g] = __float2bfloat16_rn(u * c.x - v * c.y);
-        dst[g + 1] = __float2bfloat16_rn(v * c.x + u * c.y);
-      }
-    } else {
-      const int e0 = g * V, e1 = e0 + p.n_pairs;
-      Pack<V> a, b;
-      a.raw = *reinterpret_cast<const T*>(src + e0);
-      b.raw = *reinterpret_cast<const T*>(src + e1);
-#pragma unroll
-      for (int e = 0; e < V; ++e) {
-        const float2 c = cs[e0 + e];
-        const float u = __bfloat162float(a.e[e]), v = __bfloat162float(b.e[e]);
-        a.e[e] = __float2bfloat16_rn(u * c.x - v * c.y);
-        b.e[e] = __float2bfloat16_rn(v * c.x + u * c.y);
-      }
-      *reinterpret_cast<T*>(dst + e0) = a.raw;
-      *reinterpret_cast<T*>(dst + e1) = b.raw;
-    }
+  for (int i = threadIdx.x; i < p.n_pairs; i += blockDim.x) {
+    const double angle = static_cast<double>(pos) * p.w[i];
+    const double turns = rint(angle * 0.15915494309189535);      // 1 / (2 pi)
+    double r = fma(-turns, 6.283185307179586, angle);            // 2 pi, high part
+    r = fma(-turns, 2.4492935982947064e-16, r);                  // and what the high part leaves
+    float s, c;
+    sincosf(static_cast<float>(r), &s, &c);
+    cs[i] = make_float2(c * p.magnitude, s * p.magnitude * p.sign);
   }
-  if (APPEND && slot >= 0) {
-    const int vecs = hd / V;
-    for (int w = threadIdx.x; w < j.n_kv_heads * vecs; w += ROPE_THREADS) {
-      const int h = w / vecs, e = (w % vecs) * V;
-      *reinterpret_cast<T*>(j.v + slot + h * j.head_stride + e) =
-          *reinterpret_cast<const T*>(row + static_cast<int64_t>(n_rot_heads + h) * hd + e);
+  __syncthreads();
+
+  for (int w = threadIdx.x; w < items; w += blockDim.x) {
+    if (w != threadIdx.x) fetch(w);
+    __nv_bfloat16* dst;
+    if (!APPEND || head < j.n_out_heads) dst = j.q_out + static_cast<int64_t>(t) * j.q_stride + static_cast<int64_t>(head) * hd + e;
+    else if (slot < 0) continue;
+    else if (head < j.n_rot_heads) dst = j.k + slot + (head - j.n_out_heads) * j.head_stride + e;
+    else dst = j.v + slot + (head - j.n_rot_heads) * j.head_stride + e;
+    if (kind == 2) {
+#pragma unroll
+      for (int k = 0; k < V; ++k) {
+        const float2 c = cs[e + k];
+        const float u = __bfloat162float(a.e[k]), v = __bfloat162float(b.e[k]);
+        a.e[k] = __float2bfloat16_rn(u * c.x - v * c.y);
+        b.e[k] = __float2bfloat16_rn(v * c.x + u * c.y);
+      }
+      *reinterpret_cast<T*>(dst + p.n_pairs) = b.raw;
+    } else if (kind == 1) {
+      if constexpr (V > 1) {
+#pragma unroll
+        for (int k = 0; k < V; k += 2) {
+          const float2 c = cs[(e + k) >> 1];
+          const float u = __bfloat162float(a.e[k]), v = __bfloat162float(a.e[k + 1]);
+          a.e[k] = __float2bfloat16_rn(u * c.x - v * c.y);
+          a.e[k + 1] = __float2bfloat16_rn(v * c.x + u * c.y);
+        }
+      } else {  // the even element's thread turns the pair
+        if (e & 1) continue;
+        const float2 c = cs[e >> 1];
+        const float u = __bfloat162float(a.e[0]), v = __bfloat162float(b.e[0]);
+        a.e[0] = __float2bfloat16_rn(u * c.x - v * c.y);
+        b.e[0] = __float2bfloat16_rn(v * c.x + u * c.y);
+        *reinterpret_cast<T*>(dst + 1) = b.raw;
+      }
     }
+    *reinterpret_cast<T*>(dst) = a.raw;
   }
 }
 
@@ -253,18 +270,32 @@ static int rope_vector(const RopeParams& p, const RopeJob& j, bool append) {
   return 1;
 }
 
-template <bool APPEND>
-static int rope_launch(const RopeParams& p, const RopeJob& j, cudaStream_t s) {
-  const dim3 grid(j.n_tokens), block(ROPE_THREADS);
-  switch (rope_vector(p, j, APPEND)) {
-    case 8: rope_kernel_op<8, APPEND><<<grid, block, 0, s>>>(p, j); break;
-    case 4: rope_kernel_op<4, APPEND><<<grid, block, 0, s>>>(p, j); break;
-    case 2: rope_kernel_op<2, APPEND><<<grid, block, 0, s>>>(p, j); break;
-    default: rope_kernel_op<1, APPEND><<<grid, block, 0, s>>>(p, j); break;
-  }
+template <int V, bool APPEND>
+static int rope_launch_v(const RopeParams& p, RopeJob j, cudaStream_t s) {
+  j.n_rot_heads = j.n_out_heads + (APPEND ? j.n_kv_heads : 0);
+  j.first_head = (APPEND && j.q_out == nullptr) ? j.n_out_heads : 0;
+  j.rot_items = (p.interleaved ? 2 * p.n_pairs : p.n_pairs) / V;
+  j.per_head = j.rot_items + (j.head_dim - 2 * p.n_pairs) / V;
+  const int64_t turned = static_cast<int64_t>(j.n_rot_heads - j.first_head) * j.per_head;
+  const int64_t items = turned + (APPEND ? static_cast<int64_t>(j.n_kv_heads) * (j.head_dim / V) : 0);
+  if (items > 0x3fffffff) return set_error(B200EMB_ERR_UNSUPPORTED, "rope: rows too wide");
+  j.turned = static_cast<int>(turned);
+  j.items = static_cast<int>(items);
+  const int threads = static_cast<int>(items < 64 ? 64 : items < ROPE_MAX_THREADS ? (items + 31) / 32 * 32 : ROPE_MAX_THREADS);
+  rope_kernel_op<V, APPEND><<<static_cast<unsigned>(j.n_tokens), threads, 0, s>>>(p, j);
   const cudaError_t e = cudaGetLastError();
   if (e != cudaSuccess) return set_error(B200EMB_ERR_CUDA, "rope launch: %s", cudaGetErrorString(e));
   return B200EMB_OK;
+}
+
+template <bool APPEND>
+static int rope_launch(const RopeParams& p, const RopeJob& j, cudaStream_t s) {
+  switch (rope_vector(p, j, APPEND)) {
+    case 8: return rope_launch_v<8, APPEND>(p, j, s);
+    case 4: return rope_launch_v<4, APPEND>(p, j, s);
+    case 2: return rope_launch_v<2, APPEND>(p, j, s);
+    default: return rope_launch_v<1, APPEND>(p, j, s);
+  }
 }
 
 int check_kv_cache(const b200emb_kv_cache* c, const char* who) {
