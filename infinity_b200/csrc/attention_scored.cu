@@ -180,6 +180,9 @@ attn_plan_kernel(const AttnJob j, const AttnMod mod, const AttnPlan p, int token
   __shared__ int64_t carry;
   __shared__ int64_t steps_of[AS_PLAN_CACHE];  // AttnEntry::before
   __shared__ int64_t cuts[AS_MAX_SLOTS + 1];
+  __shared__ int2 rows_s[AS_PLAN_CACHE];        // as_rows_of, for so many sequences
+  __shared__ int first_s[AS_PLAN_CACHE];        // AttnPlan::seq_first
+  __shared__ int2 docs_s[AS_PLAN_CACHE];        // AttnPlan::doc_range
   pdl_launch_dependents();
   pdl_wait();
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -190,16 +193,27 @@ attn_plan_kernel(const AttnJob j, const AttnMod mod, const AttnPlan p, int token
   for (int i = tid; i < 2 * max_slots; i += static_cast<int>(blockDim.x)) p.counter[i] = 0;
   for (int i = tid; i < max_slots; i += static_cast<int>(blockDim.x)) p.slot[i] = AttnSlot{0, 0, 0, 0};
   __syncthreads();
+  // the device copies of the lengths, read once
+  const bool few = j.n_seqs <= AS_PLAN_CACHE;
+  if (few)
+    for (int s = tid; s < j.n_seqs; s += static_cast<int>(blockDim.x)) rows_s[s] = as_rows_of(j, s);
+  __syncthreads();
+  auto rows_of = [&](int s) { return few ? rows_s[s] : as_rows_of(j, s); };
+  auto first_of = [&](int s) { return few ? first_s[s] : p.seq_first[s]; };
   // entries of each sequence
   for (int base = 0; base < j.n_seqs; base += static_cast<int>(blockDim.x)) {
     const int s = base + tid;
     int count = 0;
     if (s < j.n_seqs) {
-      const int2 r = as_rows_of(j, s);
+      const int2 r = rows_of(s);
       count = (r.y - r.x + tokens_per_entry - 1) / tokens_per_entry;
     }
     const int64_t at = as_block_sum(count, &carry, scratch);
-    if (s < j.n_seqs) p.seq_first[s] = static_cast<int>(min(at, static_cast<int64_t>(p.max_entries)));
+    if (s < j.n_seqs) {
+      const int e0 = static_cast<int>(min(at, static_cast<int64_t>(p.max_entries)));
+      p.seq_first[s] = e0;
+      if (few) first_s[s] = e0;
+    }
   }
   const int n_entries = static_cast<int>(min(carry, static_cast<int64_t>(p.max_entries)));
   if (tid == 0) p.seq_first[j.n_seqs] = n_entries;
@@ -208,7 +222,7 @@ attn_plan_kernel(const AttnJob j, const AttnMod mod, const AttnPlan p, int token
     int lo = 0, hi = j.n_seqs;
     while (hi - lo > 1) {
       const int mid = (lo + hi) >> 1;
-      if (p.seq_first[mid] <= e) lo = mid;
+      if (first_of(mid) <= e) lo = mid;
       else hi = mid;
     }
     return lo;
@@ -220,10 +234,10 @@ attn_plan_kernel(const AttnJob j, const AttnMod mod, const AttnPlan p, int token
       int lo = 0, hi = j.n_seqs;
       while (hi - lo > 1) {
         const int mid = (lo + hi) >> 1;
-        if (as_doc_base(as_rows_of(j, mid).x, mid, kv) <= i) lo = mid;
+        if (as_doc_base(rows_of(mid).x, mid, kv) <= i) lo = mid;
         else hi = mid;
       }
-      const int2 r = as_rows_of(j, lo);
+      const int2 r = rows_of(lo);
       const int t0 = r.x + (i - as_doc_base(r.x, lo, kv)) * kv;
       if (t0 < r.x) continue;  // only where cu_seqlens is not sorted
       int dmin = INT_MAX, dmax = -1;
@@ -236,19 +250,24 @@ attn_plan_kernel(const AttnJob j, const AttnMod mod, const AttnPlan p, int token
       }
       dmin = __reduce_min_sync(0xffffffffu, dmin);
       dmax = __reduce_max_sync(0xffffffffu, dmax);
-      if (lane == 0 && t0 < r.y) p.doc_range[i] = make_int2(dmin, dmax);
+      if (lane == 0 && t0 < r.y) {
+        p.doc_range[i] = make_int2(dmin, dmax);
+        if (i < AS_PLAN_CACHE) docs_s[i] = make_int2(dmin, dmax);
+      }
     }
     __syncthreads();
     // first and past-the-last key tile whose documents meet an entry's (kept in its record), a warp an entry, 32 key tiles at a time
     for (int e = warp; e < n_entries; e += static_cast<int>(blockDim.x) >> 5) {
       const int s = sequence_of_entry(e);
-      const int2 r = as_rows_of(j, s);
-      const int q0 = (e - p.seq_first[s]) * tokens_per_entry, tiles = (r.y - r.x + kv - 1) / kv;
-      const int2* range = p.doc_range + as_doc_base(r.x, s, kv);
+      const int2 r = rows_of(s);
+      const int q0 = (e - first_of(s)) * tokens_per_entry, tiles = (r.y - r.x + kv - 1) / kv;
+      const int base = as_doc_base(r.x, s, kv);
+      auto range = [&](int t) { return base + t < AS_PLAN_CACHE ? docs_s[base + t] : p.doc_range[base + t]; };
       int dmin = INT_MAX, dmax = -1;
       for (int t = q0 / kv + lane; t <= min(q0 + tokens_per_entry, r.y - r.x) / kv && t < tiles; t += 32) {
-        dmin = min(dmin, range[t].x);
-        dmax = max(dmax, range[t].y);
+        const int2 d = range(t);
+        dmin = min(dmin, d.x);
+        dmax = max(dmax, d.y);
       }
       dmin = __reduce_min_sync(0xffffffffu, dmin);
       dmax = __reduce_max_sync(0xffffffffu, dmax);
@@ -256,7 +275,7 @@ attn_plan_kernel(const AttnJob j, const AttnMod mod, const AttnPlan p, int token
       for (int t0 = 0; t0 < tiles; t0 += 32) {
         bool meets = false;
         if (t0 + lane < tiles) {
-          const int2 d = range[t0 + lane];
+          const int2 d = range(t0 + lane);
           meets = d.x <= dmax && d.y >= dmin;
         }
         const uint32_t m = __ballot_sync(0xffffffffu, meets);
@@ -280,8 +299,8 @@ attn_plan_kernel(const AttnJob j, const AttnMod mod, const AttnPlan p, int token
     int doc_lo = 0, doc_hi = INT_MAX;
     if (e < n_entries) {
       const int lo = sequence_of_entry(e);
-      const int2 r = as_rows_of(j, lo);
-      const int q0 = (e - p.seq_first[lo]) * tokens_per_entry;
+      const int2 r = rows_of(lo);
+      const int q0 = (e - first_of(lo)) * tokens_per_entry;
       x.seq = lo;
       x.tok0 = r.x + q0;
       x.n_tok = min(tokens_per_entry, r.y - r.x - q0);
@@ -332,7 +351,9 @@ attn_plan_kernel(const AttnJob j, const AttnMod mod, const AttnPlan p, int token
   // Parts of equal cost; a cut moves to an item's edge that is nearer than 1/16 of a part.
   const int heads = j.n_kv_heads;
   const int64_t total = carry * heads, total_cost = (carry + static_cast<int64_t>(AS_ITEM_STEPS) * n_entries) * heads;
-  const int slots = static_cast<int>(min(total, static_cast<int64_t>(max_slots)));
+  // a part of an item has two steps or more: what a part costs to join is more than a step
+  const int64_t most = max(min(total, static_cast<int64_t>(n_entries) * heads), (total + 1) / 2);
+  const int slots = static_cast<int>(min(most, static_cast<int64_t>(max_slots)));
   __syncthreads();
   if (slots == 0) return;
   auto before_of = [&](int e) { return e < AS_PLAN_CACHE ? steps_of[e] : p.entry[e].before; };
@@ -918,14 +939,18 @@ attn_scored_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_cons
             const int key = kv0 + q * 32;
             uint32_t seen = (as_below(key_hi() - key) & ~as_below(key_lo() - key)) | as_below(cold[C_PREFIX] - key);
             if (MODE == AS_ANY && mod.docs != nullptr) {
-              // the keys of each document that some row of the warp belongs to
               const int key_doc = q == 0 ? key_docs[0] : key_docs[1];
-              uint32_t same = 0, todo = __ballot_sync(0xffffffffu, doc >= 0);
-              while (todo) {
-                const int d = __shfl_sync(0xffffffffu, doc, __ffs(todo) - 1);
-                const uint32_t keys = __ballot_sync(0xffffffffu, key_doc == d);
-                if (doc == d) same = keys;
-                todo &= ~__ballot_sync(0xffffffffu, doc == d);
+              uint32_t same = 0;
+              if (one_doc >= 0) {
+                same = __ballot_sync(0xffffffffu, key_doc == one_doc);
+              } else {  // the keys of each document that some row of the warp belongs to
+                uint32_t todo = __ballot_sync(0xffffffffu, doc >= 0);
+                while (todo) {
+                  const int d = __shfl_sync(0xffffffffu, doc, __ffs(todo) - 1);
+                  const uint32_t keys = __ballot_sync(0xffffffffu, key_doc == d);
+                  if (doc == d) same = keys;
+                  todo &= ~__ballot_sync(0xffffffffu, doc == d);
+                }
               }
               seen &= same;
             }
@@ -1015,7 +1040,7 @@ attn_scored_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_cons
           // Most steps: every row sees all 64 keys, the reference stands, nothing is asked of a score one by one. What does not fit
           // (a sum out of range, a score beyond the cap, a wait that gave up) is taken again below, from the same scores.
           bool done = false;
-          if (whole && (MODE == AS_CAP || !first) && (MODE != AS_SLOPES || kv0 + KV <= pos_first || kv0 > pos_last)) {
+          if (whole && (MODE != AS_SLOPES || (!first && (kv0 + KV <= pos_first || kv0 > pos_last)))) {
             uint32_t z[2][32];
             tmem_ld_32x32b_x32(s_at, z[0]);
             tmem_ld_32x32b_x32(s_at + 32, z[1]);
@@ -1051,6 +1076,19 @@ attn_scored_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_cons
                 e2[i >> 4][i & 15] = tanh_near(v, __fmul2_rn(v, v));
               }
             }
+            if (MODE != AS_CAP && MODE != AS_SLOPES && first) {  // the reference, from these scores (nothing is summed yet)
+              float m0 = -INFINITY, m1 = -INFINITY;
+#pragma unroll
+              for (int i = 0; i < 16; ++i) {
+                m0 = as_max3(m0, e2[0][i].x, e2[0][i].y);
+                m1 = as_max3(m1, e2[1][i].x, e2[1][i].y);
+              }
+              float by = ceilf(fmaxf(m0, m1));
+              if (by == -INFINITY) by = 0.f;
+              ref += by;
+#pragma unroll
+              for (int i = 0; i < 32; ++i) e2[i >> 4][i & 15] = __fadd2_rn(e2[i >> 4][i & 15], make_float2(-by, -by));
+            }
             uint32_t pk[2][16];
             float total = exponentials(e2[0], pk[0]);
             total += exponentials(e2[1], pk[1]);
@@ -1070,6 +1108,11 @@ attn_scored_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_cons
             const int key32 = kv0 + q * 32;
             uint32_t seen = 0xffffffffu;
             if (!whole) seen = seen_of(q);
+            if ((__ballot_sync(0xffffffffu, seen != 0u) & real_rows) == 0u && !(first && q == 0)) {  // no row of the warp sees one of them
+              uint32_t none[16] = {};
+              tmem_st_32x32b_x16(s_at + q * 32, none);
+              continue;
+            }
             bool moves = MODE != AS_CAP && first && q == 0 && real;  // the segment's first scores set the reference
             bool again = false;
             float total;
@@ -1269,18 +1312,20 @@ attn_scored_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_cons
           for (int i = row; i < n_rows * pieces; i += 128) {
             const int piece = i / n_rows, r = i - piece * n_rows, col = piece * 8;
             float top = -INFINITY, l = 0.f, o[8] = {};
+            // four parts' reads at a time
+#pragma unroll 4
             for (int s = s0; s <= s1; ++s) {
               const float2 ml = __ldcg(&plan.part_ml[part_of(s, s == s0) * plan.rows + r]);
-              if (ml.y > 0.f) top = fmaxf(top, ml.x + __log2f(ml.y));  // a reference alone may be far from its sum
+              top = fmaxf(top, ml.y > 0.f ? ml.x + __log2f(ml.y) : -INFINITY);  // a reference alone may be far from its sum
             }
-#pragma unroll 2
+#pragma unroll 4
             for (int s = s0; s <= s1; ++s) {
               const int64_t id2 = part_of(s, s == s0);
               const float2 ml = __ldcg(&plan.part_ml[id2 * plan.rows + r]);
-              const float f = ml.y > 0.f ? as_ex2(ml.x - top) : ml.y;  // nothing seen: 0, and NaN stays NaN
               const float* src = plan.part_o + ((id2 * (D / 4) + 2 * piece) * plan.rows + r) * 4;
               const float4 x = __ldcg(reinterpret_cast<const float4*>(src));
               const float4 y = __ldcg(reinterpret_cast<const float4*>(src + static_cast<int64_t>(plan.rows) * 4));
+              const float f = ml.y > 0.f ? as_ex2(ml.x - top) : ml.y;  // nothing seen: 0, and NaN stays NaN
               l = fmaf(f, ml.y, l);
               o[0] = fmaf(f, x.x, o[0]);
               o[1] = fmaf(f, x.y, o[1]);
@@ -1444,7 +1489,7 @@ static int as_launch(const AsMaps& m, const AttnJob& j, const AttnMod& mod, cons
   }
   const int slots = static_cast<int>(PAIR ? grid : 2 * grid);
   // few entries are planned by fewer threads: their barriers are what it takes
-  const int threads = plan.max_entries <= 256 && j.n_seqs <= 256 ? 256 : AS_PLAN_THREADS;
+  const int threads = plan.max_entries <= 256 && j.n_seqs <= 256 && mod.docs == nullptr ? 256 : AS_PLAN_THREADS;
   cudaError_t e = launch_pdl(attn_plan_kernel, dim3(1), dim3(threads), 0, s, j, mod, plan, (PAIR ? 2 : 1) * j.tile_tokens, slots, AsCfg<D>::KV);
   if (e == cudaSuccess)
     e = launch_pdl(attn_scored_kernel<D, PAGED, PAIR, MODE>, dim3(static_cast<unsigned>(grid)), dim3(AS_THREADS), AsCfg<D>::SMEM_BYTES, s, m.q, m.k,
