@@ -441,7 +441,8 @@ int b200emb_op_kv_append(const void* qkv, int64_t qkv_row_stride, const int32_t*
  *   s = scale * q_i . k_j;  cap > 0: s = cap * tanh(s / cap);  slopes: s -= slopes[h] * |i - j|;
  *   bias: s += bias[h * (2 R + 1) + clamp(j - i, -R, R) + R], R = bias_radius
  * Key j is visible to query i when (j <= i + window_right and j >= i - window_left) or j < prefix_lens[s], and with
- * doc_ids only when doc_ids of both tokens are equal and not negative. A row that sees no key (or only -inf) is zero.
+ * doc_ids only when doc_ids of both tokens are equal and not negative. A row that sees no key is zero, and so is one whose visible
+ * scores are all -inf; a bias below -1e38 counts as -inf.
  * Masked scores are selected away, so keys may hold anything there; a VALUE that is not finite reaches every row of its own
  * sequence whose tiles cover it (0 * inf), never another sequence, and slots past the sequence's end never count. */
 typedef struct b200emb_attn_opts {
@@ -470,7 +471,8 @@ int b200emb_op_workspace_status(const void* workspace, void* stream);
 
 /* Packed variable-length attention: q [n_tokens, n_heads * head_dim], k and v [n_tokens, n_kv_heads * head_dim], out
  * [n_tokens, n_heads * head_dim], each with its own row stride (elements, a multiple of 8) and 16-byte aligned, so the packed qkv
- * buffer serves with three pointers. n_heads a multiple of n_kv_heads and at most 128 times it; head_dim a multiple of 8, 8 .. 128.
+ * buffer serves with three pointers. n_heads a multiple of n_kv_heads and at most 128 times it; head_dim a multiple of 8, 8 .. 128; up to
+ * 2^30 tokens. The kernels are loaded by the first call on a device: make one before a stream capture, as with the other operators.
  * opts null: plain bidirectional attention. Query i of a sequence is at position i. */
 int b200emb_op_attention_scored(const void* q, int64_t q_row_stride, const void* k, int64_t k_row_stride, const void* v,
                                 int64_t v_row_stride, void* out, int64_t out_row_stride, const int32_t* d_cu_seqlens,
@@ -479,7 +481,7 @@ int b200emb_op_attention_scored(const void* q, int64_t q_row_stride, const void*
 
 /* Attention of new tokens (a chunk of any length, or one) over the paged cache, which already holds their own keys
  * (b200emb_op_kv_append). The new tokens of sequence s are rows cu_seqlens[s] .. cu_seqlens[s + 1] - 1 of q and out and take the last
- * positions below kv_lens[s]. kv_lens is cut to table_stride * page_size. page_size a multiple of 8; the three cache
+ * positions below kv_lens[s]. kv_lens is cut to table_stride * page_size. page_size a multiple of 8, table_stride * page_size up to 2^30; the three cache
  * strides multiples of 8, k and v 16-byte aligned. opts null: causal. Few rows over long caches are split over the keys
  * and joined in a fixed order: results depend on the batch's lengths and the device alone. */
 int b200emb_op_attention_paged(const void* q, int64_t q_row_stride, void* out, int64_t out_row_stride,

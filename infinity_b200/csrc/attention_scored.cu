@@ -41,6 +41,7 @@ namespace b2 {
 
 static constexpr int AS_MAX_RADIUS = 1023;
 static constexpr int AS_MAX_GROUP = 128;
+static constexpr int AS_MAX_POSITIONS = 1 << 30;   // a tile's end stays inside 32 bits
 static constexpr int64_t AS_ALIGN = 256;
 static constexpr int AS_MAX_CTAS = 160;
 static constexpr int AS_MAX_SLOTS = 2 * AS_MAX_CTAS;
@@ -988,17 +989,19 @@ attn_scored_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_cons
               tmem_st_wait();
             }
           };
-          // probabilities of 32 keys, two to a register, and their sum
+          // probabilities of 32 keys, two to a register, and the sum of what the rounding left of them: the weights that reach O then add
+          // up to one, and the rounding of a key that dominates its row cancels (error against 64 bits 0.0024 -> 0.0020 on an
+          // indexing batch, 0.0017 of it the rounding of the output, for 3 % of the time)
           auto exponentials = [&](const float2 (&e2)[16], uint32_t (&pk)[16]) -> float {
             float2 sum = make_float2(0.f, 0.f), sum1 = make_float2(0.f, 0.f);
 #pragma unroll
             for (int i = 0; i < 16; i += 2) {
-              const float2 a = make_float2(as_ex2(e2[i].x), as_ex2(e2[i].y)), b = make_float2(as_ex2(e2[i + 1].x), as_ex2(e2[i + 1].y));
-              sum = __fadd2_rn(sum, a);
-              sum1 = __fadd2_rn(sum1, b);
-              const __nv_bfloat162 ha = __floats2bfloat162_rn(a.x, a.y), hb = __floats2bfloat162_rn(b.x, b.y);
-              pk[i] = *reinterpret_cast<const uint32_t*>(&ha);
-              pk[i + 1] = *reinterpret_cast<const uint32_t*>(&hb);
+              const __nv_bfloat162 a = __floats2bfloat162_rn(as_ex2(e2[i].x), as_ex2(e2[i].y));
+              const __nv_bfloat162 b = __floats2bfloat162_rn(as_ex2(e2[i + 1].x), as_ex2(e2[i + 1].y));
+              pk[i] = *reinterpret_cast<const uint32_t*>(&a);
+              pk[i + 1] = *reinterpret_cast<const uint32_t*>(&b);
+              sum = __fadd2_rn(sum, make_float2(__uint_as_float(pk[i] << 16), __uint_as_float(pk[i] & 0xffff0000u)));
+              sum1 = __fadd2_rn(sum1, make_float2(__uint_as_float(pk[i + 1] << 16), __uint_as_float(pk[i + 1] & 0xffff0000u)));
             }
             return (sum.x + sum1.x) + (sum.y + sum1.y);
           };
@@ -1379,6 +1382,7 @@ attn_scored_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_cons
 static int check_shape(int n_seqs, int n_tokens, int n_heads, int n_kv_heads, int head_dim, const char* who) {
   if (n_seqs < 0 || n_tokens < 0 || n_heads <= 0 || n_kv_heads <= 0)
     return set_error(B200EMB_ERR_INVALID, "%s: bad sizes", who);
+  if (n_tokens > AS_MAX_POSITIONS) return set_error(B200EMB_ERR_UNSUPPORTED, "%s: more than %d tokens", who, AS_MAX_POSITIONS);
   if (n_heads % n_kv_heads != 0)
     return set_error(B200EMB_ERR_INVALID, "%s: %d query heads are no multiple of %d key heads", who, n_heads, n_kv_heads);
   if (n_heads / n_kv_heads > AS_MAX_GROUP)
@@ -1637,6 +1641,8 @@ extern "C" int b200emb_op_attention_paged(const void* q, int64_t q_row_stride, v
   AttnMod mod;
   if (!rc) rc = make_mod(opts, cache->head_dim, true, who, &mod);
   if (rc) return rc;
+  if (static_cast<int64_t>(cache->table_stride) * cache->page_size > AS_MAX_POSITIONS)
+    return set_error(B200EMB_ERR_UNSUPPORTED, "%s: a page table of more than %d positions", who, AS_MAX_POSITIONS);
   if (cache->page_size % 8 != 0)
     return set_error(B200EMB_ERR_UNSUPPORTED, "%s: page_size %d is no multiple of 8", who, cache->page_size);
   if (cache->page_stride % 8 != 0 || cache->token_stride % 8 != 0 || cache->head_stride % 8 != 0 ||
