@@ -446,7 +446,7 @@ int b200emb_op_kv_append(const void* qkv, int64_t qkv_row_stride, const int32_t*
  * Masked scores are selected away, so keys may hold anything there; a VALUE that is not finite reaches every row of its own
  * sequence whose tiles cover it (0 * inf), never another sequence, and slots past the sequence's end never count. */
 typedef struct b200emb_attn_opts {
-  float scale;              /* 0 = 1 / sqrt(head_dim) */
+  float scale;              /* 0 = 1 / sqrt(head_dim); finite, magnitude up to 2e38, as cap */
   float cap;                /* 0 = none */
   int32_t causal;           /* 1 = window_right 0 (window_right must then be <= 0) */
   int32_t window_left;      /* < 0 = unlimited */
@@ -472,8 +472,7 @@ int b200emb_op_workspace_status(const void* workspace, void* stream);
 /* Packed variable-length attention: q [n_tokens, n_heads * head_dim], k and v [n_tokens, n_kv_heads * head_dim], out
  * [n_tokens, n_heads * head_dim], each with its own row stride (elements, a multiple of 8) and 16-byte aligned, so the packed qkv
  * buffer serves with three pointers. n_heads a multiple of n_kv_heads and at most 128 times it; head_dim a multiple of 8, 8 .. 128; up to
- * 2^30 tokens. The kernels are loaded by the first call on a device: make one before a stream capture, as with the other operators.
- * opts null: plain bidirectional attention. Query i of a sequence is at position i. */
+ * 2^30 tokens. opts null: plain bidirectional attention. Query i of a sequence is at position i. */
 int b200emb_op_attention_scored(const void* q, int64_t q_row_stride, const void* k, int64_t k_row_stride, const void* v,
                                 int64_t v_row_stride, void* out, int64_t out_row_stride, const int32_t* d_cu_seqlens,
                                 int32_t n_seqs, int32_t n_tokens, int32_t n_heads, int32_t n_kv_heads, int32_t head_dim,

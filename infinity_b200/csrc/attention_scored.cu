@@ -3,7 +3,7 @@
 //
 // Rows. The G query heads that share a key head are packed into one 128-row tile: row r of a tile is token r / G, head
 // r % G, so a single new token of a grouped model fills G rows of one tile instead of one row of G tiles, and its keys are read
-// once. An item is a query tile of one key head with the key tiles (128 keys) its masks can reach: at most two runs of
+// once. An item is a query tile of one key head with the key tiles (64 keys) its masks can reach: at most two runs of
 // tiles, the prefix and the window (a document mask cuts both to the tiles whose documents meet the query tile's).
 //
 // Split. A planning kernel (one block) lists the items and cuts the row of all (item, key tile) steps into equal parts, one
@@ -126,8 +126,14 @@ __device__ __forceinline__ float as_max3_abs(float a, float b, float c) {  // ma
   asm("max.abs.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
   return d;
 }
-// 1 - 2 / (1 + e^2x)
+// 1 - 2 / (1 + e^2x), off by about 2^-22 of one
 __device__ __forceinline__ float as_tanh(float x) { return fmaf(-2.f, as_rcp(1.f + as_ex2(x * (2.f * AS_LOG2E))), 1.f); }
+// The same with small values taken from the series x - x^3/3 + 2x^5/15 (next term below 2^-24 of x up to 0.1): a large cap
+// multiplies the error, and nearly all of its scores are small here.
+__device__ __forceinline__ float as_tanh_any(float x) {
+  const float u = x * x;
+  return fabsf(x) < 0.1f ? fmaf(x * u, fmaf(u, 2.f / 15.f, -1.f / 3.f), x) : as_tanh(x);
+}
 // 32-bit mask of the x lowest bits, x clamped to 0 .. 32
 __device__ __forceinline__ uint32_t as_below(int x) {
   uint32_t m;
@@ -819,7 +825,8 @@ attn_scored_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_cons
     const int row_tok = (row * j.group_inv) >> 16, g = row - row_tok * j.group;
     const int my_slot = PAIR ? blockIdx.x : blockIdx.x + t * gridDim.x;
     const float scale_log2 = mod.scale * AS_LOG2E, cap_out = mod.cap * AS_LOG2E;
-    const float cap_in = mod.cap > 0.f ? mod.scale / mod.cap : 0.f;
+    // held finite: a score of zero stays zero under the smallest caps
+    const float cap_in = mod.cap > 0.f ? fminf(fmaxf(mod.scale / mod.cap, -FLT_MAX), FLT_MAX) : 0.f;
     const float cap_far = mod.cap > 0.f ? fabsf(mod.cap / mod.scale) : 0.f;
     const float2 scale2 = make_float2(scale_log2, scale_log2);
     // exponent of a capped score v = scale_log2 * s: cap_out tanh(v / cap_out), see AsTanh
@@ -1012,7 +1019,7 @@ attn_scored_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_cons
             for (int i = 0; i < 32; ++i) y[i] = __uint_as_float(z[i]);
             if (mod.cap > 0.f) {
 #pragma unroll
-              for (int i = 0; i < 32; ++i) y[i] = fmaf(cap_out, as_tanh(y[i] * cap_in), -ref);
+              for (int i = 0; i < 32; ++i) y[i] = fmaf(cap_out, as_tanh_any(y[i] * cap_in), -ref);
             } else {
 #pragma unroll
               for (int i = 0; i < 32; ++i) y[i] = fmaf(y[i], scale_log2, -ref);
@@ -1396,8 +1403,8 @@ static int check_shape(int n_seqs, int n_tokens, int n_heads, int n_kv_heads, in
 static int make_mod(const b200emb_attn_opts* o, int head_dim, bool paged, const char* who, AttnMod* m) {
   *m = AttnMod{1.f / sqrtf(static_cast<float>(head_dim)), 0.f, INT_MAX, paged ? 0 : INT_MAX, 0, nullptr, nullptr, nullptr, nullptr};
   if (o == nullptr) return B200EMB_OK;
-  if (!isfinite(o->scale) || !isfinite(o->cap) || o->cap < 0.f)
-    return set_error(B200EMB_ERR_INVALID, "%s: scale must be finite and cap finite and not negative", who);
+  if (!isfinite(o->scale * AS_LOG2E) || !isfinite(o->cap * AS_LOG2E) || o->cap < 0.f)  // both in the units of the exponent
+    return set_error(B200EMB_ERR_INVALID, "%s: scale and cap must be finite and at most 2e38, cap not negative", who);
   if (o->causal != 0 && o->causal != 1) return set_error(B200EMB_ERR_INVALID, "%s: causal must be 0 or 1", who);
   if (o->causal == 1 && o->window_right > 0)
     return set_error(B200EMB_ERR_INVALID, "%s: causal together with window_right %d", who, o->window_right);

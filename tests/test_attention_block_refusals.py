@@ -73,7 +73,7 @@ def opts(**kw):
     return _lib.AttnOpts(**d)
 
 
-BAD_OPTS = [dict(scale=math.nan), dict(scale=math.inf), dict(cap=-1.0), dict(cap=math.inf), dict(cap=math.nan), dict(causal=2),
+BAD_OPTS = [dict(scale=math.nan), dict(scale=math.inf), dict(scale=3e38), dict(scale=-3e38), dict(cap=3e38), dict(cap=-1.0), dict(cap=math.inf), dict(cap=math.nan), dict(causal=2),
             dict(causal=1, window_right=3), dict(slopes=P, bias=P), dict(reserved=(C.c_int32 * 4)(1, 0, 0, 0))]
 
 
@@ -94,7 +94,8 @@ def test_scored_refuses(lib, kw):
 
 
 @pytest.mark.parametrize("kw", [dict(dim=4), dict(dim=60), dict(dim=136, strides=(1024,) * 4), dict(heads=130, kv_heads=1),
-                                dict(o=opts(bias_radius=1024, bias=P)), dict(o=opts(bias_radius=-1, bias=P))], ids=str)
+                                dict(o=opts(bias_radius=1024, bias=P)), dict(o=opts(bias_radius=-1, bias=P)),
+                                dict(n_tokens=(1 << 30) + 1)], ids=str)
 def test_scored_does_not_cover(lib, kw):
     assert scored(lib, **kw) == UNSUPPORTED
 
@@ -114,7 +115,8 @@ def test_paged_refuses(lib, kw):
     assert paged(lib, **kw) == INVALID and _lib.last_error()
 
 
-@pytest.mark.parametrize("kw", [dict(page_size=12, page_stride=12 * 128), dict(head_dim=60), dict(table_stride=1 << 28)], ids=str)
+@pytest.mark.parametrize("kw", [dict(page_size=12, page_stride=12 * 128), dict(head_dim=60), dict(table_stride=1 << 28),
+                                dict(table_stride=(1 << 26) + 1), dict(n_tokens=(1 << 30) + 1)], ids=str)
 def test_paged_does_not_cover(lib, kw):
     assert paged(lib, **kw) == UNSUPPORTED
 

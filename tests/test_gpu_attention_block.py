@@ -2,6 +2,9 @@
 cache append, packed attention with modified scores, paged attention, and a run of them together."""
 import ctypes as C
 import math
+import os
+import subprocess
+import sys
 
 import pytest
 import torch
@@ -238,6 +241,40 @@ def test_scored_long(lib, shape, name):
     _check_scored(out, q, k, v, lens, heads, kv_heads, dim, mod, slopes, bias, prefix, docs)
 
 
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("mod", [dict(cap=100.0), dict(cap=1e4, causal=1), dict(cap=1e7), dict(cap=2e38), dict(cap=1e-3), dict(cap=1e-42),
+                                 dict(cap=1e6, slopes=True), dict(scale=-0.2), dict(scale=-0.1, cap=9.0), dict(scale=-0.3, slopes=True, causal=1),
+                                 dict(scale=1e-42, slopes=True)], ids=str)
+def test_scored_caps_and_scales_of_any_size(lib, mod, dim):
+    lens, heads, kv_heads = [3, 200, 64], 4, 2
+    x, mod, slopes, bias, prefix, docs = _scored_case(lens, heads, kv_heads, dim, mod)
+    q, k, v = _split(x, heads, kv_heads, dim)
+    q[1] = 0.0  # scores of zero
+    out = R.scored(lib, q, k, v, R.cu_of(lens), heads, kv_heads, R.options(slopes=slopes, **mod))
+    _check_scored(out, q, k, v, lens, heads, kv_heads, dim, mod, slopes, bias, prefix, docs)
+
+
+def test_scored_slopes_that_grow_with_the_distance(lib):
+    lens, heads, dim = [1100, 70], 2, 64
+    x = R.normal(3, sum(lens), 3 * heads * dim)
+    q, k, v = _split(x, heads, heads, dim)
+    slopes = torch.tensor([-0.5, -0.0625], device="cuda")
+    out = R.scored(lib, q, k, v, R.cu_of(lens), heads, heads, R.options(slopes=slopes))
+    # biases of up to 550, rounded to fp32 after the slope's log2(e) is: off by at most 3 * 2^-24 * 800 = 1.4e-4 in log2 units
+    _check_scored(out, q, k, v, lens, heads, heads, dim, {}, slopes, None, None, None)
+
+
+@pytest.mark.parametrize("name", ["causal", "slopes", "docs"])
+@pytest.mark.parametrize("lens,heads,kv_heads,dim", [([1, 0, 5, 2, 70, 3] * 260, 2, 1, 64),  # more sequences than the planner keeps at hand
+                                                     ([2200, 40], 64, 1, 32),               # and more query tiles
+                                                     ([1, 9, 131], 128, 1, 128), ([4, 1], 2304, 24, 8)], ids=["sequences", "tiles", "group", "heads"])
+def test_scored_counts_beyond_the_common(lib, lens, heads, kv_heads, dim, name):
+    x, mod, slopes, bias, prefix, docs = _scored_case(lens, heads, kv_heads, dim, MODS[name])
+    q, k, v = _split(x, heads, kv_heads, dim)
+    out = R.scored(lib, q, k, v, R.cu_of(lens), heads, kv_heads, R.options(slopes=slopes, docs=docs, **mod))
+    _check_scored(out, q, k, v, lens, heads, kv_heads, dim, mod, slopes, bias, prefix, docs)
+
+
 def test_scored_options_null_is_plain_attention(lib):
     lens = [30, 61]
     x = R.normal(1, 91, 3 * 2 * 64)
@@ -358,6 +395,16 @@ def test_paged(lib, case, name):
     out = R.paged(lib, q, R.cu_of(new), R.ints(kv), heads, pages, o)
     _check_paged(out, q, new, kv, heads, pages, mod, slopes, bias, prefix)
     assert torch.equal(out, R.paged(lib, q, R.cu_of(new), R.ints(kv), heads, pages, o))
+
+
+def test_paged_counts_beyond_the_common(lib):
+    """More sequences than the planner keeps at hand, most of one new token, some of none."""
+    new = [(1, 1, 0, 2)[i % 4] for i in range(1300)]
+    kv = [n + (7 * i) % 90 for i, n in enumerate(new)]
+    pages = R.Pages(kv, 1, 64, 16, False).fill(4)
+    q = R.normal(5, sum(new), 2 * 64, gain=2.0)
+    out = R.paged(lib, q, R.cu_of(new), R.ints(kv), 2, pages, R.options(causal=1, cap=20.0))
+    _check_paged(out, q, new, kv, 2, pages, dict(cap=20.0))
 
 
 def test_paged_options_null_is_causal_and_rows_behind_stay(lib):
@@ -481,6 +528,30 @@ def test_captured_step_follows_the_lengths(lib):
         _check_paged(out, q_out, [1, 1, 1], lens, heads, pages, {})
         assert torch.equal(other_out, want_other)
         _lib.check(lib.b200emb_op_workspace_status(ws.data_ptr(), R.stream()))
+
+
+FIRST = """
+import torch, attention_block_reference as R
+from infinity_b200 import _lib
+lib = _lib.load()
+lens, heads, dim = [40, 9], 2, 64
+q, k, v = (R.normal(i, 49, heads * dim) for i in range(3))
+cu, out, ws = R.cu_of(lens), torch.empty_like(q), R.workspace(lib, 2, 49, heads, heads, dim)
+g = torch.cuda.CUDAGraph()
+torch.cuda.synchronize()
+with torch.cuda.graph(g):
+    R.scored(lib, q, k, v, cu, heads, heads, R.options(causal=1, cap=20.0), out=out, ws=ws)
+g.replay()
+torch.cuda.synchronize()
+assert torch.equal(out, R.scored(lib, q, k, v, cu, heads, heads, R.options(causal=1, cap=20.0)))
+"""
+
+
+def test_the_first_call_of_a_process_may_be_captured():
+    here = os.path.dirname(os.path.abspath(__file__))
+    env = dict(os.environ, PYTHONPATH=os.pathsep.join([here, os.path.dirname(here)]))
+    done = subprocess.run([sys.executable, "-c", FIRST], env=env, capture_output=True, text=True, timeout=600)
+    assert done.returncode == 0, done.stderr
 
 
 def test_two_streams_with_their_own_workspaces(lib):
