@@ -12,8 +12,9 @@
 // stream that finishes last joins them in the order of the parts, so the result depends on the lengths and not on timing.
 //
 // A CTA (one per SM) runs two streams, A and B, each with its own 128-row tile, softmax warpgroup and tensor-memory
-// accumulators, so that one stream's exponentials run under the other's matrix products. With long queries the two streams take
-// neighbouring tiles of the same item row and share every key and value tile ("pair"); otherwise each walks its own part.
+// accumulators, so that one stream's exponentials run under the other's matrix products. Each walks its own part. (Streams on
+// neighbouring tiles of one item row that share every key and value tile read half as much, but what bounds the kernel is the softmax:
+// 4 sequences of 4000 tokens, 28/4 heads of 128, 1058 us so and 993 us apart; 16 heads of 64 513 and 517.)
 // Per step of a stream, 64 keys:
 //   S = Q K^T     tcgen05.mma 128 x N x 16 (N = valid keys rounded up to 16), fp32 in tensor memory
 //   softmax       128 threads, one row each, in one pass over the row: a score becomes its exponential against the row's reference
@@ -69,7 +70,7 @@ struct AttnMod {
   const int32_t* docs;
 };
 
-// One query tile (PAIR: two neighbouring ones) of one sequence; the same for every key head.
+// One query tile of one sequence; the same for every key head.
 struct __align__(16) AttnEntry {
   int32_t seq, tok0, n_tok, pos0;     // first row of q and out, tokens, position of the first
   int32_t kv_len, kv_row0, prefix, n; // keys; packed: first row of k and v; visible prefix; key tiles visited
@@ -87,11 +88,11 @@ struct AttnPlan {  // views into the workspace
   int32_t* status;
   int64_t* bound;        // [slots + 1] first step of each slot
   AttnSlot* slot;        // [slots]
-  int32_t* counter;      // [2 * slots] finished parts of the item that starts in a slot (PAIR: per stream)
+  int32_t* counter;      // [slots] finished parts of the item that starts in a slot
   int32_t* seq_first;    // [n_seqs + 1] first entry of a sequence
   int2* doc_range;       // [n_tokens / keys of a tile + n_seqs + 1] smallest and largest document of a key tile
   AttnEntry* entry;
-  float2* part_ml;       // [2 * slots * streams][rows] maximum (log2 units) and denominator
+  float2* part_ml;       // [2 * slots][rows] maximum (log2 units) and denominator
   float* part_o;         // [...][rows][Dp]
   int32_t max_entries, rows;
 };
@@ -197,7 +198,7 @@ attn_plan_kernel(const AttnJob j, const AttnMod mod, const AttnPlan p, int token
     *p.status = 0;
     carry = 0;
   }
-  for (int i = tid; i < 2 * max_slots; i += static_cast<int>(blockDim.x)) p.counter[i] = 0;
+  for (int i = tid; i < max_slots; i += static_cast<int>(blockDim.x)) p.counter[i] = 0;
   for (int i = tid; i < max_slots; i += static_cast<int>(blockDim.x)) p.slot[i] = AttnSlot{0, 0, 0, 0};
   __syncthreads();
   // the device copies of the lengths, read once
@@ -609,7 +610,7 @@ struct AsTanh {
   }
 };
 
-template <int D, bool PAGED, bool PAIR, int MODE>
+template <int D, bool PAGED, int MODE>
 __global__ void __launch_bounds__(AS_THREADS, 1)
 attn_scored_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constant__ CUtensorMap tmap_k,
                    const __grid_constant__ CUtensorMap tmap_v, const __grid_constant__ AttnJob j, const __grid_constant__ AttnMod mod,
@@ -617,8 +618,8 @@ attn_scored_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_cons
   using Cfg = AsCfg<D>;
   constexpr int RING = Cfg::RING, KV = Cfg::KV;
   constexpr uint32_t Q_BUFS = Cfg::Q_BUFS;
-  // A stream's own tiles in flight, so that neither stream waits for the other's; a pair has one ring.
-  constexpr uint32_t SLOTS = PAIR ? RING : RING / 2;
+  // A stream's own tiles in flight, so that neither stream waits for the other's.
+  constexpr uint32_t SLOTS = RING / 2;
   extern __shared__ uint8_t as_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(as_raw) + 1023) & ~uintptr_t(1023));
   uint8_t* q_s = smem;
@@ -644,9 +645,9 @@ attn_scored_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_cons
   if (threadIdx.x == 0) {
     for (int i = 0; i < RING; ++i) {
       mbar_init(&k_full[i], 1);
-      mbar_init(&k_empty[i], PAIR ? 2 : 1);  // a tile is read by both streams of a pair
+      mbar_init(&k_empty[i], 1);
       mbar_init(&v_full[i], 1);
-      mbar_init(&v_empty[i], PAIR ? 2 : 1);
+      mbar_init(&v_empty[i], 1);
     }
     for (int t = 0; t < 2; ++t) {
       for (int b = 0; b < 2; ++b) {
@@ -683,8 +684,7 @@ attn_scored_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_cons
     }
     AsWalk<KV> w[2];
     w[0].start(plan, blockIdx.x);
-    if (PAIR) w[1].left = 0;
-    else w[1].start(plan, blockIdx.x + gridDim.x);
+    w[1].start(plan, blockIdx.x + gridDim.x);
     uint32_t fills[2] = {0, 0}, q_fills[2] = {0, 0};
     AsPatience patience;
     bool ok = true;
@@ -692,29 +692,23 @@ attn_scored_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_cons
     while (ok && (w[0].left > 0 || w[1].left > 0)) {
       bool moved = false;
 #pragma unroll
-      for (int t = 0; t < (PAIR ? 1 : 2); ++t) {
+      for (int t = 0; t < 2; ++t) {
         if (w[t].left <= 0) continue;
         const uint32_t slot = t * SLOTS + fills[t] % SLOTS;
         bool ready = as_test(&empty[slot], ((fills[t] / SLOTS) & 1u) ^ 1u);
-        if (is_k && w[t].first) {
-#pragma unroll
-          for (int u = t; u < (PAIR ? 2 : t + 1); ++u) ready = ready && as_test(&q_empty[2 * u + q_fills[u] % Q_BUFS], ((q_fills[u] / Q_BUFS) & 1u) ^ 1u);
-        }
+        if (is_k && w[t].first) ready = ready && as_test(&q_empty[2 * t + q_fills[t] % Q_BUFS], ((q_fills[t] / Q_BUFS) & 1u) ^ 1u);
         if (!__all_sync(0xffffffffu, ready)) continue;
         moved = true;
         if (is_k && w[t].first) {
+          if (lane == 0) {
+            const uint32_t qb = q_fills[t] % Q_BUFS;
+            mbar_arrive_expect_tx(&q_full[2 * t + qb], j.group * j.tile_tokens * 128 * Cfg::BLOCKS);
 #pragma unroll
-          for (int u = t; u < (PAIR ? 2 : t + 1); ++u) {
-            if (lane == 0) {
-              const uint32_t qb = q_fills[u] % Q_BUFS;
-              mbar_arrive_expect_tx(&q_full[2 * u + qb], j.group * j.tile_tokens * 128 * Cfg::BLOCKS);
-#pragma unroll
-              for (int b = 0; b < Cfg::BLOCKS; ++b)
-                as_tma_3d(q_s + (u * Q_BUFS + qb) * Cfg::Q_TILE + b * Cfg::Q_BLOCK, &tmap_q, &q_full[2 * u + qb], b * 64, w[t].h * j.group,
-                          w[t].f0.y + (PAIR ? u * j.tile_tokens : 0));
-            }
-            ++q_fills[u];
+            for (int b = 0; b < Cfg::BLOCKS; ++b)
+              as_tma_3d(q_s + (t * Q_BUFS + qb) * Cfg::Q_TILE + b * Cfg::Q_BLOCK, &tmap_q, &q_full[2 * t + qb], b * 64, w[t].h * j.group,
+                        w[t].f0.y);
           }
+          ++q_fills[t];
         }
         as_load_tile<D, PAGED>(j, w[t], tmap, ring + slot * Cfg::KV_TILE, &full[slot], lane);
         ++fills[t];
@@ -725,7 +719,7 @@ attn_scored_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_cons
     if (is_k) pdl_launch_dependents();
     if (!ok) {
       if (lane == 0) atomicExch(plan.status, is_k ? 5 : 8);
-      for (int t = 0; t < (PAIR ? 1 : 2); ++t) as_drain(&full[t * SLOTS], fills[t], SLOTS);
+      for (int t = 0; t < 2; ++t) as_drain(&full[t * SLOTS], fills[t], SLOTS);
       if (is_k)
         for (int u = 0; u < 2; ++u) as_drain(&q_full[2 * u], q_fills[u], Q_BUFS);
     }
@@ -735,14 +729,12 @@ attn_scored_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_cons
     const int t = warp - AS_MMA_WARP;
     const uint32_t tmem_u = __shfl_sync(0xffffffffu, tmem_base, 0);
     const uint32_t q_addr = smem_u32(q_s) + t * Q_BUFS * Cfg::Q_TILE, k_addr = smem_u32(k_s), v_addr = smem_u32(v_s);
-    const uint32_t ring0 = PAIR ? 0 : t * SLOTS;
+    const uint32_t ring0 = t * SLOTS;
     AsWalk<KV> sw, pw;  // the next S, and the next P V
-    sw.start(plan, PAIR ? blockIdx.x : blockIdx.x + t * gridDim.x);
+    sw.start(plan, blockIdx.x + t * gridDim.x);
     pw = sw;
     uint32_t q_uses = 0, n_s = 0, n_pv = 0;
     const uint32_t idesc_pv = make_idesc_bf16_f32_b_mn(128, D);
-    // In a pair stream B may have no tokens (the item ends in A's tile): its steps are then only counted.
-    auto has_rows = [&](const AsWalk<KV>& w) { return !PAIR || t == 0 || w.f0.z > j.tile_tokens; };
     auto wait_all = [](uint64_t* bar, uint32_t parity) -> bool { return __all_sync(0xffffffffu, mbar_wait(bar, parity)); };
     auto issue_s = [&]() -> bool {
       const uint32_t slot = ring0 + n_s % SLOTS, buf = n_s % 2;
@@ -754,13 +746,11 @@ attn_scored_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_cons
       if (!wait_all(&k_full[slot], (n_s / SLOTS) & 1u)) return false;
       tc_fence_after_sync();
       const uint32_t idesc = make_idesc_bf16_f32(128, as_round16(sw.n_valid()));
-      if (has_rows(sw)) {
 #pragma unroll
-        for (int k = 0; k < D / 16; ++k) {
-          const uint64_t a = make_kmajor_sw128_desc(q_addr + qb * Cfg::Q_TILE + (k / 4) * Cfg::Q_BLOCK) + 2 * (k % 4);
-          const uint64_t b = make_kmajor_sw128_desc(k_addr + slot * Cfg::KV_TILE + (k / 4) * Cfg::KV_BLOCK) + 2 * (k % 4);
-          if (elect_one()) tc_mma_f16(tmem_u + t * Cfg::S(1, 0) + buf * Cfg::S(0, 1), a, b, idesc, k != 0);
-        }
+      for (int k = 0; k < D / 16; ++k) {
+        const uint64_t a = make_kmajor_sw128_desc(q_addr + qb * Cfg::Q_TILE + (k / 4) * Cfg::Q_BLOCK) + 2 * (k % 4);
+        const uint64_t b = make_kmajor_sw128_desc(k_addr + slot * Cfg::KV_TILE + (k / 4) * Cfg::KV_BLOCK) + 2 * (k % 4);
+        if (elect_one()) tc_mma_f16(tmem_u + t * Cfg::S(1, 0) + buf * Cfg::S(0, 1), a, b, idesc, k != 0);
       }
       if (elect_one()) {
         tc_commit(&s_full[2 * t + buf]);
@@ -776,8 +766,7 @@ attn_scored_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_cons
       if (!wait_all(&v_full[slot], (n_pv / SLOTS) & 1u)) return false;
       const int n_valid = pw.n_valid(), n_eff = as_round16(n_valid);
       if (n_valid < n_eff) {
-        // value rows behind the last key: whatever lies there must not meet a zero probability (0 * NaN). In a pair both warps write
-        // these zeros, each before its own instructions.
+        // value rows behind the last key: whatever lies there must not meet a zero probability (0 * NaN)
         uint8_t* tile = v_s + slot * Cfg::KV_TILE;
         for (int i = lane; i < (n_eff - n_valid) * 8 * Cfg::BLOCKS; i += 32) {
           const int b = i / ((n_eff - n_valid) * 8), at = i - b * ((n_eff - n_valid) * 8);
@@ -788,15 +777,13 @@ attn_scored_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_cons
       }
       if (!wait_all(&p_full[2 * t + buf], (n_pv / 2) & 1u)) return false;
       tc_fence_after_sync();
-      if (has_rows(pw)) {
-        const uint64_t v_desc = make_mnmajor_sw128_desc(v_addr + slot * Cfg::KV_TILE, Cfg::KV_BLOCK);
-        const uint32_t p_at = tmem_u + t * Cfg::S(1, 0) + buf * Cfg::S(0, 1);
+      const uint64_t v_desc = make_mnmajor_sw128_desc(v_addr + slot * Cfg::KV_TILE, Cfg::KV_BLOCK);
+      const uint32_t p_at = tmem_u + t * Cfg::S(1, 0) + buf * Cfg::S(0, 1);
 #pragma unroll
-        for (int k = 0; k < KV / 16; ++k)
-          if (k * 16 < n_eff && elect_one())
-            tc_mma_f16_tmem_a(tmem_u + Cfg::O(0) + t * (Cfg::O(1) - Cfg::O(0)), p_at + (k / 2) * 32 + (k % 2) * 8, v_desc + k * 128,
-                              idesc_pv, !pw.first || k != 0);
-      }
+      for (int k = 0; k < KV / 16; ++k)
+        if (k * 16 < n_eff && elect_one())
+          tc_mma_f16_tmem_a(tmem_u + Cfg::O(0) + t * (Cfg::O(1) - Cfg::O(0)), p_at + (k / 2) * 32 + (k % 2) * 8, v_desc + k * 128,
+                            idesc_pv, !pw.first || k != 0);
       if (elect_one()) {
         tc_commit(&pv_done[2 * t + buf]);
         tc_commit(&v_empty[slot]);
@@ -823,7 +810,7 @@ attn_scored_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_cons
     volatile int* cold = reinterpret_cast<volatile int*>(smem + Cfg::SMEM_BYTES - 1024 - Cfg::COLD_BYTES) + warp * AS_COLD;
     float* table = table_s + t * AS_TABLE;
     const int row_tok = (row * j.group_inv) >> 16, g = row - row_tok * j.group;
-    const int my_slot = PAIR ? blockIdx.x : blockIdx.x + t * gridDim.x;
+    const int my_slot = blockIdx.x + t * gridDim.x;
     const float scale_log2 = mod.scale * AS_LOG2E, cap_out = mod.cap * AS_LOG2E;
     // held finite: a score of zero stays zero under the smallest caps
     const float cap_in = mod.cap > 0.f ? fminf(fmaxf(mod.scale / mod.cap, -FLT_MAX), FLT_MAX) : 0.f;
@@ -851,7 +838,7 @@ attn_scored_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_cons
     // P V of step s, one of the last two. A barrier is told by its parity alone, so each of two score buffers has its own: of the P V
     // of two steps before, the scores of step s + 1 have already told.
     auto pv_wait = [&](uint32_t s) { return mbar_wait(&pv_done[2 * t + s % 2], (s / 2) & 1u); };
-    auto part_of = [&](int slot, bool tail) -> int64_t { return (2 * slot + (tail ? 1 : 0)) * (PAIR ? 2 : 1) + (PAIR ? t : 0); };
+    auto part_of = [&](int slot, bool tail) -> int64_t { return 2 * slot + (tail ? 1 : 0); };
     float slope = 0.f;
     const float* tab = nullptr;
     float tab_unit = 1.f;
@@ -868,7 +855,7 @@ attn_scored_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_cons
         const int h = cold[C_H];
         const int4* entry = reinterpret_cast<const int4*>(plan.entry + cold[C_E]);
         const int4 f0 = entry[0], f1 = entry[1], f2 = entry[2];
-        const int skip = PAIR ? t * j.tile_tokens : 0, n_tok = min(max(f0.z - skip, 0), j.tile_tokens);
+        const int n_tok = f0.z;
         i_k = cold[C_K];
         i_end = min(f1.w, i_k + cold[C_LEFT]);
         run0 = f2.x;
@@ -876,11 +863,11 @@ attn_scored_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_cons
         run1 = f2.z;
         run_near = f2.w;
         kv_len = f1.x;
-        pos = f0.w + skip + row_tok;
+        pos = f0.w + row_tok;
         n_rows = n_tok * j.group;
         __syncwarp();
         if (lane == 0) {
-          cold[C_TOK0] = f0.y + skip;
+          cold[C_TOK0] = f0.y;
           cold[C_NTOK] = n_tok;
           cold[C_KVROW0] = f1.y;
           cold[C_PREFIX] = f1.z;
@@ -1310,7 +1297,7 @@ attn_scored_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_cons
         if (failed) break;
         if (row == 0) {
           __threadfence();
-          const int old = atomicAdd(&plan.counter[2 * s0 + (PAIR ? t : 0)], 1);
+          const int old = atomicAdd(&plan.counter[s0], 1);
           __threadfence();
           joins[t] = old == s1 - s0;
         }
@@ -1463,7 +1450,7 @@ static int64_t as_layout(void* workspace, int n_seqs, int n_tokens, int n_heads,
   q.status = reinterpret_cast<int32_t*>(take(sizeof(int32_t)));
   q.bound = reinterpret_cast<int64_t*>(take((AS_MAX_SLOTS + 1) * sizeof(int64_t)));
   q.slot = reinterpret_cast<AttnSlot*>(take(AS_MAX_SLOTS * sizeof(AttnSlot)));
-  q.counter = reinterpret_cast<int32_t*>(take(2 * AS_MAX_SLOTS * sizeof(int32_t)));
+  q.counter = reinterpret_cast<int32_t*>(take(AS_MAX_SLOTS * sizeof(int32_t)));
   q.seq_first = reinterpret_cast<int32_t*>(take((seqs + 1) * sizeof(int32_t)));
   q.doc_range = reinterpret_cast<int2*>(take((tokens / 64 + seqs + 1) * sizeof(int2)));
   q.entry = reinterpret_cast<AttnEntry*>(take(entries * sizeof(AttnEntry)));
@@ -1486,53 +1473,44 @@ struct AsMaps {
   CUtensorMap q, k, v;
 };
 
-// Two neighbouring tiles share their keys where sequences have two tiles of rows on average; shorter ones would leave stream B idle.
-// Documents keep each tile to its own few keys. (8 sequences of 2048, causal, 28/4 heads of 128: 404 us in pairs, 423 without; 192 of 8 to
-// 512, 16 heads of 64: 219 and 193.)
-static bool as_pair(const AttnJob& j, const AttnMod& mod) { return mod.docs == nullptr && static_cast<int64_t>(j.n_tokens) * j.group >= 256ll * j.n_seqs; }
-
-template <int D, bool PAGED, bool PAIR, int MODE>
+template <int D, bool PAGED, int MODE>
 static int as_launch(const AsMaps& m, const AttnJob& j, const AttnMod& mod, const AttnPlan& plan, int sms, cudaStream_t s) {
   int64_t grid = sms < AS_MAX_CTAS ? sms : AS_MAX_CTAS;
   if (!PAGED) {  // no more CTAs than steps there can be
     const int64_t steps = static_cast<int64_t>(plan.max_entries) * j.n_kv_heads * ((j.n_tokens + AsCfg<D>::KV - 1) / AsCfg<D>::KV);
     if (steps < grid) grid = steps;
   }
-  const int slots = static_cast<int>(PAIR ? grid : 2 * grid);
+  const int slots = static_cast<int>(2 * grid);
   // few entries are planned by fewer threads: their barriers are what it takes
   const int threads = plan.max_entries <= 256 && j.n_seqs <= 256 && mod.docs == nullptr ? 256 : AS_PLAN_THREADS;
-  cudaError_t e = launch_pdl(attn_plan_kernel, dim3(1), dim3(threads), 0, s, j, mod, plan, (PAIR ? 2 : 1) * j.tile_tokens, slots, AsCfg<D>::KV);
+  cudaError_t e = launch_pdl(attn_plan_kernel, dim3(1), dim3(threads), 0, s, j, mod, plan, j.tile_tokens, slots, AsCfg<D>::KV);
   if (e == cudaSuccess)
-    e = launch_pdl(attn_scored_kernel<D, PAGED, PAIR, MODE>, dim3(static_cast<unsigned>(grid)), dim3(AS_THREADS), AsCfg<D>::SMEM_BYTES, s, m.q, m.k,
+    e = launch_pdl(attn_scored_kernel<D, PAGED, MODE>, dim3(static_cast<unsigned>(grid)), dim3(AS_THREADS), AsCfg<D>::SMEM_BYTES, s, m.q, m.k,
                    m.v, j, mod, plan);
   if (e != cudaSuccess) return set_error(B200EMB_ERR_CUDA, "attention launch: %s", cudaGetErrorString(e));
   return B200EMB_OK;
 }
 
-template <int D, bool PAGED, bool PAIR, int MODE>
+template <int D, bool PAGED, int MODE>
 static int as_init_one() {
-  B2_CUDA_CHECK(cudaFuncSetAttribute(attn_scored_kernel<D, PAGED, PAIR, MODE>, cudaFuncAttributeMaxDynamicSharedMemorySize, AsCfg<D>::SMEM_BYTES));
+  B2_CUDA_CHECK(cudaFuncSetAttribute(attn_scored_kernel<D, PAGED, MODE>, cudaFuncAttributeMaxDynamicSharedMemorySize, AsCfg<D>::SMEM_BYTES));
   return B200EMB_OK;
 }
 
-template <int D, bool PAGED, bool PAIR>
+template <int D, bool PAGED>
 static int as_init_modes() {
-  int rc = as_init_one<D, PAGED, PAIR, AS_PLAIN>();
-  if (!rc) rc = as_init_one<D, PAGED, PAIR, AS_SLOPES>();
-  if (!rc) rc = as_init_one<D, PAGED, PAIR, AS_CAP>();
-  if (!rc) rc = as_init_one<D, PAGED, PAIR, AS_ANY>();
+  int rc = as_init_one<D, PAGED, AS_PLAIN>();
+  if (!rc) rc = as_init_one<D, PAGED, AS_SLOPES>();
+  if (!rc) rc = as_init_one<D, PAGED, AS_CAP>();
+  if (!rc) rc = as_init_one<D, PAGED, AS_ANY>();
   return rc;
 }
 
 int attention_scored_init_device() {
-  int rc = as_init_modes<64, false, false>();
-  if (!rc) rc = as_init_modes<64, false, true>();
-  if (!rc) rc = as_init_modes<64, true, false>();
-  if (!rc) rc = as_init_modes<64, true, true>();
-  if (!rc) rc = as_init_modes<128, false, false>();
-  if (!rc) rc = as_init_modes<128, false, true>();
-  if (!rc) rc = as_init_modes<128, true, false>();
-  if (!rc) rc = as_init_modes<128, true, true>();
+  int rc = as_init_modes<64, false>();
+  if (!rc) rc = as_init_modes<64, true>();
+  if (!rc) rc = as_init_modes<128, false>();
+  if (!rc) rc = as_init_modes<128, true>();
   return rc;
 }
 
@@ -1555,15 +1533,15 @@ static int as_map_pages(CUtensorMap* m, const void* base, const b200emb_kv_cache
   return encode_tmap_bf16(m, base, 4, dims, strides, box);
 }
 
-template <int D, bool PAGED, bool PAIR>
+template <int D, bool PAGED>
 static int as_launch_mode(const AsMaps& m, const AttnJob& j, const AttnMod& mod, const AttnPlan& plan, int sms, cudaStream_t s) {
-  if (mod.docs != nullptr) return as_launch<D, PAGED, PAIR, AS_ANY>(m, j, mod, plan, sms, s);
-  if (mod.cap == 0.f && mod.slopes == nullptr && mod.bias == nullptr) return as_launch<D, PAGED, PAIR, AS_PLAIN>(m, j, mod, plan, sms, s);
-  if (mod.cap == 0.f && mod.slopes != nullptr) return as_launch<D, PAGED, PAIR, AS_SLOPES>(m, j, mod, plan, sms, s);
+  if (mod.docs != nullptr) return as_launch<D, PAGED, AS_ANY>(m, j, mod, plan, sms, s);
+  if (mod.cap == 0.f && mod.slopes == nullptr && mod.bias == nullptr) return as_launch<D, PAGED, AS_PLAIN>(m, j, mod, plan, sms, s);
+  if (mod.cap == 0.f && mod.slopes != nullptr) return as_launch<D, PAGED, AS_SLOPES>(m, j, mod, plan, sms, s);
   const float cap = mod.cap * AS_LOG2E;
   if (cap >= AS_CAP_LOW && cap <= AS_CAP_HIGH && mod.slopes == nullptr && mod.bias == nullptr)
-    return as_launch<D, PAGED, PAIR, AS_CAP>(m, j, mod, plan, sms, s);
-  return as_launch<D, PAGED, PAIR, AS_ANY>(m, j, mod, plan, sms, s);
+    return as_launch<D, PAGED, AS_CAP>(m, j, mod, plan, sms, s);
+  return as_launch<D, PAGED, AS_ANY>(m, j, mod, plan, sms, s);
 }
 
 template <bool PAGED>
@@ -1574,10 +1552,7 @@ static int as_dispatch(const AsMaps& m, const AttnJob& j, const AttnMod& mod, vo
   if (rc) return rc;
   AttnPlan plan;
   as_layout(workspace, j.n_seqs, j.n_tokens, j.n_heads, j.n_kv_heads, j.head_dim, &plan);
-  const bool pair = as_pair(j, mod);
-  if (j.head_dim <= 64)
-    return pair ? as_launch_mode<64, PAGED, true>(m, j, mod, plan, sms, s) : as_launch_mode<64, PAGED, false>(m, j, mod, plan, sms, s);
-  return pair ? as_launch_mode<128, PAGED, true>(m, j, mod, plan, sms, s) : as_launch_mode<128, PAGED, false>(m, j, mod, plan, sms, s);
+  return j.head_dim <= 64 ? as_launch_mode<64, PAGED>(m, j, mod, plan, sms, s) : as_launch_mode<128, PAGED>(m, j, mod, plan, sms, s);
 }
 
 }  // namespace b2
