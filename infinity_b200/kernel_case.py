@@ -4,8 +4,12 @@
     python -m infinity_b200.kernel_case attention --seqs 256 --len 384 --heads 16 --head-dim 64 --launches 3
     python -m infinity_b200.kernel_case add_ln --rows 65536 --hidden 1024 --launches 3
     python -m infinity_b200.kernel_case nvfp4 --m 1024 --n 37888 --k 3584 --epi swiglu --launches 5
+    python -m infinity_b200.kernel_case rope --seqs 16 --len 1024 --heads 28 --kv-heads 4 --head-dim 128
+    python -m infinity_b200.kernel_case scored --seqs 8 --len 2048 --heads 28 --kv-heads 4 --head-dim 128 --causal 1 --cap 50
+    python -m infinity_b200.kernel_case paged --seqs 48 --len 4096 --new 1 --heads 28 --kv-heads 4 --head-dim 128 --page 16
 
-The nvfp4 case also times its two ways of multiplying by NVFP4 weights (CUDA events, best of the launches):
+The paged case appends --new tokens of each sequence to a cache that holds the rest of its --len (b200emb_op_kv_append, rotating) and
+attends to it (b200emb_op_attention_paged); rope, scored and paged print the best time of the launches. The nvfp4 case also times its two ways of multiplying by NVFP4 weights (CUDA events, best of the launches):
 expansion inside the GEMM (b200emb_op_gemm_nvfp4) against the expansion kernel followed by the bf16 GEMM.
 
 Every case checks its result against a torch computation before exiting 0.
@@ -13,6 +17,7 @@ Every case checks its result against a torch computation before exiting 0.
 from __future__ import annotations
 
 import argparse
+import ctypes as C
 import math
 
 import numpy as np
@@ -22,9 +27,95 @@ from . import _lib
 from . import configs as cf
 
 
+def _best(fn, launches: int) -> float:
+    """Best time of the launches in microseconds (CUDA events)."""
+    best = float("inf")
+    for _ in range(launches):
+        e0, e1 = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+        e0.record()
+        fn()
+        e1.record()
+        torch.cuda.synchronize()
+        best = min(best, e0.elapsed_time(e1) * 1e3)
+    return best
+
+
+def _attend(q, k, v, first, a, slopes):
+    """Attention of one sequence in fp32: q [n, heads, d] at positions first .., k and v [m, kv heads, d]."""
+    rep, pos = q.shape[1] // k.shape[1], torch.arange(q.shape[0], device=q.device)[:, None] + first
+    k, v = (z.float().repeat_interleave(rep, 1) for z in (k, v))
+    s = torch.einsum("nhd,mhd->hnm", q.float(), k) / math.sqrt(q.shape[2])
+    if a.cap > 0:
+        s = a.cap * torch.tanh(s / a.cap)
+    key = torch.arange(k.shape[0], device=q.device)[None]
+    if slopes is not None:
+        s = s - slopes[:, None, None] * (key - pos).abs()
+    seen = torch.ones_like(s[0], dtype=torch.bool) if not a.causal and a.kernel != "paged" else key <= pos
+    if a.window >= 0:
+        seen &= key >= pos - a.window
+    return torch.einsum("hnm,mhd->nhd", s.masked_fill(~seen, float("-inf")).softmax(-1), v).reshape(q.shape[0], -1)
+
+
+def _attention_block(a, lib, stream) -> None:
+    """Rotary positions, the cache append and the attention over it, and attention with modified scores."""
+    nkv, d, new = a.kv_heads or a.heads, a.head_dim, a.new if a.kernel == "paged" else a.len
+    T, width = a.seqs * new, (a.heads + 2 * nkv) * d
+    qkv = torch.randn(T, width, device="cuda").to(torch.bfloat16)
+    q, k, v = qkv[:, : a.heads * d], qkv[:, a.heads * d: (a.heads + nkv) * d], qkv[:, (a.heads + nkv) * d:]
+    cu = torch.arange(a.seqs + 1, device="cuda", dtype=torch.int32) * new
+    rope = _lib.RopeDesc(rot_dim=d, layout=_lib.ROPE_LAYOUT["half"], scaling=_lib.ROPE_SCALING["none"], original_max_pos=2048, theta=1e6, factor=1.0)
+    angle = torch.arange(a.len, device="cuda").double()[:, None] * 1e6 ** (-torch.arange(0, d, 2, device="cuda").double() / d)
+    turn = torch.cat([angle, angle], 1)[:, None]
+
+    def rotated(x, first):  # [n, heads, d] at positions first ..
+        x, t = x.double(), turn[first: first + x.shape[0]]
+        return x * t.cos() + torch.cat([-x[..., d // 2:], x[..., : d // 2]], -1) * t.sin()
+
+    if a.kernel == "rope":
+        out = torch.empty(T, (a.heads + nkv) * d, dtype=torch.bfloat16, device="cuda")
+        us = _best(lambda: _lib.check(lib.b200emb_op_rope(qkv.data_ptr(), width, out.data_ptr(), out.stride(0), None, cu.data_ptr(), None, a.seqs, T,
+                                                          a.heads + nkv, d, C.byref(rope), stream)), a.launches)
+        ref = rotated(qkv[: a.len, : (a.heads + nkv) * d].view(a.len, -1, d), 0).view(a.len, -1)
+        err = (out[: a.len].double() - ref).abs().max().item()
+        assert err < 3e-2, err
+        print(f"rope {T} tokens of {a.heads + nkv} heads of {d} ok, max abs err {err:.4f}, {us:.1f} us, {4e-3 * out.numel() / us:.0f} GB/s")
+        return
+    slopes = torch.tensor([2.0 ** (-8 * (h + 1) / a.heads) for h in range(a.heads)], device="cuda") if a.slopes else None
+    opts = _lib.AttnOpts(cap=a.cap, causal=int(a.kernel == "paged" or a.causal), window_left=a.window, window_right=-1,
+                         slopes=None if slopes is None else slopes.data_ptr())
+    out = torch.empty(T, a.heads * d, dtype=torch.bfloat16, device="cuda")
+    ws = torch.empty(lib.b200emb_attention_workspace_bytes(a.seqs, T, a.heads, nkv, d), dtype=torch.uint8, device="cuda")
+    if a.kernel == "scored":
+        us = _best(lambda: _lib.check(lib.b200emb_op_attention_scored(
+            q.data_ptr(), width, k.data_ptr(), width, v.data_ptr(), width, out.data_ptr(), out.stride(0), cu.data_ptr(), a.seqs, T, a.heads, nkv, d,
+            C.byref(opts), ws.data_ptr(), ws.numel(), stream)), a.launches)
+        ref = _attend(q[: a.len].view(a.len, a.heads, d), k[: a.len].view(a.len, nkv, d), v[: a.len].view(a.len, nkv, d), 0, a, slopes)
+    else:
+        per = -(-a.len // a.page)
+        cache = torch.randn(2, a.seqs * per, a.page, nkv, d, device="cuda").to(torch.bfloat16)
+        table = torch.randperm(a.seqs * per, device="cuda").to(torch.int32).view(a.seqs, per)
+        lens = torch.full((a.seqs,), a.len, dtype=torch.int32, device="cuda")
+        desc = _lib.KvCache(k=cache[0].data_ptr(), v=cache[1].data_ptr(), page_table=table.data_ptr(), n_pages=a.seqs * per, page_size=a.page,
+                            n_kv_heads=nkv, head_dim=d, table_stride=per, page_stride=a.page * nkv * d, token_stride=nkv * d, head_stride=d)
+        turned = torch.empty(T, a.heads * d, dtype=torch.bfloat16, device="cuda")
+        _lib.check(lib.b200emb_op_kv_append(qkv.data_ptr(), width, cu.data_ptr(), lens.data_ptr(), a.seqs, T, a.heads, C.byref(rope),
+                                            turned.data_ptr(), turned.stride(0), C.byref(desc), stream))
+        us = _best(lambda: _lib.check(lib.b200emb_op_attention_paged(
+            turned.data_ptr(), turned.stride(0), out.data_ptr(), out.stride(0), cu.data_ptr(), lens.data_ptr(), a.seqs, T, a.heads, C.byref(desc),
+            C.byref(opts), ws.data_ptr(), ws.numel(), stream)), a.launches)
+        kc, vc = (z[table[0].long()].view(-1, nkv, d)[: a.len] for z in cache)
+        fresh = rotated(k[:new].view(new, nkv, d), a.len - new)
+        assert (kc[a.len - new:].double() - fresh).abs().max().item() < 3e-2 and torch.equal(vc[a.len - new:].reshape(new, -1), v[:new])
+        ref = _attend(turned[:new].view(new, a.heads, d), kc, vc, a.len - new, a, slopes)
+    _lib.check(lib.b200emb_op_workspace_status(ws.data_ptr(), stream))
+    err = (out[: ref.shape[0]].float() - ref).abs().max().item()
+    assert err < 2e-2 * max(1.0, ref.abs().max().item()), err
+    print(f"{a.kernel} {a.seqs} sequences, {T} tokens over {a.seqs * a.len} keys, {a.heads}/{nkv} heads of {d} ok, max abs err {err:.4f}, {us:.1f} us")
+
+
 def main() -> None:
     ap = argparse.ArgumentParser()
-    ap.add_argument("kernel", choices=["gemm", "attention", "add_ln", "nvfp4", "mxfp8"])
+    ap.add_argument("kernel", choices=["gemm", "attention", "add_ln", "nvfp4", "mxfp8", "rope", "scored", "paged"])
     ap.add_argument("--m", type=int, default=32768)
     ap.add_argument("--n", type=int, default=3072)
     ap.add_argument("--k", type=int, default=1024)
@@ -36,6 +127,11 @@ def main() -> None:
     ap.add_argument("--kv-heads", type=int, default=0)
     ap.add_argument("--head-dim", type=int, default=64)
     ap.add_argument("--causal", type=int, default=0)
+    ap.add_argument("--new", type=int, default=1, help="paged: new tokens of each sequence")
+    ap.add_argument("--page", type=int, default=16, help="paged: tokens of a page")
+    ap.add_argument("--cap", type=float, default=0.0, help="scored, paged: scores become cap tanh(score / cap)")
+    ap.add_argument("--window", type=int, default=-1, help="scored, paged: keys visible to the left")
+    ap.add_argument("--slopes", type=int, default=0, help="scored, paged: 1 takes a slope per head times the distance off the scores")
     ap.add_argument("--rows", type=int, default=65536)
     ap.add_argument("--hidden", type=int, default=1024)
     ap.add_argument("--launches", type=int, default=3)
@@ -129,6 +225,8 @@ def main() -> None:
         flops = 2.0 * a.m * a.n * a.k
         print(f"nvfp4 gemm {a.m}x{a.n}x{a.k} {a.epi}: expansion in the kernel {t_fused:.3f} ms ({flops / t_fused / 1e9:.0f} TFLOP/s), "
               f"expansion kernel + bf16 gemm {t_exp:.3f} ms ({flops / t_exp / 1e9:.0f} TFLOP/s)")
+    elif a.kernel in ("rope", "scored", "paged"):
+        _attention_block(a, lib, stream)
     elif a.kernel == "attention":
         nkv = a.kv_heads or a.heads
         if a.lengths_of:

@@ -554,6 +554,15 @@ def test_the_first_call_of_a_process_may_be_captured():
     assert done.returncode == 0, done.stderr
 
 
+@pytest.mark.parametrize("args", ["rope --seqs 3 --len 200 --heads 6 --kv-heads 2", "scored --seqs 3 --len 200 --heads 6 --kv-heads 2 --causal 1 --cap 20",
+                                  "scored --seqs 2 --len 150 --heads 4 --slopes 1 --window 40", "paged --seqs 3 --len 300 --new 2 --heads 6 --kv-heads 2",
+                                  "paged --seqs 1 --len 90 --new 90 --heads 4 --slopes 1 --page 24 --head-dim 128"])
+def test_kernel_case_runs_them(args):
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    done = subprocess.run([sys.executable, "-m", "infinity_b200.kernel_case", *args.split()], cwd=root, capture_output=True, text=True, timeout=600)
+    assert done.returncode == 0 and " ok" in done.stdout, done.stderr
+
+
 def test_two_streams_with_their_own_workspaces(lib):
     x = [R.normal(i, 700, 3 * 4 * 64) for i in range(2)]
     cu = R.cu_of([400, 300])
