@@ -587,7 +587,8 @@ __device__ __forceinline__ void as_load_tile(const AttnJob& j, const AsWalk<AsCf
 
 // What happens to a score before it is masked. The kernel is built for each: a row of scores is worked on in straight-line
 // code, and one body with every branch in it is 120 KB of instructions, which the instruction caches do not hold (7 us a step).
-enum { AS_PLAIN = 0, AS_SLOPES = 1, AS_CAP = 2, AS_ANY = 3 };
+enum { AS_PLAIN = 0, AS_SLOPES = 1, AS_CAP = 2, AS_BIAS = 3, AS_DOCS = 4, AS_ANY = 5 };
+// (AS_BIAS: a bias table alone; AS_DOCS: documents, with or without one)
 
 // tanh(x) = x (c0 + c1 u + ... + c5 u^5), u = x^2, within 2.5e-7 on [-1, 1]: the odd polynomial with the smallest largest error there
 // (fitted to tanh in 64 bits by reweighted least squares). It spares the two special-function instructions of
@@ -623,6 +624,7 @@ attn_scored_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_cons
   using Cfg = AsCfg<D>;
   constexpr int RING = Cfg::RING, KV = Cfg::KV;
   constexpr uint32_t Q_BUFS = Cfg::Q_BUFS;
+  constexpr bool DOCS = MODE == AS_DOCS || MODE == AS_ANY, TABLES = DOCS || MODE == AS_BIAS;
   // A stream's own tiles in flight, so that neither stream waits for the other's.
   constexpr uint32_t SLOTS = RING / 2;
   extern __shared__ uint8_t as_raw[];
@@ -881,7 +883,7 @@ attn_scored_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_cons
         __syncwarp();
         if ((MODE == AS_SLOPES || MODE == AS_ANY) && mod.slopes != nullptr)
           slope = slopes_here ? table_s[h * j.group + g] : __ldg(mod.slopes + h * j.group + g) * AS_LOG2E;
-        if (MODE == AS_ANY && mod.bias != nullptr) {
+        if (TABLES && mod.bias != nullptr) {
           const int width = 2 * mod.radius + 1, n = j.group * width;
           if (n <= AS_TABLE) {
             meet();  // the previous item's reads are over
@@ -897,7 +899,7 @@ attn_scored_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_cons
         }
       }
       const bool active = wq * 32 < n_rows, real = row < n_rows;
-      const int doc = MODE == AS_ANY && mod.docs != nullptr && real ? __ldg(mod.docs + cold[C_TOK0] + row_tok) : -1;
+      const int doc = DOCS && mod.docs != nullptr && real ? __ldg(mod.docs + cold[C_TOK0] + row_tok) : -1;
       // first and past-the-last visible key of the window of this row
       auto key_lo = [&]() { return mod.left >= pos ? 0 : pos - mod.left; };
       auto key_hi = [&]() { return mod.right >= kv_len - pos ? kv_len : pos + mod.right + 1; };
@@ -906,7 +908,7 @@ attn_scored_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_cons
       const int all_lo = __reduce_max_sync(0xffffffffu, real ? key_lo() : INT_MIN), all_hi = __reduce_min_sync(0xffffffffu, real ? key_hi() : INT_MAX);
       const int pos_first = __reduce_min_sync(0xffffffffu, real ? pos : INT_MAX), pos_last = __reduce_max_sync(0xffffffffu, real ? pos : INT_MIN);
       int one_doc = -1;  // the document of all rows, or -1
-      if (MODE == AS_ANY && mod.docs != nullptr) {
+      if (DOCS && mod.docs != nullptr) {
         const int least = __reduce_min_sync(0xffffffffu, real ? doc : INT_MAX), most = __reduce_max_sync(0xffffffffu, real ? doc : -1);
         one_doc = least == most ? most : -1;
       }
@@ -922,23 +924,23 @@ attn_scored_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_cons
 #pragma unroll
         for (int q = 0; q < 2; ++q) next_docs[q] = key + q * 32 + lane < kv_len ? __ldg(mod.docs + cold[C_KVROW0] + key + q * 32 + lane) : -1;
       };
-      if (MODE == AS_ANY && mod.docs != nullptr) docs_of(kv0);
+      if (DOCS && mod.docs != nullptr) docs_of(kv0);
       for (; i_k < i_end; ++i_k) {
         const int buf = step % 2, n_valid = min(max(kv_len - kv0, 0), KV), n_rem = as_round16(n_valid);
         const int next_kv0 = i_k + 1 < i_end ? key0_of(i_k + 1) : 0;
         int key_docs[2] = {next_docs[0], next_docs[1]};
-        if (MODE == AS_ANY && mod.docs != nullptr) docs_of(next_kv0);
+        if (DOCS && mod.docs != nullptr) docs_of(next_kv0);
         if (!mbar_wait(&s_full[2 * t + buf], (step / 2) & 1u)) failed = true;  // looked at below, once a step
         tc_fence_after_sync();
         if (active) {
           const uint32_t s_at = lanes + t * Cfg::S(1, 0) + buf * Cfg::S(0, 1);
           bool whole = all_lo <= kv0 && all_hi >= kv0 + KV;  // no masks
-          if (MODE == AS_ANY && mod.docs != nullptr && whole)
+          if (DOCS && mod.docs != nullptr && whole)
             whole = one_doc >= 0 && __all_sync(0xffffffffu, key_docs[0] == one_doc && key_docs[1] == one_doc);
           auto seen_of = [&](int q) -> uint32_t {
             const int key = kv0 + q * 32;
             uint32_t seen = (as_below(key_hi() - key) & ~as_below(key_lo() - key)) | as_below(cold[C_PREFIX] - key);
-            if (MODE == AS_ANY && mod.docs != nullptr) {
+            if (DOCS && mod.docs != nullptr) {
               const int key_doc = q == 0 ? key_docs[0] : key_docs[1];
               uint32_t same = 0;
               if (one_doc >= 0) {
@@ -1004,12 +1006,12 @@ attn_scored_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_cons
             }
             return (sum.x + sum1.x) + (sum.y + sum1.y);
           };
-          // AS_ANY: 32 scores into exponents against the reference
+          // AS_BIAS, AS_DOCS, AS_ANY: 32 scores into exponents against the reference
           auto any_scores = [&](const uint32_t (&z)[32], int key32, float2 (&e2)[16]) {
             float y[32];
 #pragma unroll
             for (int i = 0; i < 32; ++i) y[i] = __uint_as_float(z[i]);
-            if (mod.cap > 0.f) {
+            if (MODE == AS_ANY && mod.cap > 0.f) {
 #pragma unroll
               for (int i = 0; i < 32; ++i) y[i] = fmaf(cap_out, as_tanh_any(y[i] * cap_in), -ref);
             } else {
@@ -1017,12 +1019,12 @@ attn_scored_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_cons
               for (int i = 0; i < 32; ++i) y[i] = fmaf(y[i], scale_log2, -ref);
             }
             const int d0 = key32 - pos;
-            if (mod.slopes != nullptr) {
+            if (MODE == AS_ANY && mod.slopes != nullptr) {
               const float f = static_cast<float>(d0);
 #pragma unroll
               for (int i = 0; i < 32; ++i) y[i] = fmaf(-slope, fabsf(f + static_cast<float>(i)), y[i]);
             }
-            if (mod.bias != nullptr) {
+            if (MODE == AS_BIAS || mod.bias != nullptr) {
               if (key32 + 31 - pos_first <= -mod.radius || key32 - pos_last >= mod.radius) {  // beyond the table for all rows
                 const float b = tab[key32 < pos_last ? -mod.radius : mod.radius] * tab_unit;
 #pragma unroll
@@ -1040,9 +1042,14 @@ attn_scored_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_cons
             for (int i = 0; i < 16; ++i) e2[i] = make_float2(y[2 * i], y[2 * i + 1]);
           };
           // Most steps: every row sees all 64 keys, the reference stands, nothing is asked of a score one by one. What does not fit
-          // (a sum out of range, a score beyond the cap, a wait that gave up) is taken again below, from the same scores.
+          // (a sum out of range, a score beyond the cap, a wait that gave up) is taken again below, from the same scores. Steps within a bias
+          // table's reach, documents and modifications together are left to the code below altogether: here they cost more in instructions
+          // fetched than they save (documents with a table, 4 sequences of 2500 to 4096, 12 heads of 32: 171 us and 142; beyond the table
+          // it pays: 8 of 2048, 28/4 heads of 128, radius 128: 1009 us without and 725).
           bool done = false;
-          if (whole && (MODE != AS_SLOPES || (!first && (kv0 + KV <= pos_first || kv0 > pos_last)))) {
+          const bool left_of = kv0 + KV - 1 - pos_first <= -mod.radius, right_of = kv0 - pos_last >= mod.radius;  // AS_BIAS: beyond the table
+          if (!DOCS && whole && (MODE != AS_SLOPES || (!first && (kv0 + KV <= pos_first || kv0 > pos_last))) &&
+              (MODE != AS_BIAS || left_of || right_of)) {
             uint32_t z[2][32];
             tmem_ld_32x32b_x32(s_at, z[0]);
             tmem_ld_32x32b_x32(s_at + 32, z[1]);
@@ -1051,8 +1058,10 @@ attn_scored_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_cons
             float2 e2[2][16];
             auto two = [&](int g2, int i) { return make_float2(__uint_as_float(z[g2][2 * i]), __uint_as_float(z[g2][2 * i + 1])); };
             bool odd = failed;
-            if (MODE == AS_PLAIN) {
-              const float2 base2 = make_float2(-ref, -ref);
+            if (MODE == AS_PLAIN || MODE == AS_BIAS) {
+              float base = -ref;
+              if (MODE == AS_BIAS) base = fmaf(tab[left_of ? -mod.radius : mod.radius], tab_unit, base);
+              const float2 base2 = make_float2(base, base);
 #pragma unroll
               for (int i = 0; i < 32; ++i) e2[i >> 4][i & 15] = __ffma2_rn(two(i >> 4, i & 15), scale2, base2);
             } else if (MODE == AS_SLOPES) {
@@ -1064,9 +1073,6 @@ attn_scored_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_cons
                 e2[i >> 4][i & 15] = __ffma2_rn(two(i >> 4, i & 15), scale2, bias2);
                 bias2 = __fadd2_rn(bias2, rise2);
               }
-            } else if (MODE == AS_ANY) {
-              any_scores(z[0], kv0, e2[0]);
-              any_scores(z[1], kv0 + 32, e2[1]);
             } else {
               float top = 0.f;
 #pragma unroll
@@ -1078,7 +1084,7 @@ attn_scored_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_cons
                 e2[i >> 4][i & 15] = tanh_near(v, __fmul2_rn(v, v));
               }
             }
-            if (MODE != AS_CAP && MODE != AS_SLOPES && first) {  // the reference, from these scores (nothing is summed yet)
+            if ((MODE == AS_PLAIN || MODE == AS_BIAS) && first) {  // the reference, from these scores (nothing is summed yet)
               float m0 = -INFINITY, m1 = -INFINITY;
 #pragma unroll
               for (int i = 0; i < 16; ++i) {
@@ -1507,6 +1513,9 @@ static int as_init_modes() {
   int rc = as_init_one<D, PAGED, AS_PLAIN>();
   if (!rc) rc = as_init_one<D, PAGED, AS_SLOPES>();
   if (!rc) rc = as_init_one<D, PAGED, AS_CAP>();
+  if (!rc) rc = as_init_one<D, PAGED, AS_BIAS>();
+  if constexpr (!PAGED)
+    if (!rc) rc = as_init_one<D, PAGED, AS_DOCS>();
   if (!rc) rc = as_init_one<D, PAGED, AS_ANY>();
   return rc;
 }
@@ -1540,9 +1549,14 @@ static int as_map_pages(CUtensorMap* m, const void* base, const b200emb_kv_cache
 
 template <int D, bool PAGED>
 static int as_launch_mode(const AsMaps& m, const AttnJob& j, const AttnMod& mod, const AttnPlan& plan, int sms, cudaStream_t s) {
-  if (mod.docs != nullptr) return as_launch<D, PAGED, AS_ANY>(m, j, mod, plan, sms, s);
-  if (mod.cap == 0.f && mod.slopes == nullptr && mod.bias == nullptr) return as_launch<D, PAGED, AS_PLAIN>(m, j, mod, plan, sms, s);
-  if (mod.cap == 0.f && mod.slopes != nullptr) return as_launch<D, PAGED, AS_SLOPES>(m, j, mod, plan, sms, s);
+  if constexpr (!PAGED)
+    if (mod.docs != nullptr)
+      return mod.cap == 0.f && mod.slopes == nullptr ? as_launch<D, PAGED, AS_DOCS>(m, j, mod, plan, sms, s)
+                                                     : as_launch<D, PAGED, AS_ANY>(m, j, mod, plan, sms, s);
+  if (mod.cap == 0.f) {
+    if (mod.slopes != nullptr) return as_launch<D, PAGED, AS_SLOPES>(m, j, mod, plan, sms, s);
+    return mod.bias != nullptr ? as_launch<D, PAGED, AS_BIAS>(m, j, mod, plan, sms, s) : as_launch<D, PAGED, AS_PLAIN>(m, j, mod, plan, sms, s);
+  }
   const float cap = mod.cap * AS_LOG2E;
   if (cap >= AS_CAP_LOW && cap <= AS_CAP_HIGH && mod.slopes == nullptr && mod.bias == nullptr)
     return as_launch<D, PAGED, AS_CAP>(m, j, mod, plan, sms, s);
