@@ -25,8 +25,9 @@
 //   O += P V      P rounded to bf16 (the tensor core's operand type; half a step of 2^-8 per probability) in tensor memory, V as an MN-major
 //                 shared-memory operand
 // What bounds it: a softmax warp's chain of dependent instructions, two such warps on each scheduler; the special-function unit is
-// busy 42 % of the time, the tensor cores less. 8 sequences of 2048 tokens, 28/4 heads of 128: 536 us (898 TFLOP/s; 546 with slopes, 629
-// capped, 343 causal); 16 heads of 64: 279 us (493 TFLOP/s; 286, 342, 187). One new token of 64 sequences over 64 to 8192 keys, 28/4
+// busy 42 to 47 % of the time, the tensor cores as much. 8 sequences of 2048 tokens, 28/4 heads of 128: 530 us (907 TFLOP/s; 543 with
+// slopes, 623 capped, 340 causal, 673 with a bias table of radius 128); 16 heads of 64: 265 us (519 TFLOP/s; 286 with slopes, 339 capped,
+// 180 causal). One new token of 64 sequences over 64 to 8192 keys, 28/4
 // heads of 128: 67 us, 3.5 TB/s, 6 of them the plan.
 // Warps: 0-3 softmax A, 4-7 softmax B, 8 loads Q and K, 9 loads V, 10 and 11 issue the matrix instructions of A and B.
 #include <cuda.h>
@@ -624,6 +625,9 @@ attn_scored_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_cons
   using Cfg = AsCfg<D>;
   constexpr int RING = Cfg::RING, KV = Cfg::KV;
   constexpr uint32_t Q_BUFS = Cfg::Q_BUFS;
+  // Whether a segment's first step may go the straight way (8 sequences of 2048, plain: 16 heads of 64, 280 us so and 266 not; 28/4 heads
+  // of 128, causal, 343 and 354).
+  constexpr bool FIRST = MODE == AS_CAP || MODE == AS_BIAS || (MODE == AS_PLAIN && D == 128);
   constexpr bool DOCS = MODE == AS_DOCS || MODE == AS_ANY, TABLES = DOCS || MODE == AS_BIAS;
   // A stream's own tiles in flight, so that neither stream waits for the other's.
   constexpr uint32_t SLOTS = RING / 2;
@@ -1048,7 +1052,7 @@ attn_scored_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_cons
           // it pays: 8 of 2048, 28/4 heads of 128, radius 128: 1009 us without and 725).
           bool done = false;
           const bool left_of = kv0 + KV - 1 - pos_first <= -mod.radius, right_of = kv0 - pos_last >= mod.radius;  // AS_BIAS: beyond the table
-          if (!DOCS && whole && (MODE != AS_SLOPES || (!first && (kv0 + KV <= pos_first || kv0 > pos_last))) &&
+          if (!DOCS && whole && (FIRST || !first) && (MODE != AS_SLOPES || kv0 + KV <= pos_first || kv0 > pos_last) &&
               (MODE != AS_BIAS || left_of || right_of)) {
             uint32_t z[2][32];
             tmem_ld_32x32b_x32(s_at, z[0]);
@@ -1084,7 +1088,7 @@ attn_scored_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_cons
                 e2[i >> 4][i & 15] = tanh_near(v, __fmul2_rn(v, v));
               }
             }
-            if ((MODE == AS_PLAIN || MODE == AS_BIAS) && first) {  // the reference, from these scores (nothing is summed yet)
+            if (FIRST && MODE != AS_CAP && first) {  // the reference, from these scores (nothing is summed yet)
               float m0 = -INFINITY, m1 = -INFINITY;
 #pragma unroll
               for (int i = 0; i < 16; ++i) {
@@ -1151,23 +1155,12 @@ attn_scored_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_cons
                   e2[i] = __ffma2_rn(two(i), scale2, make_float2(fmaf(-slope, fabsf(f + static_cast<float>(2 * i)), -ref),
                                                                  fmaf(-slope, fabsf(f + static_cast<float>(2 * i + 1)), -ref)));
               } else if (MODE == AS_CAP) {
-                // Which way the tanh goes is decided by what is seen alone: columns that no key wrote and rows of no token hold whatever was
-                // there before, and results must not depend on it.
-                float top = 0.f;
+                // good for every score; the polynomial beside it for those within the cap costs more to fetch than it saves (8 sequences of 600
+                // to 2048, 28/4 heads of 128, causal, window 1023: 209 us, 221 with both)
 #pragma unroll
-                for (int i = 0; i < 32; ++i) top = fmaxf(top, (seen >> i) & 1u ? fabsf(__uint_as_float(z[i])) : 0.f);
-                if ((__ballot_sync(0xffffffffu, top > cap_far) & real_rows) == 0u) {
-#pragma unroll
-                  for (int i = 0; i < 16; ++i) {
-                    const float2 v = __fmul2_rn(two(i), scale2);
-                    e2[i] = tanh_near(v, __fmul2_rn(v, v));
-                  }
-                } else {
-#pragma unroll
-                  for (int i = 0; i < 16; ++i) {
-                    const float2 v = two(i);
-                    e2[i] = make_float2(cap_out * as_tanh(v.x * cap_in), cap_out * as_tanh(v.y * cap_in));
-                  }
+                for (int i = 0; i < 16; ++i) {
+                  const float2 v = two(i);
+                  e2[i] = make_float2(cap_out * as_tanh(v.x * cap_in), cap_out * as_tanh(v.y * cap_in));
                 }
               } else {
                 any_scores(z, key32, e2);
