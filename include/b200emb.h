@@ -371,7 +371,7 @@ int b200emb_op_pool(const void* x, const int32_t* d_cu_seqlens, int32_t n_seqs, 
  * captured graph follows their values; nothing in them can move an access out of its buffer: sequences are
  * cut to [0, n_tokens), a page index outside [0, n_pages) reads as zeros and is never written. Rows from
  * cu_seqlens[n_seqs] on are left as they were. Empty sequences are allowed. n_tokens == 0 or n_seqs == 0: nothing
- * is done. None has a counterpart function in the reference: its models reach such attention through
+ * is done (the attention calls clear the status that b200emb_op_workspace_status reads). None has a counterpart function in the reference: its models reach such attention through
  * third-party torch code behind sentence_transformer.py:124. */
 
 /* b200emb_rope_desc.layout */
@@ -466,7 +466,8 @@ int64_t b200emb_attention_workspace_bytes(int32_t n_seqs, int32_t n_tokens, int3
                                           int32_t head_dim);
 
 /* Waits for the stream and reports whether a bounded device-side wait of the last attention call on this workspace gave up
- * (B200EMB_ERR_DEVICE_WAIT; its output is then not valid). The calls themselves do not wait and so cannot report it. */
+ * (B200EMB_ERR_DEVICE_WAIT; its output is then not valid). The calls themselves do not wait and so cannot report it. Before the first
+ * call on a workspace there is nothing to report, and what is returned says nothing. */
 int b200emb_op_workspace_status(const void* workspace, void* stream);
 
 /* Packed variable-length attention: q [n_tokens, n_heads * head_dim], k and v [n_tokens, n_kv_heads * head_dim], out

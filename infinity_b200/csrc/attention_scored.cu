@@ -1435,6 +1435,20 @@ static int check_workspace(const void* ws, int64_t have, int64_t want, const cha
   return B200EMB_OK;
 }
 
+// A call without rows launches nothing: it clears what an earlier call, or whatever used the memory before, left in the status word at
+// the start of the workspace. A workspace that is not device memory is left alone, as such a call leaves all its pointers.
+static int as_clear_status(void* workspace, int64_t bytes, cudaStream_t s) {
+  if (workspace == nullptr || bytes < static_cast<int64_t>(sizeof(int32_t))) return B200EMB_OK;
+  cudaPointerAttributes a;
+  if (cudaPointerGetAttributes(&a, workspace) != cudaSuccess) {
+    cudaGetLastError();  // not a pointer of this process's devices, or no device at all: nobody's error
+    return B200EMB_OK;
+  }
+  if (a.type != cudaMemoryTypeDevice && a.type != cudaMemoryTypeManaged) return B200EMB_OK;
+  B2_CUDA_CHECK(cudaMemsetAsync(workspace, 0, sizeof(int32_t), s));
+  return B200EMB_OK;
+}
+
 static int as_tile_tokens(int n_heads, int n_kv_heads) { return 128 / (n_heads / n_kv_heads); }
 
 // Carves the workspace (null: only measures it); returns its size.
@@ -1596,7 +1610,7 @@ extern "C" int b200emb_op_attention_scored(const void* q, int64_t q_row_stride, 
   AttnMod mod;
   if (!rc) rc = make_mod(opts, head_dim, false, who, &mod);
   if (rc) return rc;
-  if (n_tokens == 0 || n_seqs == 0) return B200EMB_OK;
+  if (n_tokens == 0 || n_seqs == 0) return as_clear_status(workspace, workspace_bytes, reinterpret_cast<cudaStream_t>(stream));
   const int64_t wq = static_cast<int64_t>(n_heads) * head_dim, wk = static_cast<int64_t>(n_kv_heads) * head_dim;
   rc = check_rows(q, q_row_stride, wq, "q", who);
   if (!rc) rc = check_rows(k, k_row_stride, wk, "k", who);
@@ -1642,7 +1656,7 @@ extern "C" int b200emb_op_attention_paged(const void* q, int64_t q_row_stride, v
   if (cache->page_stride % 8 != 0 || cache->token_stride % 8 != 0 || cache->head_stride % 8 != 0 ||
       reinterpret_cast<uintptr_t>(cache->k) % 16 != 0 || reinterpret_cast<uintptr_t>(cache->v) % 16 != 0)
     return set_error(B200EMB_ERR_INVALID, "%s: the cache must be 16-byte aligned with strides that are multiples of 8", who);
-  if (n_tokens == 0 || n_seqs == 0) return B200EMB_OK;
+  if (n_tokens == 0 || n_seqs == 0) return as_clear_status(workspace, workspace_bytes, reinterpret_cast<cudaStream_t>(stream));
   const int64_t wq = static_cast<int64_t>(n_heads) * cache->head_dim;
   rc = check_rows(q, q_row_stride, wq, "q", who);
   if (!rc) rc = check_rows(out, out_row_stride, wq, "out", who);

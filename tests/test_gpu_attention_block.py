@@ -590,3 +590,37 @@ def test_nothing_to_do(lib):
     pages = R.Pages([20], 1, 64, 16).fill(1)
     R.paged(lib, q, R.cu_of([0]), R.ints([20]), 1, pages, None, out=out)
     assert (out == 3.0).all()
+
+
+@pytest.mark.parametrize("n_seqs,n_tokens", [(1, 0), (0, 4), (0, 0)])
+@pytest.mark.parametrize("left", [0xFF, 7], ids=["fresh", "of an older call"])
+@pytest.mark.parametrize("captured", [False, True])
+def test_status_after_a_call_without_rows(lib, n_seqs, n_tokens, left, captured):
+    """Neither what a fresh workspace holds nor what an older call left is reported for a call that had nothing to do."""
+    x = R.normal(1, 4, 3 * 64)
+    q, k, v = _split(x, 1, 1, 64)
+    cu, kv, out, pages = R.cu_of([4]), R.ints([20]), torch.full((4, 64), 3.0, dtype=R.BF16, device="cuda"), R.Pages([20], 1, 64, 16).fill(1)
+    desc = pages.desc()
+
+    def calls(ws, stream):
+        return (lambda: lib.b200emb_op_attention_scored(q.data_ptr(), 192, k.data_ptr(), 192, v.data_ptr(), 192, out.data_ptr(), 64, cu.data_ptr(), n_seqs,
+                                                        n_tokens, 1, 1, 64, None, ws.data_ptr(), ws.numel(), stream),
+                lambda: lib.b200emb_op_attention_paged(q.data_ptr(), 192, out.data_ptr(), 64, cu.data_ptr(), kv.data_ptr(), n_seqs, n_tokens, 1,
+                                                       C.byref(desc), None, ws.data_ptr(), ws.numel(), stream))
+
+    for which in range(2):
+        ws = R.workspace(lib, 1, 4, 1, 1, 64)
+        ws[:4] = torch.tensor([left, 0, 0, 0] if left == 7 else [left] * 4, dtype=torch.uint8)
+        before = ws.clone()
+        if captured:
+            graph = torch.cuda.CUDAGraph()
+            torch.cuda.synchronize()
+            with torch.cuda.graph(graph):
+                _lib.check(calls(ws, R.stream())[which]())
+            assert torch.equal(ws, before)  # in the graph, not before it
+            graph.replay()
+            torch.cuda.synchronize()
+        else:
+            _lib.check(calls(ws, R.stream())[which]())
+        _lib.check(lib.b200emb_op_workspace_status(ws.data_ptr(), R.stream()))
+        assert torch.equal(ws[4:], before[4:]) and (out == 3.0).all()
