@@ -442,7 +442,8 @@ int b200emb_op_kv_append(const void* qkv, int64_t qkv_row_stride, const int32_t*
  *   bias: s += bias[h * (2 R + 1) + clamp(j - i, -R, R) + R], R = bias_radius
  * Key j is visible to query i when (j <= i + window_right and j >= i - window_left) or j < prefix_lens[s], and with
  * doc_ids only when doc_ids of both tokens are equal and not negative. A row that sees no key is zero, and so is one whose visible
- * scores are all -inf; a bias below -1e38 counts as -inf.
+ * scores are all -inf; a bias below -2.4e38 counts as -inf (the lowest values of fp32 and bf16 do). Any other is a number: fp32 sums
+ * with it round the digits of the scores away as it grows.
  * Masked scores are selected away, so keys may hold anything there; a VALUE that is not finite reaches every row of its own
  * sequence whose tiles cover it (0 * inf), never another sequence, and slots past the sequence's end never count. */
 typedef struct b200emb_attn_opts {

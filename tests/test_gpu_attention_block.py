@@ -340,6 +340,27 @@ def test_scored_bias_of_minus_infinity_and_the_lowest_value(lib):
         assert torch.isfinite(out).all()
 
 
+@pytest.mark.parametrize("low", [-math.inf, torch.finfo(torch.float32).min, torch.finfo(torch.bfloat16).min, -2.41e38])
+@pytest.mark.parametrize("lens,heads,kv_heads,radius", [([140], 2, 2, 70), ([1100], 4, 1, 150), ([1100], 2, 2, 600)],
+                         ids=["staged", "beyond a table read in place", "in a table read in place"])
+@pytest.mark.parametrize("docs", [False, True])
+def test_scored_bias_below_the_limit_is_minus_infinity(lib, lens, heads, kv_heads, radius, low, docs):
+    """Rows whose visible biases are all below -2.4e38 are zero, and no key with such a bias counts elsewhere: head 0 sees no key ahead of -10, head 1
+    none from radius on. Tables of up to 1024 entries of a key head are staged, larger ones are read where they lie."""
+    n, dim = lens[0], 64
+    x = R.normal(5, n, (heads + 2 * kv_heads) * dim)
+    q, k, v = _split(x, heads, kv_heads, dim)
+    bias = _bias(heads, radius)
+    bias[0, radius - 10:] = low
+    bias[1, 2 * radius:] = low
+    ids = torch.zeros(n, dtype=torch.int32, device="cuda") if docs else None
+    out = R.scored(lib, q, k, v, R.cu_of(lens), heads, kv_heads, R.options(bias=bias, docs=ids)).view(n, heads, dim)
+    bias[bias < -2.4e38] = -math.inf
+    want, size = R.attend(q.reshape(n, heads, dim), k.reshape(n, kv_heads, dim), v.reshape(n, kv_heads, dim), 0, bias=bias)
+    assert (want[:11, 0] == 0).all() and (out[:11, 0] == 0).all()
+    R.assert_attended(out, want, size)
+
+
 def test_scored_large_scores(lib):
     """Scores that differ by thousands between keys, growing and falling along the row."""
     lens, heads, dim = [400], 2, 64
