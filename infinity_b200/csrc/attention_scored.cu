@@ -135,12 +135,6 @@ __device__ __forceinline__ float as_max3_abs(float a, float b, float c) {  // ma
 }
 // 1 - 2 / (1 + e^2x), off by about 2^-22 of one
 __device__ __forceinline__ float as_tanh(float x) { return fmaf(-2.f, as_rcp(1.f + as_ex2(x * (2.f * AS_LOG2E))), 1.f); }
-// The same with small values taken from the series x - x^3/3 + 2x^5/15 (next term below 2^-24 of x up to 0.1): a large cap
-// multiplies the error, and nearly all of its scores are small here.
-__device__ __forceinline__ float as_tanh_any(float x) {
-  const float u = x * x;
-  return fabsf(x) < 0.1f ? fmaf(x * u, fmaf(u, 2.f / 15.f, -1.f / 3.f), x) : as_tanh(x);
-}
 // 32-bit mask of the x lowest bits, x clamped to 0 .. 32
 __device__ __forceinline__ uint32_t as_below(int x) {
   uint32_t m;
@@ -1022,9 +1016,13 @@ attn_scored_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_cons
             float y[32];
 #pragma unroll
             for (int i = 0; i < 32; ++i) y[i] = __uint_as_float(z[i]);
-            if (MODE == AS_ANY && mod.cap > 0.f) {
+            if (MODE == AS_ANY && cap_out > AS_CAP_HIGH) {
+              // the cap multiplies the error: 2^-22 of one is 2^-16 of a score's unit at a cap of 55, and 0.24 of it at 1e6
 #pragma unroll
-              for (int i = 0; i < 32; ++i) y[i] = fmaf(cap_out, as_tanh_any(y[i] * cap_in), -ref);
+              for (int i = 0; i < 32; ++i) y[i] = fmaf(cap_out, tanhf(y[i] * cap_in), -ref);
+            } else if (MODE == AS_ANY && mod.cap > 0.f) {
+#pragma unroll
+              for (int i = 0; i < 32; ++i) y[i] = fmaf(cap_out, as_tanh(y[i] * cap_in), -ref);
             } else {
 #pragma unroll
               for (int i = 0; i < 32; ++i) y[i] = fmaf(y[i], scale_log2, -ref);

@@ -254,6 +254,35 @@ def test_scored_caps_and_scales_of_any_size(lib, mod, dim):
     _check_scored(out, q, k, v, lens, heads, kv_heads, dim, mod, slopes, bias, prefix, docs)
 
 
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("cap", [56.0, 1e3, 1e5, 1e6])
+def test_scored_large_caps_at_scores_of_their_size(lib, cap, dim):
+    """Scores of a hundredth of the cap up to all of it, keys a few units apart, and values that show each key's weight. The products are exact
+    (small whole numbers), so what is left is the arithmetic of cap * tanh(s / cap) in fp32: two roundings of the argument, one unit in the last
+    place of tanh, two roundings of cap * log2(e), one of the sum with the reference, 7 * 2^-24 of the score altogether."""
+    n, far = 48, [0.01, 0.05, 0.0999, 0.1001, 0.102, 0.11, 0.13, 0.16, 0.2, 0.25, 0.3, 0.35, 0.4, 0.45, 0.5, 0.6, 0.8, 1.0]
+    rows = len(far) * 16
+    g = torch.Generator().manual_seed(7)
+    want_at = torch.tensor(far).repeat_interleave(16) * cap
+    q, k = torch.zeros(rows, dim), torch.zeros(rows, dim)
+    # s = 128 q0 + q1 + k1: q0 and q1 of the row, k1 of the key
+    q[:, 0] = (want_at / 128).floor().clamp(max=255) if cap < 3e4 else (want_at / 128).to(R.BF16).float()
+    q[:, 1], q[:, 2] = torch.randint(0, 128, (rows,), generator=g).float() * (cap > 500), 1.0
+    k[:, 0], k[:, 1], k[:, 2] = 128.0, 1.0, torch.randint(-3, 4, (rows,), generator=g).float()
+    v = torch.eye(dim)[torch.arange(rows) % n]
+    q, k, v = (z.to(R.BF16).cuda() for z in (q, k, v))
+    # blocks of one document: every query sees the n keys of its own block
+    docs = (torch.arange(rows) // n).to(torch.int32).cuda()
+    out = R.scored(lib, q, k, v, R.cu_of([rows]), 1, 1, R.options(scale=1.0, cap=cap, docs=docs)).double()
+    want, size = R.attend(*(z.view(rows, 1, dim) for z in (q, k, v)), 0, scale=1.0, cap=cap, q_docs=docs, k_docs=docs)
+    s = (q.double() @ k.double().T).abs()
+    top = (cap * torch.tanh(torch.where(docs[:, None] == docs[None], s, 0.0) / cap)).amax(1)
+    off = torch.expm1(2 * 7 * 2.0 ** -24 * top)[:, None]  # of a weight: its own exponent, and those of the sum
+    tol = size.view(rows, dim) * (R.HALF_STEP * (1 + off) + off) + want.view(rows, dim) * R.HALF_STEP * (1 + off)
+    bad = ((out - want.view(rows, dim)).abs() - tol).amax(1)
+    assert torch.isfinite(out).all() and (bad <= 0).all(), [(f, round(b, 4)) for f, b in zip(far, bad.view(-1, 16).amax(1).tolist())]
+
+
 def test_scored_slopes_that_grow_with_the_distance(lib):
     lens, heads, dim = [1100, 70], 2, 64
     x = R.normal(3, sum(lens), 3 * heads * dim)
