@@ -444,6 +444,9 @@ int b200emb_op_kv_append(const void* qkv, int64_t qkv_row_stride, const int32_t*
  * doc_ids only when doc_ids of both tokens are equal and not negative. A row that sees no key is zero, and so is one whose visible
  * scores are all -inf; a bias below -2.4e38 counts as -inf (the lowest values of fp32 and bf16 do). Any other is a number: fp32 sums
  * with it round the digits of the scores away as it grows.
+ * The weighted sums of the values are kept in fp32 times up to 2^48, and times e^+-cap under a cap of up to 55: with such a cap, values between
+ * 2^-40 and 2^17 in magnitude come out right whatever the scores, without one those between 2^-60 and 2^79. Beyond that a row whose scores
+ * ask for it may be infinite, or zero, although its result is a number.
  * Masked scores are selected away, so keys may hold anything there; a VALUE that is not finite reaches every row of its own
  * sequence whose tiles cover it (0 * inf), never another sequence, and slots past the sequence's end never count. */
 typedef struct b200emb_attn_opts {

@@ -19,9 +19,9 @@
 //   S = Q K^T     tcgen05.mma 128 x N x 16 (N = valid keys rounded up to 16), fp32 in tensor memory
 //   softmax       128 threads, one row each, in one pass over the row: a score becomes its exponential against the row's reference
 //                 at once. The reference is a guess (from the first 32 scores of the row's first step) and is only replaced, by the
-//                 exact maximum and a second pass, when the sum leaves 2^-60 .. 2^80: numerators and denominator share its
-//                 scale, and fp32 sums and bf16 probabilities keep their relative precision anywhere in between. Capped scores
-//                 lie within +-cap and need no reference at all.
+//                 exact maximum and a second pass, when the sum leaves 2^-60 .. 2^48: numerators and denominator share its
+//                 scale, and fp32 sums and bf16 probabilities keep their relative precision anywhere in between; the numerators of values
+//                 up to 2^79 stay finite. Capped scores lie within +-cap and need no reference at all (caps up to 55: 2^+-80).
 //   O += P V      P rounded to bf16 (the tensor core's operand type; half a step of 2^-8 per probability) in tensor memory, V as an MN-major
 //                 shared-memory operand
 // What bounds it: a softmax warp's chain of dependent instructions, two such warps on each scheduler; the special-function unit is
@@ -64,7 +64,7 @@ static constexpr int AS_COLD = 12;                 // words of a softmax warp's 
 static constexpr int AS_PACKED_BOX = 32;           // rows of one copy of a packed key tile: short sequences copy few rows
 static constexpr int AS_TABLE = 1024;              // floats of a stream's staged bias tables
 static constexpr float AS_LOG2E = 1.4426950408889634f;
-static constexpr float AS_SUM_LOW = 0x1p-60f, AS_SUM_HIGH = 0x1p80f;  // sums that keep the reference, see above
+static constexpr float AS_SUM_LOW = 0x1p-60f, AS_SUM_HIGH = 0x1p48f;  // sums that keep the reference, see above
 static constexpr float AS_CAP_LOW = 0x1p-7f, AS_CAP_HIGH = 80.f;      // cap * log2(e) that AS_CAP serves: 2^+-80 keeps fp32 sums in range
 
 struct AttnMod {

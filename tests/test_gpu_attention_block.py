@@ -390,6 +390,45 @@ def test_scored_bias_below_the_limit_is_minus_infinity(lib, lens, heads, kv_head
     R.assert_attended(out, want, size)
 
 
+@pytest.mark.parametrize("power", [79, -60])
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("mod", [{}, dict(causal=1), dict(slopes=True), dict(bias=9), dict(cap=200.0), dict(docs=True)], ids=str)
+def test_scored_values_of_any_magnitude(lib, mod, dim, power):
+    """Values as large, and as small, as the header allows without a cap up to 55, with scores that rise by 50 along the row after its first keys, and
+    that fall by as much before them: sums that follow a first reference would pass fp32's range."""
+    lens, heads, kv_heads = [300], 4, 2
+    x, mod, slopes, bias, prefix, docs = _scored_case(lens, heads, kv_heads, dim, mod)
+    q, k, v = _split(x, heads, kv_heads, dim)
+    x[:, :(heads + kv_heads) * dim] *= 0.05
+    q[:, ::dim], k[:, ::dim] = dim ** 0.5, 0.0
+    k[100:200, ::dim], k[200:, ::dim] = 25.0, 50.0
+    if power < 0:
+        k[:100, ::dim] = 50.0  # the first reference is far above all that follows in the rows that do not see these keys
+    v[:] = (R.normal(3, 300, kv_heads * dim).float().clamp(-1, 1) * 2.0 ** power).to(R.BF16)
+    docs = torch.arange(300, dtype=torch.int32, device="cuda") // 250 if docs is not None else None
+    out = R.scored(lib, q, k, v, R.cu_of(lens), heads, kv_heads, R.options(slopes=slopes, bias=bias, docs=docs, **mod))
+    scale = 2.0 ** -power  # exact: compared at the values' own scale
+    _check_scored(out.double() * scale, q, k, v.double() * scale, lens, heads, kv_heads, dim, mod, slopes, bias, prefix, docs)
+
+
+@pytest.mark.parametrize("power", [17, -40])
+@pytest.mark.parametrize("sign", [1.0, -1.0])
+@pytest.mark.parametrize("dim", [64, 128])
+def test_scored_values_of_any_magnitude_under_a_cap(lib, dim, sign, power):
+    """The largest and smallest values that the header allows under a cap, where all scores lie at one end of it, and at both."""
+    lens, heads = [500, 70], 2
+    for mixed in (False, True):
+        x, mod, slopes, bias, prefix, docs = _scored_case(lens, heads, heads, dim, dict(cap=55.0))
+        q, k, v = _split(x, heads, heads, dim)
+        q[:, ::dim], k[:, ::dim] = 8.0 * dim ** 0.5, sign * 100.0
+        if mixed:
+            k[::7, ::dim] = -sign * 100.0
+        v[:] = (R.normal(3, sum(lens), heads * dim).float().clamp(-1, 1) * 2.0 ** power).to(R.BF16)
+        out = R.scored(lib, q, k, v, R.cu_of(lens), heads, heads, R.options(**mod))
+        scale = 2.0 ** -power
+        _check_scored(out.double() * scale, q, k, v.double() * scale, lens, heads, heads, dim, mod, slopes, bias, prefix, docs)
+
+
 def test_scored_large_scores(lib):
     """Scores that differ by thousands between keys, growing and falling along the row."""
     lens, heads, dim = [400], 2, 64
