@@ -38,6 +38,8 @@
 #include <math.h>
 #include <stdint.h>
 
+#include <atomic>
+
 #include "kernels.h"
 // waits here are short and on the chain softmax -> MMA -> softmax: plain polling, as in attention_tc2.cu
 #define B2_MBAR_SUSPEND_NS 0
@@ -1480,20 +1482,31 @@ static int64_t as_layout(void* workspace, int n_seqs, int n_tokens, int n_heads,
   return at;
 }
 
-static int as_sm_count(int* out) {
-  int dev = 0;
-  B2_CUDA_CHECK(cudaGetDevice(&dev));
-  B2_CUDA_CHECK(cudaDeviceGetAttribute(out, cudaDevAttrMultiProcessorCount, dev));
-  return B200EMB_OK;
-}
-
 struct AsMaps {
   CUtensorMap q, k, v;
 };
 
+struct AsDevice {
+  int id, sms;
+};
+
+// Opt-in shared memory of one kernel, at its first launch on a device: setting it loads the kernel, and who never launches one of the 22 is
+// not to wait for it (all of them at the library's first call: see kernels_init_device, which leaves them out).
 template <int D, bool PAGED, int MODE>
-static int as_launch(const AsMaps& m, const AttnJob& j, const AttnMod& mod, const AttnPlan& plan, int sms, cudaStream_t s) {
-  int64_t grid = sms < AS_MAX_CTAS ? sms : AS_MAX_CTAS;
+static int as_init_kernel(int device) {
+  static std::atomic<uint64_t> ready{0};
+  const uint64_t bit = device >= 0 && device < 64 ? uint64_t(1) << device : 0;
+  if (ready.load(std::memory_order_acquire) & bit) return B200EMB_OK;
+  B2_CUDA_CHECK(cudaFuncSetAttribute(attn_scored_kernel<D, PAGED, MODE>, cudaFuncAttributeMaxDynamicSharedMemorySize, AsCfg<D>::SMEM_BYTES));
+  ready.fetch_or(bit, std::memory_order_release);
+  return B200EMB_OK;
+}
+
+template <int D, bool PAGED, int MODE>
+static int as_launch(const AsMaps& m, const AttnJob& j, const AttnMod& mod, const AttnPlan& plan, const AsDevice& dev, cudaStream_t s) {
+  const int rc = as_init_kernel<D, PAGED, MODE>(dev.id);
+  if (rc) return rc;
+  int64_t grid = dev.sms < AS_MAX_CTAS ? dev.sms : AS_MAX_CTAS;
   if (!PAGED) {  // no more CTAs than steps there can be
     const int64_t steps = static_cast<int64_t>(plan.max_entries) * j.n_kv_heads * ((j.n_tokens + AsCfg<D>::KV - 1) / AsCfg<D>::KV);
     if (steps < grid) grid = steps;
@@ -1507,32 +1520,6 @@ static int as_launch(const AsMaps& m, const AttnJob& j, const AttnMod& mod, cons
                    m.v, j, mod, plan);
   if (e != cudaSuccess) return set_error(B200EMB_ERR_CUDA, "attention launch: %s", cudaGetErrorString(e));
   return B200EMB_OK;
-}
-
-template <int D, bool PAGED, int MODE>
-static int as_init_one() {
-  B2_CUDA_CHECK(cudaFuncSetAttribute(attn_scored_kernel<D, PAGED, MODE>, cudaFuncAttributeMaxDynamicSharedMemorySize, AsCfg<D>::SMEM_BYTES));
-  return B200EMB_OK;
-}
-
-template <int D, bool PAGED>
-static int as_init_modes() {
-  int rc = as_init_one<D, PAGED, AS_PLAIN>();
-  if (!rc) rc = as_init_one<D, PAGED, AS_SLOPES>();
-  if (!rc) rc = as_init_one<D, PAGED, AS_CAP>();
-  if (!rc) rc = as_init_one<D, PAGED, AS_BIAS>();
-  if constexpr (!PAGED)
-    if (!rc) rc = as_init_one<D, PAGED, AS_DOCS>();
-  if (!rc) rc = as_init_one<D, PAGED, AS_ANY>();
-  return rc;
-}
-
-int attention_scored_init_device() {
-  int rc = as_init_modes<64, false>();
-  if (!rc) rc = as_init_modes<64, true>();
-  if (!rc) rc = as_init_modes<128, false>();
-  if (!rc) rc = as_init_modes<128, true>();
-  return rc;
 }
 
 // rows of n heads: [tokens, heads, head_dim] with a row stride
@@ -1555,30 +1542,29 @@ static int as_map_pages(CUtensorMap* m, const void* base, const b200emb_kv_cache
 }
 
 template <int D, bool PAGED>
-static int as_launch_mode(const AsMaps& m, const AttnJob& j, const AttnMod& mod, const AttnPlan& plan, int sms, cudaStream_t s) {
+static int as_launch_mode(const AsMaps& m, const AttnJob& j, const AttnMod& mod, const AttnPlan& plan, const AsDevice& dev, cudaStream_t s) {
   if constexpr (!PAGED)
     if (mod.docs != nullptr)
-      return mod.cap == 0.f && mod.slopes == nullptr ? as_launch<D, PAGED, AS_DOCS>(m, j, mod, plan, sms, s)
-                                                     : as_launch<D, PAGED, AS_ANY>(m, j, mod, plan, sms, s);
+      return mod.cap == 0.f && mod.slopes == nullptr ? as_launch<D, PAGED, AS_DOCS>(m, j, mod, plan, dev, s)
+                                                     : as_launch<D, PAGED, AS_ANY>(m, j, mod, plan, dev, s);
   if (mod.cap == 0.f) {
-    if (mod.slopes != nullptr) return as_launch<D, PAGED, AS_SLOPES>(m, j, mod, plan, sms, s);
-    return mod.bias != nullptr ? as_launch<D, PAGED, AS_BIAS>(m, j, mod, plan, sms, s) : as_launch<D, PAGED, AS_PLAIN>(m, j, mod, plan, sms, s);
+    if (mod.slopes != nullptr) return as_launch<D, PAGED, AS_SLOPES>(m, j, mod, plan, dev, s);
+    return mod.bias != nullptr ? as_launch<D, PAGED, AS_BIAS>(m, j, mod, plan, dev, s) : as_launch<D, PAGED, AS_PLAIN>(m, j, mod, plan, dev, s);
   }
   const float cap = mod.cap * AS_LOG2E;
   if (cap >= AS_CAP_LOW && cap <= AS_CAP_HIGH && mod.slopes == nullptr && mod.bias == nullptr)
-    return as_launch<D, PAGED, AS_CAP>(m, j, mod, plan, sms, s);
-  return as_launch<D, PAGED, AS_ANY>(m, j, mod, plan, sms, s);
+    return as_launch<D, PAGED, AS_CAP>(m, j, mod, plan, dev, s);
+  return as_launch<D, PAGED, AS_ANY>(m, j, mod, plan, dev, s);
 }
 
 template <bool PAGED>
 static int as_dispatch(const AsMaps& m, const AttnJob& j, const AttnMod& mod, void* workspace, cudaStream_t s) {
-  int rc = kernels_init_device();
-  int sms = 0;
-  if (!rc) rc = as_sm_count(&sms);
-  if (rc) return rc;
+  AsDevice dev = {};
+  B2_CUDA_CHECK(cudaGetDevice(&dev.id));
+  B2_CUDA_CHECK(cudaDeviceGetAttribute(&dev.sms, cudaDevAttrMultiProcessorCount, dev.id));
   AttnPlan plan;
   as_layout(workspace, j.n_seqs, j.n_tokens, j.n_heads, j.n_kv_heads, j.head_dim, &plan);
-  return j.head_dim <= 64 ? as_launch_mode<64, PAGED>(m, j, mod, plan, sms, s) : as_launch_mode<128, PAGED>(m, j, mod, plan, sms, s);
+  return j.head_dim <= 64 ? as_launch_mode<64, PAGED>(m, j, mod, plan, dev, s) : as_launch_mode<128, PAGED>(m, j, mod, plan, dev, s);
 }
 
 }  // namespace b2

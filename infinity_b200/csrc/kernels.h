@@ -55,7 +55,8 @@ inline cudaError_t launch_pdl(void (*kern)(KArgs...), dim3 grid, dim3 block, siz
   return cudaLaunchKernelEx(&cfg, kern, static_cast<KArgs>(args)...);
 }
 
-// Opt-in shared-memory attributes of every kernel, for the current device. Idempotent.
+// Opt-in shared-memory attributes of the forward's and the single operators' kernels, for the current device. Idempotent. Attention with
+// modified scores sets its kernels up by itself, one by one (attention_scored.cu).
 int kernels_init_device();
 
 // ---- GEMM (gemm_bf16.cu) ----
@@ -134,7 +135,6 @@ int launch_attention_tc2(const void* qkv, void* out, const AttnTile* d_tiles, in
                          int n_kv_heads, int head_dim, int causal, int sm_count, int* err_flag, cudaStream_t stream);
 int attention_tc_init_device();
 int attention_tc2_init_device();
-int attention_scored_init_device();  // attention with modified scores, packed and paged (attention_scored.cu)
 
 // ---- block-format weight quantisers (quant.cu) ----
 // w bf16 [rows, cols] -> q (packed elements), scales (one byte per block, row-major [rows, cols / block]);

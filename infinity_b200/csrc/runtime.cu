@@ -59,7 +59,6 @@ int kernels_init_device() {
   if (!rc) rc = attention_init_device();
   if (!rc) rc = attention_tc_init_device();
   if (!rc) rc = attention_tc2_init_device();
-  if (!rc) rc = attention_scored_init_device();
   if (!rc) rc = gemm_mxfp8_init_device();
   if (!rc) rc = gemm_w4_init_device();
   if (!rc) rc = moe_init_device();
