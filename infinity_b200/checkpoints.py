@@ -60,6 +60,16 @@ def _strip_prefix(sd: Dict[str, torch.Tensor], marker: str) -> Tuple[Dict[str, t
     return body, rest
 
 
+def _check_rope(config: dict) -> None:
+    """Refuses rotary positions that the decoder does not turn by: it has unscaled angles only. ``dynamic`` scaling begins beyond
+    max_position_embeddings, which no input passes."""
+    for key in ("rope_scaling", "rope_parameters"):
+        rope = config.get(key) or {}
+        kind = rope.get("rope_type") or rope.get("type") or ("unnamed" if "factor" in rope else "default")
+        if kind not in ("default", "dynamic") and not (kind == "linear" and rope.get("factor") == 1.0):
+            raise ValueError(f"{key} of type '{kind}' is not supported (unscaled rotary positions only)")
+
+
 def spec_from_hf_config(config: dict, *, name: str = "checkpoint", pooling: Optional[str] = None,
                         normalize: Optional[bool] = None, head: Optional[str] = None) -> ModelSpec:
     """The runtime's model descriptor for a transformers ``config.json``."""
@@ -89,6 +99,7 @@ def spec_from_hf_config(config: dict, *, name: str = "checkpoint", pooling: Opti
             max_len=config["max_position_embeddings"] - pos_offset)
     if mt == "qwen2":
         H, nh = config["hidden_size"], config["num_attention_heads"]
+        _check_rope(config)
         rope = config.get("rope_theta") or (config.get("rope_parameters") or {}).get("rope_theta", 10000.0)
         return ModelSpec(
             name=name, arch="decoder", n_layers=config["num_hidden_layers"], hidden=H, n_heads=nh,

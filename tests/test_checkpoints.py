@@ -151,3 +151,25 @@ def test_converted_checkpoint_runs_like_transformers(tmp_path, kind):
         cos = (got * ref).sum(1) / (np.linalg.norm(got, axis=1) * np.linalg.norm(ref, axis=1))
         assert cos.min() >= 0.9999, cos
     gpu.close()
+
+
+_DECODER = dict(model_type="qwen2", hidden_size=128, num_attention_heads=4, num_hidden_layers=2, intermediate_size=256, vocab_size=1000,
+                max_position_embeddings=128, rope_theta=1e6)
+
+
+@pytest.mark.parametrize("rope", [dict(type="yarn", factor=4.0, original_max_position_embeddings=32), dict(rope_type="linear", factor=2.0),
+                                  dict(rope_type="longrope", factor=8.0), dict(factor=2.0)], ids=str)
+@pytest.mark.parametrize("key", ["rope_scaling", "rope_parameters"])
+def test_scaled_rotary_positions_are_refused(key, rope):
+    """The decoder's angles are unscaled: such a checkpoint would load and give other embeddings than its model."""
+    with pytest.raises(ValueError, match="rotary"):
+        ck.spec_from_hf_config(dict(_DECODER, **{key: rope}))
+
+
+@pytest.mark.parametrize("rope", [None, {}, dict(rope_type="default", rope_theta=1e6), dict(type="default"), dict(rope_type="linear", factor=1.0),
+                                  dict(type="dynamic", factor=4.0)], ids=str)
+def test_unscaled_rotary_positions_are_taken(rope):
+    """``dynamic`` scaling starts beyond max_position_embeddings, and the descriptor takes no longer input."""
+    spec = ck.spec_from_hf_config(dict(_DECODER, rope_scaling=rope))
+    assert spec.rope_theta == 1e6 and spec.max_len == 128
+    assert ck.spec_from_hf_config(dict(_DECODER, rope_parameters=rope)).rope_theta == 1e6
