@@ -21,8 +21,10 @@ int set_error(int code, const char* fmt, ...);
 #define B2_CUDA_CHECK(expr)                                                                  \
   do {                                                                                       \
     cudaError_t e__ = (expr);                                                                \
-    if (e__ != cudaSuccess)                                                                  \
+    if (e__ != cudaSuccess) {                                                                \
+      cudaGetLastError(); /* reported here: the next call's launch check is not to find it */ \
       return ::b2::set_error(B200EMB_ERR_CUDA, "%s: %s", #expr, cudaGetErrorString(e__));    \
+    }                                                                                        \
   } while (0)
 
 // Programmatic dependent launch: a kernel launched through launch_pdl may be scheduled while its predecessor
@@ -52,7 +54,9 @@ inline cudaError_t launch_pdl(void (*kern)(KArgs...), dim3 grid, dim3 block, siz
   attr[0].val.programmaticStreamSerializationAllowed = pdl_enabled() ? 1 : 0;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, kern, static_cast<KArgs>(args)...);
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, kern, static_cast<KArgs>(args)...);
+  if (e != cudaSuccess) cudaGetLastError();  // as B2_CUDA_CHECK
+  return e;
 }
 
 // Opt-in shared-memory attributes of the forward's and the single operators' kernels, for the current device. Idempotent. Attention with

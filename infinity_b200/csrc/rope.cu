@@ -282,8 +282,11 @@ static int rope_launch_v(const RopeParams& p, RopeJob j, cudaStream_t s) {
   j.turned = static_cast<int>(turned);
   j.items = static_cast<int>(items);
   const int threads = static_cast<int>(items < 64 ? 64 : items < ROPE_MAX_THREADS ? (items + 31) / 32 * 32 : ROPE_MAX_THREADS);
-  rope_kernel_op<V, APPEND><<<static_cast<unsigned>(j.n_tokens), threads, 0, s>>>(p, j);
-  const cudaError_t e = cudaGetLastError();
+  cudaLaunchConfig_t cfg = {};  // returns this launch's own error: what an earlier call left behind is not this one's
+  cfg.gridDim = dim3(static_cast<unsigned>(j.n_tokens));
+  cfg.blockDim = dim3(static_cast<unsigned>(threads));
+  cfg.stream = s;
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, rope_kernel_op<V, APPEND>, p, j);
   if (e != cudaSuccess) return set_error(B200EMB_ERR_CUDA, "rope launch: %s", cudaGetErrorString(e));
   return B200EMB_OK;
 }
