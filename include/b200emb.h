@@ -431,7 +431,8 @@ typedef struct b200emb_kv_cache {
  * qkv is the packed buffer of b200emb_op_attention with row stride qkv_row_stride. kv_lens[s] counts the keys of
  * sequence s INCLUDING its new tokens: token t of sequence s gets position kv_lens[s] - (new tokens of s) + t - cu_seqlens[s].
  * q_out [n_tokens, n_heads * head_dim] (row stride q_out_row_stride) receives the queries (copied when rope is null);
- * q_out null: they are not touched. Tokens at a negative position, past the page table or on a page outside [0, n_pages)
+ * q_out null: they are not touched; q_out == qkv with the same row stride: they are turned in place. No other overlap of qkv, q_out and
+ * the cache is allowed. Tokens at a negative position, past the page table or on a page outside [0, n_pages)
  * are not stored. A slot written by two tokens holds one of the two. */
 int b200emb_op_kv_append(const void* qkv, int64_t qkv_row_stride, const int32_t* d_cu_seqlens, const int32_t* d_kv_lens,
                          int32_t n_seqs, int32_t n_tokens, int32_t n_heads, const b200emb_rope_desc* rope, void* q_out,
@@ -477,7 +478,8 @@ int b200emb_op_workspace_status(const void* workspace, void* stream);
 /* Packed variable-length attention: q [n_tokens, n_heads * head_dim], k and v [n_tokens, n_kv_heads * head_dim], out
  * [n_tokens, n_heads * head_dim], each with its own row stride (elements, a multiple of 8) and 16-byte aligned, so the packed qkv
  * buffer serves with three pointers. n_heads a multiple of n_kv_heads and at most 128 times it; head_dim a multiple of 8, 8 .. 128; up to
- * 2^30 tokens. opts null: plain bidirectional attention. Query i of a sequence is at position i. */
+ * 2^30 tokens. opts null: plain bidirectional attention. Query i of a sequence is at position i. out may be q itself with the same row
+ * stride; it may not overlap q, k or v in any other way. */
 int b200emb_op_attention_scored(const void* q, int64_t q_row_stride, const void* k, int64_t k_row_stride, const void* v,
                                 int64_t v_row_stride, void* out, int64_t out_row_stride, const int32_t* d_cu_seqlens,
                                 int32_t n_seqs, int32_t n_tokens, int32_t n_heads, int32_t n_kv_heads, int32_t head_dim,
@@ -486,7 +488,7 @@ int b200emb_op_attention_scored(const void* q, int64_t q_row_stride, const void*
 /* Attention of new tokens (a chunk of any length, or one) over the paged cache, which already holds their own keys
  * (b200emb_op_kv_append). The new tokens of sequence s are rows cu_seqlens[s] .. cu_seqlens[s + 1] - 1 of q and out and take the last
  * positions below kv_lens[s]. kv_lens is cut to table_stride * page_size. page_size a multiple of 8, table_stride * page_size up to 2^30; the three cache
- * strides multiples of 8, k and v 16-byte aligned. opts null: causal. Few rows over long caches are split over the keys
+ * strides multiples of 8, k and v 16-byte aligned. opts null: causal. out may be q itself with the same row stride. Few rows over long caches are split over the keys
  * and joined in a fixed order: results depend on the batch's lengths and the device alone. */
 int b200emb_op_attention_paged(const void* q, int64_t q_row_stride, void* out, int64_t out_row_stride,
                                const int32_t* d_cu_seqlens, const int32_t* d_kv_lens, int32_t n_seqs, int32_t n_tokens,

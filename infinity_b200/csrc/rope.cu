@@ -367,6 +367,8 @@ extern "C" int b200emb_op_kv_append(const void* qkv, int64_t qkv_row_stride, con
   if (n_tokens == 0 || n_seqs == 0) return B200EMB_OK;
   if (qkv == nullptr || d_cu_seqlens == nullptr || d_kv_lens == nullptr)
     return set_error(B200EMB_ERR_INVALID, "kv_append: null pointer");
+  if (q_out == qkv && q_out_row_stride != qkv_row_stride)
+    return set_error(B200EMB_ERR_INVALID, "kv_append: queries in place need equal row strides");
   RopeJob j = {};
   j.x = static_cast<const __nv_bfloat16*>(qkv);
   j.x_stride = qkv_row_stride;

@@ -63,6 +63,10 @@ def test_append_refuses(lib, kw):
     assert append(lib, **kw) == INVALID and _lib.last_error()
 
 
+def test_append_refuses_queries_in_place_with_another_stride(lib):
+    assert append(lib, qkv=P, q_out=P, stride=512, q_stride=256) == INVALID and "in place" in _lib.last_error()
+
+
 def test_append_refuses_positions_that_pass_32_bits(lib):
     assert append(lib, table_stride=1 << 28) == UNSUPPORTED
 

@@ -546,6 +546,37 @@ def test_paged_offsets_beyond_32_bits(lib):
     _check_paged(out, q_out[39:], [1], [40], 2, pages, {})
 
 
+# -- in place -------------------------------------------------------------------------------------
+@pytest.mark.parametrize("rope", [None, dict(rot=32, layout="interleaved"), dict(rot=6), dict(rot=6, layout="interleaved")], ids=str)
+def test_append_turns_queries_in_place(lib, rope):
+    heads, kv_heads, dim, kv = 6, 2, 32, [41, 3]
+    pages, again = (R.Pages(kv, kv_heads, dim, 16) for _ in range(2))
+    qkv, cu = R.normal(9, 44, (heads + 2 * kv_heads) * dim), R.cu_of(kv)
+    d = None if rope is None else R.rope_desc(**rope)
+    q_out, same = torch.empty(44, heads * dim, dtype=R.BF16, device="cuda"), qkv.clone()
+    R.append(lib, qkv, cu, R.ints(kv), heads, pages, d, q_out)
+    R.append(lib, same, cu, R.ints(kv), heads, again, d, same)
+    assert torch.equal(same[:, :heads * dim], q_out) and torch.equal(same[:, heads * dim:], qkv[:, heads * dim:])
+    assert torch.equal(again.k.view(torch.int16), pages.k.view(torch.int16)) and torch.equal(again.v.view(torch.int16), pages.v.view(torch.int16))
+
+
+@pytest.mark.parametrize("lens,heads,kv_heads,dim", [([300, 1, 70], 4, 2, 64), ([2600], 7, 1, 128), ([40] * 50, 2, 2, 32)], ids=str)
+def test_attention_in_place_of_its_queries(lib, lens, heads, kv_heads, dim):
+    """Items that several streams share are joined after the last of them has read its queries."""
+    t = sum(lens)
+    x, cu = R.normal(4, t, (heads + 2 * kv_heads) * dim, gain=1.5), R.cu_of(lens)
+    q, k, v = _split(x, heads, kv_heads, dim)
+    want = R.scored(lib, q, k, v, cu, heads, kv_heads, R.options(causal=1))
+    R.scored(lib, q, k, v, cu, heads, kv_heads, R.options(causal=1), out=q)
+    assert torch.equal(q, want)
+    new, kv = [1, 3, 130], [1500, 3, 400]
+    pages = R.Pages(kv, kv_heads, dim, 16).fill(2)
+    q = R.normal(3, sum(new), heads * dim, gain=2.0)
+    want = R.paged(lib, q, R.cu_of(new), R.ints(kv), heads, pages, None)
+    R.paged(lib, q, R.cu_of(new), R.ints(kv), heads, pages, None, out=q)
+    assert torch.equal(q, want)
+
+
 # -- together, captured, on other streams --------------------------------------------------------
 @pytest.mark.parametrize("heads,kv_heads,dim,page", [(4, 2, 64, 16), (7, 1, 128, 24)])
 def test_chunks_over_the_cache_match_one_pass(lib, heads, kv_heads, dim, page):
