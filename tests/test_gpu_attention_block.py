@@ -304,6 +304,22 @@ def test_scored_counts_beyond_the_common(lib, lens, heads, kv_heads, dim, name):
     _check_scored(out, q, k, v, lens, heads, kv_heads, dim, mod, slopes, bias, prefix, docs)
 
 
+@pytest.mark.parametrize("name", ["slopes_prefix", "slopes_prefix_window", "slopes_window", "steep_prefix", "bias_prefix", "cap_prefix", "docs_slopes_prefix"])
+@pytest.mark.parametrize("lens,heads,kv_heads,dim", [([5, 200, 0, 700], 4, 2, 64), ([1500, 90], 7, 1, 128)], ids=["64", "128"])
+def test_scored_prefix_with_the_others(lib, lens, heads, kv_heads, dim, name):
+    """A prefix is walked before the window: with slopes its keys, the farthest of all, give a row its first reference."""
+    mods = {"slopes_prefix": dict(causal=1, slopes=True, prefix=True), "slopes_prefix_window": dict(causal=1, left=40, slopes=True, prefix=True),
+            "slopes_window": dict(left=70, right=130, slopes=True), "steep_prefix": dict(causal=1, left=3, slopes=True, prefix=True),
+            "bias_prefix": dict(causal=1, left=20, bias=33, prefix=True), "cap_prefix": dict(causal=1, left=20, cap=20.0, prefix=True),
+            "docs_slopes_prefix": dict(causal=1, left=90, slopes=True, prefix=True, docs=True)}
+    x, mod, slopes, bias, prefix, docs = _scored_case(lens, heads, kv_heads, dim, mods[name])
+    if name == "steep_prefix":
+        slopes = slopes * 16
+    q, k, v = _split(x, heads, kv_heads, dim)
+    out = R.scored(lib, q, k, v, R.cu_of(lens), heads, kv_heads, R.options(slopes=slopes, bias=bias, prefix=prefix, docs=docs, **mod))
+    _check_scored(out, q, k, v, lens, heads, kv_heads, dim, mod, slopes, bias, prefix, docs)
+
+
 def test_scored_options_null_is_plain_attention(lib):
     lens = [30, 61]
     x = R.normal(1, 91, 3 * 2 * 64)
@@ -484,6 +500,15 @@ def test_paged(lib, case, name):
     out = R.paged(lib, q, R.cu_of(new), R.ints(kv), heads, pages, o)
     _check_paged(out, q, new, kv, heads, pages, mod, slopes, bias, prefix)
     assert torch.equal(out, R.paged(lib, q, R.cu_of(new), R.ints(kv), heads, pages, o))
+
+
+@pytest.mark.parametrize("left", [-1, 25])
+def test_paged_slopes_with_a_prefix(lib, left):
+    new, kv, heads, kv_heads, dim = [1, 40, 130], [900, 41, 600], 8, 2, 64
+    pages = R.Pages(kv, kv_heads, dim, 16).fill(3)
+    q, slopes, prefix = R.normal(12, sum(new), heads * dim, gain=2.0), _slopes(heads), R.ints([300, 0, 599])
+    out = R.paged(lib, q, R.cu_of(new), R.ints(kv), heads, pages, R.options(causal=1, left=left, slopes=slopes, prefix=prefix))
+    _check_paged(out, q, new, kv, heads, pages, dict(left=left), slopes, None, prefix)
 
 
 def test_paged_counts_beyond_the_common(lib):
