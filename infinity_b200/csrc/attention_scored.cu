@@ -25,10 +25,10 @@
 //   O += P V      P rounded to bf16 (the tensor core's operand type; half a step of 2^-8 per probability) in tensor memory, V as an MN-major
 //                 shared-memory operand
 // What bounds it: a softmax warp's chain of dependent instructions, two such warps on each scheduler; the special-function unit is
-// busy 42 to 47 % of the time, the tensor cores as much. 8 sequences of 2048 tokens, 28/4 heads of 128: 530 us (907 TFLOP/s; 543 with
-// slopes, 623 capped, 340 causal, 673 with a bias table of radius 128); 16 heads of 64: 265 us (519 TFLOP/s; 286 with slopes, 339 capped,
-// 180 causal). One new token of 64 sequences over 64 to 8192 keys, 28/4
-// heads of 128: 67 us, 3.5 TB/s, 6 of them the plan.
+// busy 15 to 47 % of the time, the tensor cores 10 to 46 %, the issue slots 38 to 51 % (single tokens over a cache: 8, 27 and 19 %, they wait
+// for memory). 8 sequences of 2048 tokens, 28/4 heads of 128, normal inputs: 541 us (890 TFLOP/s; 580 with slopes, 668 capped, 373 causal, 709 with a bias table of radius 128);
+// 16 heads of 64: 266 us (517 TFLOP/s; 281 with slopes, 334 capped, 177 causal). One new token of 64 sequences over 64 to 8192 keys, 28/4
+// heads of 128: 66 us, 3.5 TB/s, 6 of them the plan.
 // Warps: 0-3 softmax A, 4-7 softmax B, 8 loads Q and K, 9 loads V, 10 and 11 issue the matrix instructions of A and B.
 #include <cuda.h>
 #include <cuda_bf16.h>
@@ -361,7 +361,7 @@ attn_plan_kernel(const AttnJob j, const AttnMod mod, const AttnPlan p, int token
   // Parts of equal cost; a cut moves to an item's edge that is nearer than 1/16 of a part.
   const int heads = j.n_kv_heads;
   const int64_t total = carry * heads, total_cost = (carry + static_cast<int64_t>(AS_ITEM_STEPS) * n_entries) * heads;
-  // a part of an item has two steps or more: what a part costs to join is more than a step
+  // parts have two steps or more on average, since what a part costs to join is more than a step (a cut by cost may still leave one)
   const int64_t most = max(min(total, static_cast<int64_t>(n_entries) * heads), (total + 1) / 2);
   const int slots = static_cast<int>(min(most, static_cast<int64_t>(max_slots)));
   __syncthreads();
@@ -629,8 +629,10 @@ attn_scored_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_cons
   using Cfg = AsCfg<D>;
   constexpr int RING = Cfg::RING, KV = Cfg::KV;
   constexpr uint32_t Q_BUFS = Cfg::Q_BUFS;
-  // Whether a segment's first step may go the straight way (8 sequences of 2048, plain: 16 heads of 64, 280 us so and 266 not; 28/4 heads
-  // of 128, causal, 343 and 354).
+  // Whether a segment's first step may go the straight way, us with it and without. Caps (they need no reference): 96 sequences of 300 tokens,
+  // 16 heads of 64, 174 and 194; 64 of 300, 28/4 heads of 128, 186 and 204; 8 of 2048 334 and 343, 670 and 690. Bias tables: the same short
+  // batches 205 and 225, 214 and 231, long ones equal. Plain scores at head_dim 128: short 153 and 156, causal 131 and 133, long 543 and 536; at 64 long
+  // ones lose more (283 and 265; short 144 and 147, causal 121 and 126). Slopes: their first step holds the queries' own positions.
   constexpr bool FIRST = MODE == AS_CAP || MODE == AS_BIAS || (MODE == AS_PLAIN && D == 128);
   constexpr bool DOCS = MODE == AS_DOCS || MODE == AS_ANY, TABLES = DOCS || MODE == AS_BIAS;
   // A stream's own tiles in flight, so that neither stream waits for the other's.
