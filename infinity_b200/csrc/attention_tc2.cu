@@ -602,11 +602,11 @@ int attention_tc2_init_device() {
 }
 
 template <int D, bool CAUSAL>
-static void t2_launch(const CUtensorMap& tm, void* out, const AttnTile* d_tiles, int n_items, int n_heads, int n_kv_heads,
-                      int grid, int* err_flag, cudaStream_t stream) {
+static cudaError_t t2_launch(const CUtensorMap& tm, void* out, const AttnTile* d_tiles, int n_items, int n_heads, int n_kv_heads,
+                             int grid, int* err_flag, cudaStream_t stream) {
   const float scale_log2 = 1.4426950408889634f / sqrtf(static_cast<float>(D));
-  launch_pdl(attn_tc2_kernel<D, CAUSAL>, dim3(grid), dim3(T2_THREADS), T2Cfg<D>::SMEM_BYTES, stream, tm,
-             reinterpret_cast<__nv_bfloat16*>(out), d_tiles, n_items, n_heads, n_kv_heads, scale_log2, err_flag);
+  return launch_pdl(attn_tc2_kernel<D, CAUSAL>, dim3(grid), dim3(T2_THREADS), T2Cfg<D>::SMEM_BYTES, stream, tm,
+                    reinterpret_cast<__nv_bfloat16*>(out), d_tiles, n_items, n_heads, n_kv_heads, scale_log2, err_flag);
 }
 
 int launch_attention_tc2(const void* qkv, void* out, const AttnTile* d_tiles, int n_tiles, int n_tokens, int n_heads,
@@ -624,14 +624,14 @@ int launch_attention_tc2(const void* qkv, void* out, const AttnTile* d_tiles, in
   if (n_items > 0x7fffffffLL) return set_error(B200EMB_ERR_UNSUPPORTED, "attention: too many tiles");
   const int grid = static_cast<int>(n_items < sm_count ? n_items : sm_count);
   const int ni = static_cast<int>(n_items);
+  cudaError_t e;
   if (head_dim == 64) {
-    if (causal) t2_launch<64, true>(tm, out, d_tiles, ni, n_heads, n_kv_heads, grid, err_flag, stream);
-    else t2_launch<64, false>(tm, out, d_tiles, ni, n_heads, n_kv_heads, grid, err_flag, stream);
+    e = causal ? t2_launch<64, true>(tm, out, d_tiles, ni, n_heads, n_kv_heads, grid, err_flag, stream)
+               : t2_launch<64, false>(tm, out, d_tiles, ni, n_heads, n_kv_heads, grid, err_flag, stream);
   } else {
-    if (causal) t2_launch<128, true>(tm, out, d_tiles, ni, n_heads, n_kv_heads, grid, err_flag, stream);
-    else t2_launch<128, false>(tm, out, d_tiles, ni, n_heads, n_kv_heads, grid, err_flag, stream);
+    e = causal ? t2_launch<128, true>(tm, out, d_tiles, ni, n_heads, n_kv_heads, grid, err_flag, stream)
+               : t2_launch<128, false>(tm, out, d_tiles, ni, n_heads, n_kv_heads, grid, err_flag, stream);
   }
-  cudaError_t e = cudaGetLastError();
   if (e != cudaSuccess) return set_error(B200EMB_ERR_CUDA, "attention launch: %s", cudaGetErrorString(e));
   return B200EMB_OK;
 }

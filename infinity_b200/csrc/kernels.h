@@ -41,8 +41,9 @@ constexpr long long PDL_MAX_WORK = 12ll << 20;
 bool pdl_enabled();
 void pdl_for_batch(int n_tokens, int hidden);
 
+// The status is the returned one alone: a failure is not left for cudaGetLastError.
 template <typename... KArgs, typename... Args>
-inline cudaError_t launch_pdl(void (*kern)(KArgs...), dim3 grid, dim3 block, size_t smem_bytes, cudaStream_t stream,
+[[nodiscard]] inline cudaError_t launch_pdl(void (*kern)(KArgs...), dim3 grid, dim3 block, size_t smem_bytes, cudaStream_t stream,
                               Args&&... args) {
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = grid;
