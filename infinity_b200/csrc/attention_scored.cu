@@ -26,9 +26,9 @@
 //                 shared-memory operand
 // What bounds it: a softmax warp's chain of dependent instructions, two such warps on each scheduler; the special-function unit is
 // busy 15 to 47 % of the time, the tensor cores 10 to 46 %, the issue slots 38 to 51 % (single tokens over a cache: 8, 27 and 19 %, they wait
-// for memory). 8 sequences of 2048 tokens, 28/4 heads of 128, normal inputs: 541 us (890 TFLOP/s; 580 with slopes, 668 capped, 373 causal, 709 with a bias table of radius 128);
-// 16 heads of 64: 266 us (517 TFLOP/s; 281 with slopes, 334 capped, 177 causal). One new token of 64 sequences over 64 to 8192 keys, 28/4
-// heads of 128: 66 us, 3.5 TB/s, 6 of them the plan.
+// for memory). 8 sequences of 2048 tokens, 28/4 heads of 128, normal inputs: 541 us (890 TFLOP/s; 580 with slopes, 668 capped, 373 causal,
+// 709 with a bias table of radius 128); 16 heads of 64: 266 us (517 TFLOP/s; 281 with slopes, 334 capped, 177 causal). One new token of 64
+// sequences over 64 to 8192 keys, 28/4 heads of 128: 66 us, 3.5 TB/s, 6 of them the plan.
 // Warps: 0-3 softmax A, 4-7 softmax B, 8 loads Q and K, 9 loads V, 10 and 11 issue the matrix instructions of A and B.
 #include <cuda.h>
 #include <cuda_bf16.h>
